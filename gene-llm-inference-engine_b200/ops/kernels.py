@@ -1556,3 +1556,52 @@ def sample(logits: torch.Tensor, scratch: torch.Tensor, temperature: torch.Tenso
                           _dev(temperature, "temperature", torch.float32), _dev(top_k, "top_k", torch.int32),
                           _dev(top_p, "top_p", torch.float32), _dev(uniform, "uniform", torch.float32),
                           _dev(out, "out", torch.int32), _stream()), "sample")
+
+
+def token_probabilities(logits: torch.Tensor, temperature: torch.Tensor, out: torch.Tensor) -> None:
+    """out[r, :] = the distribution that ``sample`` draws row r from without filters: exp((l - max l) / T) times the 32-bit
+    reciprocal of its sum (taken in 64 bits), T = temperature[r]; one-hot at the argmax for T <= 0 (NaN where a row has no
+    distribution). ``logits`` [rows, vocab] 32-bit or bfloat16, ``out`` 32-bit: what a drafter keeps for ``verify_drafts``."""
+    rows, V = logits.shape
+    if out.shape != logits.shape or temperature.numel() != rows:
+        raise KernelError("token_probabilities: shapes of logits, temperature and out do not agree")
+    check(lib().gi_token_probabilities(_dev(logits, "logits"), dtype_code(logits.dtype), rows, V, _dev(temperature, "temperature", torch.float32),
+                                       _dev(out, "out", torch.float32), _stream()), "token_probabilities")
+
+
+def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafted: torch.Tensor, counts: torch.Tensor,
+                  draft_probs: Optional[torch.Tensor], temperature: torch.Tensor, accept_uniform: torch.Tensor,
+                  draw_uniform: torch.Tensor, tokens: torch.Tensor, accepted: torch.Tensor, work: torch.Tensor) -> None:
+    """Drafted tokens against the target's distribution. Request r has counts[r] (0 to D) drafts drafted[r, :] and counts[r] + 1
+    rows of ``logits`` [N, vocab] (32-bit or bfloat16) from row_start[r] on; row j judges draft j. With T = temperature[r] > 0 and p_j the
+    row's distribution (``token_probabilities``), draft x_j is kept while accept_uniform[r, j] * q_j(x_j) < p_j(x_j); the first one
+    refused is replaced by a draw from max(p_j - q_j, 0) (from p_j where nothing of that is left), and with all of them kept one
+    more token is drawn from the last row. T <= 0: kept while it is the argmax (the lowest index among equals), which also
+    replaces it. A draw takes the first token of some weight at which the running sum passes draw_uniform[r] times the whole.
+
+    ``draft_probs`` [R, D, vocab] 32-bit: q (its first two dimensions may have any strides); None: the drafts come from no
+    distribution (a look-up), q is one at the draft. ``tokens`` [R, D + 1]: the kept drafts, the new token, then -1; ``accepted`` [R]: how many
+    drafts were kept (-1, and no token, for a request whose rows do not lie in ``logits``). A row without a distribution (a logit
+    that is no number or +infinity, or all of them -infinity) refuses its draft and gives the last token of the vocabulary, as
+    ``sample`` does. No two requests may share a row. ``work`` [N, 4] 32-bit scratch. Two launches."""
+    N, V = logits.shape
+    R, D = drafted.shape
+    if row_start.numel() != R or counts.numel() != R or temperature.numel() != R or draw_uniform.numel() != R or accepted.numel() != R \
+            or accept_uniform.shape != (R, D) or tokens.shape != (R, D + 1):
+        raise KernelError("verify_drafts: the sizes of the requests' arrays do not agree")
+    if work.numel() < 4 * N:
+        raise KernelError("verify_drafts: work must hold four values a row of logits")
+    q, q_request, q_place = 0, 0, 0
+    if draft_probs is not None:
+        if draft_probs.shape != (R, D, V):
+            raise KernelError("verify_drafts: draft_probs must be [R, D, vocab]")
+        if not draft_probs.is_cuda or draft_probs.dtype != torch.float32 or (V > 1 and draft_probs.stride(2) != 1):
+            raise KernelError("verify_drafts: draft_probs must be 32-bit values on the device, the vocabulary's neighbours in memory")
+        q_request, q_place, _ = draft_probs.stride()
+        q = draft_probs.data_ptr() if D else 0
+    check(lib().gi_verify_drafts(
+        _dev(logits, "logits"), dtype_code(logits.dtype), N, V, R, D, _dev(row_start, "row_start", torch.int32),
+        _dev(drafted, "drafted", torch.int32), _dev(counts, "counts", torch.int32), q, q_request, q_place,
+        _dev(temperature, "temperature", torch.float32), _dev(accept_uniform, "accept_uniform", torch.float32),
+        _dev(draw_uniform, "draw_uniform", torch.float32), _dev(tokens, "tokens", torch.int32), _dev(accepted, "accepted", torch.int32),
+        _dev(work, "work", torch.float32), _stream()), "verify_drafts")
