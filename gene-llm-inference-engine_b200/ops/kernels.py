@@ -1605,3 +1605,43 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafted: torch.
         _dev(temperature, "temperature", torch.float32), _dev(accept_uniform, "accept_uniform", torch.float32),
         _dev(draw_uniform, "draw_uniform", torch.float32), _dev(tokens, "tokens", torch.int32), _dev(accepted, "accepted", torch.int32),
         _dev(work, "work", torch.float32), _stream()), "verify_drafts")
+
+
+def _table_args(lengths, tables, held, free_pages, n_free, status):
+    R = lengths.numel()
+    if tables.dim() != 2 or tables.shape[0] != R or held.numel() != R or n_free.numel() != 1 or status.numel() != 1:
+        raise KernelError("step_tables: the sizes of lengths, tables, held, n_free and status do not agree")
+    return R, (_dev(tables, "tables", torch.int32), tables.shape[1], _dev(held, "held", torch.int32), _dev(free_pages, "free_pages", torch.int32),
+               _dev(n_free, "n_free", torch.int32), free_pages.numel())
+
+
+def step_tables(lengths: torch.Tensor, counts: torch.Tensor, tables: torch.Tensor, held: torch.Tensor, free_pages: torch.Tensor,
+                n_free: torch.Tensor, page_size: int, row_start: torch.Tensor, row_req: torch.Tensor, positions: torch.Tensor,
+                slots: torch.Tensor, status: torch.Tensor) -> None:
+    """A step's tables on the device (all int32). Request r has lengths[r] cached positions, brings counts[r] tokens and holds held[r]
+    pages, named by ``tables`` [R, stride]; ``free_pages`` is a stack of n_free[0] free pages (its size: the most it can hold). Every
+    request gets the pages that lengths + counts positions need; pages beyond go back, the last request's last first, before any
+    is taken (entries given back become -1). ``row_start`` [R + 1]: the requests' first rows and the number of rows;
+    ``row_req``, ``positions``, ``slots`` (as many places as a step may have rows): every row's request, position and slot
+    (page * page_size + place in the page); rows beyond the step's: -1, 0, -1. A request's pages must be its own: shared
+    prefixes are the host manager's business.
+
+    ``status`` [1]: 0; else nothing but the status has been written: the number of pages missing, -1 (more rows than places), -2 (a
+    request beyond its table), -3 (a negative number, or more pages held than the table has), -4 (more free pages than the stack holds)."""
+    R, args = _table_args(lengths, tables, held, free_pages, n_free, status)
+    rows = row_req.numel()
+    if counts.numel() != R or row_start.numel() != R + 1 or positions.numel() != rows or slots.numel() != rows:
+        raise KernelError("step_tables: the sizes of counts, row_start, row_req, positions and slots do not agree")
+    check(lib().gi_step_tables(_dev(lengths, "lengths", torch.int32), _dev(counts, "counts", torch.int32), R, *args, int(page_size),
+                               _dev(row_start, "row_start", torch.int32), _dev(row_req, "row_req", torch.int32),
+                               _dev(positions, "positions", torch.int32), _dev(slots, "slots", torch.int32), rows,
+                               _dev(status, "status", torch.int32), _stream()), "step_tables")
+
+
+def trim_tables(lengths: torch.Tensor, tables: torch.Tensor, held: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor,
+                page_size: int, status: torch.Tensor) -> None:
+    """The block tables of ``step_tables`` after a rewind (drafts that were refused) or the end of a request (length 0): every request
+    keeps the pages that lengths[r] positions need (and gets those it lacks), the others go back on the stack."""
+    R, args = _table_args(lengths, tables, held, free_pages, n_free, status)
+    check(lib().gi_step_tables(_dev(lengths, "lengths", torch.int32), 0, R, *args, int(page_size), 0, 0, 0, 0, 0,
+                               _dev(status, "status", torch.int32), _stream()), "trim_tables")

@@ -129,6 +129,8 @@ _SIGNATURES = {
     "gi_program_run": [c_void_p, c_void_p],
     "gi_program_free": [c_void_p],
     "gi_argmax": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+    "gi_step_tables": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                       c_void_p, c_int, c_void_p, c_void_p],
     "gi_token_probabilities": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "gi_verify_drafts": [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong,
                          c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
