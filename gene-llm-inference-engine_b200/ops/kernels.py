@@ -1645,3 +1645,77 @@ def trim_tables(lengths: torch.Tensor, tables: torch.Tensor, held: torch.Tensor,
     R, args = _table_args(lengths, tables, held, free_pages, n_free, status)
     check(lib().gi_step_tables(_dev(lengths, "lengths", torch.int32), 0, R, *args, int(page_size), 0, 0, 0, 0, 0,
                                _dev(status, "status", torch.int32), _stream()), "trim_tables")
+
+
+class AdapterPlan:
+    """The rows of a step in the order of their adapters (``adapter_plan``), for every ``adapter_product`` of the step."""
+
+    __slots__ = ("buffer", "rows", "adapters", "tile_rows", "tiles")
+
+    def __init__(self, buffer: torch.Tensor, rows: int, adapters: int, tile_rows: int, tiles: int):
+        self.buffer, self.rows, self.adapters, self.tile_rows, self.tiles = buffer, rows, adapters, tile_rows, tiles
+
+
+def _adapter_tiles(rows: int, adapters: int) -> Tuple[int, int]:
+    """(rows of a tile, the most tiles): few rows (single tokens, each with an adapter of its own as a rule) in small tiles."""
+    tile_rows = 16 if rows <= 256 else 64
+    return tile_rows, rows // tile_rows + min(adapters, rows)
+
+
+def adapter_plan_size(rows: int, adapters: int) -> int:
+    """Values (int32) of the buffer that ``adapter_plan`` needs for up to ``rows`` rows."""
+    return max(1 + rows + 3 * _adapter_tiles(n, adapters)[1] for n in (min(rows, 256), rows))
+
+
+def adapter_plan(row_adapter: torch.Tensor, adapters: int, buffer: Optional[torch.Tensor] = None) -> AdapterPlan:
+    """Puts the rows of a step in the order of their adapters: ``row_adapter`` [T] int32 on the device, an adapter's number or, for
+    a row without one, anything outside 0 .. adapters - 1. ``buffer``: where to (``adapter_plan_size`` int32 values; new memory without it).
+    Once a step: every product of the step takes the same plan."""
+    T = row_adapter.numel()
+    if not 1 <= adapters:
+        raise KernelError("adapter_plan: there must be an adapter")
+    tile_rows, tiles = _adapter_tiles(T, adapters)
+    if buffer is None:
+        buffer = torch.empty(1 + T + 3 * tiles, dtype=torch.int32, device=row_adapter.device)
+    elif buffer.numel() < 1 + T + 3 * tiles:
+        raise KernelError("adapter_plan: the buffer is too small")
+    check(lib().gi_adapter_plan(_dev(row_adapter, "row_adapter", torch.int32), T, int(adapters), tile_rows, _dev(buffer, "buffer", torch.int32),
+                                _stream()), "adapter_plan")
+    return AdapterPlan(buffer, T, int(adapters), tile_rows, tiles)
+
+
+def _rows_of(t: torch.Tensor, name: str) -> int:
+    if not t.is_cuda:
+        raise KernelError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise KernelError(f"{name} must have rows of neighbouring values that do not overlap")
+    return t.data_ptr()
+
+
+def adapter_product(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scales: torch.Tensor, plan: AdapterPlan, out: torch.Tensor,
+                    slices=None) -> None:
+    """Every row's low-rank adapter added to a projection's output: out[t, :] += scales[a] * up[a] (down[a] x[t, :]) with a the
+    row's adapter (rows without one are left alone). ``x`` [T, K] and the weights of one dtype, ``down`` [adapters, S * rank, K],
+    ``up`` [adapters, N, rank], ``scales`` [adapters] 32-bit; ``out`` [T, N] 32-bit or, with bfloat16 weights, bfloat16 (rounded
+    once). ``slices``: the widths of S projections stacked in one output ([q; k; v], [gate; up]), each with ``rank`` rows of
+    ``down`` of its own; None: one. x and out may be columns of wider tensors. Sums in 32 bits."""
+    T, K = x.shape
+    A, N, r = up.shape
+    S = 1 if slices is None else len(slices)
+    if out.shape != (T, N) or down.shape != (A, S * r, K) or scales.numel() != A:
+        raise KernelError("adapter_product: shapes of x, down, up, scales and out do not agree")
+    if plan.rows != T or plan.adapters != A:
+        raise KernelError("adapter_product: the plan is of other rows or adapters")
+    if down.dtype != x.dtype or up.dtype != x.dtype:
+        raise KernelError("adapter_product: x and the weights must have one dtype")
+    if x.dtype == torch.float32 and out.dtype != torch.float32:
+        raise KernelError("adapter_product: 32-bit weights give 32-bit output")
+    if not 1 <= S <= 4:
+        raise KernelError("adapter_product: one to four slices")
+    ends, at = [0, 0, 0, 0], 0
+    for i in range(S):
+        at += N if slices is None else int(slices[i])
+        ends[i] = at
+    check(lib().gi_adapter_product(_rows_of(x, "x"), x.stride(0), dtype_code(x.dtype), _dev(down, "down"), _dev(up, "up"),
+                                   _dev(scales, "scales", torch.float32), plan.buffer.data_ptr(), T, plan.tile_rows, plan.tiles, _rows_of(out, "out"),
+                                   out.stride(0), dtype_code(out.dtype), K, N, r, S, *ends, _stream()), "adapter_product")
