@@ -16,7 +16,7 @@ namespace gi {
 
 namespace cg = cooperative_groups;
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024, kPlanEach = 8;
 constexpr int kPlanAdaptersMost = 8192;        // counters of the plan's block in shared memory
 constexpr int kAdapterRanksMost = 512;         // S * r
 constexpr int kAdapterSlicesMost = 4;
@@ -41,15 +41,22 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const int* r
     for (int a = threadIdx.x; a < A; a += kPlanThreads) counts[a] = 0;
     if (threadIdx.x == 0) base_rows = base_tiles = 0;
     __syncthreads();
+    // up to kPlanEach rows a thread stay in registers, all asked for at once; further ones are read again
     auto adapter = [&](int t) {
         const int a = t < T ? row_adapter[t] : -1;
         return a >= 0 && a < A ? a : -1;
     };
-    for (int t0 = 0; t0 < T; t0 += kPlanThreads) {
-        const int a = adapter(t0 + threadIdx.x);
+    int held[kPlanEach];
+#pragma unroll
+    for (int i = 0; i < kPlanEach; ++i) held[i] = adapter(i * kPlanThreads + threadIdx.x);
+    auto count = [&](int a) {
         const unsigned same = __match_any_sync(0xffffffffu, a);
         if (a >= 0 && lane == __ffs(same) - 1) atomicAdd(&counts[a], __popc(same));
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kPlanEach; ++i)
+        if (i * kPlanThreads < T) count(held[i]);
+    for (int t0 = kPlanEach * kPlanThreads; t0 < T; t0 += kPlanThreads) count(adapter(t0 + threadIdx.x));
     __syncthreads();
     int* tiles = plan + 1 + T;
     for (int a0 = 0; a0 < A; a0 += kPlanThreads) {
@@ -76,15 +83,18 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const int* r
         __syncthreads();
     }
     if (threadIdx.x == 0) plan[0] = base_tiles;
-    for (int t0 = 0; t0 < T; t0 += kPlanThreads) {
-        const int t = t0 + threadIdx.x, a = adapter(t);
+    auto put = [&](int t, int a) {
         const unsigned same = __match_any_sync(0xffffffffu, a);
         const int leader = __ffs(same) - 1;
         int place = 0;
         if (a >= 0 && lane == leader) place = atomicAdd(&counts[a], __popc(same));
         place = __shfl_sync(0xffffffffu, place, leader) + __popc(same & ((1u << lane) - 1));
         if (a >= 0) plan[1 + place] = t;
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kPlanEach; ++i)
+        if (i * kPlanThreads < T) put(i * kPlanThreads + threadIdx.x, held[i]);
+    for (int t0 = kPlanEach * kPlanThreads; t0 < T; t0 += kPlanThreads) put(t0 + threadIdx.x, adapter(t0 + threadIdx.x));
 }
 
 struct AdapterArgs {
@@ -96,29 +106,87 @@ struct AdapterArgs {
     PlanView plan;
     void* out;
     long long ldo;
-    int K, N, r, S, tile_rows;
+    int A, K, N, r, S, tile_rows;              // tile_rows 0: no plan, plan.p are the rows' adapters
     int ends[kAdapterSlicesMost];              // a slice's last column + 1
+    int wide;                                  // eight neighbouring columns from a multiple of eight on lie on 16 bytes in every row of out
 };
 
+constexpr int kAdapterThreads = 256, kAdapterWarps = kAdapterThreads / 32;
+constexpr int kDirectRows = kAdapterThreads;   // steps of up to so many rows have no plan: a tile's block looks its rows up itself
+constexpr int kDirectTile = 16, kDirectAdapters = 1024;       // (of so many adapters)
+
+// The rows of the block's tile (or of the `M` rows from `piece` on of a plan's tile) into rows[0 .. M); false: there are none.
+template <int M>
+__device__ __forceinline__ bool find_rows(const PlanView& plan, int A, int tile_rows, int which, int* rows, int& adapter, int& n, int* scratch) {
+    if (tile_rows == 0) {
+        // rows counted by adapter, the adapters' first tiles by a scan, then the ranks of the rows of the one that has tile `which`
+        __shared__ int s_counts[kDirectAdapters], s_adapter, s_tile;
+        constexpr int kEach = kDirectAdapters / kAdapterThreads;
+        const int i = threadIdx.x, lane = i & 31, warp = i >> 5;
+        const int mine = i < plan.T ? plan.p[i] : -1;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) s_counts[i + k * kAdapterThreads] = 0;
+        if (i < M) rows[i] = -1;
+        if (i == 0) s_adapter = -1;
+        __syncthreads();
+        if (mine >= 0 && mine < A) atomicAdd(&s_counts[mine], 1);
+        __syncthreads();
+        int tiles[kEach], sum = 0;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) { tiles[k] = (s_counts[i * kEach + k] + kDirectTile - 1) / kDirectTile; sum += tiles[k]; }
+        int run = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += v;
+        }
+        if (lane == 31) scratch[warp] = run;
+        __syncthreads();
+        run -= sum;
+        for (int w = 0; w < warp; ++w) run += scratch[w];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            if (which >= run && which < run + tiles[k]) { s_adapter = i * kEach + k; s_tile = which - run; }
+            run += tiles[k];
+        }
+        __syncthreads();
+        adapter = s_adapter;
+        if (adapter < 0) return false;
+        const unsigned same = __ballot_sync(0xffffffffu, mine == adapter);
+        if (lane == 0) scratch[warp] = __popc(same);
+        __syncthreads();
+        int place = __popc(same & ((1u << lane) - 1)) - s_tile * kDirectTile;
+        for (int w = 0; w < warp; ++w) place += scratch[w];
+        const bool in = mine == adapter && place >= 0 && place < kDirectTile;
+        if (in) rows[place] = i;
+        n = __syncthreads_count(in);
+    } else {
+        const int per_tile = (tile_rows + M - 1) / M, tile = which / per_tile, piece = which % per_tile;
+        const int* info = plan.tile(tile);     // (there, if not written, for every tile of the launch)
+        const int of = info[0], first = info[1], all = info[2];
+        if (tile >= plan.tiles()) return false;
+        adapter = of;
+        n = min(M, all - piece * M);
+        if (n <= 0) return false;
+        for (int i = threadIdx.x; i < M; i += kAdapterThreads) rows[i] = i < n ? plan.rows()[first + piece * M + i] : -1;
+    }
+    __syncthreads();
+    return true;
+}
+
 // ---- any type, any size: on the CUDA cores, in 32 bits ----
-constexpr int kPlainThreads = 256, kPlainRows = 32, kPlainCols = 64, kPlainK = 32;
+constexpr int kPlainThreads = kAdapterThreads, kPlainRows = 32, kPlainCols = 64, kPlainK = 32;
 
 template <typename T, typename TO>
 __global__ void __launch_bounds__(kPlainThreads) adapter_plain_kernel(AdapterArgs a) {
     pdl_prologue();
     extern __shared__ float h[];               // [2][kPlainRows][S r]: this CTA's partial sums, then the whole sums
     __shared__ float xs[kPlainRows][kPlainK + 1], ds[kPlainCols][kPlainK + 1];
-    __shared__ int s_rows[kPlainRows];
+    __shared__ int s_rows[kPlainRows], s_scratch[kAdapterWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int part = cluster.block_rank(), parts = cluster.num_blocks();
-    const int per_tile = (a.tile_rows + kPlainRows - 1) / kPlainRows;
-    const int which = blockIdx.x / parts, tile = which / per_tile, piece = which % per_tile;
-    if (tile >= a.plan.tiles()) return;        // (the whole cluster)
-    const int* info = a.plan.tile(tile);
-    const int adapter = info[0], first = info[1] + piece * kPlainRows, rows = min(kPlainRows, info[2] - piece * kPlainRows);
-    if (rows <= 0) return;
-    if (threadIdx.x < kPlainRows) s_rows[threadIdx.x] = threadIdx.x < rows ? a.plan.rows()[first + threadIdx.x] : -1;
-    __syncthreads();
+    int adapter, rows;
+    if (!find_rows<kPlainRows>(a.plan, a.A, a.tile_rows, blockIdx.x / parts, s_rows, adapter, rows, s_scratch)) return;     // (the whole cluster)
     const int cols = a.S * a.r;
     const T* down = static_cast<const T*>(a.down) + static_cast<size_t>(adapter) * cols * a.K;
     const T* x = static_cast<const T*>(a.x);
@@ -187,6 +255,467 @@ __global__ void __launch_bounds__(kPlainThreads) adapter_plain_kernel(AdapterArg
     }
 }
 
+// ---- bfloat16 on the tensor cores (mma.sync m16n8k16) ----
+// Rows are the M side in both products, the ranks (then the output's columns) the N side. Lane (g, c) = (lane / 4, lane % 4) holds of A rows g and
+// g + 8, of B column g, and of both the k slots 2c, 2c + 1, 2c + 8, 2c + 9. Which values of k sit in these slots is free as long as A and B agree: reading
+// straight from memory a lane takes neighbours of a row (8 c .. 8 c + 7 for two steps of k, or 4 c .. 4 c + 3 for one), 64 or 32 bytes a row for its four lanes.
+// Between the products a row's r sums are kept as bfloat16 pieces, each what the ones before leave: three for 32-bit outputs hold all 24 bits (two
+// showed as 1.8e-6 of the result against 2e-7), two for bfloat16 outputs (16 bits under a result rounded to 8).
+constexpr int kFewRows = 16, kBlockCols = 32;
+template <typename TO> struct Pieces { static constexpr int n = sizeof(TO) == 4 ? 3 : 2; };
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void load_matrices(unsigned (&m)[4], unsigned address) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ unsigned shared_address(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
+
+// The k slot of a rank within its 16: ranks 4 c .. 4 c + 3 sit in slots 2c, 2c + 1, 2c + 8, 2c + 9.
+__device__ __forceinline__ int rank_slot(int j) { return (j & ~15) + 2 * ((j >> 2) & 3) + ((j & 2) << 2) + (j & 1); }
+
+// The next piece of two neighbouring values (an even rank first), which is taken off them.
+__device__ __forceinline__ unsigned next_piece(float& v0, float& v1) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(v0, v1);
+    const float p0 = __bfloat162float(p.x), p1 = __bfloat162float(p.y);
+    v0 = fabsf(p0) < INFINITY ? v0 - p0 : 0.f;             // (an infinity leaves nothing)
+    v1 = fabsf(p1) < INFINITY ? v1 - p1 : 0.f;
+    return *reinterpret_cast<const unsigned*>(&p);
+}
+
+// kSteps steps of k (16 ranks each) of 32 columns of `up`. Which column is column g of tile q is chosen so that a lane's values of a row are runs
+// of 16 bytes and the runs of its four lanes fill whole sectors: 32-bit outputs 16 (q / 2) + 4 (g / 2) + 2 (q % 2) + g % 2, two runs of
+// four; bfloat16 ones 8 (g / 2) + 2 q + g % 2, one run of eight.
+template <int kSteps> struct UpFragments {
+    unsigned b[4][kSteps][2];                  // [tile of columns][step][half]
+};
+template <int kSteps, typename TO>
+__device__ __forceinline__ void load_up(UpFragments<kSteps>& f, const __nv_bfloat16* up, int r, int rank0, int cols) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int col = sizeof(TO) == 4 ? 16 * (q >> 1) + 4 * (g >> 1) + 2 * (q & 1) + (g & 1) : 8 * (g >> 1) + 2 * q + (g & 1);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int j = rank0 + 16 * s + 4 * c;
+            uint2 v = {0u, 0u};
+            if (col < cols && j < r) v = __ldg(reinterpret_cast<const uint2*>(up + static_cast<size_t>(col) * r + j));
+            f.b[q][s][0] = v.x;
+            f.b[q][s][1] = v.y;
+        }
+    }
+}
+
+// A block of up to 32 columns within one slice.
+struct ColumnBlock {
+    int col, cols, slice;
+};
+__device__ __forceinline__ ColumnBlock column_block(const AdapterArgs& a, int i) {
+    int begin = 0;
+#pragma unroll
+    for (int s = 0; s < kAdapterSlicesMost - 1; ++s) {
+        const int n = (a.ends[s] - begin + kBlockCols - 1) / kBlockCols;
+        if (i < n || s == a.S - 1) return {begin + i * kBlockCols, min(kBlockCols, a.ends[s] - begin - i * kBlockCols), s};
+        i -= n;
+        begin = a.ends[s];
+    }
+    return {begin + i * kBlockCols, min(kBlockCols, a.ends[kAdapterSlicesMost - 1] - begin - i * kBlockCols), kAdapterSlicesMost - 1};
+}
+
+// What a bfloat16 output holds in a lane's runs of a block, asked for ahead of the products (32-bit outputs are added to at the memory's side).
+template <int MT, typename TO> struct OldValues {
+    uint4 v[sizeof(TO) == 2 ? MT : 1][2];
+};
+__device__ __forceinline__ bool is_wide(const AdapterArgs& a, const ColumnBlock& block) { return a.wide && block.col % 8 == 0 && block.cols == kBlockCols; }
+template <int MT, typename TO>
+__device__ __forceinline__ void load_old(OldValues<MT, TO>& old, const AdapterArgs& a, const ColumnBlock& block, int row0, const int* rows) {
+    if constexpr (sizeof(TO) == 2) {
+        if (!is_wide(a, block)) return;
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        const TO* out = static_cast<const TO*>(a.out) + block.col + 8 * c;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int row = rows[row0 + 16 * m + 8 * half + g];
+                if (row >= 0) old.v[m][half] = *reinterpret_cast<const uint4*>(out + row * a.ldo);
+            }
+    }
+}
+
+// The second product of a warp: a block's columns for `MT` tiles of 16 rows from row0 on. pieces: shared [piece][`piece_bytes`: rows x ld] bfloat16
+// in the ranks' slots. fresh: f does not hold the block's first ranks yet.
+template <int MT, int kSteps, typename TO>
+__device__ __forceinline__ void expand(const AdapterArgs& a, UpFragments<kSteps>& f, bool fresh, const OldValues<MT, TO>& old, const __nv_bfloat16* up,
+                                       const ColumnBlock& block, unsigned pieces, unsigned piece_bytes, int ld, int row0, const int* rows) {
+    constexpr int kRun = 16 / sizeof(TO), kRuns = 8 / kRun;
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const bool wide = is_wide(a, block);
+    TO* out = static_cast<TO*>(a.out) + block.col + kRun * c;
+    float acc[MT][4][4] = {};
+    for (int rank0 = 0; rank0 < (kSteps == 4 ? a.r : 1); rank0 += 64) {
+        if (fresh || rank0) load_up<kSteps, TO>(f, up, a.r, rank0, block.cols);
+        const int k0 = block.slice * ((a.r + 15) & ~15) + rank0;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            if (kSteps < 4 || rank0 + 16 * s < a.r) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const unsigned at = ((row0 + 16 * m + (lane & 15)) * ld + k0 + 16 * s + 8 * (lane >> 4)) * 2;
+#pragma unroll
+                    for (int p = 0; p < Pieces<TO>::n; ++p) {
+                        unsigned h[4];
+                        load_matrices(h, pieces + p * piece_bytes + at);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) mma_bf16(acc[m][q], h[0], h[1], h[2], h[3], f.b[q][s][0], f.b[q][s][1]);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int row = rows[row0 + 16 * m + 8 * half + g];
+            if (row < 0) continue;
+            float v[8];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { v[2 * q] = acc[m][q][2 * half]; v[2 * q + 1] = acc[m][q][2 * half + 1]; }
+            TO* at = out + row * a.ldo;
+#pragma unroll
+            for (int u = 0; u < kRuns; ++u) {
+                if (wide && sizeof(TO) == 4) {
+                    // every value is added to once a call, so an addition at the memory's side, with nothing to wait for, gives the same bits in
+                    // any order (2,048 rows x 6,144 columns: 16 us for the second product, 22 us with loads and stores)
+                    const float* y = v + 4 * u;
+                    asm volatile("red.global.add.v4.f32 [%0], {%1,%2,%3,%4};" :: "l"(at + 16 * u), "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]) : "memory");
+                } else if (wide) {
+                    uint4 x = old.v[sizeof(TO) == 2 ? m : 0][half];
+                    unsigned* w = reinterpret_cast<unsigned*>(&x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const __nv_bfloat162 s = __floats2bfloat162_rn(__uint_as_float(w[i] << 16) + v[2 * i], __uint_as_float(w[i] & 0xffff0000u) + v[2 * i + 1]);
+                        w[i] = *reinterpret_cast<const unsigned*>(&s);
+                    }
+                    *reinterpret_cast<uint4*>(at + 16 * u) = x;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kRun; ++i)
+                        if (kRun * c + 16 * u + i < block.cols) at[16 * u + i] = from_float<TO>(to_float(at[16 * u + i]) + v[kRun * u + i]);
+                }
+            }
+        }
+}
+
+__device__ __forceinline__ int column_blocks(const AdapterArgs& a) {
+    int n = 0, begin = 0;
+#pragma unroll
+    for (int s = 0; s < kAdapterSlicesMost; ++s)
+        if (s < a.S) { n += (a.ends[s] - begin + kBlockCols - 1) / kBlockCols; begin = a.ends[s]; }
+    return n;
+}
+
+// Four sums of a row of the tile over the cluster's CTAs (whose partial sums lie at the same place), times scale.
+__device__ __forceinline__ float4 cluster_total(const float* at, float scale, cg::cluster_group& cluster, int parts) {
+    float4 x[kAdapterClusterMost];
+#pragma unroll
+    for (int p = 0; p < kAdapterClusterMost; ++p)
+        if (p < parts) x[p] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(at, p));
+    float4 v = x[0];
+#pragma unroll
+    for (int p = 1; p < kAdapterClusterMost; ++p)
+        if (p < parts) { v.x += x[p].x; v.y += x[p].y; v.z += x[p].z; v.w += x[p].w; }
+    return make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
+}
+
+// Few rows (single tokens): everything comes straight from memory into the lanes that multiply it. A warp takes every eighth 32 values of the CTA's
+// share of K; the warps' sums meet in shared memory, the CTAs' through the cluster.
+constexpr int kFewCols = 64;
+template <int kSteps, typename TO>
+__global__ void __launch_bounds__(kAdapterThreads, 2) adapter_few_kernel(AdapterArgs a) {
+    pdl_prologue();
+    extern __shared__ __align__(16) float h[]; // [kFewRows][S r], then the pieces
+    __shared__ float2 sums[kAdapterWarps][kFewRows][kFewCols / 2 + 4];
+    __shared__ int s_rows[kFewRows], s_scratch[kAdapterWarps];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int part = cluster.block_rank(), parts = cluster.num_blocks();
+    int adapter, n;
+    if (!find_rows<kFewRows>(a.plan, a.A, a.tile_rows, blockIdx.x / parts, s_rows, adapter, n, s_scratch)) return;     // (the whole cluster)
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+    const int cols = a.S * a.r, rp = (a.r + 15) & ~15, ld = a.S * rp + 8;
+    const __nv_bfloat16* down = static_cast<const __nv_bfloat16*>(a.down) + static_cast<size_t>(adapter) * cols * a.K;
+    const __nv_bfloat16* up = static_cast<const __nv_bfloat16*>(a.up) + static_cast<size_t>(adapter) * a.N * a.r;
+    __nv_bfloat16* pieces = reinterpret_cast<__nv_bfloat16*>(h + kFewRows * cols);
+    const float scale = a.scales[adapter];
+    if (rp != a.r)                             // the slots of ranks that are not there
+        for (int i = threadIdx.x; i < kFewRows * ld / 2 * Pieces<TO>::n; i += kAdapterThreads) reinterpret_cast<unsigned*>(pieces)[i] = 0u;
+    const int share = ((a.K + parts - 1) / parts + 31) / 32 * 32, k_begin = min(a.K, part * share), k_end = min(a.K, k_begin + share);
+    const int row_g = s_rows[g], row_h = s_rows[g + 8];
+    const __nv_bfloat16* x_g = static_cast<const __nv_bfloat16*>(a.x) + max(row_g, 0) * a.ldx;
+    const __nv_bfloat16* x_h = static_cast<const __nv_bfloat16*>(a.x) + max(row_h, 0) * a.ldx;
+    // the warp's first columns of the second product, asked for ahead of all (they wait for nobody)
+    const int blocks = column_blocks(a), per = (blocks + parts - 1) / parts, first = part * per + warp, last = min(blocks, (part + 1) * per);
+    UpFragments<kSteps> f;
+    ColumnBlock block = {0, 0, 0};
+    if (first < last) {
+        block = column_block(a, first);
+        load_up<kSteps, TO>(f, up + static_cast<size_t>(block.col) * a.r, a.r, 0, block.cols);
+    }
+    for (int c0 = 0; c0 < cols; c0 += kFewCols) {
+        float acc[kFewCols / 8][4] = {};
+        for (int k0 = k_begin + 32 * warp; k0 < k_end; k0 += 32 * kAdapterWarps) {
+            const int k = k0 + 8 * c;
+            const bool there = k < k_end;
+            uint4 x0 = {0u, 0u, 0u, 0u}, x1 = x0, w[kFewCols / 8];
+            if (there && row_g >= 0) x0 = __ldg(reinterpret_cast<const uint4*>(x_g + k));
+            if (there && row_h >= 0) x1 = __ldg(reinterpret_cast<const uint4*>(x_h + k));
+#pragma unroll
+            for (int t = 0; t < kFewCols / 8; ++t) {
+                const int j = c0 + 8 * t + g;
+                w[t] = make_uint4(0u, 0u, 0u, 0u);
+                if (there && j < cols) w[t] = __ldg(reinterpret_cast<const uint4*>(down + static_cast<size_t>(j) * a.K + k));
+            }
+#pragma unroll
+            for (int t = 0; t < kFewCols / 8; ++t) {
+                if (c0 + 8 * t < cols) {
+                    mma_bf16(acc[t], x0.x, x1.x, x0.y, x1.y, w[t].x, w[t].y);
+                    mma_bf16(acc[t], x0.z, x1.z, x0.w, x1.w, w[t].z, w[t].w);
+                }
+            }
+        }
+        if (c0) __syncthreads();
+#pragma unroll
+        for (int t = 0; t < kFewCols / 8; ++t)
+            if (c0 + 8 * t < cols) {
+                sums[warp][g][4 * t + c] = make_float2(acc[t][0], acc[t][1]);
+                sums[warp][g + 8][4 * t + c] = make_float2(acc[t][2], acc[t][3]);
+            }
+        __syncthreads();
+        const int some = min(kFewCols, cols - c0);
+        for (int i = threadIdx.x; i < kFewRows * kFewCols / 2; i += kAdapterThreads) {
+            const int row = i / (kFewCols / 2), pair = i % (kFewCols / 2);
+            if (2 * pair >= some) continue;
+            float2 v = sums[0][row][pair];
+#pragma unroll
+            for (int w = 1; w < kAdapterWarps; ++w) { const float2 y = sums[w][row][pair]; v.x += y.x; v.y += y.y; }
+            *reinterpret_cast<float2*>(h + row * cols + c0 + 2 * pair) = v;
+        }
+    }
+    cluster.sync();
+    for (int i = threadIdx.x; i < kFewRows * cols / 4; i += kAdapterThreads) {
+        const int row = 4 * i / cols, col = 4 * i % cols;
+        float4 v = cluster_total(h + row * cols + col, scale, cluster, parts);
+        __nv_bfloat16* to = pieces + row * ld + (col / a.r) * rp + rank_slot(col % a.r);
+#pragma unroll
+        for (int p = 0; p < Pieces<TO>::n; ++p, to += kFewRows * ld) {
+            *reinterpret_cast<unsigned*>(to) = next_piece(v.x, v.y);
+            *reinterpret_cast<unsigned*>(to + 8) = next_piece(v.z, v.w);
+        }
+    }
+    cluster.barrier_arrive();                  // no CTA leaves while another reads its sums
+    __syncthreads();
+    for (int i = first; i < last; i += kAdapterWarps) {
+        const ColumnBlock now = block;
+        UpFragments<kSteps> next;
+        if (i + kAdapterWarps < last) {
+            block = column_block(a, i + kAdapterWarps);
+            load_up<kSteps, TO>(next, up + static_cast<size_t>(block.col) * a.r, a.r, 0, block.cols);
+        }
+        OldValues<1, TO> old;
+        load_old<1, TO>(old, a, now, 0, s_rows);
+        expand<1, kSteps, TO>(a, f, false, old, up + static_cast<size_t>(now.col) * a.r, now, shared_address(pieces), 2 * kFewRows * ld, ld, 0, s_rows);
+        f = next;
+    }
+    cluster.barrier_wait();
+}
+
+// Many rows: x and `down` pass through a ring of stages of 64 values of K in shared memory (rows of 128 bytes, 16-byte pieces exchanged by the row's last
+// three bits); warps share the rows in groups of 32 (16 where the tile has 64) and a stage's steps of k in two halves. With one pass over K (S r up to 64)
+// the sums and their pieces lie where the ring was, else the sums have a place of their own.
+template <int M, bool kOnePass> struct ManyShape {
+    static constexpr int kStageBytes = (M + 64) * 128;
+    static constexpr int kStages = M == 128 ? 4 : kOnePass ? 6 : 5;
+    static constexpr int kGroups = 4, kSplits = kAdapterWarps / kGroups, kTiles = M / 16 / kGroups;
+};
+constexpr int kManyCols = 64;                  // ranks of a pass over K
+
+__device__ __forceinline__ void copy_16(unsigned to, const void* from, int bytes) {      // bytes: 16, or 0 for zeros (from is then an address of some memory)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to), "l"(from), "r"(bytes) : "memory");
+}
+
+template <int M, bool kOnePass, int kSteps, typename TO>
+__global__ void __launch_bounds__(kAdapterThreads, 2) adapter_many_kernel(AdapterArgs a) {
+    pdl_prologue();
+    using Shape = ManyShape<M, kOnePass>;
+    constexpr int kTiles = Shape::kTiles;
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ int s_rows[M], s_scratch[kAdapterWarps];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int part = cluster.block_rank(), parts = cluster.num_blocks();
+    int adapter, n;
+    if (!find_rows<M>(a.plan, a.A, a.tile_rows, blockIdx.x / parts, s_rows, adapter, n, s_scratch)) return;     // (the whole cluster)
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+    const int cols = a.S * a.r, rp = (a.r + 15) & ~15, ld = a.S * rp + 8, hs = cols + 8;
+    const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(a.x);
+    const __nv_bfloat16* down = static_cast<const __nv_bfloat16*>(a.down) + static_cast<size_t>(adapter) * cols * a.K;
+    const __nv_bfloat16* up = static_cast<const __nv_bfloat16*>(a.up) + static_cast<size_t>(adapter) * a.N * a.r;
+    float* h = reinterpret_cast<float*>(ring + (kOnePass ? 0 : Shape::kStages * Shape::kStageBytes));        // [M][hs]
+    __nv_bfloat16* pieces = reinterpret_cast<__nv_bfloat16*>(ring + (kOnePass ? M * hs * sizeof(float) : 0));
+    const float scale = a.scales[adapter];
+    const int share = ((a.K + parts - 1) / parts + 63) / 64 * 64, k_begin = min(a.K, part * share), k_end = min(a.K, k_begin + share);
+    const int stages = (k_end - k_begin + 63) / 64;
+    const unsigned ring_at = shared_address(ring);
+    const int group = warp % Shape::kGroups, split = warp / Shape::kGroups;
+    // what a thread copies: 16 bytes of every 32nd row, always the same ones of the 128
+    const int copy_row = threadIdx.x >> 3, copy_k = 8 * (threadIdx.x & 7);
+    const unsigned copy_to = copy_row * 128 + (((threadIdx.x & 7) ^ (copy_row & 7)) << 4);
+    const __nv_bfloat16* x_rows[M / 32];
+    int x_bytes[M / 32];
+#pragma unroll
+    for (int i = 0; i < M / 32; ++i) {
+        const int row = s_rows[copy_row + 32 * i];
+        x_bytes[i] = row >= 0 ? 16 : 0;
+        x_rows[i] = x + max(row, 0) * a.ldx + (row >= 0 ? k_begin + copy_k : 0);
+    }
+    // where a lane's fragments lie in a stage: their 16-byte piece for step s is exchanged by 2 s
+    const unsigned x_at = (group * kTiles * 16 + (lane & 15)) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+    const int w_row = (lane & 7) + ((lane >> 4) << 3);
+    const unsigned w_at = (M + w_row) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+    for (int c0 = 0; c0 < (kOnePass ? 1 : cols); c0 += kManyCols) {
+        const int some = min(kManyCols, cols - c0);
+        const int w_rows = (some + 15) & ~15;
+        int w_bytes[2];
+        const __nv_bfloat16* w_from[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const bool there = copy_row + 32 * i < some;
+            w_bytes[i] = there ? 16 : 0;
+            w_from[i] = down + (there ? static_cast<size_t>(c0 + copy_row + 32 * i) * a.K + k_begin + copy_k : 0);
+        }
+        auto fetch = [&](int stage, int slot) {
+            const unsigned at = ring_at + slot * Shape::kStageBytes + copy_to;
+            const int k = 64 * stage;
+            if (k_begin + k + 64 <= k_end) {
+#pragma unroll
+                for (int i = 0; i < M / 32; ++i) copy_16(at + i * 32 * 128, x_rows[i] + (x_bytes[i] ? k : 0), x_bytes[i]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (copy_row + 32 * i < w_rows) copy_16(at + (M + i * 32) * 128, w_from[i] + (w_bytes[i] ? k : 0), w_bytes[i]);
+            } else {                           // the last stage may end early
+                const bool in = k_begin + k + copy_k < k_end;
+#pragma unroll
+                for (int i = 0; i < M / 32; ++i) copy_16(at + i * 32 * 128, in && x_bytes[i] ? x_rows[i] + k : x, in ? x_bytes[i] : 0);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (copy_row + 32 * i < w_rows) copy_16(at + (M + i * 32) * 128, in && w_bytes[i] ? w_from[i] + k : down, in ? w_bytes[i] : 0);
+            }
+        };
+        float acc[kTiles][kManyCols / 8][4] = {};
+#pragma unroll
+        for (int i = 0; i < Shape::kStages - 1; ++i) {
+            if (i < stages) fetch(i, i);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        int slot = 0, next = Shape::kStages - 1;
+        for (int i = 0; i < stages; ++i) {
+            asm volatile("cp.async.wait_group %0;" :: "n"(Shape::kStages - 2) : "memory");
+            __syncthreads();                   // the stage is there for all, and the one before it is free
+            if (i + Shape::kStages - 1 < stages) fetch(i + Shape::kStages - 1, next);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            const unsigned at = ring_at + slot * Shape::kStageBytes;
+            next = slot;
+            slot = slot + 1 == Shape::kStages ? 0 : slot + 1;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int step = 2 * split + s;
+                unsigned xa[kTiles][4], w[kManyCols / 16][4];          // (a step's fragments first: its products then wait for nothing)
+#pragma unroll
+                for (int m = 0; m < kTiles; ++m) load_matrices(xa[m], (at + x_at + m * 16 * 128) ^ (step << 5));
+#pragma unroll
+                for (int t = 0; t < kManyCols / 16; ++t)
+                    if (16 * t < some) load_matrices(w[t], (at + w_at + t * 16 * 128) ^ (step << 5));
+#pragma unroll
+                for (int t = 0; t < kManyCols / 16; ++t)
+                    if (16 * t < some) {
+#pragma unroll
+                        for (int m = 0; m < kTiles; ++m) {
+                            mma_bf16(acc[m][2 * t], xa[m][0], xa[m][1], xa[m][2], xa[m][3], w[t][0], w[t][1]);
+                            mma_bf16(acc[m][2 * t + 1], xa[m][0], xa[m][1], xa[m][2], xa[m][3], w[t][2], w[t][3]);
+                        }
+                    }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+        for (int p = 0; p < Shape::kSplits; ++p) {          // the warps that share the steps add up in their order
+            __syncthreads();
+            if (p == split)
+#pragma unroll
+                for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+                    for (int t = 0; t < kManyCols / 8; ++t)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const int row = (group * kTiles + m) * 16 + g + 8 * half, col = 8 * t + 2 * c;
+                            if (col < some) {
+                                float2* to = reinterpret_cast<float2*>(h + row * hs + c0 + col);
+                                float2 v = make_float2(acc[m][t][2 * half], acc[m][t][2 * half + 1]);
+                                if (p) { v.x += to->x; v.y += to->y; }
+                                *to = v;
+                            }
+                        }
+        }
+    }
+    __syncthreads();
+    if (rp != a.r)                             // the slots of ranks that are not there
+        for (int i = threadIdx.x; i < M * ld / 2 * Pieces<TO>::n; i += kAdapterThreads) reinterpret_cast<unsigned*>(pieces)[i] = 0u;
+    // the warp's first columns of the second product are asked for before the cluster meets
+    const int blocks = column_blocks(a), per = (blocks + parts - 1) / parts, first = part * per + warp, last = min(blocks, (part + 1) * per);
+    UpFragments<kSteps> f;
+    ColumnBlock block = {0, 0, 0};
+    if (first < last) {
+        block = column_block(a, first);
+        load_up<kSteps, TO>(f, up + static_cast<size_t>(block.col) * a.r, a.r, 0, block.cols);
+    }
+    cluster.sync();
+    // every CTA adds up its share of the tile's sums and gives their pieces to all
+    const int fours = M * cols / 4, four_share = (fours + parts - 1) / parts, fours_end = min(fours, (part + 1) * four_share);
+    for (int i = part * four_share + threadIdx.x; i < fours_end; i += kAdapterThreads) {
+        const int row = 4 * i / cols, col = 4 * i % cols;
+        float4 v = cluster_total(h + row * hs + col, scale, cluster, parts);
+        __nv_bfloat16* to = pieces + row * ld + (col / a.r) * rp + rank_slot(col % a.r);
+#pragma unroll
+        for (int q = 0; q < Pieces<TO>::n; ++q, to += M * ld) {
+            const unsigned p0 = next_piece(v.x, v.y), p1 = next_piece(v.z, v.w);
+#pragma unroll
+            for (int p = 0; p < kAdapterClusterMost; ++p)
+                if (p < parts) {
+                    *reinterpret_cast<unsigned*>(cluster.map_shared_rank(to, p)) = p0;
+                    *reinterpret_cast<unsigned*>(cluster.map_shared_rank(to + 8, p)) = p1;
+                }
+        }
+    }
+    cluster.sync();
+    OldValues<2, TO> old;
+    if (first < last) load_old<2, TO>(old, a, block, 0, s_rows);
+    for (int i = first; i < last; i += kAdapterWarps) {
+        const ColumnBlock now = block;
+        const __nv_bfloat16* from = up + static_cast<size_t>(now.col) * a.r;
+        if (i + kAdapterWarps < last) block = column_block(a, i + kAdapterWarps);
+        for (int row0 = 0; row0 < n; row0 += 32) {
+            OldValues<2, TO> next;             // of the turn that follows
+            if (row0 + 32 < n) load_old<2, TO>(next, a, now, row0 + 32, s_rows);
+            else if (i + kAdapterWarps < last) load_old<2, TO>(next, a, block, 0, s_rows);
+            expand<2, kSteps, TO>(a, f, kSteps == 4 && a.r > 64 && row0 > 0, old, from, now, shared_address(pieces), 2 * M * ld, ld, row0, s_rows);
+            old = next;
+        }
+        if (i + kAdapterWarps < last) load_up<kSteps, TO>(f, up + static_cast<size_t>(block.col) * a.r, a.r, 0, block.cols);
+    }
+}
+
 template <typename... KArgs, typename... Args>
 inline void launch_tile_clusters(void (*kernel)(KArgs...), long long tiles, int parts, int threads, size_t smem, cudaStream_t stream, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
@@ -206,27 +735,83 @@ inline void launch_tile_clusters(void (*kernel)(KArgs...), long long tiles, int 
     counted(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
 }
 
-// CTAs of a tile's cluster: enough for two on every multiprocessor.
-inline int cluster_parts(long long tiles) {
+// The clusters of a launch, and how many of them will have rows as a rule: every adapter could leave a tile that is not full, in large steps few do.
+struct TileCount { long long all, busy; };
+inline TileCount tile_count(const AdapterArgs& a, long long tiles, int rows) {
+    if (a.tile_rows == 0) return {tiles, tiles};
+    return {tiles * ((a.tile_rows + rows - 1) / rows), (a.plan.T + rows - 1) / rows};
+}
+// CTAs of a cluster: as many as two a multiprocessor have room for.
+inline int cluster_parts(long long tiles, int slack) {
     int parts = 1;
-    while (parts < kAdapterClusterMost && tiles * parts < 2LL * sm_count()) parts *= 2;
+    while (parts < kAdapterClusterMost && 2 * parts * tiles <= 2LL * sm_count() * slack) parts *= 2;
     return parts;
+}
+
+template <typename Kernel>
+int launch_adapter(Kernel kernel, SharedLimit& limit, const AdapterArgs& a, TileCount tiles, size_t smem, size_t most, cudaStream_t st) {
+    const cudaError_t e = limit.allow(reinterpret_cast<const void*>(kernel), static_cast<int>(most));
+    GI_REQUIRE(e == cudaSuccess, "adapter_product: %s", cudaGetErrorString(e));
+    launch_tile_clusters(kernel, tiles.all, cluster_parts(tiles.busy, a.tile_rows ? 1 : 2), kAdapterThreads, smem, st, a);
+    return check_launch("adapter_product");
 }
 
 template <typename T, typename TO>
 int launch_plain(const AdapterArgs& a, long long tiles, cudaStream_t st) {
     static SharedLimit limit;
-    const long long pieces = tiles * ((a.tile_rows + kPlainRows - 1) / kPlainRows);
-    const size_t smem = 2ull * kPlainRows * a.S * a.r * sizeof(float);
-    const cudaError_t e = limit.allow(reinterpret_cast<const void*>(&adapter_plain_kernel<T, TO>), 2 * kPlainRows * kAdapterRanksMost * sizeof(float));
-    GI_REQUIRE(e == cudaSuccess, "adapter_product: %s", cudaGetErrorString(e));
-    launch_tile_clusters((adapter_plain_kernel<T, TO>), pieces, cluster_parts(pieces), kPlainThreads, smem, st, a);
-    return check_launch("adapter_product");
+    return launch_adapter(&adapter_plain_kernel<T, TO>, limit, a, tile_count(a, tiles, kPlainRows), 2ull * kPlainRows * a.S * a.r * sizeof(float),
+                          2ull * kPlainRows * kAdapterRanksMost * sizeof(float), st);
+}
+
+template <typename TO> inline size_t pieces_bytes(const AdapterArgs& a, int rows) {
+    return 2ull * Pieces<TO>::n * rows * (a.S * ((a.r + 15) / 16 * 16) + 8);
+}
+inline size_t sums_bytes(const AdapterArgs& a, int rows) { return 4ull * rows * (a.S * a.r + 8); }
+template <typename Shape> constexpr size_t ring_bytes() { return static_cast<size_t>(Shape::kStages) * Shape::kStageBytes; }
+
+template <int kSteps, typename TO>
+int launch_few(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+    static SharedLimit limit;
+    return launch_adapter(&adapter_few_kernel<kSteps, TO>, limit, a, tile_count(a, tiles, kFewRows), 4ull * kFewRows * a.S * a.r + pieces_bytes<TO>(a, kFewRows),
+                          150 * 1024, st);
+}
+
+template <int M, bool kOnePass, int kSteps, typename TO>
+int launch_many(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+    static SharedLimit limit;
+    const size_t ring = ring_bytes<ManyShape<M, kOnePass>>();
+    return launch_adapter(&adapter_many_kernel<M, kOnePass, kSteps, TO>, limit, a, tile_count(a, tiles, M), kOnePass ? ring : ring + sums_bytes(a, M),
+                          210 * 1024, st);
+}
+
+template <int kSteps, typename TO>
+int launch_steps(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+    using Wide = ManyShape<128, true>;
+    using Tall = ManyShape<64, true>;
+    using Passes = ManyShape<64, false>;
+    if (a.tile_rows == 0) return launch_few<kSteps, TO>(a, tiles, st);
+    const bool one = a.S * a.r <= kManyCols;
+    if (one && a.plan.T >= 4096 && sums_bytes(a, 128) + pieces_bytes<TO>(a, 128) <= ring_bytes<Wide>()) return launch_many<128, true, kSteps, TO>(a, tiles, st);
+    if (one && sums_bytes(a, 64) + pieces_bytes<TO>(a, 64) <= ring_bytes<Tall>()) return launch_many<64, true, kSteps, TO>(a, tiles, st);
+    if (pieces_bytes<TO>(a, 64) <= ring_bytes<Passes>()) return launch_many<64, false, kSteps, TO>(a, tiles, st);
+    return launch_few<kSteps, TO>(a, tiles, st);
+}
+
+template <typename TO>
+int launch_bf16(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+    // 16-byte pieces of x and `down`, 8-byte ones of `up`
+    const bool pieces = a.K % 8 == 0 && a.ldx % 8 == 0 && a.r % 4 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
+                        reinterpret_cast<uintptr_t>(a.down) % 16 == 0 && reinterpret_cast<uintptr_t>(a.up) % 8 == 0;
+    if (!pieces) return launch_plain<__nv_bfloat16, TO>(a, tiles, st);
+    return a.r <= 16 ? launch_steps<1, TO>(a, tiles, st) : a.r <= 32 ? launch_steps<2, TO>(a, tiles, st) : launch_steps<4, TO>(a, tiles, st);
 }
 
 }  // namespace gi
 
 using namespace gi;
+
+// Rows of a step whose products need no plan, with so many adapters.
+extern "C" int gi_adapter_direct_rows(int A) { return A <= kDirectAdapters ? kDirectRows : 0; }
 
 static int gi_adapter_plan_impl(const int* row_adapter, int T, int A, int tile_rows, int* plan, void* stream) {
     GI_REQUIRE(T >= 0 && A > 0 && tile_rows > 0, "adapter_plan: sizes must be positive (T=%d, adapters=%d, tile rows=%d)", T, A, tile_rows);
@@ -235,27 +820,31 @@ static int gi_adapter_plan_impl(const int* row_adapter, int T, int A, int tile_r
     return check_launch("adapter_plan");
 }
 
-// x [T, K] with ldx values between rows; down [A, S r, K]; up [A, N, r]; out [T, N] with ldo values between rows; ends [S]: host memory, read
-// during the call; tiles: the most that the plan can have.
+// x [T, K] with ldx values between rows; down [A, S r, K]; up [A, N, r]; out [T, N] with ldo values between rows; end0 ..: the slices' last columns + 1.
+// tile_rows > 0: plan is adapter_plan's, tiles the most it can have; 0 (up to gi_adapter_direct_rows() rows): plan is row_adapter [T] itself, tiles
+// the most that its rows can make in tiles of 16.
 static int gi_adapter_product_impl(const void* x, long long ldx, int dtype, const void* down, const void* up, const float* scales, const int* plan, int T,
-                                   int tile_rows, int tiles, void* out, long long ldo, int out_dtype, int K, int N, int r, int S, int end0, int end1, int end2,
-                                   int end3, void* stream) {
+                                   int A, int tile_rows, int tiles, void* out, long long ldo, int out_dtype, int K, int N, int r, int S, int end0, int end1,
+                                   int end2, int end3, void* stream) {
     if (T == 0 || tiles == 0) return 0;
-    GI_REQUIRE(T > 0 && K > 0 && N > 0 && r > 0 && tile_rows > 0 && tiles > 0, "adapter_product: sizes must be positive (T=%d, K=%d, N=%d, rank=%d)", T, K, N, r);
+    GI_REQUIRE(T > 0 && A > 0 && K > 0 && N > 0 && r > 0 && tile_rows >= 0 && tiles > 0, "adapter_product: sizes must be positive (T=%d, adapters=%d, K=%d, N=%d, rank=%d)",
+               T, A, K, N, r);
+    GI_REQUIRE(tile_rows > 0 || T <= gi_adapter_direct_rows(A), "adapter_product: %d rows need a plan", T);
     GI_REQUIRE(S >= 1 && S <= kAdapterSlicesMost, "adapter_product: %d slices (1 to %d)", S, kAdapterSlicesMost);
     GI_REQUIRE(static_cast<long long>(S) * r <= kAdapterRanksMost, "adapter_product: %d slices of rank %d exceed %d", S, r, kAdapterRanksMost);
-    AdapterArgs a = {x, ldx, down, up, scales, {plan, T}, out, ldo, K, N, r, S, tile_rows, {end0, end1, end2, end3}};
+    AdapterArgs a = {x, ldx, down, up, scales, {plan, T}, out, ldo, A, K, N, r, S, tile_rows, {end0, end1, end2, end3}, 0};
     int before = 0;
     for (int s = 0; s < S; ++s) {
         GI_REQUIRE(a.ends[s] > before, "adapter_product: a slice without columns");
         before = a.ends[s];
     }
     GI_REQUIRE(before == N, "adapter_product: the slices have %d columns, the output %d", before, N);
-    GI_REQUIRE(static_cast<long long>(tiles) * tile_rows <= INT_MAX / kAdapterClusterMost, "adapter_product: %d tiles exceed the grid limit", tiles);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    GI_REQUIRE(static_cast<long long>(tiles) * (tile_rows + kDirectTile) <= INT_MAX / kAdapterClusterMost, "adapter_product: %d tiles exceed the grid limit", tiles);
+    a.wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ldo * (out_dtype == kF32 ? 4 : 2) % 16 == 0;
     GI_REQUIRE(dtype == kBF16 || out_dtype == kF32, "adapter_product: 32-bit weights give 32-bit output");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == kF32) return launch_plain<float, float>(a, tiles, st);
-    return out_dtype == kF32 ? launch_plain<__nv_bfloat16, float>(a, tiles, st) : launch_plain<__nv_bfloat16, __nv_bfloat16>(a, tiles, st);
+    return out_dtype == kF32 ? launch_bf16<float>(a, tiles, st) : launch_bf16<__nv_bfloat16>(a, tiles, st);
 }
 
 extern "C" int gi_adapter_plan(const int* row_adapter, int T, int A, int tile_rows, int* plan, void* stream) {
@@ -263,8 +852,8 @@ extern "C" int gi_adapter_plan(const int* row_adapter, int T, int A, int tile_ro
 }
 
 extern "C" int gi_adapter_product(const void* x, long long ldx, int dtype, const void* down, const void* up, const float* scales, const int* plan, int T,
-                                  int tile_rows, int tiles, void* out, long long ldo, int out_dtype, int K, int N, int r, int S, int end0, int end1, int end2,
-                                  int end3, void* stream) {
-    return gi::dispatch(gi_adapter_product_impl, x, ldx, dtype, down, up, scales, plan, T, tile_rows, tiles, out, ldo, out_dtype, K, N, r, S, end0, end1, end2,
-                        end3, stream);
+                                  int A, int tile_rows, int tiles, void* out, long long ldo, int out_dtype, int K, int N, int r, int S, int end0, int end1,
+                                  int end2, int end3, void* stream) {
+    return gi::dispatch(gi_adapter_product_impl, x, ldx, dtype, down, up, scales, plan, T, A, tile_rows, tiles, out, ldo, out_dtype, K, N, r, S, end0, end1,
+                        end2, end3, stream);
 }

@@ -1656,32 +1656,32 @@ class AdapterPlan:
         self.buffer, self.rows, self.adapters, self.tile_rows, self.tiles = buffer, rows, adapters, tile_rows, tiles
 
 
-def _adapter_tiles(rows: int, adapters: int) -> Tuple[int, int]:
-    """(rows of a tile, the most tiles): few rows (single tokens, each with an adapter of its own as a rule) in small tiles."""
-    tile_rows = 16 if rows <= 256 else 64
-    return tile_rows, rows // tile_rows + min(adapters, rows)
+ADAPTER_TILE_ROWS = 128
+ADAPTER_DIRECT_ROWS, ADAPTER_DIRECT_ADAPTERS = 256, 1024      # steps of up to so many rows (and adapters) need no plan on the device: the products look rows up themselves
 
 
 def adapter_plan_size(rows: int, adapters: int) -> int:
     """Values (int32) of the buffer that ``adapter_plan`` needs for up to ``rows`` rows."""
-    return max(1 + rows + 3 * _adapter_tiles(n, adapters)[1] for n in (min(rows, 256), rows))
+    return 1 + rows + 3 * (rows // ADAPTER_TILE_ROWS + min(adapters, rows))
 
 
 def adapter_plan(row_adapter: torch.Tensor, adapters: int, buffer: Optional[torch.Tensor] = None) -> AdapterPlan:
     """Puts the rows of a step in the order of their adapters: ``row_adapter`` [T] int32 on the device, an adapter's number or, for
     a row without one, anything outside 0 .. adapters - 1. ``buffer``: where to (``adapter_plan_size`` int32 values; new memory without it).
-    Once a step: every product of the step takes the same plan."""
+    Once a step: every product of the step takes the same plan, which reads ``row_adapter`` when it runs."""
     T = row_adapter.numel()
-    if not 1 <= adapters:
-        raise KernelError("adapter_plan: there must be an adapter")
-    tile_rows, tiles = _adapter_tiles(T, adapters)
+    if not 1 <= adapters <= 8192:
+        raise KernelError(f"adapter_plan: {adapters} adapters (1 to 8192)")
+    rows = _dev(row_adapter, "row_adapter", torch.int32)
+    if T <= ADAPTER_DIRECT_ROWS and adapters <= ADAPTER_DIRECT_ADAPTERS:
+        return AdapterPlan(row_adapter, T, int(adapters), 0, T // 16 + min(adapters, T))
+    tiles = T // ADAPTER_TILE_ROWS + min(adapters, T)
     if buffer is None:
         buffer = torch.empty(1 + T + 3 * tiles, dtype=torch.int32, device=row_adapter.device)
     elif buffer.numel() < 1 + T + 3 * tiles:
         raise KernelError("adapter_plan: the buffer is too small")
-    check(lib().gi_adapter_plan(_dev(row_adapter, "row_adapter", torch.int32), T, int(adapters), tile_rows, _dev(buffer, "buffer", torch.int32),
-                                _stream()), "adapter_plan")
-    return AdapterPlan(buffer, T, int(adapters), tile_rows, tiles)
+    check(lib().gi_adapter_plan(rows, T, int(adapters), ADAPTER_TILE_ROWS, _dev(buffer, "buffer", torch.int32), _stream()), "adapter_plan")
+    return AdapterPlan(buffer, T, int(adapters), ADAPTER_TILE_ROWS, tiles)
 
 
 def _rows_of(t: torch.Tensor, name: str) -> int:
@@ -1717,5 +1717,5 @@ def adapter_product(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale
         at += N if slices is None else int(slices[i])
         ends[i] = at
     check(lib().gi_adapter_product(_rows_of(x, "x"), x.stride(0), dtype_code(x.dtype), _dev(down, "down"), _dev(up, "up"),
-                                   _dev(scales, "scales", torch.float32), plan.buffer.data_ptr(), T, plan.tile_rows, plan.tiles, _rows_of(out, "out"),
+                                   _dev(scales, "scales", torch.float32), plan.buffer.data_ptr(), T, A, plan.tile_rows, plan.tiles, _rows_of(out, "out"),
                                    out.stride(0), dtype_code(out.dtype), K, N, r, S, *ends, _stream()), "adapter_product")
