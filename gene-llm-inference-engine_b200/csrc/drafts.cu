@@ -7,14 +7,16 @@
 // the target alone. T <= 0: a draft is kept while it is the row's argmax, which is also what replaces it. The draw takes the first index i of
 // weight w_i > 0 with w_0 + .. + w_i > v * sum(w); the random numbers u and v come from the caller.
 //
-// Two launches: one cluster of CTAs per row finds max and sum (a row is read once and stays in registers), one cluster per request
-// finds the stop and draws. The answer is a whole number, so sums run in 64 bits: their order moves a boundary between two tokens by
+// A cluster of CTAs per row finds max and sum and whether the row's draft is kept; a cluster per request finds the stop and draws there. Where there
+// are many more rows than the GPU holds at a time, the drafts' places are taken a few at a launch, and rows whose request has met a
+// refusal in an earlier one are left out. The answer is a whole number, so sums run in 64 bits: their order moves a boundary between two tokens by
 // 1e-13 of the mass, where 32-bit sums would move all 128,000 of them by 1e-7, a different token in one draw of a hundred.
 #include <climits>
 
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "device_limit.h"
 
 namespace gi {
 
@@ -23,19 +25,57 @@ namespace cg = cooperative_groups;
 constexpr int kRowThreads = 512, kRowWarps = kRowThreads / 32;
 constexpr int kRowCtasMost = 8;           // CTAs of a row's cluster
 constexpr int kRowUnitsMost = 10;         // groups of four values that a thread holds: vocabularies of up to 163,840 stay in registers
+constexpr int kEdge = 4;                  // places at either end of a row that may lie in no whole group
 
-// (l - max) / T. With y the rounded reciprocal of T, q = l y and one correction by the exact remainder give the rounded
-// quotient (P. Markstein, IBM J. Res. Dev. 34, 1990): three multiply-adds instead of the general division. Temperatures whose
-// reciprocal could leave the normal range take the division. The dividend is bounded below, where exp gives 0 anyway: an infinite one has no remainder.
+// Two 32-bit operations an instruction, each rounded as its single form.
+__device__ __forceinline__ float2 add_2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul_2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fma_2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+// exp((l - max) / T). With y the rounded reciprocal of T, q = a y and one correction by the exact remainder give the rounded
+// quotient a / T (P. Markstein, IBM J. Res. Dev. 34, 1990): three multiply-adds, two values at a time, instead of the general division. Temperatures
+// whose reciprocal could leave the normal range take the division. The dividend is bounded below, where exp gives 0 anyway: an infinite one
+// has no remainder.
 struct ByTemperature {
-    float t, y;
+    float max, t, y;
     bool plain;
-    __device__ explicit ByTemperature(float temp) : t(temp), y(1.0f / temp), plain(!(temp > 1e-3f && temp < 1e3f)) {}
-    __device__ __forceinline__ float operator()(float a) const {
-        if (plain) return a / t;
-        a = fmaxf(a, -1e30f);
-        const float q = __fmul_rn(a, y);
-        return __fmaf_rn(__fmaf_rn(-q, t, a), y, q);
+    __device__ ByTemperature(float mx, float temp) : max(mx), t(temp), y(1.0f / temp), plain(!(temp > 1e-3f && temp < 1e3f)) {}
+    __device__ __forceinline__ float operator()(float l) const {
+        float v[2] = {l, l};
+        if (plain) general(v);
+        else usual(v);
+        return v[0];
+    }
+    template <int n> __device__ __forceinline__ void general(float (&v)[n]) const {
+#pragma unroll
+        for (int i = 0; i < n; ++i) v[i] = expf((v[i] - max) / t);
+    }
+    template <int n> __device__ __forceinline__ void usual(float (&v)[n]) const {
+        const float2 y2 = {y, y}, t2 = {-t, -t}, m2 = {-max, -max};
+#pragma unroll
+        for (int i = 0; i < n; i += 2) {
+            float2 a = add_2(make_float2(v[i], v[i + 1]), m2);
+            a.x = fmaxf(a.x, -1e30f);
+            a.y = fmaxf(a.y, -1e30f);
+            const float2 q = mul_2(a, y2), x = fma_2(fma_2(q, t2, a), y2, q);
+            v[i] = expf(x.x);
+            v[i + 1] = expf(x.y);
+        }
     }
 };
 
@@ -45,34 +85,53 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
     return r;
 }
 
+__device__ __forceinline__ float max_or_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // A row in groups of four neighbours on a boundary of four elements: the first and the last group may reach beyond the row.
 template <typename T> struct Row {
     const T* row;
     int V, off, units, begin, end;         // begin, end: this CTA's groups
-    __device__ Row(const T* p, int vocab, int part, int parts) : row(p), V(vocab) {
+    int first_whole, end_whole;            // the groups that lie within the row
+    __device__ Row(const T* p, int vocab, int part, int log_parts) : row(p), V(vocab) {
         off = static_cast<int>((reinterpret_cast<uintptr_t>(p) / sizeof(T)) & 3);
-        units = static_cast<int>((static_cast<long long>(V) + off + 3) / 4);
-        const int per = ((units + parts - 1) / parts + 31) / 32 * 32;
+        units = (V + off + 3) / 4;             // (V leaves room for the sum)
+        const int per = (((units - 1) >> log_parts) + 32) & ~31;          // the groups over the CTAs, rounded up, in whole warps
         begin = min(units, part * per);
         end = min(units, begin + per);
+        first_whole = off > 0;
+        end_whole = (V + off) / 4;
     }
     __device__ __forceinline__ int index(int unit) const { return 4 * unit - off; }
-    __device__ __forceinline__ bool whole(int unit) const { return index(unit) >= 0 && index(unit) <= V - 4; }
-    // the group's values, `none` beyond the row
-    __device__ __forceinline__ void load(int unit, float none, float (&v)[4]) const {
+    // the i-th place ahead of the first whole group, or behind the last one; -1: there is none
+    __device__ __forceinline__ int head(int i) const { return i < min((4 - off) & 3, V) ? i : -1; }
+    __device__ __forceinline__ int tail(int i) const {
+        const int at = max(min((4 - off) & 3, V), index(end_whole)) + i;
+        return at < V ? at : -1;
+    }
+    // asks the CTA's whole groups (of this row, or of the same places of a row of 32-bit values) into L2 at once: the passes' own loads, a few a thread
+    // at a time, then wait for L2 only
+    __device__ __forceinline__ void ask() const { ask(row); }
+    template <typename U> __device__ __forceinline__ void ask(const U* values) const {
+        const int from = max(begin, first_whole), to = min(end, end_whole);
+        const U* at = values + index(from);
+        const int skip = static_cast<int>((16 - reinterpret_cast<uintptr_t>(at) % 16) % 16 / sizeof(U));          // (the groups need not lie on 16 bytes)
+        const long long bytes = (static_cast<long long>(to - from) * 4 - skip) * sizeof(U) / 16 * 16;
+        if (threadIdx.x == 0 && bytes > 0)
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(at + skip), "r"(static_cast<int>(bytes)) : "memory");
+    }
+    __device__ __forceinline__ void load_whole(int unit, float (&v)[4]) const {
         const int i = index(unit);
-        if (whole(unit)) {
-            if constexpr (sizeof(T) == 4) {
-                const float4 x = *reinterpret_cast<const float4*>(row + i);
-                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-            } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(row + i);
-                v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xffff0000u);
-                v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xffff0000u);
-            }
+        if constexpr (sizeof(T) == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(row + i);
+            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
         } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = i + e >= 0 && i + e < V ? to_float(row[i + e]) : none;
+            const uint2 x = *reinterpret_cast<const uint2*>(row + i);
+            v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xffff0000u);
+            v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xffff0000u);
         }
     }
 };
@@ -90,8 +149,15 @@ struct RowShared {
     double warp_sum[kRowWarps];
     float cta_max[kRowCtasMost];
     int cta_at[kRowCtasMost];
-    double cta_sum[kRowCtasMost];
+    double cta_sum[3][kRowCtasMost];       // of the exponentials, of the weights, of the weights where those are nothing
 };
+
+// All threads of the cluster meet behind the remote stores of every CTA's first warp: only that warp's arrival has to wait for its stores to be seen.
+__device__ __forceinline__ void meet_behind_first_warps() {
+    if (threadIdx.x < 32) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    else asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 // The largest value of the cluster's row (NaN if any value is none); every thread has it.
 __device__ __forceinline__ float cluster_max(float mx, RowShared& s, cg::cluster_group& cluster, int part, int parts) {
@@ -107,14 +173,14 @@ __device__ __forceinline__ float cluster_max(float mx, RowShared& s, cg::cluster
         for (int o = kRowWarps / 2; o > 0; o >>= 1) mx = max_or_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         if (lane < parts) *cluster.map_shared_rank(&s.cta_max[part], lane) = mx;
     }
-    cluster.sync();
+    meet_behind_first_warps();
     mx = s.cta_max[0];
     for (int p = 1; p < parts; ++p) mx = max_or_nan(mx, s.cta_max[p]);
     return mx;
 }
 
-// The cluster's sum, in the order of the CTAs; every thread has it.
-__device__ __forceinline__ double cluster_sum(double v, RowShared& s, cg::cluster_group& cluster, int part, int parts) {
+// The cluster's sum, in the order of the CTAs; every thread has it. The warps' sums stay in s.warp_sum, the CTAs' in s.cta_sum[turn].
+__device__ __forceinline__ double cluster_sum(double v, RowShared& s, int turn, cg::cluster_group& cluster, int part, int parts) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     v = warp_total(v);
     if (lane == 0) s.warp_sum[warp] = v;
@@ -123,11 +189,11 @@ __device__ __forceinline__ double cluster_sum(double v, RowShared& s, cg::cluste
         v = s.warp_sum[lane & (kRowWarps - 1)];
 #pragma unroll
         for (int o = kRowWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane < parts) *cluster.map_shared_rank(&s.cta_sum[part], lane) = v;
+        if (lane < parts) *cluster.map_shared_rank(&s.cta_sum[turn][part], lane) = v;
     }
-    cluster.sync();
-    v = s.cta_sum[0];
-    for (int p = 1; p < parts; ++p) v += s.cta_sum[p];
+    meet_behind_first_warps();
+    v = s.cta_sum[turn][0];
+    for (int p = 1; p < parts; ++p) v += s.cta_sum[turn][p];
     return v;
 }
 
@@ -159,37 +225,72 @@ __device__ __forceinline__ int cluster_argmax(const Each& each, RowShared& s, cg
             *cluster.map_shared_rank(&s.cta_at[part], p) = at;
         }
     }
-    cluster.sync();
+    meet_behind_first_warps();
     best = s.cta_max[0];
     at = s.cta_at[0];
     for (int p = 1; p < parts; ++p) keep_best(s.cta_max[p], s.cta_at[p], best, at);
     return at == INT_MAX ? 0 : at;
 }
 
-// Values of a CTA's groups: held in registers (kUnits groups of four a thread) or, kUnits = 0, read again in every pass.
-template <typename T, int kUnits> struct Values {
+// Values of a CTA's whole groups: held in registers (kUnits groups of four a thread) or, kUnits = 0, read again in every pass (the cluster's row is then
+// in L2). kOrdered: a warp's groups are neighbours, as a draw wants them; else the block's threads take turns (a little faster). The places
+// in no whole group: one each for the first lanes of the first CTA's first warp and of the last CTA's last warp.
+template <typename T, int kUnits, bool kOrdered> struct Values {
+    static constexpr int kBatch = 4;       // groups whose loads are in flight together
+    static constexpr int kStep = kOrdered ? 32 : kRowThreads;
     const Row<T>& r;
+    int first, last, edge_at;
+    float edge;
     float held[kUnits > 0 ? kUnits : 1][4];
-    __device__ explicit Values(const Row<T>& row) : r(row) {
+    __device__ Values(const Row<T>& row, int part, int parts) : r(row) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        last = min(r.end, r.end_whole);
+        if constexpr (kOrdered) {
+            const int share = ((r.end - r.begin + kRowWarps - 1) / kRowWarps + 31) & ~31;
+            first = r.begin + warp * share + lane;
+            last = min(last, r.begin + (warp + 1) * share);
+        } else {
+            first = max(r.begin, r.first_whole) + threadIdx.x;
+        }
+        edge_at = part == 0 && warp == 0 && lane < kEdge ? r.head(lane) : part == parts - 1 && warp == kRowWarps - 1 && lane >= kEdge && lane < 2 * kEdge ? r.tail(lane - kEdge) : -1;
+        edge = edge_at >= 0 ? to_float(r.row[edge_at]) : -INFINITY;
         if constexpr (kUnits > 0) {
 #pragma unroll
             for (int u = 0; u < kUnits; ++u) {
-                const int unit = r.begin + u * kRowThreads + threadIdx.x;
-                if (unit < r.end) r.load(unit, -INFINITY, held[u]);
-                else held[u][0] = held[u][1] = held[u][2] = held[u][3] = -INFINITY;
+                held[u][0] = held[u][1] = held[u][2] = held[u][3] = -INFINITY;
+                if (there(first + kStep * u)) r.load_whole(first + kStep * u, held[u]);
             }
         }
     }
-    // f(group, values): every group of the thread, in order
+    __device__ __forceinline__ bool there(int unit) const { return unit < last && (!kOrdered || unit >= r.first_whole); }
+    // f(group, values): every group of the thread, in order, until it says stop (kOrdered: by the warp); values of a group that is not there are -infinity
     template <typename F> __device__ __forceinline__ void groups(F f) {
+        groups_with([](int, float (&)[4]) {}, [&](int unit, float (&v)[4], float (&)[4]) { return f(unit, v); });
+    }
+    // f(group, values, others) where more(group, others) fetches four further values of a group that is there (0 where it is not)
+    template <typename G, typename F> __device__ __forceinline__ void groups_with(G more, F f) {
         if constexpr (kUnits > 0) {
+            float none[4];
 #pragma unroll
-            for (int u = 0; u < kUnits; ++u) f(r.begin + u * kRowThreads + static_cast<int>(threadIdx.x), held[u]);
+            for (int u = 0; u < kUnits; ++u)
+                if (f(first + kStep * u, held[u], none)) return;
         } else {
-            for (int unit = r.begin + threadIdx.x; unit < r.end; unit += kRowThreads) {
-                float v[4];
-                r.load(unit, -INFINITY, v);
-                f(unit, v);
+            // whole batches of the warp (of the thread, where nothing hangs on the warp) without a look at what is there, the rest one by one
+            const int lane = kOrdered ? threadIdx.x & 31 : 0;
+            int unit = first;
+            for (; unit + (31 - lane) * kOrdered + kStep * (kBatch - 1) < last && (!kOrdered || unit - lane >= r.first_whole); unit += kBatch * kStep) {
+                float v[kBatch][4], w[kBatch][4];
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) { r.load_whole(unit + kStep * u, v[u]); more(unit + kStep * u, w[u]); }
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u)
+                    if (f(unit + kStep * u, v[u], w[u])) return;
+            }
+#pragma unroll 1
+            for (; unit - lane < last; unit += kStep) {
+                float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, w[4] = {0.f, 0.f, 0.f, 0.f};
+                if (there(unit)) { r.load_whole(unit, v); more(unit, w); }
+                if (f(unit, v, w)) return;
             }
         }
     }
@@ -198,7 +299,7 @@ template <typename T, int kUnits> struct Values {
 struct RowArgs {
     const void* logits;
     long long stride;                      // values from row to row
-    int N, V;
+    int N, V, log_parts;                   // CTAs of a row's cluster: 2^log_parts
     const float* temperature;              // per row (probabilities) or per request
     float* out;                            // probabilities [N, V]
     // verification
@@ -211,8 +312,8 @@ struct RowArgs {
     const float* draw;
     int* tokens;
     int* accepted;
-    float4* work;                          // per row: max, 1 / sum, kept (1) or not (0), argmax (as an integer's bits)
-    int R, D;
+    float4* work;                          // per row: max, 1 / sum, draft kept (1) or not (0), argmax of a greedy row (an integer's bits)
+    int R, D, place;                       // place: the first of the drafts' places that a launch takes
 };
 
 // The request's drafts, or -1 where its rows do not lie in the logits.
@@ -221,107 +322,232 @@ __device__ __forceinline__ int drafts_of(const RowArgs& a, int r) {
     return start < 0 || start > a.N - 1 - d ? -1 : d;
 }
 
-// One cluster per row. kProbs: row i's distribution goes to out; else: row j of request r, its max and sum and whether its draft is kept.
+// What a draw needs of a row: q's row (or null), the token that a draft without a distribution leaves out, both for refused drafts only.
+template <typename T>
+__device__ __forceinline__ int draw_token(Values<T, 0, true>& values, const ByTemperature& by, float inv, const float* q, int without, float number, int V,
+                                          RowShared& s, cg::cluster_group& cluster, int part, int parts) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool q_wide = q != nullptr && (reinterpret_cast<uintptr_t>(q) / 4 & 3) == static_cast<unsigned>(values.r.off);
+    bool subtract = q != nullptr || without >= 0;
+    auto taken = [&](int unit, float (&take)[4]) {
+        take[0] = take[1] = take[2] = take[3] = 0.f;
+        if (q == nullptr || !subtract) return;
+        const int i = values.r.index(unit);
+        if (q_wide) {
+            const float4 x = *reinterpret_cast<const float4*>(q + i);
+            take[0] = x.x; take[1] = x.y; take[2] = x.z; take[3] = x.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) take[e] = q[i + e];
+        }
+    };
+    // the four weights of a group in the place of its values, and their sum
+    auto weigh = [&](int unit, float (&w)[4], float (&take)[4]) {
+        const int i = values.r.index(unit);
+        if (by.plain) by.general(w);
+        else by.usual(w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float pe = __fmul_rn(w[e], inv);
+            if (i + e == without && subtract) take[e] = 1.0f;
+            w[e] = pe > take[e] ? __fsub_rn(pe, take[e]) : 0.f;      // (a q that is no number takes all)
+        }
+        return (static_cast<double>(w[0]) + static_cast<double>(w[1])) + (static_cast<double>(w[2]) + static_cast<double>(w[3]));
+    };
+    auto weigh_edge = [&]() {
+        if (values.edge_at < 0) return 0.f;
+        const float pe = __fmul_rn(by(values.edge), inv), take = !subtract ? 0.f : q != nullptr ? q[values.edge_at] : values.edge_at == without ? 1.0f : 0.0f;
+        return pe > take ? __fsub_rn(pe, take) : 0.f;
+    };
+    double total;
+    int turn = 1;
+    for (;; ++turn) {
+        double mine = static_cast<double>(weigh_edge());
+        values.groups_with(taken, [&](int unit, float (&w)[4], float (&take)[4]) {
+            mine += weigh(unit, w, take);
+            return false;
+        });
+        if (turn == 1) cluster.barrier_wait();              // (arrived at when the kernel began)
+        total = cluster_sum(mine, s, turn, cluster, part, parts);
+        if (!subtract || total > 0.0) break;
+        subtract = false;                                   // nothing is left of p behind q: the draw is from p (the whole cluster takes this turn)
+        __syncthreads();                                    // all have read the warps' sums
+    }
+    const double target = static_cast<double>(number) * total;
+    // The CTA, the warp, the group and the value in which the running sum passes the target, every sum taken the same way by all who
+    // compare it; where rounding (or a number of 1 and more) lets none, the last that weighs anything.
+    double run = 0.0, ahead = 0.0;
+    int owner = -1;
+    bool found = false;
+    for (int c = 0; c < parts && !found; ++c) {
+        const double t = s.cta_sum[turn][c];
+        if (t > 0.0) { owner = c; ahead = run; found = run + t > target; }
+        run += t;
+    }
+    if (owner != part) return -1;
+    run = ahead;
+    owner = -1;
+    found = false;
+    for (int w = 0; w < kRowWarps && !found; ++w) {
+        const double t = s.warp_sum[w];
+        if (t > 0.0) { owner = w; ahead = run; found = run + t > target; }
+        run += t;
+    }
+    if (owner != warp) return -1;
+    int pick = V - 1;
+    // the lanes' sums t in order: the lane that passes the target (or the last that weighs anything), and what lies ahead of it
+    auto look = [&](double t, bool& over_any, double& before) {
+        double cum = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double m = __shfl_up_sync(0xffffffffu, cum, o);
+            if (lane >= o) cum += m;
+        }
+        const unsigned some = __ballot_sync(0xffffffffu, t > 0.0), over = __ballot_sync(0xffffffffu, t > 0.0 && ahead + cum > target);
+        before = ahead + (cum - t);
+        ahead += __shfl_sync(0xffffffffu, cum, 31);
+        over_any = over != 0;
+        return over ? __ffs(over) - 1 : some ? 31 - __clz(some) : -1;
+    };
+    bool done = false;
+    double before;
+    auto look_edge = [&](bool mine) {
+        const float w = mine ? weigh_edge() : 0.f;
+        const int at = look(static_cast<double>(w), done, before);
+        if (at >= 0) pick = __shfl_sync(0xffffffffu, values.edge_at, at);
+    };
+    if (part == 0 && warp == 0) look_edge(lane < kEdge);
+    if (!done)
+        values.groups_with(taken, [&](int unit, float (&w)[4], float (&take)[4]) {
+            const double t = weigh(unit, w, take);
+            const int at = look(t, done, before);
+            if (at >= 0) {
+                int place = 0;
+                bool passed = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (w[e] > 0.f && !passed) { before += static_cast<double>(w[e]); place = e; passed = before > target; }
+                pick = __shfl_sync(0xffffffffu, values.r.index(unit) + place, at);
+            }
+            return done;
+        });
+    if (!done && part == parts - 1 && warp == kRowWarps - 1) look_edge(lane >= kEdge);
+    return lane == 0 ? pick : -1;
+}
+
+// One cluster per row. kProbs: row i's distribution goes to out; else row j of request r: whether its draft is kept, and if there is none or it is not, the
+// token that a draw at this row gives.
 template <typename T, int kUnits, bool kProbs>
-__global__ void __launch_bounds__(kRowThreads, 2) row_softmax_kernel(RowArgs a) {
+__global__ void __launch_bounds__(kRowThreads, kUnits ? 2 : 3) row_softmax_kernel(RowArgs a) {
     pdl_prologue();
     __shared__ RowShared s;
     cg::cluster_group cluster = cg::this_cluster();
-    const int part = cluster.block_rank(), parts = cluster.num_blocks();
-    const int which = blockIdx.x / parts;
-    int row = which, j = 0, d = 0, r = which;
+    const int parts = 1 << a.log_parts, part = blockIdx.x & (parts - 1);
+    const int r = blockIdx.x >> a.log_parts;                // the row, or the request
+    int row = r, j = 0, d = 0;
     if constexpr (!kProbs) {
-        r = which / (a.D + 1);
-        j = which % (a.D + 1);
+        j = a.place + blockIdx.y;
         d = drafts_of(a, r);
         if (j > d) return;                 // (the whole cluster)
         row = a.row_start[r] + j;
+        for (int i = 0; i < a.place; ++i)
+            if (a.work[row - j + i].z == 0.f) return;       // a refusal in an earlier launch: nobody asks for this row (the whole cluster)
     }
     cluster.barrier_arrive();              // every CTA of the cluster runs before another writes into its shared memory
     const T* p = static_cast<const T*>(a.logits) + row * a.stride;
-    const Row<T> span(p, a.V, part, parts);
-    Values<T, kUnits> values(span);
+    const Row<T> span(p, a.V, part, a.log_parts);
+    if constexpr (kUnits == 0) span.ask();
+    Values<T, kUnits, false> values(span, part, parts);
     const float temp = a.temperature[r];
+    // the draft, its logit, its probability in q and the number that decides (the same in every thread)
+    int x = -1;
+    float lx = 0.f, qx = 1.f, number = 0.f;
+    const float* q = nullptr;
+    if constexpr (!kProbs) {
+        if (j < d) {
+            x = a.drafted[static_cast<size_t>(r) * a.D + j];
+            number = a.accept[static_cast<size_t>(r) * a.D + j];
+            if (x < 0 || x >= a.V) x = -1;
+            if (a.q) q = a.q + r * a.q_request + j * a.q_place;
+            if (x >= 0) {
+                lx = to_float(p[x]);
+                if (q) qx = q[x];
+            }
+        }
+    }
     if (!(temp > 0.f)) {
         const int best = cluster_argmax([&](auto f) {
             values.groups([&](int unit, float (&v)[4]) {
+                if (values.there(unit))
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (v[e] > -INFINITY || (unit < span.end && span.index(unit) + e >= 0 && span.index(unit) + e < a.V && v[e] == -INFINITY)) f(span.index(unit) + e, v[e]);
+                    for (int e = 0; e < 4; ++e) f(span.index(unit) + e, v[e]);
+                return false;
             });
+            if (values.edge_at >= 0) f(values.edge_at, values.edge);
         }, s, cluster, part, parts);
         if constexpr (kProbs) {
             float* out = a.out + static_cast<size_t>(row) * a.V;
-            for (int unit = span.begin + threadIdx.x; unit < span.end; unit += kRowThreads)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = span.index(unit) + e;
-                    if (i >= 0 && i < a.V) out[i] = i == best ? 1.0f : 0.0f;
-                }
+            const int share = ((a.V - 1) >> a.log_parts) + 1, end = static_cast<int>(min(static_cast<long long>(a.V), static_cast<long long>(part + 1) * share));
+            for (int i = part * share + threadIdx.x; i < end; i += kRowThreads) out[i] = i == best ? 1.0f : 0.0f;
         } else if (part == 0 && threadIdx.x == 0) {
-            const bool kept = j < d && a.drafted[static_cast<size_t>(r) * a.D + j] == best;
-            a.work[row] = make_float4(0.f, 0.f, kept ? 1.f : 0.f, __int_as_float(best));
+            a.work[row] = make_float4(0.f, 0.f, x == best ? 1.f : 0.f, __int_as_float(best));
         }
         return;
     }
-    float mx = -INFINITY;
-    values.groups([&](int, float (&v)[4]) { mx = max_or_nan(max_or_nan(mx, max_or_nan(v[0], v[1])), max_or_nan(v[2], v[3])); });
+    float mx = values.edge;
+    values.groups([&](int, float (&v)[4]) { mx = max_or_nan(max_or_nan(mx, v[0], v[1]), v[2], v[3]); return false; });
     mx = cluster_max(mx, s, cluster, part, parts);
     const bool some = mx > -INFINITY && mx < INFINITY;      // else there are no probabilities (a value is none, or infinite, or all are -infinity)
-    const ByTemperature by(temp);
+    const ByTemperature by(mx, temp);
     double sum = 0.0;
-    if (some)
+    auto weigh = [&](auto exponentials) {                   // sum += exp of every value; the probabilities keep them
         values.groups([&](int, float (&v)[4]) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = expf(by(v[e] - mx));
-                sum += static_cast<double>(x);
-                if constexpr (kProbs) v[e] = x;
-            }
+            float y[4] = {v[0], v[1], v[2], v[3]};
+            exponentials(y);
+            sum += (static_cast<double>(y[0]) + static_cast<double>(y[1])) + (static_cast<double>(y[2]) + static_cast<double>(y[3]));
+            if constexpr (kProbs) { v[0] = y[0]; v[1] = y[1]; v[2] = y[2]; v[3] = y[3]; }
+            return false;
         });
-    sum = cluster_sum(sum, s, cluster, part, parts);
+        if (threadIdx.x < 32 || threadIdx.x >= kRowThreads - 32) sum += static_cast<double>(by(values.edge));     // (the warps that can have one)
+    };
+    if (some && !by.plain) weigh([&](float (&y)[4]) { by.usual(y); });
+    else if (some) weigh([&](float (&y)[4]) { by.general(y); });
+    sum = cluster_sum(sum, s, 0, cluster, part, parts);
     const float inv = some ? static_cast<float>(1.0 / sum) : NAN;
     if constexpr (kProbs) {
         float* out = a.out + static_cast<size_t>(row) * a.V;
         const bool wide = (reinterpret_cast<uintptr_t>(out) / 4 & 3) == static_cast<unsigned>(span.off);
         values.groups([&](int unit, float (&v)[4]) {
-            if (unit >= span.end) return;
+            if (!values.there(unit)) return false;
             float y[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(kUnits > 0 ? v[e] : expf(by(v[e] - mx)), inv);
+            for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(kUnits > 0 ? v[e] : by(v[e]), inv);
             const int i = span.index(unit);
-            if (wide && span.whole(unit)) {
+            if (wide) {
                 *reinterpret_cast<float4*>(out + i) = make_float4(y[0], y[1], y[2], y[3]);
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (i + e >= 0 && i + e < a.V) out[i + e] = y[e];
+                for (int e = 0; e < 4; ++e) out[i + e] = y[e];
             }
+            return false;
         });
-    } else if (part == 0 && threadIdx.x == 0) {
-        bool kept = false;
-        if (j < d) {
-            const int x = a.drafted[static_cast<size_t>(r) * a.D + j];
-            if (x >= 0 && x < a.V) {
-                const float q = a.q ? a.q[r * a.q_request + j * a.q_place + x] : 1.0f;
-                const float px = __fmul_rn(expf(by(to_float(p[x]) - mx)), inv);
-                kept = __fmul_rn(a.accept[static_cast<size_t>(r) * a.D + j], q) < px;
-            }
+        if (values.edge_at >= 0) out[values.edge_at] = __fmul_rn(by(values.edge), inv);
+    } else {
+        if (part == 0 && threadIdx.x == 0) {
+            const bool kept = some && x >= 0 && __fmul_rn(number, qx) < __fmul_rn(by(lx), inv);
+            a.work[row] = make_float4(mx, inv, kept ? 1.f : 0.f, 0.f);
         }
-        a.work[row] = make_float4(mx, inv, kept ? 1.f : 0.f, 0.f);
     }
 }
 
-// One cluster per request: the stop among its rows, and the token there. A warp owns neighbouring groups; the row and q's row are read once, then
-// once more (from the caches) by the one warp in whose piece the draw falls.
+// One cluster per request: the stop among its rows, and the token there.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, 2) draft_draw_kernel(RowArgs a) {
     pdl_prologue();
     __shared__ RowShared s;
     cg::cluster_group cluster = cg::this_cluster();
-    const int part = cluster.block_rank(), parts = cluster.num_blocks();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int r = blockIdx.x / parts, d = drafts_of(a, r);
+    const int parts = 1 << a.log_parts, part = blockIdx.x & (parts - 1);
+    const int r = blockIdx.x >> a.log_parts, d = drafts_of(a, r);
     int* tokens = a.tokens + static_cast<size_t>(r) * (a.D + 1);
     if (d < 0) {
         if (part == 0) {
@@ -331,8 +557,12 @@ __global__ void __launch_bounds__(kRowThreads, 2) draft_draw_kernel(RowArgs a) {
         return;
     }
     const int start = a.row_start[r];
-    int stop = 0;
-    while (stop < d && a.work[start + stop].z != 0.f) ++stop;
+    int stop = d;
+    for (int j0 = 0; j0 < d && stop == d; j0 += 32) {       // (rows behind the first refusal may not have been written)
+        const int j = j0 + (threadIdx.x & 31);
+        const unsigned refused = __ballot_sync(0xffffffffu, j < d && a.work[start + j].z == 0.f);
+        if (refused) stop = j0 + __ffs(refused) - 1;
+    }
     if (part == 0) {
         for (int j = threadIdx.x; j <= a.D; j += kRowThreads)
             if (j != stop) tokens[j] = j < stop ? a.drafted[static_cast<size_t>(r) * a.D + j] : -1;
@@ -344,133 +574,21 @@ __global__ void __launch_bounds__(kRowThreads, 2) draft_draw_kernel(RowArgs a) {
         if (part == 0 && threadIdx.x == 0) tokens[stop] = temp > 0.f ? a.V - 1 : __float_as_int(stat.w);
         return;
     }
-    cluster.barrier_arrive();              // every CTA of the cluster runs before another writes into its shared memory
-    const Row<T> span(static_cast<const T*>(a.logits) + (start + stop) * a.stride, a.V, part, parts);
-    const ByTemperature by(temp);
-    const float mx = stat.x, inv = stat.y;
-    const bool refused = stop < d;
-    const float* q = refused && a.q ? a.q + r * a.q_request + stop * a.q_place : nullptr;
-    const int without = refused && !a.q ? a.drafted[static_cast<size_t>(r) * a.D + stop] : -1;
-    const bool q_wide = q != nullptr && (reinterpret_cast<uintptr_t>(q) / 4 & 3) == static_cast<unsigned>(span.off);
-    bool subtract = refused;
-
-    // what is taken off a group's probabilities
-    auto taken = [&](int unit, float (&take)[4]) {
-        const int i = span.index(unit);
-        take[0] = take[1] = take[2] = take[3] = 0.f;
-        if (q_wide && span.whole(unit)) {
-            const float4 x = *reinterpret_cast<const float4*>(q + i);
-            take[0] = x.x; take[1] = x.y; take[2] = x.z; take[3] = x.w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (i + e >= 0 && i + e < a.V) take[e] = q ? q[i + e] : i + e == without ? 1.0f : 0.0f;
-        }
-    };
-    // the four weights of a group, and their sum; beyond the row none
-    auto weigh = [&](const float (&take)[4], float (&w)[4]) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float pe = __fmul_rn(expf(by(w[e] - mx)), inv);
-            w[e] = pe > take[e] ? __fsub_rn(pe, take[e]) : 0.f;      // (a q that is no number takes all)
-        }
-        return (static_cast<double>(w[0]) + static_cast<double>(w[1])) + (static_cast<double>(w[2]) + static_cast<double>(w[3]));
-    };
-    const int share = (((span.end - span.begin) + kRowWarps - 1) / kRowWarps + 31) / 32 * 32;
-    const int begin = min(span.end, span.begin + warp * share), end = min(span.end, begin + share);
-    constexpr int kBatch = 4;                               // turns whose loads are in flight together
-    // f(group, weights, sum) of every turn of 32 groups, until it says stop
-    auto turns = [&](auto f) {
-        for (int base = begin; base < end; base += 32 * kBatch) {
-            float w[kBatch][4], take[kBatch][4];
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const int unit = base + 32 * b + lane;
-                w[b][0] = w[b][1] = w[b][2] = w[b][3] = -INFINITY;
-                take[b][0] = take[b][1] = take[b][2] = take[b][3] = 0.f;
-                if (unit < end) {
-                    span.load(unit, -INFINITY, w[b]);
-                    if (subtract) taken(unit, take[b]);
-                }
-            }
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const double t = weigh(take[b], w[b]);
-                if (f(base + 32 * b + lane, w[b], t)) return;
-            }
-        }
-    };
-
-    double total;
-    for (bool first = true;; first = false) {
-        double mine = 0.0;
-        turns([&](int, const float (&)[4], double t) { mine += t; return false; });
-        mine = warp_total(mine);
-        if (lane == 0) s.warp_sum[warp] = mine;
-        __syncthreads();
-        if (first) cluster.barrier_wait();
-        if (warp == 0) {
-            double t = 0.0;
-            for (int w = 0; w < kRowWarps; ++w) t += s.warp_sum[w];
-            if (lane < parts) *cluster.map_shared_rank(&s.cta_sum[part], lane) = t;
-        }
-        cluster.sync();
-        total = 0.0;
-        for (int c = 0; c < parts; ++c) total += s.cta_sum[c];
-        if (!subtract || total > 0.0) break;
-        subtract = false;                                   // nothing is left of p behind q: the draw is from p (the whole cluster takes this turn)
-        cluster.sync();                                     // all have read the sums
-    }
-    const double target = static_cast<double>(a.draw[r]) * total;
-    // The CTA, the warp, the group and the value in which the running sum passes the target, every sum taken the same way by all who
-    // compare it; where rounding (or a number of 1 and more) lets none, the last that weighs anything.
-    double run = 0.0, ahead = 0.0;
-    int owner = -1;
-    bool found = false;
-    for (int c = 0; c < parts && !found; ++c) {
-        const double t = s.cta_sum[c];
-        if (t > 0.0) { owner = c; ahead = run; found = run + t > target; }
-        run += t;
-    }
-    if (owner != part) return;
-    run = ahead;
-    owner = -1;
-    found = false;
-    for (int w = 0; w < kRowWarps && !found; ++w) {
-        const double t = s.warp_sum[w];
-        if (t > 0.0) { owner = w; ahead = run; found = run + t > target; }
-        run += t;
-    }
-    if (owner != warp) return;
-    int pick = a.V - 1;
-    turns([&](int unit, const float (&w)[4], double t) {
-        double cum = t;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double m = __shfl_up_sync(0xffffffffu, cum, o);
-            if (lane >= o) cum += m;
-        }
-        const unsigned some = __ballot_sync(0xffffffffu, t > 0.0), over = __ballot_sync(0xffffffffu, t > 0.0 && ahead + cum > target);
-        if (some) {
-            const int at = over ? __ffs(over) - 1 : 31 - __clz(some);
-            double c = ahead + (cum - t);
-            int place = 0;
-            bool passed = false;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (w[e] > 0.f && !passed) { c += static_cast<double>(w[e]); place = e; passed = c > target; }
-            pick = __shfl_sync(0xffffffffu, span.index(unit) + place, at);
-        }
-        ahead += __shfl_sync(0xffffffffu, cum, 31);
-        return over != 0;
-    });
-    if (lane == 0) tokens[stop] = pick;
+    cluster.barrier_arrive();                               // every CTA of the cluster runs before another writes into its shared memory
+    const Row<T> span(static_cast<const T*>(a.logits) + (start + stop) * a.stride, a.V, part, a.log_parts);
+    const float* q = stop < d && a.q ? a.q + r * a.q_request + stop * a.q_place : nullptr;
+    span.ask();
+    if (q) span.ask(q);
+    Values<T, 0, true> values(span, part, parts);
+    const int without = stop < d && !a.q ? a.drafted[static_cast<size_t>(r) * a.D + stop] : -1;
+    const int pick = draw_token<T>(values, ByTemperature(stat.x, temp), stat.y, q, without, a.draw[r], a.V, s, cluster, part, parts);
+    if (pick >= 0) tokens[stop] = pick;
 }
 
 template <typename... KArgs, typename... Args>
-inline void launch_row_clusters(void (*kernel)(KArgs...), long long rows, int parts, cudaStream_t stream, Args&&... args) {
+inline void launch_row_clusters(void (*kernel)(KArgs...), dim3 grid, int parts, cudaStream_t stream, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(rows * parts));
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(kRowThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -485,33 +603,56 @@ inline void launch_row_clusters(void (*kernel)(KArgs...), long long rows, int pa
     counted(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
 }
 
-// CTAs of a row's cluster and groups a thread holds (0: read again in every pass).
-struct RowPlan { int parts, units; };
-inline RowPlan row_plan(int V) {
-    const long long groups = (static_cast<long long>(V) + 6) / 4;         // with an edge on either side
-    int parts = 1;
-    while (parts < kRowCtasMost && groups > 2LL * kRowThreads * parts) parts *= 2;
-    const long long per = ((groups + parts - 1) / parts + 31) / 32 * 32, units = (per + kRowThreads - 1) / kRowThreads;
-    return {parts, units <= 2 ? 2 : units <= 4 ? 4 : units <= 8 ? 8 : units <= kRowUnitsMost ? kRowUnitsMost : 0};
+// CTAs of a row's cluster and groups a thread holds (0: read again in every pass, out of L2). Few rows: as many CTAs as fit the GPU at once, and
+// registers where those hold the row, for the shortest way from first read to answer. Many rows: about kSlice values a CTA and nothing held, three CTAs a
+// multiprocessor: what a row costs besides its values (the exchanges within warps, block and cluster) is spread over more of them, and rows in flight stay
+// within L2 (742 rows of 128,256: clusters of four 112 us, clusters of eight with rows in registers 168 us). Probabilities (`keeps`) need every
+// exponential twice and keep it in registers wherever those hold the row (512 rows of 151,669: 170 us, 193 us without).
+constexpr int kSlice = 32768;
+struct RowPlan { int log_parts, units; };
+inline RowPlan row_plan(int V, long long rows, bool keeps = false) {
+    const long long groups = (static_cast<long long>(V) + 6) / 4, sms = sm_count();         // with an edge on either side
+    int log_parts = 0;
+    while ((1 << log_parts) < kRowCtasMost && ((static_cast<long long>(kSlice) << log_parts) < V ||
+                                               ((keeps || (rows << log_parts) * 2 <= 3 * sms) && groups > (2LL * kRowThreads << log_parts)))) ++log_parts;
+    const long long per = (((groups - 1) >> log_parts) + 32) & ~31LL, units = (per + kRowThreads - 1) / kRowThreads;
+    if (!keeps && rows << log_parts > 2 * sms) return {log_parts, 0};
+    return {log_parts, units <= 2 ? 2 : units <= 4 ? 4 : units <= 8 ? 8 : units <= kRowUnitsMost ? kRowUnitsMost : 0};
 }
 
 template <typename T, bool kProbs>
-int launch_rows(const RowArgs& a, long long rows, cudaStream_t st, const char* what) {
-    const RowPlan plan = row_plan(a.V);
-    GI_REQUIRE(rows <= INT_MAX / plan.parts, "%s: %lld rows exceed the grid limit", what, rows);
+int launch_rows(RowArgs a, int rows, int places, cudaStream_t st, const char* what) {
+    const RowPlan plan = row_plan(a.V, static_cast<long long>(rows) * places, kProbs);
+    a.log_parts = plan.log_parts;
+    GI_REQUIRE(rows <= INT_MAX >> plan.log_parts && places <= 65535, "%s: %d rows of %d places exceed the grid limit", what, rows, places);
+    const dim3 grid(static_cast<unsigned>(rows) << plan.log_parts, places);
+    const int parts = 1 << plan.log_parts;
     switch (plan.units) {
-        case 2: launch_row_clusters((row_softmax_kernel<T, 2, kProbs>), rows, plan.parts, st, a); break;
-        case 4: launch_row_clusters((row_softmax_kernel<T, 4, kProbs>), rows, plan.parts, st, a); break;
-        case 8: launch_row_clusters((row_softmax_kernel<T, 8, kProbs>), rows, plan.parts, st, a); break;
-        case kRowUnitsMost: launch_row_clusters((row_softmax_kernel<T, kRowUnitsMost, kProbs>), rows, plan.parts, st, a); break;
-        default: launch_row_clusters((row_softmax_kernel<T, 0, kProbs>), rows, plan.parts, st, a); break;
+        case 2: launch_row_clusters((row_softmax_kernel<T, 2, kProbs>), grid, parts, st, a); break;
+        case 4: launch_row_clusters((row_softmax_kernel<T, 4, kProbs>), grid, parts, st, a); break;
+        case 8: launch_row_clusters((row_softmax_kernel<T, 8, kProbs>), grid, parts, st, a); break;
+        case kRowUnitsMost: launch_row_clusters((row_softmax_kernel<T, kRowUnitsMost, kProbs>), grid, parts, st, a); break;
+        default: launch_row_clusters((row_softmax_kernel<T, 0, kProbs>), grid, parts, st, a); break;
     }
     return check_launch(what);
 }
 
+// Places of the drafts that a launch takes: all, unless there are kRounds times the rows that the GPU holds at a time, for every launch (128 requests of six
+// drafts, 2.8 kept: two launches 152 us, one 170 us; a launch's last clusters leave SMs idle for about half a round).
+constexpr int kRounds = 4;
+inline int places_of_launch(const RowArgs& a) {
+    const long long rows = static_cast<long long>(a.R) * (a.D + 1), held = 3LL * sm_count() >> row_plan(a.V, rows).log_parts;
+    const long long launches = rows / (kRounds * held);
+    return launches <= 1 ? a.D + 1 : launches > a.D ? 1 : static_cast<int>((a.D + launches) / launches);
+}
+
 template <typename T>
-int launch_draw(const RowArgs& a, cudaStream_t st) {
-    launch_row_clusters((draft_draw_kernel<T>), a.R, row_plan(a.V).parts, st, a);
+int launch_verify(RowArgs a, cudaStream_t st) {
+    const int places = places_of_launch(a);
+    for (a.place = 0; a.place <= a.D; a.place += places)
+        if (const int rc = launch_rows<T, false>(a, a.R, a.D + 1 - a.place < places ? a.D + 1 - a.place : places, st, "verify_drafts")) return rc;
+    a.log_parts = row_plan(a.V, 1).log_parts;
+    launch_row_clusters((draft_draw_kernel<T>), dim3(static_cast<unsigned>(a.R) << a.log_parts), 1 << a.log_parts, st, a);
     return check_launch("verify_drafts");
 }
 
@@ -525,7 +666,7 @@ static int gi_token_probabilities_impl(const void* logits, int dtype, int rows, 
     RowArgs a = {};
     a.logits = logits; a.stride = V; a.N = rows; a.V = V; a.temperature = temperature; a.out = out;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return dtype == kF32 ? launch_rows<float, true>(a, rows, st, "token_probabilities") : launch_rows<__nv_bfloat16, true>(a, rows, st, "token_probabilities");
+    return dtype == kF32 ? launch_rows<float, true>(a, rows, 1, st, "token_probabilities") : launch_rows<__nv_bfloat16, true>(a, rows, 1, st, "token_probabilities");
 }
 
 // logits [N, V]; request r's rows start at row_start[r]; drafted, accept [R, D]; q (or null): q_request / q_place values between
@@ -534,17 +675,14 @@ static int gi_verify_drafts_impl(const void* logits, int dtype, int N, int V, in
                                  const float* q, long long q_request, long long q_place, const float* temperature, const float* accept, const float* draw,
                                  int* tokens, int* accepted, void* work, void* stream) {
     if (R == 0) return 0;
-    GI_REQUIRE(N > 0 && V > 0 && V <= INT_MAX - 8 && R > 0 && D >= 0, "verify_drafts: sizes must be positive (N=%d, V=%d, R=%d, D=%d)", N, V, R, D);
+    GI_REQUIRE(N > 0 && V > 0 && V <= INT_MAX - 8 && R > 0 && D >= 0 && D < INT_MAX, "verify_drafts: sizes must be positive (N=%d, V=%d, R=%d, D=%d)", N, V, R, D);
     GI_REQUIRE(reinterpret_cast<uintptr_t>(work) % 16 == 0, "verify_drafts: the workspace must lie on a boundary of 16 bytes");
     RowArgs a = {};
     a.logits = logits; a.stride = V; a.N = N; a.V = V; a.temperature = temperature; a.row_start = row_start; a.drafted = drafted; a.counts = counts;
     a.q = q; a.q_request = q_request; a.q_place = q_place; a.accept = accept; a.draw = draw; a.tokens = tokens; a.accepted = accepted;
     a.work = static_cast<float4*>(work); a.R = R; a.D = D;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const long long rows = static_cast<long long>(R) * (D + 1);
-    const int rc = dtype == kF32 ? launch_rows<float, false>(a, rows, st, "verify_drafts") : launch_rows<__nv_bfloat16, false>(a, rows, st, "verify_drafts");
-    if (rc) return rc;
-    return dtype == kF32 ? launch_draw<float>(a, st) : launch_draw<__nv_bfloat16>(a, st);
+    return dtype == kF32 ? launch_verify<float>(a, st) : launch_verify<__nv_bfloat16>(a, st);
 }
 
 extern "C" int gi_token_probabilities(const void* logits, int dtype, int rows, int V, const float* temperature, float* out, void* stream) {
