@@ -716,6 +716,156 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_many_kernel(Adapte
     }
 }
 
+// ---- 32-bit on the CUDA cores ----
+// x and `down` pass through a ring of stages of 32 values of K (rows of 128 bytes, 16-byte pieces exchanged by the row's last three bits). Of 16 neighbouring
+// threads each has four columns of `kRows` rows, or with few ranks (S r below 64) a share of every stage's K instead, so that none is idle.
+template <int kRows> struct FloatShape {
+    static constexpr int kTile = 16 * kRows, kStageBytes = (kTile + 64) * 128, kStages = kRows == 2 ? 6 : 5;
+};
+template <int kRows>
+__global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(AdapterArgs a) {
+    pdl_prologue();
+    using Shape = FloatShape<kRows>;
+    constexpr int M = Shape::kTile;
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ int s_rows[M], s_scratch[kAdapterWarps];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int part = cluster.block_rank(), parts = cluster.num_blocks();
+    int adapter, n;
+    if (!find_rows<M>(a.plan, a.A, a.tile_rows, blockIdx.x / parts, s_rows, adapter, n, s_scratch)) return;     // (the whole cluster)
+    const int cols = a.S * a.r, hs = cols + 4;
+    const float* x = static_cast<const float*>(a.x);
+    const float* down = static_cast<const float*>(a.down) + static_cast<size_t>(adapter) * cols * a.K;
+    const float* up = static_cast<const float*>(a.up) + static_cast<size_t>(adapter) * a.N * a.r;
+    float* h = reinterpret_cast<float*>(ring + Shape::kStages * Shape::kStageBytes);         // [M][hs]: this CTA's sums
+    float* sums = reinterpret_cast<float*>(ring);                                            // [M][hs]: the whole ones, where the ring was
+    const float scale = a.scales[adapter];
+    const int share = ((a.K + parts - 1) / parts + 31) / 32 * 32, k_begin = min(a.K, part * share), k_end = min(a.K, k_begin + share);
+    const int stages = (k_end - k_begin + 31) / 32;
+    const unsigned ring_at = shared_address(ring);
+    const int copy_row = threadIdx.x >> 3, copy_k = 4 * (threadIdx.x & 7);
+    const unsigned copy_to = copy_row * 128 + (((threadIdx.x & 7) ^ (copy_row & 7)) << 4);
+    const float* x_rows[M / 32];
+    int x_bytes[M / 32];
+#pragma unroll
+    for (int i = 0; i < M / 32; ++i) {
+        const int row = s_rows[copy_row + 32 * i];
+        x_bytes[i] = row >= 0 ? 16 : 0;
+        x_rows[i] = x + max(row, 0) * a.ldx;
+    }
+    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+    for (int c0 = 0; c0 < cols; c0 += 64) {
+        const int some = min(64, cols - c0);
+        int log_groups = 0;                    // threads across the columns: 2^log_groups of 16, the others share K
+        while ((4 << log_groups) < some) ++log_groups;
+        const int groups = 1 << log_groups, across = tx & (groups - 1), split = tx >> log_groups, splits = 16 >> log_groups;
+        auto fetch = [&](int stage, int slot) {
+            const unsigned at = ring_at + slot * Shape::kStageBytes + copy_to;
+            const int k = k_begin + 32 * stage + copy_k;
+            const bool in = k < k_end;
+#pragma unroll
+            for (int i = 0; i < M / 32; ++i) copy_16(at + i * 32 * 128, in ? x_rows[i] + k : x, in ? x_bytes[i] : 0);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (copy_row + 32 * i < 4 * groups) {
+                    const bool there = in && copy_row + 32 * i < some;
+                    copy_16(at + (M + i * 32) * 128, there ? down + static_cast<size_t>(c0 + copy_row + 32 * i) * a.K + k : down, there ? 16 : 0);
+                }
+        };
+        float acc[kRows][4] = {};
+        __syncthreads();                       // (a further pass: the ring is free again)
+#pragma unroll
+        for (int i = 0; i < Shape::kStages - 1; ++i) {
+            if (i < stages) fetch(i, i);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        int slot = 0, next = Shape::kStages - 1;
+        for (int i = 0; i < stages; ++i) {
+            asm volatile("cp.async.wait_group %0;" :: "n"(Shape::kStages - 2) : "memory");
+            __syncthreads();                   // the stage is there for all, and the one before it is free
+            if (i + Shape::kStages - 1 < stages) fetch(i + Shape::kStages - 1, next);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            const unsigned char* at = ring + slot * Shape::kStageBytes;
+            next = slot;
+            slot = slot + 1 == Shape::kStages ? 0 : slot + 1;
+            for (int q = split; q < 8; q += splits) {
+                float4 xv[kRows], w[4];
+#pragma unroll
+                for (int m = 0; m < kRows; ++m) {
+                    const int row = ty + 16 * m;
+                    xv[m] = *reinterpret_cast<const float4*>(at + row * 128 + ((q ^ (row & 7)) << 4));
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int col = across + groups * j;
+                    w[j] = *reinterpret_cast<const float4*>(at + (M + col) * 128 + ((q ^ (col & 7)) << 4));
+                }
+#pragma unroll
+                for (int m = 0; m < kRows; ++m)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        acc[m][j] = fmaf(xv[m].x, w[j].x, acc[m][j]);
+                        acc[m][j] = fmaf(xv[m].y, w[j].y, acc[m][j]);
+                        acc[m][j] = fmaf(xv[m].z, w[j].z, acc[m][j]);
+                        acc[m][j] = fmaf(xv[m].w, w[j].w, acc[m][j]);
+                    }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+        for (int m = 0; m < kRows; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float v = acc[m][j];
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) {
+                    const float y = __shfl_xor_sync(0xffffffffu, v, o);
+                    if (o >= groups) v += y;   // (the threads that share K)
+                }
+                const int col = across + groups * j;
+                if (split == 0 && col < some) h[(ty + 16 * m) * hs + c0 + col] = v;
+            }
+    }
+    cluster.sync();
+    // every CTA adds up its share of the tile's sums and gives them to all
+    const int fours = M * cols / 4, four_share = (fours + parts - 1) / parts, fours_end = min(fours, (part + 1) * four_share);
+    for (int i = part * four_share + threadIdx.x; i < fours_end; i += kAdapterThreads) {
+        const int row = 4 * i / cols, col = 4 * i % cols;
+        const float4 v = cluster_total(h + row * hs + col, scale, cluster, parts);
+#pragma unroll
+        for (int p = 0; p < kAdapterClusterMost; ++p)
+            if (p < parts) *reinterpret_cast<float4*>(cluster.map_shared_rank(sums + row * hs + col, p)) = v;
+    }
+    cluster.sync();
+    // a column a thread, half of the rows a warp
+    constexpr int kHalf = M / 2;
+    const int row0 = (threadIdx.x >> 7) * kHalf;
+    if (row0 >= n) return;
+    float* out = static_cast<float*>(a.out);
+    const int n_share = (a.N + parts - 1) / parts, n_begin = min(a.N, part * n_share), n_end = min(a.N, n_begin + n_share);
+    for (int col = n_begin + (threadIdx.x & 127); col < n_end; col += 128) {
+        int slice = 0;
+#pragma unroll
+        for (int s = 0; s < kAdapterSlicesMost - 1; ++s) slice += s < a.S - 1 && col >= a.ends[s];
+        const float* at = sums + row0 * hs + slice * a.r;
+        const float* w_at = up + static_cast<size_t>(col) * a.r;
+        float acc[kHalf] = {};
+        for (int j = 0; j < a.r; j += 4) {
+            const float4 w = __ldg(reinterpret_cast<const float4*>(w_at + j));
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) {
+                const float4 v = *reinterpret_cast<const float4*>(at + i * hs + j);
+                acc[i] = fmaf(v.x, w.x, fmaf(v.y, w.y, fmaf(v.z, w.z, fmaf(v.w, w.w, acc[i]))));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kHalf; ++i) {
+            const int row = s_rows[row0 + i];
+            if (row >= 0) asm volatile("red.global.add.f32 [%0], %1;" :: "l"(out + row * a.ldo + col), "f"(acc[i]) : "memory");
+        }
+    }
+}
+
 template <typename... KArgs, typename... Args>
 inline void launch_tile_clusters(void (*kernel)(KArgs...), long long tiles, int parts, int threads, size_t smem, cudaStream_t stream, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
@@ -784,6 +934,22 @@ int launch_many(const AdapterArgs& a, long long tiles, cudaStream_t st) {
                           210 * 1024, st);
 }
 
+template <int kRows>
+int launch_float(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+    static SharedLimit limit;
+    using Shape = FloatShape<kRows>;
+    return launch_adapter(&adapter_float_kernel<kRows>, limit, a, tile_count(a, tiles, Shape::kTile),
+                          ring_bytes<Shape>() + 4ull * Shape::kTile * (a.S * a.r + 4), 160 * 1024, st);
+}
+
+int launch_f32(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+    const bool pieces = a.K % 4 == 0 && a.ldx % 4 == 0 && a.r % 4 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
+                        reinterpret_cast<uintptr_t>(a.down) % 16 == 0 && reinterpret_cast<uintptr_t>(a.up) % 16 == 0;
+    if (!pieces) return launch_plain<float, float>(a, tiles, st);
+    if (a.tile_rows && a.plan.T >= 4096 && a.S * a.r <= 256) return launch_float<4>(a, tiles, st);
+    return launch_float<2>(a, tiles, st);
+}
+
 template <int kSteps, typename TO>
 int launch_steps(const AdapterArgs& a, long long tiles, cudaStream_t st) {
     using Wide = ManyShape<128, true>;
@@ -843,7 +1009,7 @@ static int gi_adapter_product_impl(const void* x, long long ldx, int dtype, cons
     a.wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ldo * (out_dtype == kF32 ? 4 : 2) % 16 == 0;
     GI_REQUIRE(dtype == kBF16 || out_dtype == kF32, "adapter_product: 32-bit weights give 32-bit output");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == kF32) return launch_plain<float, float>(a, tiles, st);
+    if (dtype == kF32) return launch_f32(a, tiles, st);
     return out_dtype == kF32 ? launch_bf16<float>(a, tiles, st) : launch_bf16<__nv_bfloat16>(a, tiles, st);
 }
 

@@ -27,12 +27,19 @@ class SharedLimit {
     std::atomic<unsigned long long> set_{0};
 };
 
-// Multiprocessors of the current device.
+// Multiprocessors of the current device, asked for once a device.
 inline int sm_count() {
+    static std::atomic<int> known[64];
     int sms = 0, device = 0;
     cudaGetDevice(&device);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    return sms > 0 ? sms : 1;
+    const bool kept = device >= 0 && device < 64;
+    if (kept) sms = known[device].load(std::memory_order_relaxed);
+    if (sms == 0) {
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+        if (sms <= 0) return 1;
+        if (kept) known[device].store(sms, std::memory_order_relaxed);
+    }
+    return sms;
 }
 
 }  // namespace gi
