@@ -7,7 +7,7 @@ from . import architectures  # noqa: F401  (fills the architecture registry)
 from . import cache, config, weights
 
 __all__ = ["cache", "config", "weights", "load_model", "StepEngine", "StepEntry", "Engine", "Scheduler",
-           "SchedulerConfig", "GenerationRequest", "RequestResult", "SamplingParams", "RandomStream"]
+           "SchedulerConfig", "GenerationRequest", "RequestResult", "SamplingParams", "RandomStream", "SpeculativeEngine"]
 
 
 def __getattr__(name):
@@ -22,6 +22,9 @@ def __getattr__(name):
     if name == "Engine":
         from .engine.generate import Engine
         return Engine
+    if name == "SpeculativeEngine":
+        from .engine.speculative import SpeculativeEngine
+        return SpeculativeEngine
     if name in ("Scheduler", "SchedulerConfig", "GenerationRequest", "RequestResult"):
         from .engine import scheduler as _sched
         return getattr(_sched, name)

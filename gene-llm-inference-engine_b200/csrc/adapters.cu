@@ -47,16 +47,22 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const int* r
         return a >= 0 && a < A ? a : -1;
     };
     int held[kPlanEach];
+    unsigned held_same[kPlanEach];             // the lanes with the same adapter
 #pragma unroll
     for (int i = 0; i < kPlanEach; ++i) held[i] = adapter(i * kPlanThreads + threadIdx.x);
-    auto count = [&](int a) {
-        const unsigned same = __match_any_sync(0xffffffffu, a);
+    auto alike = [&](int a) {                  // (neighbouring rows mostly have one adapter)
+        return __all_sync(0xffffffffu, a == __shfl_sync(0xffffffffu, a, 0)) ? 0xffffffffu : __match_any_sync(0xffffffffu, a);
+    };
+    auto count = [&](int a, unsigned same) {
         if (a >= 0 && lane == __ffs(same) - 1) atomicAdd(&counts[a], __popc(same));
     };
 #pragma unroll
     for (int i = 0; i < kPlanEach; ++i)
-        if (i * kPlanThreads < T) count(held[i]);
-    for (int t0 = kPlanEach * kPlanThreads; t0 < T; t0 += kPlanThreads) count(adapter(t0 + threadIdx.x));
+        if (i * kPlanThreads < T) { held_same[i] = alike(held[i]); count(held[i], held_same[i]); }
+    for (int t0 = kPlanEach * kPlanThreads; t0 < T; t0 += kPlanThreads) {
+        const int a = adapter(t0 + threadIdx.x);
+        count(a, alike(a));
+    }
     __syncthreads();
     int* tiles = plan + 1 + T;
     for (int a0 = 0; a0 < A; a0 += kPlanThreads) {
@@ -83,8 +89,7 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const int* r
         __syncthreads();
     }
     if (threadIdx.x == 0) plan[0] = base_tiles;
-    auto put = [&](int t, int a) {
-        const unsigned same = __match_any_sync(0xffffffffu, a);
+    auto put = [&](int t, int a, unsigned same) {
         const int leader = __ffs(same) - 1;
         int place = 0;
         if (a >= 0 && lane == leader) place = atomicAdd(&counts[a], __popc(same));
@@ -93,8 +98,11 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const int* r
     };
 #pragma unroll
     for (int i = 0; i < kPlanEach; ++i)
-        if (i * kPlanThreads < T) put(i * kPlanThreads + threadIdx.x, held[i]);
-    for (int t0 = kPlanEach * kPlanThreads; t0 < T; t0 += kPlanThreads) put(t0 + threadIdx.x, adapter(t0 + threadIdx.x));
+        if (i * kPlanThreads < T) put(i * kPlanThreads + threadIdx.x, held[i], held_same[i]);
+    for (int t0 = kPlanEach * kPlanThreads; t0 < T; t0 += kPlanThreads) {
+        const int a = adapter(t0 + threadIdx.x);
+        put(t0 + threadIdx.x, a, alike(a));
+    }
 }
 
 struct AdapterArgs {
@@ -946,7 +954,8 @@ int launch_f32(const AdapterArgs& a, long long tiles, cudaStream_t st) {
     const bool pieces = a.K % 4 == 0 && a.ldx % 4 == 0 && a.r % 4 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
                         reinterpret_cast<uintptr_t>(a.down) % 16 == 0 && reinterpret_cast<uintptr_t>(a.up) % 16 == 0;
     if (!pieces) return launch_plain<float, float>(a, tiles, st);
-    if (a.tile_rows && a.plan.T >= 4096 && a.S * a.r <= 256) return launch_float<4>(a, tiles, st);
+    // (2,048 rows of 14,336 into 4,096 at rank 64: tiles of 64 rows 215 us, of 32 263 us; 1,024 rows of 2,048 at rank 16: 27 and 22 us)
+    if (a.tile_rows && a.plan.T >= 2048 && a.S * a.r <= 256) return launch_float<4>(a, tiles, st);
     return launch_float<2>(a, tiles, st);
 }
 

@@ -23,14 +23,16 @@ class Engine:
     def __init__(self, model_dir: str, dtype: str = "bfloat16", device: str = "cuda:0",
                  max_seq_len: Optional[int] = None, page_size: int = 16, kv_pages: Optional[int] = None,
                  max_running: int = 8, step_tokens: int = 2048, prefill_chunk: int = 0, prefix_cache: bool = True,
-                 decode_weight_copy: bool = True, nvtx: bool = False, debug_checks: bool = False):
+                 decode_weight_copy: bool = True, nvtx: bool = False, debug_checks: bool = False,
+                 adapter_slots: int = 0, adapter_rank: int = 16):
         """``model_dir``: folder with config.json and model.safetensors. ``dtype``: "bfloat16"
         (serving kernels) or "float32" (everything in true 32-bit). ``max_seq_len`` lowers the
         context length. ``kv_pages``: pages of ``page_size`` positions in the pool (default: room
         for ``max_running`` full contexts, within 80 % of the free device memory).
         ``decode_weight_copy`` (bfloat16): a second copy of the matrices laid out for decode steps, which
         then stream the weights faster; False saves that memory. ``nvtx`` wraps steps, layers and the head in NVTX
-        ranges; ``debug_checks`` validates every step's descriptor (positions, page ids) on the host before launch."""
+        ranges; ``debug_checks`` validates every step's descriptor (positions, page ids) on the host before launch.
+        ``adapter_slots``: how many low-rank adapters of up to ``adapter_rank`` can be held (``load_adapter``); every request names its own."""
         self.model = load_model(model_dir, dtype=dtype, device=device, max_position=max_seq_len,
                                 weight_tiles=decode_weight_copy)
         context = self.model.max_position
@@ -51,6 +53,8 @@ class Engine:
         self.steps = StepEngine(self.model, page_size=page_size, n_pages=kv_pages, max_requests=max_running,
                                 max_step_tokens=step_tokens, max_logit_rows=max_running, nvtx=nvtx,
                                 debug_checks=debug_checks)
+        if adapter_slots:
+            self.steps.enable_adapters(adapter_slots, adapter_rank)
         self.sampler = DeviceSampler(self.model.vocab_size, self.model.device, ids=self.steps.feedback)
         self.scheduler = Scheduler(self.steps, self.sampler.sample,
                                    SchedulerConfig(max_running, step_tokens, prefill_chunk, prefix_cache),
@@ -58,9 +62,18 @@ class Engine:
 
     # ------------------------------------------------------------------ the reference's Engine interface
     def submit(self, prompt: Sequence[int], max_positions: int = 0, sampling: Optional[SamplingParams] = None,
-               stop_ids: Sequence[int] = (), on_token=None) -> int:
+               stop_ids: Sequence[int] = (), on_token=None, adapter: int = -1) -> int:
+        if adapter >= 0 and (self.steps.adapter_step is None or adapter >= self.steps.adapter_step.slots):
+            raise ValueError(f"submit: there is no adapter slot {adapter}")
         return self.scheduler.submit(GenerationRequest(list(prompt), max_positions, sampling or SamplingParams(),
-                                                       tuple(stop_ids), on_token))
+                                                       tuple(stop_ids), on_token, adapter))
+
+    def load_adapter(self, slot: int, folder: str) -> None:
+        """Reads the low-rank adapter in ``folder`` (adapter_config.json, adapter_model.safetensors) into a slot; no request
+        that names the slot may be running."""
+        from ..weights.adapters import read_adapter
+        pairs, scale = read_adapter(folder)
+        self.steps.put_adapter(slot, pairs, scale)
 
     def step(self) -> bool:
         return self.scheduler.step()
@@ -97,16 +110,18 @@ class Engine:
 
     # ------------------------------------------------------------------ convenience
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 16, temperature: float = 0.0,
-                 top_k: int = 0, top_p: float = 1.0, seed: int = 1, stop_ids: Sequence[int] = ()) -> List[List[int]]:
+                 top_k: int = 0, top_p: float = 1.0, seed: int = 1, stop_ids: Sequence[int] = (),
+                 adapters: Optional[Sequence[int]] = None) -> List[List[int]]:
         """Generates up to ``max_new_tokens`` for every prompt (all requests run together) and
-        returns the generated token ids. Request i samples with seed ``seed + i``."""
+        returns the generated token ids. Request i samples with seed ``seed + i`` and runs with the adapter in slot ``adapters[i]``
+        (-1, or no list: none)."""
         if max_new_tokens <= 0:
             return [[] for _ in prompts]
         ids = []
         for i, p in enumerate(prompts):
             params = SamplingParams(temperature, top_k, top_p, seed + i)
             # the token sampled at the last fed position is kept but not fed: positions = prompt + new - 1
-            ids.append(self.submit(p, len(p) + max_new_tokens - 1, params, stop_ids))
+            ids.append(self.submit(p, len(p) + max_new_tokens - 1, params, stop_ids, adapter=adapters[i] if adapters is not None else -1))
         self.run_until_idle()
         out = []
         for i in ids:

@@ -56,6 +56,7 @@ class GenerationRequest:
     sampling: SamplingParams = field(default_factory=SamplingParams)
     stop_ids: Sequence[int] = ()
     on_token: Optional[Callable[[int], None]] = None
+    adapter: int = -1            # the slot of the adapter it runs with; -1 for none
 
 
 @dataclass
@@ -179,7 +180,7 @@ class Scheduler:
             job = self.waiting.popleft()
             job.cache = self.backend.open(("job", job.id))
             job.fed = job.cached_upto = 0
-            if self.prefix is not None:
+            if self.prefix is not None and job.request.adapter < 0:          # (keys and values of one adapter are no other's)
                 # at least one token must still be fed (it gives the logits) and the limit must leave a row
                 usable = min(len(job.tokens) - 1, job.limit - 1)
                 pages = self.prefix.match(job.tokens, usable) if usable > 0 else []
@@ -193,7 +194,7 @@ class Scheduler:
         self.stats.max_running_seen = max(self.stats.max_running_seen, len(self.running))
 
     def _index_new_pages(self, job: _Job) -> None:
-        if self.prefix is None:
+        if self.prefix is None or job.request.adapter >= 0:
             return
         ps = self.backend.cache.page_size
         if job.fed // ps <= job.cached_upto // ps:
@@ -279,7 +280,8 @@ class Scheduler:
             if take == 0:
                 continue
             last = job.fed + take == len(job.tokens)
-            entries.append(StepEntry(("job", job.id), job.tokens[job.fed:job.fed + take], [take - 1] if last else []))
+            entries.append(StepEntry(("job", job.id), job.tokens[job.fed:job.fed + take], [take - 1] if last else [],
+                                     adapter=job.request.adapter))
             jobs.append(job)
             fed_takes.append(take)
             if last:
@@ -314,7 +316,7 @@ class Scheduler:
             needed += cache.pages_needed(job.cache, 1)
         if needed > cache.free_pages():
             return None                                   # eviction or preemption: decided with all ids known
-        entries = [StepEntry(("job", job.id), [-(k + 1)], [0]) for k, job in enumerate(cur.owners)]
+        entries = [StepEntry(("job", job.id), [-(k + 1)], [0], adapter=job.request.adapter) for k, job in enumerate(cur.owners)]
         return self._run(entries, list(cur.owners), [1] * len(entries), list(cur.owners))
 
     def _complete(self, cur: _InFlight) -> None:

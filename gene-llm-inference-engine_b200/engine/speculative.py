@@ -1,0 +1,280 @@
+"""Generation with drafted tokens: a small model proposes, the served model checks several positions in one step.
+
+A round: the draft model decodes ``drafts`` tokens for every request, one after another, and leaves the distribution of each
+(``kernels.token_probabilities``); the target model runs the last token and the drafts as one step with logits at all of them;
+``kernels.verify_drafts`` keeps a prefix and draws one more token, distributed as the target model alone would have drawn it (greedy
+requests get exactly the target's tokens). What a round leaves on the device (tokens, how many were kept, the requests'
+lengths) is what the next one starts from: the block tables of both models follow the lengths there (``kernels.step_tables`` ahead
+of a step, ``kernels.trim_tables`` behind the verification), and the host reads a round's tokens while the next one runs.
+
+Every request may run the target with a low-rank adapter of its own (``adapter_slots``); the draft model runs as it is, which
+costs accepted drafts, not correctness.
+"""
+from __future__ import annotations
+
+from typing import List, Optional, Sequence
+
+import torch
+
+from ..ops import kernels
+from ..sampling.params import RandomStream, SamplingParams
+from .loading import load_model
+from .step import Segment, StepContext, StepEngine
+
+
+class _Side:
+    """One of the two models with pages of its own and block tables that live on the device."""
+
+    def __init__(self, model, page_size: int, requests: int, positions: int, step_tokens: int, logit_rows: int):
+        stride = (positions + page_size - 1) // page_size
+        pool = requests * stride
+        self.model, self.page_size, self.requests = model, page_size, requests
+        self.steps = StepEngine(model, page_size=page_size, n_pages=pool, max_requests=requests, max_step_tokens=step_tokens, max_logit_rows=logit_rows)
+        cache = self.steps.cache
+        if len(cache.groups) != 1 or cache.groups[0].need.window or cache.groups[0].need.chunk or cache.state_layers:
+            raise ValueError("drafted tokens: the models' layers must keep the keys and values of every position, and no other state (a refused "
+                             "draft is taken back by forgetting its positions)")
+        dev = model.device
+        self.tables = torch.full((requests, stride), -1, dtype=torch.int32, device=dev)
+        self.held = torch.zeros(requests, dtype=torch.int32, device=dev)
+        self.free = torch.arange(pool, dtype=torch.int32, device=dev)
+        self.n_free = torch.full((1,), pool, dtype=torch.int32, device=dev)
+        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.row_start = torch.empty(requests + 1, dtype=torch.int32, device=dev)
+        self.row_req, self.positions, self.slots = (torch.empty(step_tokens, dtype=torch.int32, device=dev) for _ in range(3))
+        self.all_rows = torch.arange(max(step_tokens, logit_rows), dtype=torch.int32, device=dev)
+        self.no_slots = torch.zeros(requests, dtype=torch.int32, device=dev)
+
+    def forward(self, tokens: torch.Tensor, counts: Sequence[int], counts_dev: torch.Tensor, lengths: torch.Tensor, bounds: Sequence[int],
+                logits: bool, row_adapter: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """A step of ``counts`` tokens a request behind the ``lengths`` cached ones (on the device; ``bounds``: what they are at
+        most), with logits at every row or none."""
+        T, R = tokens.numel(), self.requests
+        kernels.step_tables(lengths, counts_dev, self.tables, self.held, self.free, self.n_free, self.page_size, self.row_start,
+                            self.row_req[:T], self.positions[:T], self.slots[:T], self.status)
+        views = {"tokens": tokens, "positions": self.positions[:T], "row_req": self.row_req[:T], "logit_rows": self.all_rows[:T if logits else 0],
+                 "state_slots": self.no_slots, "seg_start": self.row_start[:R], "seg_len": counts_dev, "tables": [self.tables]}
+        if row_adapter is not None:
+            views["row_adapter"] = row_adapter
+        segments, row = [], 0
+        for r, n in enumerate(counts):
+            segments.append(Segment(r, row, n, bounds[r], 0, False))
+            row += n
+        steps = self.steps
+        steps._poll_status(wait=False)
+        failures = kernels.status_failures(steps.device)
+        steps._aux_calls = 0
+        ctx = StepContext(steps, T, R, T if logits else 0, segments, views)
+        with kernels.on_current_stream():
+            steps._begin_adapters(ctx)
+            out = self.model.forward(ctx)
+        steps._post_status(failures)
+        return out
+
+    def trim(self, lengths: torch.Tensor) -> None:
+        kernels.trim_tables(lengths, self.tables, self.held, self.free, self.n_free, self.page_size, self.status)
+
+    def check(self) -> None:
+        self.steps.check_status()
+        status = int(self.status)
+        if status:
+            raise RuntimeError(f"step tables were refused (status {status})")
+
+
+class SpeculativeEngine:
+    def __init__(self, model_dir: str, draft_dir: str, drafts: int = 4, dtype: str = "bfloat16", device: str = "cuda:0", max_running: int = 8,
+                 max_seq_len: int = 2048, page_size: int = 16, step_tokens: int = 2048, decode_weight_copy: bool = True,
+                 adapter_slots: int = 0, adapter_rank: int = 16):
+        """``model_dir``, ``draft_dir``: the served and the proposing model, of one vocabulary. ``drafts``: tokens proposed a
+        round. ``max_seq_len``: positions of a request at most (prompt and generated tokens). The other arguments are ``Engine``'s."""
+        if drafts < 1 or max_running < 1:
+            raise ValueError("drafted tokens: drafts and max_running must be positive")
+        self.drafts, self.requests, self.page_size = drafts, max_running, page_size
+        room = max_seq_len + drafts + 1            # positions that a round may write behind the last one that stays
+        target = load_model(model_dir, dtype=dtype, device=device, max_position=room, weight_tiles=decode_weight_copy)
+        draft = load_model(draft_dir, dtype=dtype, device=device, max_position=room, weight_tiles=decode_weight_copy)
+        if target.vocab_size != draft.vocab_size:
+            raise ValueError(f"drafted tokens: the models' vocabularies differ ({target.vocab_size} and {draft.vocab_size})")
+        self.context = min(target.max_position, draft.max_position) - drafts - 1
+        if self.context < 2:
+            raise ValueError("drafted tokens: the context is too short")
+        self.vocab, self.device = target.vocab_size, target.device
+        R, K, V = max_running, drafts, target.vocab_size
+        self.step_tokens = max(step_tokens, R * (K + 1))
+        self.target = _Side(target, page_size, R, self.context + K + 1, self.step_tokens, R * (K + 1))
+        self.draft = _Side(draft, page_size, R, self.context + K + 1, self.step_tokens, R)
+        if adapter_slots:
+            self.target.steps.enable_adapters(adapter_slots, adapter_rank)
+        dev = self.device
+        ints = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=dev)      # noqa: E731
+        self._lengths, self._current, self._ends = ints(R), ints(R), ints(R)
+        self._at = ints(K + 1, R)                                   # lengths of the drafting steps
+        self._ids, self._drafted, self._fed = ints(K, R), ints(R, K), ints(R, K + 1)
+        self._ones, self._counts, self._rows = ints(R) + 1, ints(R), ints(R) + (K + 1)
+        self._starts = torch.arange(R, dtype=torch.int32, device=dev) * (K + 1)
+        self._tokens, self._accepted = ints(R, K + 1), ints(R)
+        self._probs = torch.empty(K, R, V, dtype=torch.float32, device=dev)
+        self._scratch = torch.empty(R, V, dtype=torch.float32, device=dev)
+        self._work = torch.empty(R * (K + 1), 4, dtype=torch.float32, device=dev)
+        self._temperature = torch.zeros(R, dtype=torch.float32, device=dev)
+        self._no_top_k, self._no_top_p = ints(R), torch.ones(R, dtype=torch.float32, device=dev)
+        self._adapters = ints(R) - 1
+        # two rounds may be in flight: numbers on their way in, tokens on their way out
+        n = R * (2 * K + 1)
+        self._numbers_host = [torch.zeros(n).pin_memory() for _ in range(3)]
+        self._numbers = [torch.zeros(n, device=dev) for _ in range(3)]
+        self._out_host = [torch.zeros(R, K + 2, dtype=torch.int32).pin_memory() for _ in range(3)]
+        self._done = [None] * 3
+        self.rounds = self.proposed = self.kept = 0
+
+    def load_adapter(self, slot: int, folder: str) -> None:
+        """Reads a low-rank adapter of the target model into a slot (``Engine.load_adapter``)."""
+        from ..weights.adapters import read_adapter
+        pairs, scale = read_adapter(folder)
+        self.target.steps.put_adapter(slot, pairs, scale)
+
+    def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 16, temperature=0.0, seed: int = 1,
+                 stop_ids: Sequence[int] = (), adapters: Optional[Sequence[int]] = None) -> List[List[int]]:
+        """Up to ``max_new_tokens`` for every prompt, ``max_running`` of them at a time; ``temperature``: one number, or one a prompt (0:
+        greedy). Request i draws with seed ``seed + i`` and runs the target with the adapter in slot ``adapters[i]`` (-1: none)."""
+        temps = list(temperature) if hasattr(temperature, "__len__") else [float(temperature)] * len(prompts)
+        slots = list(adapters) if adapters is not None else [-1] * len(prompts)
+        if len(temps) != len(prompts) or len(slots) != len(prompts):
+            raise ValueError("generate: a temperature and an adapter for every prompt")
+        have = self.target.steps.adapter_step.slots if self.target.steps.adapter_step is not None else 0
+        for p, t, a in zip(prompts, temps, slots):
+            SamplingParams(temperature=float(t))               # (refuses what is no temperature)
+            if not 1 <= len(p) or len(p) + max_new_tokens > self.context:
+                raise ValueError(f"generate: a prompt of {len(p)} tokens and {max_new_tokens} more do not fit in {self.context} positions")
+            if any(not 0 <= int(x) < self.vocab for x in p):
+                raise ValueError("generate: token id out of range")
+            if a >= have:
+                raise ValueError(f"generate: there is no adapter slot {a}")
+        out: List[List[int]] = []
+        for at in range(0, len(prompts), self.requests):
+            some = slice(at, at + self.requests)
+            out += self._batch([list(p) for p in prompts[some]], max_new_tokens, temps[some], [seed + at + i for i in range(len(prompts[some]))],
+                               set(stop_ids), slots[some])
+        return out
+
+    # ------------------------------------------------------------------ one batch
+    def _batch(self, prompts, max_new, temps, seeds, stop_ids, slots) -> List[List[int]]:
+        R, n, dev = self.requests, len(prompts), self.device
+        if max_new <= 0:
+            return [[] for _ in prompts]
+        fill = lambda t, values, rest: t.copy_(torch.tensor(list(values) + [rest] * (R - n), dtype=t.dtype))      # noqa: E731
+        self._lengths.zero_()
+        for side in (self.target, self.draft):
+            side.trim(self._lengths)                           # (whatever an earlier batch held)
+        fill(self._temperature, temps, 0.0)
+        fill(self._adapters, slots, -1)
+        fill(self._current, [p[-1] for p in prompts], 0)
+        # places without a request run along on position 0; a request that has ended stays at its end
+        ends = [len(p) - 1 + max_new for p in prompts] + [0] * (R - n)
+        self._ends.copy_(torch.tensor(ends, dtype=torch.int32))
+        adapted = any(a >= 0 for a in slots)
+        self._prefill(prompts, adapted)
+        streams = [RandomStream(s) for s in seeds]
+        lengths = [len(p) - 1 for p in prompts] + [0] * (R - n)
+        results: List[List[int]] = [[] for _ in prompts]
+        alive = [True] * n
+        pending = None
+        rounds = 0
+        while True:
+            now = None
+            if any(alive) and rounds < max_new:                # (a round gives every request a token at least)
+                bounds = [min(l + rounds * (self.drafts + 1), e) for l, e in zip(lengths, ends)]
+                now = self._round(rounds % 3, streams, temps, bounds, adapted)
+                rounds += 1
+            if pending is not None:
+                self._collect(pending, results, alive, max_new, stop_ids)
+            if now is None:
+                break
+            pending = now
+        for side in (self.target, self.draft):
+            side.check()
+        return results
+
+    def _prefill(self, prompts, adapted: bool) -> None:
+        """All of every prompt but its last token, in portions of the step's token limit."""
+        R, dev = self.requests, self.device
+        fed = [0] * R
+        total = [len(p) - 1 for p in prompts] + [0] * (R - len(prompts))
+        while any(f < t for f, t in zip(fed, total)):
+            budget, counts, tokens, rows = self.step_tokens, [], [], []
+            for r in range(R):
+                take = min(total[r] - fed[r], budget)
+                budget -= take
+                counts.append(take)
+                if take:
+                    tokens += prompts[r][fed[r]:fed[r] + take]
+                    rows += [r] * take
+            ids = torch.tensor(tokens, dtype=torch.int32).to(dev)
+            self._counts.copy_(torch.tensor(counts, dtype=torch.int32))
+            row_adapter = self._adapters[torch.tensor(rows).to(dev)].contiguous() if adapted else None
+            self.target.forward(ids, counts, self._counts, self._lengths, fed, False, row_adapter)
+            self.draft.forward(ids, counts, self._counts, self._lengths, fed, False)
+            self._lengths += self._counts
+            fed = [f + c for f, c in zip(fed, counts)]
+
+    def _round(self, turn: int, streams, temps, bounds, adapted: bool):
+        """Launches a round; its tokens are on their way to the host behind the returned event."""
+        R, K = self.requests, self.drafts
+        if self._done[turn] is not None:
+            self._done[turn].synchronize()
+        host, numbers = self._numbers_host[turn], self._numbers[turn]
+        for r, stream in enumerate(streams):
+            if temps[r] > 0:
+                for j in range(K):
+                    host[j * R + r] = stream.next_uniform()                      # the draft's draw
+                for j in range(K):
+                    host[K * R + r * K + j] = stream.next_uniform()              # whether it is kept
+                host[2 * K * R + r] = stream.next_uniform()                      # the token behind the kept ones
+        numbers.copy_(host, non_blocking=True)
+        accept, draw = numbers[K * R:2 * K * R].view(R, K), numbers[2 * K * R:]
+        # the drafts, and one step more that only leaves the last one's keys and values
+        torch.add(self._lengths, torch.arange(K + 1, dtype=torch.int32, device=self.device)[:, None], out=self._at)
+        ones = [1] * R
+        for j in range(K + 1):
+            tokens = self._current if j == 0 else self._ids[j - 1]
+            logits = self.draft.forward(tokens, ones, self._ones, self._at[j], [b + j for b in bounds], j < K)
+            if j < K:
+                kernels.token_probabilities(logits, self._temperature, self._probs[j])
+                kernels.argmax(logits, self._ids[j])
+                kernels.sample(logits, self._scratch, self._temperature, self._no_top_k, self._no_top_p, numbers[j * R:(j + 1) * R], self._ids[j])
+        self._drafted.copy_(self._ids.t())
+        self._fed[:, 0].copy_(self._current)
+        self._fed[:, 1:].copy_(self._drafted)
+        row_adapter = self._adapters[:, None].expand(R, K + 1).reshape(-1).contiguous() if adapted else None
+        logits = self.target.forward(self._fed.view(-1), [K + 1] * R, self._rows, self._lengths, bounds, True, row_adapter)
+        self._counts.fill_(K)
+        kernels.verify_drafts(logits, self._starts, self._drafted, self._counts, self._probs.transpose(0, 1), self._temperature, accept, draw,
+                              self._tokens, self._accepted, self._work)
+        # the next round starts behind what was kept
+        self._current.copy_(self._tokens.gather(1, self._accepted.long()[:, None])[:, 0])
+        self._lengths.copy_(torch.minimum(self._lengths + self._accepted + 1, self._ends))
+        for side in (self.target, self.draft):
+            side.trim(self._lengths)
+        out = self._out_host[turn]
+        out[:, :K + 1].copy_(self._tokens, non_blocking=True)
+        out[:, K + 1].copy_(self._accepted, non_blocking=True)
+        event = torch.cuda.Event()
+        event.record()
+        self._done[turn] = event
+        return turn, event
+
+    def _collect(self, pending, results, alive, max_new: int, stop_ids) -> None:
+        turn, event = pending
+        event.synchronize()
+        out = self._out_host[turn].tolist()
+        self.rounds += 1
+        for r, result in enumerate(results):
+            if not alive[r]:
+                continue
+            self.proposed += self.drafts
+            self.kept += out[r][-1]
+            for token in out[r][:out[r][-1] + 1]:
+                result.append(int(token))
+                if token in stop_ids or len(result) == max_new:
+                    alive[r] = False
+                    break

@@ -17,6 +17,7 @@ import torch
 
 from ..cache import CacheManager, OutOfPages, RequestCache
 from ..ops import kernels
+from ..ops.adapters import AdapterSet, AdapterStep
 from ..parts import DecoderModel
 
 _STATE_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "int32": torch.int32}
@@ -26,10 +27,12 @@ _STATE_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "int32": 
 class StepEntry:
     """The next tokens of one request and the places among them whose logits are wanted. A token
     given as -(k + 1) is taken on the device from place k of the engine's ``feedback`` buffer, where
-    a sampler left the id it drew from the step before (the host need not know it yet)."""
+    a sampler left the id it drew from the step before (the host need not know it yet). ``adapter``: the slot of the
+    adapter that the request's rows run with (``StepEngine.enable_adapters``), -1 for none."""
     key: Hashable
     tokens: Sequence[int]
     want: Sequence[int] = field(default_factory=list)
+    adapter: int = -1
 
 
 @dataclass
@@ -68,6 +71,7 @@ class StepContext:
         self.seg_start = views["seg_start"]
         self.seg_len = views["seg_len"]
         self._tables = views["tables"]
+        self.row_adapter = views.get("row_adapter")      # the rows' adapters where some row of the step has one
         self._cache: Dict = {}
         self.carry: Dict = {}      # what a part leaves ready for the part that runs next (cleared when a forward pass starts)
         self.all_single = all(s.length == 1 for s in segments)
@@ -108,7 +112,7 @@ class StepContext:
         if not eng.use_programs or eng.tap is not None:
             launch()
             return
-        full = (id(owner), key)
+        full = (id(owner), key, self.row_adapter is not None)
         program = eng._programs.get(full)
         if program is None:
             with kernels.record() as rec:
@@ -238,6 +242,8 @@ class StepEngine:
             self.layer_state[layer] = torch.zeros((max_requests, *need.shape), dtype=_STATE_DTYPES[need.dtype],
                                                   device=self.device)
         self._scratch: Dict[Tuple, torch.Tensor] = {}
+        self.adapter_step = None            # set by enable_adapters
+        self.adapter_sets: Dict[int, Dict[str, object]] = {}
         self._init_descriptor()
         self.row_index = torch.arange(max(max_step_tokens, max_requests), dtype=torch.int32, device=self.device)
         self.no_work = torch.zeros((0, 3), dtype=torch.int32, device=self.device)
@@ -302,8 +308,11 @@ class StepEngine:
         stride = self.cache.max_pages_per_request
         self._layout: Dict[str, Tuple[int, int]] = {}
         off = 0
-        for name, n in (("tokens", T), ("positions", T), ("row_req", T), ("logit_rows", self.max_logit_rows),
-                        ("state_slots", R), ("seg_start", R), ("seg_len", R)):
+        arrays = [("tokens", T), ("positions", T), ("row_req", T), ("logit_rows", self.max_logit_rows),
+                  ("state_slots", R), ("seg_start", R), ("seg_len", R)]
+        if self.adapter_step is not None:
+            arrays.append(("row_adapter", T))
+        for name, n in arrays:
             self._layout[name] = (off, n)
             off += n
         self._table_stride = max(stride, 1)
@@ -357,6 +366,51 @@ class StepEngine:
         self._aux_events[k][turn] = ev
         return dev[:n]
 
+    # ------------------------------------------------------------------ adapters
+    def enable_adapters(self, slots: int, rank: int) -> None:
+        """Room for ``slots`` low-rank adapters of up to ``rank`` beside the projections of every layer; entries then name a
+        slot each. Before the first step."""
+        if self.adapter_step is not None:
+            raise RuntimeError("adapters are enabled already")
+        found = {}
+        for run in self.model.runs:
+            layer = self.model.layers[run.layer]
+            for part in (layer.mixer, getattr(layer, "feed_forward", None)):
+                projections = getattr(part, "adaptable", list)()
+                if part is not None and not projections:
+                    raise ValueError(f"adapters: layer {run.layer} has a part ({type(part).__name__}) that takes none")
+                for name, linear, widths in projections:
+                    found.setdefault(run.layer, {})[name] = (linear, widths)
+        step = AdapterStep(slots, self.max_step_tokens, self.device)
+        for layer, projections in found.items():
+            for name, (linear, widths) in projections.items():
+                adapters = AdapterSet(slots, rank, linear.in_features, widths, linear.compute_dtype, self.device)
+                linear.adapt(adapters, step)
+                self.adapter_sets.setdefault(layer, {})[name] = adapters
+        self.adapter_step = step
+        self._init_descriptor()
+        self._drop_captures()
+
+    def put_adapter(self, slot: int, pairs, scale: float) -> None:
+        """``pairs``: {(layer, projection): a (down, up) or None for every part stacked in it}; projections that are not
+        named get none. The slot's requests run with it from the next step on."""
+        if self.adapter_step is None:
+            raise RuntimeError("adapters are not enabled")
+        known = {(layer, name) for layer, sets in self.adapter_sets.items() for name in sets}
+        unknown = sorted(str(k) for k in set(pairs) - known)
+        if unknown:
+            raise ValueError(f"adapters: no such projection: {', '.join(unknown[:5])}")
+        for layer, sets in self.adapter_sets.items():
+            for name, adapters in sets.items():
+                if pairs.get((layer, name)) is None:
+                    adapters.clear(slot)
+                else:
+                    adapters.put(slot, pairs[(layer, name)], scale)
+
+    def _begin_adapters(self, ctx: "StepContext") -> None:
+        if self.adapter_step is not None:
+            self.adapter_step.begin(ctx.row_adapter)
+
     # ------------------------------------------------------------------ requests
     def open(self, key: Hashable) -> RequestCache:
         return self.cache.open(key)
@@ -394,6 +448,8 @@ class StepEngine:
             seen.add(e.key)
             if e.key not in self.cache.requests:
                 raise KeyError(f"request {e.key!r} is not open")
+            if e.adapter >= 0 and (self.adapter_step is None or e.adapter >= self.adapter_step.slots):
+                raise ValueError(f"request {e.key!r}: there is no adapter slot {e.adapter}")
             n = len(e.tokens)
             for tok in e.tokens:
                 if not (0 <= int(tok) < V) and not (-self.max_logit_rows <= int(tok) < 0):
@@ -450,6 +506,9 @@ class StepEngine:
             host[t_off + row:t_off + row + n] = np.asarray(e.tokens, dtype=np.int32)
             host[p_off + row:p_off + row + n] = np.arange(rc.length, rc.length + n, dtype=np.int32)
             host[r_off + row:r_off + row + n] = r
+            if self.adapter_step is not None:
+                a_off = lay["row_adapter"][0]
+                host[a_off + row:a_off + row + n] = e.adapter
             for w in e.want:
                 host[l_off + k] = row + int(w)
                 k += 1
@@ -477,6 +536,8 @@ class StepEngine:
             "seg_len": dev[lay["seg_len"][0]:lay["seg_len"][0] + R],
             "tables": [dev[o:o + R * self._table_stride].view(R, self._table_stride) for o in self._table_off],
         }
+        if any(e.adapter >= 0 for e in entries):
+            views["row_adapter"] = dev[lay["row_adapter"][0]:lay["row_adapter"][0] + total]
         for seg in segments:                       # state of a new request starts from zero
             if seg.fresh_state:
                 for st in self.layer_state.values():
@@ -500,15 +561,18 @@ class StepEngine:
         fresh = any(s.fresh_state for s in ctx.segments) and self.layer_state
         if not (self.use_graphs and ctx.all_single and not fresh and self.tap is None):
             with kernels.on_current_stream():
+                self._begin_adapters(ctx)
                 return self.model.forward(ctx)
-        key = (ctx.n_tokens, ctx.n_logit_rows, ctx.longest_single)
+        key = (ctx.n_tokens, ctx.n_logit_rows, ctx.longest_single, ctx.row_adapter is not None)
         entry = self._graphs.get(key)
         if entry is None:
             with kernels.on_current_stream():
+                self._begin_adapters(ctx)
                 out = self.model.forward(ctx)      # also sizes scratch and configures the kernels
             before = kernels.launch_count()
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph), kernels.on_current_stream():
+                self._begin_adapters(ctx)
                 captured = self.model.forward(ctx)
             n_kernels = kernels.launch_count() - before
             kernels.count_launches(-n_kernels)     # captured, not launched

@@ -21,7 +21,10 @@ from . import kernels
 
 
 class Linear:
-    not_weights = ("weight_tiles",)      # a second layout of the same weights, not counted among a model's weight bytes
+    # not counted among a model's weight bytes: a second layout of the same weights, and adapters that rows may have beside them
+    not_weights = ("weight_tiles", "adapters", "adapter_step")
+    adapters = None         # AdapterSet of this projection
+    adapter_step = None     # which of the current step's rows have one (AdapterStep)
 
     def __init__(self, weight: torch.Tensor, compute_dtype: torch.dtype, device: torch.device, tiles: bool = True):
         if weight.dim() != 2:
@@ -52,19 +55,34 @@ class Linear:
             new.weight_tiles = kernels.tile_weight(weight)
         return new
 
+    def adapt(self, adapters, adapter_step) -> None:
+        """From now on rows of a step may have an adapter of ``adapters`` (AdapterSet) beside this projection."""
+        if (adapters.in_features, adapters.out_features) != (self.in_features, self.out_features):
+            raise ValueError("Linear: the adapters are of another projection")
+        self.adapters, self.adapter_step = adapters, adapter_step
+
+    @property
+    def adapted(self) -> bool:
+        """Whether a row of the current step has an adapter here: the product's output is then added to, so nothing that
+        follows it (a norm, a rotation, an activation) can ride in its last pass."""
+        return self.adapters is not None and self.adapter_step.plan is not None
+
     def forward(self, a: torch.Tensor, out: torch.Tensor, accumulate: bool = False, then: "Linear" = None, norm=None) -> torch.Tensor:
         """``norm`` = (weight, eps, xn): the norm of out's rows goes to xn (``kernels.gemm_tc``). ``then``: the Linear whose
         product runs next but one (after a small kernel); a product of few tokens asks the start of its weights into L2
         meanwhile (``kernels.gemm_tc``: ``ahead``)."""
         if a.dtype != self.compute_dtype:
             raise kernels.KernelError(f"Linear: activations are {a.dtype}, the weight is {self.compute_dtype}")
+        adapted = self.adapted
         if self.compute_dtype is torch.bfloat16 and self.in_features % 8 == 0:
-            fused = norm is not None and kernels.gemm_tc_takes_norm(a, self.weight, out, accumulate, norm)
+            fused = norm is not None and not adapted and kernels.gemm_tc_takes_norm(a, self.weight, out, accumulate, norm)
             kernels.gemm_tc(a, self.weight, out, accumulate, w_tiles=self.weight_tiles,   # tensor cores (TMA needs 16-byte rows)
                             ahead=then.weight_tiles if then is not None else None, norm=norm if fused else None)
         else:
             fused = False
             kernels.gemm_simt(a, self.weight, out, accumulate, w_constant=True)
+        if adapted:
+            self.adapters.add(a, self.adapter_step.plan, out)
         if norm is not None and not fused:        # (an operation of its own, also for who times them one by one)
             kernels.rmsnorm(out, norm[0], norm[2], norm[1])
         return out

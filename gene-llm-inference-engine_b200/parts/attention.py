@@ -222,6 +222,14 @@ class AttentionMixer:
                 raise ValueError("attention: the query temperature's blocks must have a positive length")
             self.temperature = (coef, every)
 
+    def adaptable(self):
+        """[(name of the projection, its Linear, widths of the parts stacked in it)]: where adapters can be (none with the options,
+        whose projections stack more than queries, keys and values)."""
+        if self.extended:
+            return []
+        H, Hkv, hd = self.num_heads, self.num_kv_heads, self.head_dim
+        return [("w_qkv", self.w_qkv, (H * hd, Hkv * hd, Hkv * hd)), ("w_o", self.w_o, (self.hidden_size,))]
+
     def prefill_on_tcgen05(self, page_size: int) -> bool:
         """Head sizes 64 and 128 with pages TMA can tile: prompt portions run on the tcgen05 kernel."""
         key = ("tc", page_size)
@@ -324,7 +332,7 @@ class AttentionMixer:
         if self.extended:
             self._forward_extended(ctx, run, xn, x, q, k_cache, v_cache, tables, then)
             return
-        if self.dtype is torch.bfloat16 and kernels.gemm_rope_store_supported(
+        if self.dtype is torch.bfloat16 and not self.w_qkv.adapted and kernels.gemm_rope_store_supported(
                 T, self.hidden_size, H, Hkv, hd, self.position.cos, self.position.interleaved):
             # rotation and page store in the epilogue of the product
             kernels.gemm_rope_store(xn, self.w_qkv.weight, ctx.positions, ctx.row_req, tables, self.position.cos,

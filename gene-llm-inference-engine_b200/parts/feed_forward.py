@@ -58,6 +58,10 @@ class SwiGLUFeedForward:
         """The Linear of the first product (a block hands it to the mixer that runs before, see AttentionMixer.forward)."""
         return self.w_gate_up
 
+    def adaptable(self):
+        """[(name of the projection, its Linear, widths of the parts stacked in it)]: where adapters can be."""
+        return [("w_gate_up", self.w_gate_up, (self.intermediate_size, self.intermediate_size)), ("w_down", self.w_down, (self.hidden_size,))]
+
     def launch_key(self, ctx):
         """Its launches depend on the token count only (which the caller's key holds)."""
         return ()
@@ -71,7 +75,7 @@ class SwiGLUFeedForward:
         """``accumulate`` False: x is set to the output instead of being added to. ``norm`` = (weight, eps, out): the norm of x then."""
         T = xn.shape[0]
         h = ctx.scratch("ffn_hidden", (T, self.intermediate_size), self.dtype)
-        if self.dtype is torch.bfloat16 and kernels.gemm_swiglu_supported(T, self.intermediate_size, self.hidden_size):
+        if self.dtype is torch.bfloat16 and not self.w_gate_up.adapted and kernels.gemm_swiglu_supported(T, self.intermediate_size, self.hidden_size):
             # activation (and bias) in the product's epilogue
             kernels.gemm_swiglu(xn, self.w_gate_up.weight, h, self.activation, self.limit, self.b_gate_up)
         else:

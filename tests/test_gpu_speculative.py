@@ -1,0 +1,261 @@
+"""Adapters and drafted tokens through the engine: a request's adapter does what its matrices added to the weights would do, and generation with
+drafts gives what the target model alone gives."""
+import json
+import os
+
+import numpy as np
+import pytest
+import torch
+
+import gpu_fixtures as gf
+import tiny_configs as tc
+
+pytestmark = pytest.mark.gpu
+
+PUBLISHED = {"self_attn.q_proj": "self_attn.q_proj.weight", "self_attn.k_proj": "self_attn.k_proj.weight", "self_attn.v_proj": "self_attn.v_proj.weight",
+             "self_attn.o_proj": "self_attn.o_proj.weight", "mlp.gate_proj": "mlp.gate_proj.weight", "mlp.up_proj": "mlp.up_proj.weight",
+             "mlp.down_proj": "mlp.down_proj.weight"}
+
+
+def adapter_and_merged(case, seed, tmp_path, rank=6, only=None, std=0.1):
+    """(adapter folder, model folder in 32-bit with the adapter added to its weights)."""
+    from geneinfer_b200.weights import SafetensorsFile, read_config, write_safetensors
+    from geneinfer_b200.weights.adapters import read_adapter, write_random_adapter, PLACES
+    source = gf.model_dir(case)
+    _, config, _ = read_config(source)
+    folder = str(tmp_path / f"adapter_{case}_{seed}")
+    write_random_adapter(config, seed, folder, rank=rank, alpha=9.0, std=std)
+    if only is not None:
+        path = os.path.join(folder, "adapter_model.safetensors")
+        with SafetensorsFile(path) as f:
+            kept = [(n, f.tensor(n).clone()) for n in f.names() if any(o in n for o in only)]
+        write_safetensors(path, kept)
+    pairs, scale = read_adapter(folder)
+    merged = str(tmp_path / f"merged_{case}_{seed}")
+    os.makedirs(merged)
+    with open(os.path.join(source, "config.json")) as f, open(os.path.join(merged, "config.json"), "w") as g:
+        g.write(f.read())
+    by_name = {}
+    for (layer, name), parts in pairs.items():
+        for published, (projection, place, _) in PLACES.items():
+            if projection == name and parts[place] is not None:
+                by_name[f"model.layers.{layer}.{PUBLISHED[published]}"] = parts[place]
+    with SafetensorsFile(os.path.join(source, "model.safetensors")) as f:
+        tensors = []
+        for n in f.names():
+            w = f.tensor(n).float()
+            if n in by_name:
+                down, up = by_name[n]
+                w = w + scale * (up.double() @ down.double()).float()
+            tensors.append((n, w))
+    assert by_name and all(any(n == m for m, _ in tensors) for n in by_name)
+    write_safetensors(os.path.join(merged, "model.safetensors"), tensors)
+    return folder, merged
+
+
+def engine_of(folder, dtype, slots=0, **options):
+    from geneinfer_b200.engine.loading import load_model
+    from geneinfer_b200.engine.step import StepEngine
+    steps = StepEngine(load_model(folder, dtype=dtype), n_pages=96, max_requests=4, max_step_tokens=512, debug_checks=True, **options)
+    if slots:
+        steps.enable_adapters(slots, 8)
+    return steps
+
+
+@pytest.mark.parametrize("case", ["a", "b", "c"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_an_adapter_does_what_added_to_the_weights_it_would_do(case, dtype, tmp_path):
+    """Two requests with adapters and one without in the same steps: a prompt, a portion beside single tokens, then single tokens (captured and replayed).
+    32-bit: both sides differ in the order of sums. bfloat16: the merged side keeps its weights unrounded in 32 bits, so the distance is the
+    model's own rounding noise, of which the fixture's comparisons allow three quarters beside the plain form; here both the weights and the
+    adapters' sums round, twice the noise."""
+    from geneinfer_b200.engine.step import StepEntry
+    from geneinfer_b200.weights.adapters import read_adapter
+    folders = [adapter_and_merged(case, s, tmp_path, std=0.1 if dtype == "float32" else 0.03) for s in (1, 2)]
+    steps = engine_of(gf.model_dir(case), dtype, slots=3)
+    for slot, (folder, _) in zip((2, 0), folders):
+        steps.put_adapter(slot, *read_adapter(folder))
+    plain = [engine_of(m, "float32") for m in (folders[0][1], folders[1][1], gf.model_dir(case))]
+    vocab = steps.model.vocab_size
+    texts = [tc.random_tokens(n, vocab, 9 + n) for n in (40, 21, 33)]
+    slots = (2, 0, -1)
+    for r in range(3):
+        steps.open(r)
+        plain[r].open(r)
+    bound = 2e-4 if dtype == "float32" else 2 * max(gf.bf16_noise(case), 1e-2)
+    at = [0, 0, 0]
+    for counts in ((40 - 6, 21 - 6, 33 - 6), (2, 1, 1), (1, 1, 1), (1, 1, 1), (1, 1, 1), (0, 2, 0)):
+        entries = [StepEntry(r, texts[r][at[r]:at[r] + n], [n - 1], adapter=slots[r]) for r, n in enumerate(counts) if n]
+        got = steps.step(entries).float().cpu().numpy().copy()
+        for row, e in zip(got, entries):
+            want = plain[e.key].step([StepEntry(e.key, e.tokens, e.want)]).cpu().numpy()[0]
+            assert np.abs(row - want).max() <= bound * max(1.0, np.abs(want).max()), (counts, e.key)
+        at = [a + n for a, n in zip(at, counts)]
+    assert steps.graph_replays > 0
+
+
+def test_adapters_of_some_projections_only_and_steps_without_any(tmp_path):
+    from geneinfer_b200.engine.step import StepEntry
+    from geneinfer_b200.weights.adapters import read_adapter
+    folder, merged = adapter_and_merged("a", 3, tmp_path, only=("layers.0.self_attn.v_proj", "layers.1.mlp.up_proj"))
+    steps, plain, base = engine_of(gf.model_dir("a"), "float32", slots=1), engine_of(merged, "float32"), engine_of(gf.model_dir("a"), "float32")
+    steps.put_adapter(0, *read_adapter(folder))
+    text = tc.random_tokens(30, 256, 5)
+    for engine in (steps, plain, base):
+        for r in range(2):
+            engine.open(r)
+    a = steps.step([StepEntry(0, text, [29], adapter=0), StepEntry(1, text, [29])]).cpu().numpy().copy()
+    b = plain.step([StepEntry(0, text, [29])]).cpu().numpy()[0].copy()
+    c = base.step([StepEntry(0, text, [29]), StepEntry(1, text, [29])]).cpu().numpy()[0].copy()
+    assert np.abs(a[0] - b).max() <= 2e-4 * np.abs(b).max() and np.abs(a[1] - c).max() <= 2e-5 * np.abs(c).max() and np.abs(a[0] - c).max() > 1e-2
+    # a step in which no request has one runs as an engine without adapters runs it, to the bit
+    d = steps.step([StepEntry(1, text[:3], [2])]).cpu().numpy().copy()
+    e = base.step([StepEntry(1, text[:3], [2])]).cpu().numpy().copy()
+    assert np.array_equal(d, e)
+    steps.adapter_sets[0]["w_qkv"].clear(0)
+    steps.adapter_sets[1]["w_gate_up"].clear(0)
+    steps.truncate(0, 0)
+    f = steps.step([StepEntry(0, text, [29], adapter=0)]).cpu().numpy()[0]
+    assert np.abs(f - c).max() <= 2e-5 * np.abs(c).max()
+
+
+def test_adapters_through_generate_and_their_refusals(tmp_path):
+    from geneinfer_b200 import Engine
+    from geneinfer_b200.engine.step import StepEntry
+    folder, merged = adapter_and_merged("a", 4, tmp_path)
+    engine = Engine(gf.model_dir("a"), dtype="float32", max_running=3, adapter_slots=2, adapter_rank=6)
+    engine.load_adapter(1, folder)
+    alone, base = Engine(merged, dtype="float32", max_running=3), Engine(gf.model_dir("a"), dtype="float32", max_running=3)
+    shared = tc.random_tokens(40, 256, 7)                     # a prefix of whole pages that must not be shared between adapters
+    prompts = [shared + [1], shared + [2], shared + [3]]
+    got = engine.generate(prompts, max_new_tokens=10, adapters=[1, -1, 1])
+    again = engine.generate(prompts, max_new_tokens=10, adapters=[-1, 1, -1])
+    want, plain = alone.generate(prompts, max_new_tokens=10), base.generate(prompts, max_new_tokens=10)
+    assert got[0] == want[0] and got[1] == plain[1] and got[2] == want[2]
+    assert again[0] == plain[0] and again[1] == want[1] and again[2] == plain[2]
+    assert want != plain
+    with pytest.raises(ValueError):
+        engine.submit([1, 2], adapter=2)
+    with pytest.raises(ValueError):
+        base.submit([1, 2], adapter=0)
+    engine.steps.open("x")
+    with pytest.raises(ValueError):
+        engine.steps.step([StepEntry("x", [1], [], adapter=2)])
+    with pytest.raises(RuntimeError):
+        engine.steps.enable_adapters(1, 4)
+    sets = engine.steps.adapter_sets[0]["w_qkv"]
+    for bad in ([None], [(torch.zeros(7, 64), torch.zeros(64, 7)), None, None], [(torch.zeros(4, 63), torch.zeros(64, 4)), None, None],
+                [(torch.zeros(4, 64), torch.zeros(64, 5)), None, None]):
+        if bad[0] is not None and bad[0][0].shape[0] == 7:
+            bad = [(torch.zeros(sets.rank + 1, 64), torch.zeros(64, sets.rank + 1)), None, None]
+        with pytest.raises(ValueError):
+            sets.put(0, bad, 1.0)
+    with pytest.raises(ValueError):
+        sets.put(2, [None, None, None], 1.0)
+    with pytest.raises(ValueError):
+        engine.steps.put_adapter(0, {(0, "w_other"): [None]}, 1.0)
+    with open(os.path.join(folder, "adapter_config.json"), "w") as f:
+        json.dump({"r": 6, "use_dora": True}, f)
+    with pytest.raises(ValueError):
+        engine.load_adapter(0, folder)
+
+
+# ---- drafted tokens
+def speculative(case, draft, dtype, **options):
+    from geneinfer_b200 import SpeculativeEngine
+    options = {"drafts": 4, "max_running": 3, "max_seq_len": 100, "step_tokens": 48, **options}
+    return SpeculativeEngine(gf.model_dir(case), gf.model_dir(draft) if draft in gf.CASES else draft, dtype=dtype, **options)
+
+
+@pytest.mark.parametrize("draft", ["a", "a_named"])
+@pytest.mark.parametrize("drafts", [1, 4])
+def test_greedy_generation_with_drafts_is_the_targets(draft, drafts):
+    """32 bits, where the target's logits do not depend on how positions are cut into steps: token for token what the engine gives alone. The target as its
+    own drafter proposes nothing that is refused."""
+    from geneinfer_b200 import Engine
+    prompts = [tc.random_tokens(n, 256, 40 + n) for n in (7, 1, 33, 60, 2)]
+    want = Engine(gf.model_dir("a"), dtype="float32", max_running=3).generate(prompts, max_new_tokens=21)
+    engine = speculative("a", draft, "float32", drafts=drafts)
+    assert engine.generate(prompts, max_new_tokens=21) == want
+    if draft == "a":
+        assert engine.kept == engine.proposed > 0
+    # again, with a stop token that comes up
+    stop = want[0][5]
+    cut = [w[:w.index(stop) + 1] if stop in w else w for w in want]
+    assert engine.generate(prompts, max_new_tokens=21, stop_ids=[stop]) == cut
+    for side in (engine.target, engine.draft):                # pages: none lost, none twice
+        held = side.tables[side.tables >= 0].tolist()
+        assert sorted(held + side.free[:int(side.n_free)].tolist()) == list(range(side.free.numel()))
+
+
+def test_sampled_generation_with_the_target_as_drafter_keeps_every_draft():
+    """p = q to the bit: u q(x) < p(x) for every u below 1."""
+    engine = speculative("a", "a", "float32")
+    out = engine.generate([tc.random_tokens(9, 256, 3), tc.random_tokens(20, 256, 4)], max_new_tokens=20, temperature=[0.9, 1.3], seed=5)
+    assert engine.kept == engine.proposed and all(len(o) == 20 for o in out)
+    assert engine.generate([tc.random_tokens(9, 256, 3), tc.random_tokens(20, 256, 4)], max_new_tokens=20, temperature=[0.9, 1.3], seed=5) == out
+    assert engine.generate([tc.random_tokens(9, 256, 3), tc.random_tokens(20, 256, 4)], max_new_tokens=20, temperature=[0.9, 1.3], seed=6) != out
+
+
+def test_sampled_generation_with_drafts_is_distributed_as_the_target():
+    """600 requests of one prompt, the first two tokens: counts of the eight likeliest first tokens and of the likeliest second ones against the target's
+    probabilities, within five standard deviations."""
+    from geneinfer_b200.engine.loading import load_model
+    from geneinfer_b200.engine.step import StepEngine, StepEntry
+    prompt, n, T = tc.random_tokens(12, 256, 8), 600, 0.7
+    engine = speculative("a", "a_named", "float32", max_running=100, max_seq_len=40, drafts=3)
+    out = engine.generate([prompt] * n, max_new_tokens=2, temperature=T, seed=1000)
+    steps = StepEngine(load_model(gf.model_dir("a"), dtype="float32"), n_pages=32, max_requests=1)
+    steps.open(0)
+    p = torch.softmax(steps.step([StepEntry(0, prompt, [11])])[0].double().cpu() / T, 0)
+    counts = torch.bincount(torch.tensor([o[0] for o in out]), minlength=256).double()
+    top = p.argsort(descending=True)[:8]
+    assert bool(((counts[top] - n * p[top]).abs() <= 5 * (n * p[top] * (1 - p[top])).sqrt()).all())
+    first = int(counts.argmax())
+    second = [o[1] for o in out if o[0] == first]
+    p2 = torch.softmax(steps.step([StepEntry(0, [first], [0])])[0].double().cpu() / T, 0)
+    best = int(p2.argmax())
+    m, share = len(second), float(p2[best])
+    assert abs(sum(t == best for t in second) - m * share) <= 5 * (m * share * (1 - share)) ** 0.5 + 1
+    assert 0 < engine.kept < engine.proposed
+
+
+def test_drafts_and_adapters_together(tmp_path):
+    """Every operator at once: requests with and without an adapter, drafts of the plain model, block tables on the device."""
+    from geneinfer_b200 import Engine
+    folder, merged = adapter_and_merged("a", 6, tmp_path)
+    prompts = [tc.random_tokens(n, 256, 70 + n) for n in (5, 31, 18)]
+    engine = speculative("a", "a", "float32", adapter_slots=1, adapter_rank=8)
+    engine.load_adapter(0, folder)
+    got = engine.generate(prompts, max_new_tokens=16, adapters=[0, -1, 0])
+    want = Engine(merged, dtype="float32").generate(prompts, max_new_tokens=16)
+    base = Engine(gf.model_dir("a"), dtype="float32").generate(prompts, max_new_tokens=16)
+    assert got == [want[0], base[1], want[2]]
+    assert 0 < engine.kept < engine.proposed
+
+
+@pytest.mark.parametrize("case", ["c", "d"])
+def test_drafts_in_bfloat16(case):
+    """The tensor-core kernels with rows of several tokens a request: against the engine alone up to the first near-tie."""
+    from geneinfer_b200 import Engine
+    vocab = gf.CASES[case][0]["vocab_size"]
+    prompts = [tc.random_tokens(n, vocab, 90 + n) for n in (17, 40)]
+    want = Engine(gf.model_dir(case), dtype="bfloat16", max_running=2).generate(prompts, max_new_tokens=24)
+    engine = speculative(case, case, "bfloat16", max_running=2)
+    got = engine.generate(prompts, max_new_tokens=24)
+    same = [next((i for i, (a, b) in enumerate(zip(g, w)) if a != b), len(w)) for g, w in zip(got, want)]
+    assert all(len(g) == 24 for g in got) and sum(same) >= 24 and engine.kept > engine.proposed / 2
+
+
+def test_speculative_refuses_what_does_not_fit():
+    from geneinfer_b200 import SpeculativeEngine
+    with pytest.raises(ValueError):
+        SpeculativeEngine(gf.model_dir("a"), gf.model_dir("b"), dtype="float32")          # other vocabularies
+    with pytest.raises(ValueError):
+        speculative("a", "a", "float32", drafts=0)
+    engine = speculative("a", "a", "float32")
+    for arguments in (dict(prompts=[[]]), dict(prompts=[[256]]), dict(prompts=[[1] * 90], max_new_tokens=30), dict(prompts=[[1]], temperature=-1.0),
+                      dict(prompts=[[1], [2]], temperature=[0.5]), dict(prompts=[[1]], adapters=[0])):
+        with pytest.raises(ValueError):
+            engine.generate(**arguments)
+    assert engine.generate([[1, 2]], max_new_tokens=0) == [[]]
