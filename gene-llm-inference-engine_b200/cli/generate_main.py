@@ -17,10 +17,14 @@ USAGE = (
     "                   [--weights native|f32 | --dtype bf16|fp32] [--device cuda] [--profile] [--temperature F]\n"
     "                   [--top-k N] [--top-p F] [--seed N] [--stop-ids \"2 7\"] [--page-size N] [--kv-pages N]\n"
     "                   [--no-echo] [--quiet] [--dump-tokens FILE] [--random-weights SEED --config FILE]\n"
+    "                   [--adapter DIR] [--draft-model DIR [--drafts N]]\n"
     "  DIR holds config.json and model.safetensors. --steps is the maximum number of positions including the\n"
     "  prompt (default: the context length). --weights f32 (= --dtype fp32) runs the whole model in true 32-bit.\n"
     "  --random-weights SEED --config FILE first writes such a folder (random bfloat16 weights from the seed, for the\n"
-    "  configuration in FILE, a config.json) to DIR, or to a temporary folder when no --model is given.\n")
+    "  configuration in FILE, a config.json) to DIR, or to a temporary folder when no --model is given.\n"
+    "  --adapter DIR: a low-rank adapter (adapter_config.json, adapter_model.safetensors) beside the model's weights.\n"
+    "  --draft-model DIR: a model of the same vocabulary proposes N tokens a step (default 4), which the model checks;\n"
+    "  the result is distributed as without it. Top-k and top-p are then off.\n")
 
 
 class UsageError(Exception):
@@ -50,9 +54,9 @@ def _ids(flag: str, text: str) -> List[int]:
 
 def parse(argv: List[str]) -> dict:
     o = {"model": "", "prompt_ids": None, "steps": 0, "max_seq_len": 0, "weights": "native", "device": "cuda",
-         "profile": False, "temperature": 0.8, "top_k": 0, "top_p": 0.9, "seed": None, "stop_ids": [],
+         "profile": False, "temperature": 0.8, "top_k": None, "top_p": None, "seed": None, "stop_ids": [],
          "page_size": 16, "kv_pages": None, "echo": True, "quiet": False, "dump_tokens": "", "random_weights": None,
-         "config": "", "help": False}
+         "config": "", "help": False, "adapter": "", "draft_model": "", "drafts": 4}
     i = 0
     while i < len(argv):
         flag = argv[i]
@@ -102,6 +106,9 @@ def parse(argv: List[str]) -> dict:
         elif flag == "--no-echo": o["echo"] = False
         elif flag == "--quiet": o["quiet"] = True
         elif flag == "--dump-tokens": o["dump_tokens"] = value()
+        elif flag == "--adapter": o["adapter"] = value()
+        elif flag == "--draft-model": o["draft_model"] = value()
+        elif flag == "--drafts": o["drafts"] = _int(flag, value())
         else:
             raise UsageError(f"unknown option {flag}")
         i += 1
@@ -117,9 +124,53 @@ def parse(argv: List[str]) -> dict:
         raise UsageError("--weights must be native or f32 (int8 is not built)")
     if not o["device"].startswith("cuda"):
         raise UsageError("--device must be cuda: this engine has no CPU or emulated device")
+    if o["draft_model"] and (o["top_k"] or (o["top_p"] is not None and o["top_p"] < 1.0)):
+        raise UsageError("--draft-model cannot be combined with --top-k or --top-p")
+    if o["draft_model"] and o["drafts"] < 1:
+        raise UsageError("--drafts must be positive")
+    if o["top_k"] is None:
+        o["top_k"] = 0
+    if o["top_p"] is None:
+        o["top_p"] = 1.0 if o["draft_model"] else 0.9
     if o["seed"] is None:
         o["seed"] = time.time_ns() & ((1 << 63) - 1)
     return o
+
+
+def _adapter_rank(folder: str) -> int:
+    import json
+    import os
+    with open(os.path.join(folder, "adapter_config.json")) as f:
+        return int(json.load(f)["r"])
+
+
+def _with_drafts(o: dict, device: str) -> int:
+    """The generation with a draft model: the whole result at once."""
+    from ..engine.speculative import SpeculativeEngine
+    from ..weights import read_config
+    prompt = o["prompt_ids"]
+    context = o["max_seq_len"] or read_config(o["model"])[1].max_position_embeddings
+    positions = min(o["steps"], context) if o["steps"] > 0 else context
+    rank = _adapter_rank(o["adapter"]) if o["adapter"] else 0
+    # (a request's own positions, and those that a refused round may touch)
+    engine = SpeculativeEngine(o["model"], o["draft_model"], drafts=o["drafts"], dtype="float32" if o["weights"] == "f32" else "bfloat16", device=device,
+                               max_running=1, max_seq_len=positions + 1, page_size=o["page_size"], adapter_slots=1 if rank else 0, adapter_rank=rank or 16)
+    if rank:
+        engine.load_adapter(0, o["adapter"])
+    new = min(positions, engine.context - 1) - len(prompt) + 1
+    if new < 1:
+        raise ValueError(f"a prompt of {len(prompt)} tokens does not fit in {positions} positions")
+    t0 = time.perf_counter()
+    out = engine.generate([prompt], new, o["temperature"], o["seed"], o["stop_ids"], [0] if rank else None)[0]
+    seconds = time.perf_counter() - t0
+    sys.stdout.write((" ".join(map(str, prompt)) + " | " if o["echo"] else " ") + " ".join(map(str, out)) + "\n")
+    if o["dump_tokens"]:
+        with open(o["dump_tokens"], "w") as f:
+            f.write(" ".join(map(str, prompt)) + "\n" + " ".join(map(str, out)) + "\n")
+    if not o["quiet"]:
+        sys.stderr.write(f"[stats] prompt {len(prompt)} tokens and {len(out)} generated in {seconds * 1e3:.1f} ms | {engine.rounds} rounds, "
+                         f"{engine.kept} of {engine.proposed} drafts kept | seed {o['seed']}\n")
+    return 0
 
 
 def main(argv: Optional[List[str]] = None) -> int:
@@ -159,10 +210,15 @@ def main(argv: Optional[List[str]] = None) -> int:
             sys.stderr.write(f"error: {e}\n")
             return 2
         device = o["device"] if ":" in o["device"] else "cuda:0"
+        if o["draft_model"]:
+            return _with_drafts(o, device)
         t0 = time.perf_counter()
+        rank = _adapter_rank(o["adapter"]) if o["adapter"] else 0
         engine = Engine(o["model"], dtype="float32" if o["weights"] == "f32" else "bfloat16", device=device,
                         max_seq_len=o["max_seq_len"] or None, page_size=o["page_size"], kv_pages=o["kv_pages"],
-                        max_running=1, prefix_cache=False)
+                        max_running=1, prefix_cache=False, adapter_slots=1 if rank else 0, adapter_rank=rank or 16)
+        if rank:
+            engine.load_adapter(0, o["adapter"])
         load_s = time.perf_counter() - t0
         prompt = o["prompt_ids"]
         if o["echo"]:
@@ -174,7 +230,7 @@ def main(argv: Optional[List[str]] = None) -> int:
             sys.stdout.flush()
 
         times = {}
-        rid = engine.submit(prompt, o["steps"], params, o["stop_ids"], on_token)
+        rid = engine.submit(prompt, o["steps"], params, o["stop_ids"], on_token, adapter=0 if rank else -1)
         torch.cuda.synchronize()
         t0 = time.perf_counter()
         while engine.step():

@@ -114,16 +114,17 @@ struct AdapterArgs {
     PlanView plan;
     void* out;
     long long ldo;
-    int A, K, N, r, S, tile_rows;              // tile_rows 0: no plan, plan.p are the rows' adapters
+    int A, used, K, N, r, S, tile_rows;        // used: adapters that occur at most; tile_rows 0: no plan, plan.p are the rows' adapters
     int ends[kAdapterSlicesMost];              // a slice's last column + 1
     int wide;                                  // eight neighbouring columns from a multiple of eight on lie on 16 bytes in every row of out
 };
 
 constexpr int kAdapterThreads = 256, kAdapterWarps = kAdapterThreads / 32;
-constexpr int kDirectRows = kAdapterThreads;   // steps of up to so many rows have no plan: a tile's block looks its rows up itself
-constexpr int kDirectTile = 16, kDirectAdapters = 1024;       // (of so many adapters)
+constexpr int kDirectRows = 2048, kDirectEach = kDirectRows / kAdapterThreads;      // steps of up to so many rows have no plan: a tile's blocks look its rows up themselves
+constexpr int kDirectAdapters = 1024;          // (of so many adapters)
+constexpr int kFewTokens = 256;                // rows up to which they are taken for single tokens, each with an adapter of its own as a rule
 
-// The rows of the block's tile (or of the `M` rows from `piece` on of a plan's tile) into rows[0 .. M); false: there are none.
+// The rows of tile `which` of `M` rows (with a plan: of the `M` rows from `piece` on of a plan's tile) into rows[0 .. M); false: there are none.
 template <int M>
 __device__ __forceinline__ bool find_rows(const PlanView& plan, int A, int tile_rows, int which, int* rows, int& adapter, int& n, int* scratch) {
     if (tile_rows == 0) {
@@ -131,17 +132,28 @@ __device__ __forceinline__ bool find_rows(const PlanView& plan, int A, int tile_
         __shared__ int s_counts[kDirectAdapters], s_adapter, s_tile;
         constexpr int kEach = kDirectAdapters / kAdapterThreads;
         const int i = threadIdx.x, lane = i & 31, warp = i >> 5;
-        const int mine = i < plan.T ? plan.p[i] : -1;
+        int mine[kDirectEach];
+#pragma unroll
+        for (int e = 0; e < kDirectEach; ++e) mine[e] = i + e * kAdapterThreads < plan.T ? plan.p[i + e * kAdapterThreads] : -1;
 #pragma unroll
         for (int k = 0; k < kEach; ++k) s_counts[i + k * kAdapterThreads] = 0;
-        if (i < M) rows[i] = -1;
+        for (int k = i; k < M; k += kAdapterThreads) rows[k] = -1;
         if (i == 0) s_adapter = -1;
         __syncthreads();
-        if (mine >= 0 && mine < A) atomicAdd(&s_counts[mine], 1);
+#pragma unroll
+        for (int e = 0; e < kDirectEach; ++e) {
+            if (e * kAdapterThreads >= plan.T) break;
+            const bool valid = mine[e] >= 0 && mine[e] < A;
+            if (__all_sync(0xffffffffu, mine[e] == __shfl_sync(0xffffffffu, mine[e], 0))) {      // (a prompt's rows)
+                if (valid && lane == 0) atomicAdd(&s_counts[mine[e]], 32);
+            } else if (valid) {
+                atomicAdd(&s_counts[mine[e]], 1);
+            }
+        }
         __syncthreads();
         int tiles[kEach], sum = 0;
 #pragma unroll
-        for (int k = 0; k < kEach; ++k) { tiles[k] = (s_counts[i * kEach + k] + kDirectTile - 1) / kDirectTile; sum += tiles[k]; }
+        for (int k = 0; k < kEach; ++k) { tiles[k] = (s_counts[i * kEach + k] + M - 1) / M; sum += tiles[k]; }
         int run = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -160,23 +172,36 @@ __device__ __forceinline__ bool find_rows(const PlanView& plan, int A, int tile_
         __syncthreads();
         adapter = s_adapter;
         if (adapter < 0) return false;
-        const unsigned same = __ballot_sync(0xffffffffu, mine == adapter);
-        if (lane == 0) scratch[warp] = __popc(same);
+        const int first = s_tile * M;
+        n = min(M, s_counts[adapter] - first);
+        __syncthreads();                       // the scratch is free again
+#pragma unroll
+        for (int e = 0; e < kDirectEach; ++e) {
+            const unsigned same = __ballot_sync(0xffffffffu, mine[e] == adapter);
+            if (lane == 0) scratch[e * kAdapterWarps + warp] = __popc(same);
+        }
         __syncthreads();
-        int place = __popc(same & ((1u << lane) - 1)) - s_tile * kDirectTile;
-        for (int w = 0; w < warp; ++w) place += scratch[w];
-        const bool in = mine == adapter && place >= 0 && place < kDirectTile;
-        if (in) rows[place] = i;
-        n = __syncthreads_count(in);
+        int before = 0;                        // the adapter's rows ahead, in the order (turn, warp, lane)
+#pragma unroll
+        for (int e = 0; e < kDirectEach; ++e) {
+            if (e * kAdapterThreads >= plan.T) break;
+            for (int w = 0; w < kAdapterWarps; ++w) {
+                if (w == warp) {
+                    const unsigned same = __ballot_sync(0xffffffffu, mine[e] == adapter);
+                    const int place = before + __popc(same & ((1u << lane) - 1)) - first;
+                    if (mine[e] == adapter && place >= 0 && place < M) rows[place] = i + e * kAdapterThreads;
+                }
+                before += scratch[e * kAdapterWarps + w];
+            }
+        }
     } else {
         const int per_tile = (tile_rows + M - 1) / M, tile = which / per_tile, piece = which % per_tile;
-        const int* info = plan.tile(tile);     // (there, if not written, for every tile of the launch)
-        const int of = info[0], first = info[1], all = info[2];
         if (tile >= plan.tiles()) return false;
-        adapter = of;
-        n = min(M, all - piece * M);
-        if (n <= 0) return false;
-        for (int i = threadIdx.x; i < M; i += kAdapterThreads) rows[i] = i < n ? plan.rows()[first + piece * M + i] : -1;
+        const int* info = plan.tile(tile);
+        adapter = info[0];
+        n = min(M, info[2] - piece * M);
+        if (n <= 0) return false;              // (the plan's tile ends ahead of this piece of it)
+        for (int i = threadIdx.x; i < M; i += kAdapterThreads) rows[i] = i < n ? plan.rows()[info[1] + piece * M + i] : -1;
     }
     __syncthreads();
     return true;
@@ -190,7 +215,7 @@ __global__ void __launch_bounds__(kPlainThreads) adapter_plain_kernel(AdapterArg
     pdl_prologue();
     extern __shared__ float h[];               // [2][kPlainRows][S r]: this CTA's partial sums, then the whole sums
     __shared__ float xs[kPlainRows][kPlainK + 1], ds[kPlainCols][kPlainK + 1];
-    __shared__ int s_rows[kPlainRows], s_scratch[kAdapterWarps];
+    __shared__ int s_rows[kPlainRows], s_scratch[kDirectEach * kAdapterWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int part = cluster.block_rank(), parts = cluster.num_blocks();
     int adapter, rows;
@@ -447,7 +472,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_few_kernel(Adapter
     pdl_prologue();
     extern __shared__ __align__(16) float h[]; // [kFewRows][S r], then the pieces
     __shared__ float2 sums[kAdapterWarps][kFewRows][kFewCols / 2 + 4];
-    __shared__ int s_rows[kFewRows], s_scratch[kAdapterWarps];
+    __shared__ int s_rows[kFewRows], s_scratch[kDirectEach * kAdapterWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int part = cluster.block_rank(), parts = cluster.num_blocks();
     int adapter, n;
@@ -560,7 +585,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_many_kernel(Adapte
     using Shape = ManyShape<M, kOnePass>;
     constexpr int kTiles = Shape::kTiles;
     extern __shared__ __align__(128) unsigned char ring[];
-    __shared__ int s_rows[M], s_scratch[kAdapterWarps];
+    __shared__ int s_rows[M], s_scratch[kDirectEach * kAdapterWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int part = cluster.block_rank(), parts = cluster.num_blocks();
     int adapter, n;
@@ -736,7 +761,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(Adapt
     using Shape = FloatShape<kRows>;
     constexpr int M = Shape::kTile;
     extern __shared__ __align__(128) unsigned char ring[];
-    __shared__ int s_rows[M], s_scratch[kAdapterWarps];
+    __shared__ int s_rows[M], s_scratch[kDirectEach * kAdapterWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int part = cluster.block_rank(), parts = cluster.num_blocks();
     int adapter, n;
@@ -848,9 +873,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(Adapt
     // a column a thread, half of the rows a warp
     constexpr int kHalf = M / 2;
     const int row0 = (threadIdx.x >> 7) * kHalf;
-    if (row0 >= n) return;
     float* out = static_cast<float*>(a.out);
-    const int n_share = (a.N + parts - 1) / parts, n_begin = min(a.N, part * n_share), n_end = min(a.N, n_begin + n_share);
+    const int n_share = (a.N + parts - 1) / parts, n_begin = min(a.N, part * n_share), n_end = row0 < n ? min(a.N, n_begin + n_share) : 0;
     for (int col = n_begin + (threadIdx.x & 127); col < n_end; col += 128) {
         int slice = 0;
 #pragma unroll
@@ -893,13 +917,15 @@ inline void launch_tile_clusters(void (*kernel)(KArgs...), long long tiles, int 
     counted(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
 }
 
-// The clusters of a launch, and how many of them will have rows as a rule: every adapter could leave a tile that is not full, in large steps few do.
-struct TileCount { long long all, busy; };
-inline TileCount tile_count(const AdapterArgs& a, long long tiles, int rows) {
-    if (a.tile_rows == 0) return {tiles, tiles};
-    return {tiles * ((a.tile_rows + rows - 1) / rows), (a.plan.T + rows - 1) / rows};
+// The tiles that a launch may have, and how many there are as a rule: every adapter could leave a tile that is not full, in large steps few do.
+struct TileCount { long long most, busy; };
+inline TileCount tile_count(const AdapterArgs& a, int rows) {
+    const long long adapters = a.used < a.plan.T ? a.used : a.plan.T, full = (a.plan.T + rows - 1) / rows;
+    if (a.tile_rows) return {(a.plan.T / a.tile_rows + adapters) * ((a.tile_rows + rows - 1) / rows), full};
+    const long long most = a.plan.T / rows + adapters;
+    return {most, a.plan.T <= kFewTokens ? most : full};
 }
-// CTAs of a cluster: as many as two a multiprocessor have room for.
+// CTAs of a cluster: as many as two a multiprocessor have room for (`slack`: twice as many).
 inline int cluster_parts(long long tiles, int slack) {
     int parts = 1;
     while (parts < kAdapterClusterMost && 2 * parts * tiles <= 2LL * sm_count() * slack) parts *= 2;
@@ -907,17 +933,19 @@ inline int cluster_parts(long long tiles, int slack) {
 }
 
 template <typename Kernel>
-int launch_adapter(Kernel kernel, SharedLimit& limit, const AdapterArgs& a, TileCount tiles, size_t smem, size_t most, cudaStream_t st) {
+int launch_adapter(Kernel kernel, SharedLimit& limit, const AdapterArgs& a, int rows, size_t smem, size_t most, cudaStream_t st) {
     const cudaError_t e = limit.allow(reinterpret_cast<const void*>(kernel), static_cast<int>(most));
     GI_REQUIRE(e == cudaSuccess, "adapter_product: %s", cudaGetErrorString(e));
-    launch_tile_clusters(kernel, tiles.all, cluster_parts(tiles.busy, a.tile_rows ? 1 : 2), kAdapterThreads, smem, st, a);
+    const TileCount tiles = tile_count(a, rows);
+    const int parts = cluster_parts(tiles.busy, a.plan.T <= kFewTokens ? 2 : 1);
+    launch_tile_clusters(kernel, tiles.most, parts, kAdapterThreads, smem, st, a);
     return check_launch("adapter_product");
 }
 
 template <typename T, typename TO>
-int launch_plain(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+int launch_plain(const AdapterArgs& a, cudaStream_t st) {
     static SharedLimit limit;
-    return launch_adapter(&adapter_plain_kernel<T, TO>, limit, a, tile_count(a, tiles, kPlainRows), 2ull * kPlainRows * a.S * a.r * sizeof(float),
+    return launch_adapter(&adapter_plain_kernel<T, TO>, limit, a, kPlainRows, 2ull * kPlainRows * a.S * a.r * sizeof(float),
                           2ull * kPlainRows * kAdapterRanksMost * sizeof(float), st);
 }
 
@@ -928,57 +956,57 @@ inline size_t sums_bytes(const AdapterArgs& a, int rows) { return 4ull * rows * 
 template <typename Shape> constexpr size_t ring_bytes() { return static_cast<size_t>(Shape::kStages) * Shape::kStageBytes; }
 
 template <int kSteps, typename TO>
-int launch_few(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+int launch_few(const AdapterArgs& a, cudaStream_t st) {
     static SharedLimit limit;
-    return launch_adapter(&adapter_few_kernel<kSteps, TO>, limit, a, tile_count(a, tiles, kFewRows), 4ull * kFewRows * a.S * a.r + pieces_bytes<TO>(a, kFewRows),
+    return launch_adapter(&adapter_few_kernel<kSteps, TO>, limit, a, kFewRows, 4ull * kFewRows * a.S * a.r + pieces_bytes<TO>(a, kFewRows),
                           150 * 1024, st);
 }
 
 template <int M, bool kOnePass, int kSteps, typename TO>
-int launch_many(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+int launch_many(const AdapterArgs& a, cudaStream_t st) {
     static SharedLimit limit;
     const size_t ring = ring_bytes<ManyShape<M, kOnePass>>();
-    return launch_adapter(&adapter_many_kernel<M, kOnePass, kSteps, TO>, limit, a, tile_count(a, tiles, M), kOnePass ? ring : ring + sums_bytes(a, M),
+    return launch_adapter(&adapter_many_kernel<M, kOnePass, kSteps, TO>, limit, a, M, kOnePass ? ring : ring + sums_bytes(a, M),
                           210 * 1024, st);
 }
 
 template <int kRows>
-int launch_float(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+int launch_float(const AdapterArgs& a, cudaStream_t st) {
     static SharedLimit limit;
     using Shape = FloatShape<kRows>;
-    return launch_adapter(&adapter_float_kernel<kRows>, limit, a, tile_count(a, tiles, Shape::kTile),
+    return launch_adapter(&adapter_float_kernel<kRows>, limit, a, Shape::kTile,
                           ring_bytes<Shape>() + 4ull * Shape::kTile * (a.S * a.r + 4), 160 * 1024, st);
 }
 
-int launch_f32(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+int launch_f32(const AdapterArgs& a, cudaStream_t st) {
     const bool pieces = a.K % 4 == 0 && a.ldx % 4 == 0 && a.r % 4 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
                         reinterpret_cast<uintptr_t>(a.down) % 16 == 0 && reinterpret_cast<uintptr_t>(a.up) % 16 == 0;
-    if (!pieces) return launch_plain<float, float>(a, tiles, st);
+    if (!pieces) return launch_plain<float, float>(a, st);
     // (2,048 rows of 14,336 into 4,096 at rank 64: tiles of 64 rows 215 us, of 32 263 us; 1,024 rows of 2,048 at rank 16: 27 and 22 us)
-    if (a.tile_rows && a.plan.T >= 2048 && a.S * a.r <= 256) return launch_float<4>(a, tiles, st);
-    return launch_float<2>(a, tiles, st);
+    if (a.plan.T >= 2048 && a.S * a.r <= 256) return launch_float<4>(a, st);
+    return launch_float<2>(a, st);
 }
 
 template <int kSteps, typename TO>
-int launch_steps(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+int launch_steps(const AdapterArgs& a, cudaStream_t st) {
     using Wide = ManyShape<128, true>;
     using Tall = ManyShape<64, true>;
     using Passes = ManyShape<64, false>;
-    if (a.tile_rows == 0) return launch_few<kSteps, TO>(a, tiles, st);
+    if (a.plan.T <= kFewTokens) return launch_few<kSteps, TO>(a, st);
     const bool one = a.S * a.r <= kManyCols;
-    if (one && a.plan.T >= 4096 && sums_bytes(a, 128) + pieces_bytes<TO>(a, 128) <= ring_bytes<Wide>()) return launch_many<128, true, kSteps, TO>(a, tiles, st);
-    if (one && sums_bytes(a, 64) + pieces_bytes<TO>(a, 64) <= ring_bytes<Tall>()) return launch_many<64, true, kSteps, TO>(a, tiles, st);
-    if (pieces_bytes<TO>(a, 64) <= ring_bytes<Passes>()) return launch_many<64, false, kSteps, TO>(a, tiles, st);
-    return launch_few<kSteps, TO>(a, tiles, st);
+    if (one && a.plan.T >= 4096 && sums_bytes(a, 128) + pieces_bytes<TO>(a, 128) <= ring_bytes<Wide>()) return launch_many<128, true, kSteps, TO>(a, st);
+    if (one && sums_bytes(a, 64) + pieces_bytes<TO>(a, 64) <= ring_bytes<Tall>()) return launch_many<64, true, kSteps, TO>(a, st);
+    if (pieces_bytes<TO>(a, 64) <= ring_bytes<Passes>()) return launch_many<64, false, kSteps, TO>(a, st);
+    return launch_few<kSteps, TO>(a, st);
 }
 
 template <typename TO>
-int launch_bf16(const AdapterArgs& a, long long tiles, cudaStream_t st) {
+int launch_bf16(const AdapterArgs& a, cudaStream_t st) {
     // 16-byte pieces of x and `down`, 8-byte ones of `up`
     const bool pieces = a.K % 8 == 0 && a.ldx % 8 == 0 && a.r % 4 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
                         reinterpret_cast<uintptr_t>(a.down) % 16 == 0 && reinterpret_cast<uintptr_t>(a.up) % 8 == 0;
-    if (!pieces) return launch_plain<__nv_bfloat16, TO>(a, tiles, st);
-    return a.r <= 16 ? launch_steps<1, TO>(a, tiles, st) : a.r <= 32 ? launch_steps<2, TO>(a, tiles, st) : launch_steps<4, TO>(a, tiles, st);
+    if (!pieces) return launch_plain<__nv_bfloat16, TO>(a, st);
+    return a.r <= 16 ? launch_steps<1, TO>(a, st) : a.r <= 32 ? launch_steps<2, TO>(a, st) : launch_steps<4, TO>(a, st);
 }
 
 }  // namespace gi
@@ -996,30 +1024,28 @@ static int gi_adapter_plan_impl(const int* row_adapter, int T, int A, int tile_r
 }
 
 // x [T, K] with ldx values between rows; down [A, S r, K]; up [A, N, r]; out [T, N] with ldo values between rows; end0 ..: the slices' last columns + 1.
-// tile_rows > 0: plan is adapter_plan's, tiles the most it can have; 0 (up to gi_adapter_direct_rows() rows): plan is row_adapter [T] itself, tiles
-// the most that its rows can make in tiles of 16.
+// used: so many adapters occur at most. tile_rows > 0: plan is adapter_plan's; 0 (up to gi_adapter_direct_rows() rows): plan is row_adapter [T] itself.
 static int gi_adapter_product_impl(const void* x, long long ldx, int dtype, const void* down, const void* up, const float* scales, const int* plan, int T,
-                                   int A, int tile_rows, int tiles, void* out, long long ldo, int out_dtype, int K, int N, int r, int S, int end0, int end1,
+                                   int A, int used, int tile_rows, void* out, long long ldo, int out_dtype, int K, int N, int r, int S, int end0, int end1,
                                    int end2, int end3, void* stream) {
-    if (T == 0 || tiles == 0) return 0;
-    GI_REQUIRE(T > 0 && A > 0 && K > 0 && N > 0 && r > 0 && tile_rows >= 0 && tiles > 0, "adapter_product: sizes must be positive (T=%d, adapters=%d, K=%d, N=%d, rank=%d)",
+    if (T == 0) return 0;
+    GI_REQUIRE(T > 0 && A > 0 && used > 0 && K > 0 && N > 0 && r > 0 && tile_rows >= 0, "adapter_product: sizes must be positive (T=%d, adapters=%d, K=%d, N=%d, rank=%d)",
                T, A, K, N, r);
     GI_REQUIRE(tile_rows > 0 || T <= gi_adapter_direct_rows(A), "adapter_product: %d rows need a plan", T);
     GI_REQUIRE(S >= 1 && S <= kAdapterSlicesMost, "adapter_product: %d slices (1 to %d)", S, kAdapterSlicesMost);
     GI_REQUIRE(static_cast<long long>(S) * r <= kAdapterRanksMost, "adapter_product: %d slices of rank %d exceed %d", S, r, kAdapterRanksMost);
-    AdapterArgs a = {x, ldx, down, up, scales, {plan, T}, out, ldo, A, K, N, r, S, tile_rows, {end0, end1, end2, end3}, 0};
+    AdapterArgs a = {x, ldx, down, up, scales, {plan, T}, out, ldo, A, used, K, N, r, S, tile_rows, {end0, end1, end2, end3}, 0};
     int before = 0;
     for (int s = 0; s < S; ++s) {
         GI_REQUIRE(a.ends[s] > before, "adapter_product: a slice without columns");
         before = a.ends[s];
     }
     GI_REQUIRE(before == N, "adapter_product: the slices have %d columns, the output %d", before, N);
-    GI_REQUIRE(static_cast<long long>(tiles) * (tile_rows + kDirectTile) <= INT_MAX / kAdapterClusterMost, "adapter_product: %d tiles exceed the grid limit", tiles);
     a.wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ldo * (out_dtype == kF32 ? 4 : 2) % 16 == 0;
     GI_REQUIRE(dtype == kBF16 || out_dtype == kF32, "adapter_product: 32-bit weights give 32-bit output");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == kF32) return launch_f32(a, tiles, st);
-    return out_dtype == kF32 ? launch_bf16<float>(a, tiles, st) : launch_bf16<__nv_bfloat16>(a, tiles, st);
+    if (dtype == kF32) return launch_f32(a, st);
+    return out_dtype == kF32 ? launch_bf16<float>(a, st) : launch_bf16<__nv_bfloat16>(a, st);
 }
 
 extern "C" int gi_adapter_plan(const int* row_adapter, int T, int A, int tile_rows, int* plan, void* stream) {
@@ -1027,8 +1053,8 @@ extern "C" int gi_adapter_plan(const int* row_adapter, int T, int A, int tile_ro
 }
 
 extern "C" int gi_adapter_product(const void* x, long long ldx, int dtype, const void* down, const void* up, const float* scales, const int* plan, int T,
-                                  int A, int tile_rows, int tiles, void* out, long long ldo, int out_dtype, int K, int N, int r, int S, int end0, int end1,
+                                  int A, int used, int tile_rows, void* out, long long ldo, int out_dtype, int K, int N, int r, int S, int end0, int end1,
                                   int end2, int end3, void* stream) {
-    return gi::dispatch(gi_adapter_product_impl, x, ldx, dtype, down, up, scales, plan, T, A, tile_rows, tiles, out, ldo, out_dtype, K, N, r, S, end0, end1,
+    return gi::dispatch(gi_adapter_product_impl, x, ldx, dtype, down, up, scales, plan, T, A, used, tile_rows, out, ldo, out_dtype, K, N, r, S, end0, end1,
                         end2, end3, stream);
 }

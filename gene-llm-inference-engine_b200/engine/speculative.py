@@ -118,7 +118,7 @@ class SpeculativeEngine:
         self._work = torch.empty(R * (K + 1), 4, dtype=torch.float32, device=dev)
         self._temperature = torch.zeros(R, dtype=torch.float32, device=dev)
         self._no_top_k, self._no_top_p = ints(R), torch.ones(R, dtype=torch.float32, device=dev)
-        self._adapters = ints(R) - 1
+        self._adapters, self._row_adapter = ints(R) - 1, ints(self.step_tokens)      # (one place for every step: recorded launches name it)
         # two rounds may be in flight: numbers on their way in, tokens on their way out
         n = R * (2 * K + 1)
         self._numbers_host = [torch.zeros(n).pin_memory() for _ in range(3)]
@@ -211,7 +211,10 @@ class SpeculativeEngine:
                     rows += [r] * take
             ids = torch.tensor(tokens, dtype=torch.int32).to(dev)
             self._counts.copy_(torch.tensor(counts, dtype=torch.int32))
-            row_adapter = self._adapters[torch.tensor(rows).to(dev)].contiguous() if adapted else None
+            row_adapter = None
+            if adapted:
+                row_adapter = self._row_adapter[:len(rows)]
+                row_adapter.copy_(self._adapters[torch.tensor(rows).to(dev)])
             self.target.forward(ids, counts, self._counts, self._lengths, fed, False, row_adapter)
             self.draft.forward(ids, counts, self._counts, self._lengths, fed, False)
             self._lengths += self._counts
@@ -245,7 +248,10 @@ class SpeculativeEngine:
         self._drafted.copy_(self._ids.t())
         self._fed[:, 0].copy_(self._current)
         self._fed[:, 1:].copy_(self._drafted)
-        row_adapter = self._adapters[:, None].expand(R, K + 1).reshape(-1).contiguous() if adapted else None
+        row_adapter = None
+        if adapted:
+            row_adapter = self._row_adapter[:R * (K + 1)]
+            row_adapter.view(R, K + 1).copy_(self._adapters[:, None].expand(R, K + 1))
         logits = self.target.forward(self._fed.view(-1), [K + 1] * R, self._rows, self._lengths, bounds, True, row_adapter)
         self._counts.fill_(K)
         kernels.verify_drafts(logits, self._starts, self._drafted, self._counts, self._probs.transpose(0, 1), self._temperature, accept, draw,

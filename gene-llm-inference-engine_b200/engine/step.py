@@ -112,7 +112,8 @@ class StepContext:
         if not eng.use_programs or eng.tap is not None:
             launch()
             return
-        full = (id(owner), key, self.row_adapter is not None)
+        # (with adapters the launches are also sized by how many different ones there can be: one a request)
+        full = (id(owner), key, 0 if self.row_adapter is None else self.n_requests)
         program = eng._programs.get(full)
         if program is None:
             with kernels.record() as rec:
@@ -409,7 +410,7 @@ class StepEngine:
 
     def _begin_adapters(self, ctx: "StepContext") -> None:
         if self.adapter_step is not None:
-            self.adapter_step.begin(ctx.row_adapter)
+            self.adapter_step.begin(ctx.row_adapter, ctx.n_requests)          # (a request has one)
 
     # ------------------------------------------------------------------ requests
     def open(self, key: Hashable) -> RequestCache:

@@ -23,9 +23,10 @@ class AdapterStep:
         self.plan: Optional[kernels.AdapterPlan] = None
         self._buffer = torch.empty(max(1, kernels.adapter_plan_size(max_rows, slots)), dtype=torch.int32, device=device)
 
-    def begin(self, row_adapter: Optional[torch.Tensor]) -> None:
-        """``row_adapter`` [rows] int32 on the device: every row's slot, or a negative number; None: no adapters in this step."""
-        self.plan = None if row_adapter is None else kernels.adapter_plan(row_adapter, self.slots, self._buffer)
+    def begin(self, row_adapter: Optional[torch.Tensor], used: Optional[int] = None) -> None:
+        """``row_adapter`` [rows] int32 on the device: every row's slot, or a negative number; None: no adapters in this step.
+        ``used``: so many different ones at most."""
+        self.plan = None if row_adapter is None else kernels.adapter_plan(row_adapter, self.slots, self._buffer, min(self.slots, used or self.slots))
 
 
 class AdapterSet:

@@ -1653,14 +1653,14 @@ def trim_tables(lengths: torch.Tensor, tables: torch.Tensor, held: torch.Tensor,
 class AdapterPlan:
     """The rows of a step in the order of their adapters (``adapter_plan``), for every ``adapter_product`` of the step."""
 
-    __slots__ = ("buffer", "rows", "adapters", "tile_rows", "tiles")
+    __slots__ = ("buffer", "rows", "adapters", "used", "tile_rows")
 
-    def __init__(self, buffer: torch.Tensor, rows: int, adapters: int, tile_rows: int, tiles: int):
-        self.buffer, self.rows, self.adapters, self.tile_rows, self.tiles = buffer, rows, adapters, tile_rows, tiles
+    def __init__(self, buffer: torch.Tensor, rows: int, adapters: int, used: int, tile_rows: int):
+        self.buffer, self.rows, self.adapters, self.used, self.tile_rows = buffer, rows, adapters, used, tile_rows
 
 
 ADAPTER_TILE_ROWS = 128
-ADAPTER_DIRECT_ROWS, ADAPTER_DIRECT_ADAPTERS = 256, 1024      # steps of up to so many rows (and adapters) need no plan on the device: the products look rows up themselves
+ADAPTER_DIRECT_ROWS, ADAPTER_DIRECT_ADAPTERS = 2048, 1024      # steps of up to so many rows (and adapters) need no plan on the device: the products look rows up themselves
 
 
 def adapter_plan_size(rows: int, adapters: int) -> int:
@@ -1668,23 +1668,27 @@ def adapter_plan_size(rows: int, adapters: int) -> int:
     return 1 + rows + 3 * (rows // ADAPTER_TILE_ROWS + min(adapters, rows))
 
 
-def adapter_plan(row_adapter: torch.Tensor, adapters: int, buffer: Optional[torch.Tensor] = None) -> AdapterPlan:
+def adapter_plan(row_adapter: torch.Tensor, adapters: int, buffer: Optional[torch.Tensor] = None, used: Optional[int] = None) -> AdapterPlan:
     """Puts the rows of a step in the order of their adapters: ``row_adapter`` [T] int32 on the device, an adapter's number or, for
     a row without one, anything outside 0 .. adapters - 1. ``buffer``: where to (``adapter_plan_size`` int32 values; new memory without it).
-    Once a step: every product of the step takes the same plan, which reads ``row_adapter`` when it runs."""
+    ``used``: so many different adapters occur at most (default: all), which bounds the blocks that find nothing to do where hundreds
+    are loaded. Once a step: every product of the step takes the same plan, which reads ``row_adapter`` when it runs."""
     T = row_adapter.numel()
     if not 1 <= adapters <= 8192:
         raise KernelError(f"adapter_plan: {adapters} adapters (1 to 8192)")
+    used = adapters if used is None else used
+    if not 1 <= used <= adapters:
+        raise KernelError(f"adapter_plan: {used} of {adapters} adapters used")
     rows = _dev(row_adapter, "row_adapter", torch.int32)
     if T <= ADAPTER_DIRECT_ROWS and adapters <= ADAPTER_DIRECT_ADAPTERS:
-        return AdapterPlan(row_adapter, T, int(adapters), 0, T // 16 + min(adapters, T))
+        return AdapterPlan(row_adapter, T, int(adapters), int(used), 0)
     tiles = T // ADAPTER_TILE_ROWS + min(adapters, T)
     if buffer is None:
         buffer = torch.empty(1 + T + 3 * tiles, dtype=torch.int32, device=row_adapter.device)
     elif buffer.numel() < 1 + T + 3 * tiles:
         raise KernelError("adapter_plan: the buffer is too small")
     check(lib().gi_adapter_plan(rows, T, int(adapters), ADAPTER_TILE_ROWS, _dev(buffer, "buffer", torch.int32), _stream()), "adapter_plan")
-    return AdapterPlan(buffer, T, int(adapters), ADAPTER_TILE_ROWS, tiles)
+    return AdapterPlan(buffer, T, int(adapters), int(used), ADAPTER_TILE_ROWS)
 
 
 def _rows_of(t: torch.Tensor, name: str) -> int:
@@ -1720,5 +1724,5 @@ def adapter_product(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale
         at += N if slices is None else int(slices[i])
         ends[i] = at
     check(lib().gi_adapter_product(_rows_of(x, "x"), x.stride(0), dtype_code(x.dtype), _dev(down, "down"), _dev(up, "up"),
-                                   _dev(scales, "scales", torch.float32), plan.buffer.data_ptr(), T, A, plan.tile_rows, plan.tiles, _rows_of(out, "out"),
+                                   _dev(scales, "scales", torch.float32), plan.buffer.data_ptr(), T, A, plan.used, plan.tile_rows, _rows_of(out, "out"),
                                    out.stride(0), dtype_code(out.dtype), K, N, r, S, *ends, _stream()), "adapter_product")

@@ -80,7 +80,8 @@ TYPES = [("float32", "float32"), ("bfloat16", "float32"), ("bfloat16", "bfloat16
     (1, 1, (1,), 1, 1), (1, 2048, (2048,), 16, 1), (2, 33, (7,), 3, 2), (8, 2048, (2048,), 16, 8), (15, 1000, (129, 3), 5, 4), (16, 64, (40,), 4, 30),
     (17, 520, (264,), 8, 3), (64, 2048, (512, 128, 128), 16, 9), (100, 256, (96,), 64, 2), (255, 2056, (1000, 520), 12, 24), (256, 1024, (512,), 32, 40),
     (257, 1024, (512,), 32, 7), (300, 4096, (640, 128, 64, 8), 24, 5), (700, 2048, (2048,), 12, 3), (1000, 136, (264,), 128, 11), (130, 72, (24,), 256, 3),
-    (1500, 328, (1028,), 16, 1), (333, 999, (257,), 7, 6), (513, 2048, (250, 250), 100, 2)])
+    (1500, 328, (1028,), 16, 1), (333, 999, (257,), 7, 6), (513, 2048, (250, 250), 100, 2), (2048, 264, (72,), 8, 1000), (2049, 264, (72,), 8, 1000),
+    (200, 128, (64,), 8, 1024), (200, 128, (64,), 8, 1025), (3000, 72, (40,), 4, 5000), (5000, 520, (96, 32), 16, 3), (4100, 264, (64,), 64, 9)])
 def test_adapters_of_many_rows(dtype, out_dtype, T, K, widths, rank, A):
     x, down, up, scales, out, ids = make(T + K + rank, T, K, widths, rank, A, dtype, out_dtype)
     compare(x, down, up, scales, out, ids, widths, run(x, down, up, scales, out, ids, widths))
@@ -150,11 +151,11 @@ def test_the_same_bits_every_time_and_in_every_batch_of_a_size(dtype):
 
 
 def test_streams_buffers_and_programs():
-    x, down, up, scales, out, ids = make(8, 300, 512, (256,), 16, 4, "bfloat16", "float32")
+    x, down, up, scales, out, ids = make(8, 2500, 512, (256,), 16, 4, "bfloat16", "float32")
     want = run(x, down, up, scales, out, ids, (256,))
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
-    buffer = torch.full((K_().adapter_plan_size(300, 4),), -7, dtype=torch.int32, device=DEV)
+    buffer = torch.full((K_().adapter_plan_size(2500, 4),), -7, dtype=torch.int32, device=DEV)
     got = out.clone()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side), K_().record() as rec:
@@ -167,12 +168,12 @@ def test_streams_buffers_and_programs():
 
 
 def test_a_plan_serves_every_number_of_rows_up_to_its_size():
-    size = K_().adapter_plan_size(1000, 9)
-    for T in (0, 1, 16, 255, 256, 257, 999, 1000):
+    size = K_().adapter_plan_size(3000, 9)
+    for T in (0, 1, 16, 255, 256, 257, 2047, 2048, 2049, 3000):
         plan = K_().adapter_plan(torch.arange(T, dtype=torch.int32, device=DEV) % 9, 9, torch.empty(size, dtype=torch.int32, device=DEV))
         assert plan.rows == T
     with pytest.raises(K_().KernelError):
-        K_().adapter_plan(torch.zeros(1001, dtype=torch.int32, device=DEV), 9, torch.empty(1000, dtype=torch.int32, device=DEV))
+        K_().adapter_plan(torch.zeros(3001, dtype=torch.int32, device=DEV), 9, torch.empty(3000, dtype=torch.int32, device=DEV))
 
 
 def test_adapters_refuse_what_does_not_fit():
@@ -199,3 +200,15 @@ def test_adapters_refuse_what_does_not_fit():
         K_().adapter_plan(ids, 0)
     with pytest.raises(K_().KernelError):
         K_().adapter_plan(ids, 8193)
+    for used in (0, 4):
+        with pytest.raises(K_().KernelError):
+            K_().adapter_plan(ids, 3, used=used)
+
+
+@pytest.mark.parametrize("T", [100, 700, 3000])
+def test_few_of_many_adapters(T):
+    x, down, up, scales, out, ids = make(11, T, 128, (72,), 8, 900, "bfloat16", "float32")
+    ids = torch.where(ids >= 0, ids % 5 * 179, ids).contiguous()
+    got = out.clone()
+    K_().adapter_product(x, down, up, scales, K_().adapter_plan(ids, 900, used=5), got)
+    compare(x, down, up, scales, out, ids, (72,), got)

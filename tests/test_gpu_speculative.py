@@ -259,3 +259,20 @@ def test_speculative_refuses_what_does_not_fit():
         with pytest.raises(ValueError):
             engine.generate(**arguments)
     assert engine.generate([[1, 2]], max_new_tokens=0) == [[]]
+
+
+def test_the_command_line_with_an_adapter_and_a_draft_model(tmp_path, capsys):
+    from geneinfer_b200.cli.generate_main import main
+    folder, merged = adapter_and_merged("a", 9, tmp_path)
+    prompt = " ".join(map(str, tc.random_tokens(11, 256, 12)))
+    common = ["--prompt-ids", prompt, "--steps", "30", "--temperature", "0", "--dtype", "fp32", "--quiet"]
+
+    def run(*more):
+        assert main([*common, *more]) == 0
+        return capsys.readouterr().out.split()
+
+    want = run("--model", merged)
+    assert run("--model", gf.model_dir("a"), "--adapter", folder) == want
+    assert run("--model", gf.model_dir("a"), "--adapter", folder, "--draft-model", gf.model_dir("a_named"), "--drafts", "3") == want
+    assert main([*common, "--model", merged, "--draft-model", merged, "--top-p", "0.9"]) == 2
+    assert main([*common, "--model", merged, "--draft-model", merged, "--drafts", "0"]) == 2
