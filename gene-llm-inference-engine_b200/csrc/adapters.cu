@@ -120,7 +120,7 @@ struct AdapterArgs {
 };
 
 constexpr int kAdapterThreads = 256, kAdapterWarps = kAdapterThreads / 32;
-constexpr int kDirectRows = 2048, kDirectEach = kDirectRows / kAdapterThreads;      // steps of up to so many rows have no plan: a tile's blocks look its rows up themselves
+constexpr int kDirectRows = 1024, kDirectEach = kDirectRows / kAdapterThreads;      // steps of up to so many rows have no plan: a tile's blocks look its rows up themselves
 constexpr int kDirectAdapters = 1024;          // (of so many adapters)
 constexpr int kFewTokens = 256;                // rows up to which they are taken for single tokens, each with an adapter of its own as a rule
 
@@ -570,8 +570,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_few_kernel(Adapter
 // the sums and their pieces lie where the ring was, else the sums have a place of their own.
 template <int M, bool kOnePass> struct ManyShape {
     static constexpr int kStageBytes = (M + 64) * 128;
-    static constexpr int kStages = M == 128 ? 4 : kOnePass ? 6 : 5;
-    static constexpr int kGroups = 4, kSplits = kAdapterWarps / kGroups, kTiles = M / 16 / kGroups;
+    static constexpr int kStages = (kOnePass ? 98304 : 81920) / kStageBytes;
+    static constexpr int kGroups = M < 64 ? M / 16 : 4, kSplits = kAdapterWarps / kGroups, kTiles = M / 16 / kGroups, kSteps = 4 / kSplits;
 };
 constexpr int kManyCols = 64;                  // ranks of a pass over K
 
@@ -662,8 +662,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_many_kernel(Adapte
             next = slot;
             slot = slot + 1 == Shape::kStages ? 0 : slot + 1;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int step = 2 * split + s;
+            for (int s = 0; s < Shape::kSteps; ++s) {
+                const int step = Shape::kSteps * split + s;
                 unsigned xa[kTiles][4], w[kManyCols / 16][4];          // (a step's fragments first: its products then wait for nothing)
 #pragma unroll
                 for (int m = 0; m < kTiles; ++m) load_matrices(xa[m], (at + x_at + m * 16 * 128) ^ (step << 5));
@@ -737,7 +737,12 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_many_kernel(Adapte
     for (int i = first; i < last; i += kAdapterWarps) {
         const ColumnBlock now = block;
         const __nv_bfloat16* from = up + static_cast<size_t>(now.col) * a.r;
-        if (i + kAdapterWarps < last) block = column_block(a, i + kAdapterWarps);
+        UpFragments<kSteps> after;             // of the next columns
+        constexpr bool kAhead = kSteps < 4;      // (with four steps of ranks the registers are full)
+        if (i + kAdapterWarps < last) {
+            block = column_block(a, i + kAdapterWarps);
+            if (kAhead) load_up<kSteps, TO>(after, up + static_cast<size_t>(block.col) * a.r, a.r, 0, block.cols);
+        }
         for (int row0 = 0; row0 < n; row0 += 32) {
             OldValues<2, TO> next;             // of the turn that follows
             if (row0 + 32 < n) load_old<2, TO>(next, a, now, row0 + 32, s_rows);
@@ -745,7 +750,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_many_kernel(Adapte
             expand<2, kSteps, TO>(a, f, kSteps == 4 && a.r > 64 && row0 > 0, old, from, now, shared_address(pieces), 2 * M * ld, ld, row0, s_rows);
             old = next;
         }
-        if (i + kAdapterWarps < last) load_up<kSteps, TO>(f, up + static_cast<size_t>(block.col) * a.r, a.r, 0, block.cols);
+        if (kAhead) f = after;
+        else if (i + kAdapterWarps < last) load_up<kSteps, TO>(f, up + static_cast<size_t>(block.col) * a.r, a.r, 0, block.cols);
     }
 }
 
@@ -925,7 +931,8 @@ inline TileCount tile_count(const AdapterArgs& a, int rows) {
     const long long most = a.plan.T / rows + adapters;
     return {most, a.plan.T <= kFewTokens ? most : full};
 }
-// CTAs of a cluster: as many as two a multiprocessor have room for (`slack`: twice as many).
+// CTAs of a cluster: as many as two a multiprocessor have room for (`slack`: twice as many). Powers of two: clusters of three and six, which would
+// fill more places, do not all find theirs at once (3,000 rows into 16,384 columns, 94 tiles: clusters of two 141 us, of three 186 us).
 inline int cluster_parts(long long tiles, int slack) {
     int parts = 1;
     while (parts < kAdapterClusterMost && 2 * parts * tiles <= 2LL * sm_count() * slack) parts *= 2;
@@ -954,6 +961,11 @@ template <typename TO> inline size_t pieces_bytes(const AdapterArgs& a, int rows
 }
 inline size_t sums_bytes(const AdapterArgs& a, int rows) { return 4ull * rows * (a.S * a.r + 8); }
 template <typename Shape> constexpr size_t ring_bytes() { return static_cast<size_t>(Shape::kStages) * Shape::kStageBytes; }
+
+// Whether what lies where the ring was fits there.
+template <int M, bool kOnePass, typename TO> inline bool fits(const AdapterArgs& a) {
+    return (kOnePass ? sums_bytes(a, M) : 0) + pieces_bytes<TO>(a, M) <= ring_bytes<ManyShape<M, kOnePass>>();
+}
 
 template <int kSteps, typename TO>
 int launch_few(const AdapterArgs& a, cudaStream_t st) {
@@ -989,14 +1001,14 @@ int launch_f32(const AdapterArgs& a, cudaStream_t st) {
 
 template <int kSteps, typename TO>
 int launch_steps(const AdapterArgs& a, cudaStream_t st) {
-    using Wide = ManyShape<128, true>;
-    using Tall = ManyShape<64, true>;
-    using Passes = ManyShape<64, false>;
     if (a.plan.T <= kFewTokens) return launch_few<kSteps, TO>(a, st);
-    const bool one = a.S * a.r <= kManyCols;
-    if (one && a.plan.T >= 4096 && sums_bytes(a, 128) + pieces_bytes<TO>(a, 128) <= ring_bytes<Wide>()) return launch_many<128, true, kSteps, TO>(a, st);
-    if (one && sums_bytes(a, 64) + pieces_bytes<TO>(a, 64) <= ring_bytes<Tall>()) return launch_many<64, true, kSteps, TO>(a, st);
-    if (pieces_bytes<TO>(a, 64) <= ring_bytes<Passes>()) return launch_many<64, false, kSteps, TO>(a, st);
+    if (a.S * a.r <= kManyCols) {
+        // (tiles of 32 rows: 2,048 rows of 4,096 into 6,144 at rank 16 38 us, of 64 48 us; 3,000 of 8,192 into 2,048 35 and 31 us)
+        if (a.plan.T <= 2048 && fits<32, true, TO>(a)) return launch_many<32, true, kSteps, TO>(a, st);
+        if (fits<64, true, TO>(a)) return launch_many<64, true, kSteps, TO>(a, st);
+    }
+    // (several passes: tiles of 32 rows leave two blocks a multiprocessor, 1,000 rows into [q; k; v] at rank 64 43 us, of 64 rows 71 us)
+    if (fits<32, false, TO>(a)) return launch_many<32, false, kSteps, TO>(a, st);
     return launch_few<kSteps, TO>(a, st);
 }
 

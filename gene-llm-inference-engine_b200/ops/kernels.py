@@ -1660,7 +1660,7 @@ class AdapterPlan:
 
 
 ADAPTER_TILE_ROWS = 128
-ADAPTER_DIRECT_ROWS, ADAPTER_DIRECT_ADAPTERS = 2048, 1024      # steps of up to so many rows (and adapters) need no plan on the device: the products look rows up themselves
+ADAPTER_DIRECT_ROWS, ADAPTER_DIRECT_ADAPTERS = 1024, 1024      # steps of up to so many rows (and adapters) need no plan on the device: the products look rows up themselves
 
 
 def adapter_plan_size(rows: int, adapters: int) -> int:

@@ -80,7 +80,7 @@ TYPES = [("float32", "float32"), ("bfloat16", "float32"), ("bfloat16", "bfloat16
     (1, 1, (1,), 1, 1), (1, 2048, (2048,), 16, 1), (2, 33, (7,), 3, 2), (8, 2048, (2048,), 16, 8), (15, 1000, (129, 3), 5, 4), (16, 64, (40,), 4, 30),
     (17, 520, (264,), 8, 3), (64, 2048, (512, 128, 128), 16, 9), (100, 256, (96,), 64, 2), (255, 2056, (1000, 520), 12, 24), (256, 1024, (512,), 32, 40),
     (257, 1024, (512,), 32, 7), (300, 4096, (640, 128, 64, 8), 24, 5), (700, 2048, (2048,), 12, 3), (1000, 136, (264,), 128, 11), (130, 72, (24,), 256, 3),
-    (1500, 328, (1028,), 16, 1), (333, 999, (257,), 7, 6), (513, 2048, (250, 250), 100, 2), (2048, 264, (72,), 8, 1000), (2049, 264, (72,), 8, 1000),
+    (1500, 328, (1028,), 16, 1), (333, 999, (257,), 7, 6), (513, 2048, (250, 250), 100, 2), (1024, 264, (72,), 8, 1000), (1025, 264, (72,), 8, 1000),
     (200, 128, (64,), 8, 1024), (200, 128, (64,), 8, 1025), (3000, 72, (40,), 4, 5000), (5000, 520, (96, 32), 16, 3), (4100, 264, (64,), 64, 9)])
 def test_adapters_of_many_rows(dtype, out_dtype, T, K, widths, rank, A):
     x, down, up, scales, out, ids = make(T + K + rank, T, K, widths, rank, A, dtype, out_dtype)
@@ -169,7 +169,7 @@ def test_streams_buffers_and_programs():
 
 def test_a_plan_serves_every_number_of_rows_up_to_its_size():
     size = K_().adapter_plan_size(3000, 9)
-    for T in (0, 1, 16, 255, 256, 257, 2047, 2048, 2049, 3000):
+    for T in (0, 1, 16, 255, 256, 257, 1023, 1024, 1025, 3000):
         plan = K_().adapter_plan(torch.arange(T, dtype=torch.int32, device=DEV) % 9, 9, torch.empty(size, dtype=torch.int32, device=DEV))
         assert plan.rows == T
     with pytest.raises(K_().KernelError):
