@@ -8,8 +8,8 @@
 // weight w_i > 0 with w_0 + .. + w_i > v * sum(w); the random numbers u and v come from the caller.
 //
 // A cluster of CTAs per row finds max and sum and whether the row's draft is kept; a cluster per request finds the stop and draws there. Where there
-// are many more rows than the GPU holds at a time, the drafts' places are taken a few at a launch, and rows whose request has met a
-// refusal in an earlier one are left out. The answer is a whole number, so sums run in 64 bits: their order moves a boundary between two tokens by
+// are more rows than the GPU holds at a time, the rows run in the order of the drafts' places, and those whose request has met a
+// refusal by then are left out. The answer is a whole number, so sums run in 64 bits: their order moves a boundary between two tokens by
 // 1e-13 of the mass, where 32-bit sums would move all 128,000 of them by 1e-7, a different token in one draw of a hundred.
 //
 // What bounds it: few rows the chain of read, exchange, exponentials, exchange (one user's five rows of 128,256: 6.5 us, the draw 9.7 us of which 4.4
@@ -164,6 +164,7 @@ __device__ __forceinline__ void meet_behind_first_warps() {
 }
 
 // The largest value of the cluster's row (NaN if any value is none); every thread has it.
+template <int kThreads>
 __device__ __forceinline__ float cluster_max(float mx, RowShared& s, cg::cluster_group& cluster, int part, int parts) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -172,9 +173,9 @@ __device__ __forceinline__ float cluster_max(float mx, RowShared& s, cg::cluster
     __syncthreads();
     cluster.barrier_wait();                // (arrived at when the kernel began)
     if (warp == 0) {
-        mx = s.warp_max[lane & (kRowWarps - 1)];
+        mx = s.warp_max[lane & ((kThreads / 32) - 1)];
 #pragma unroll
-        for (int o = kRowWarps / 2; o > 0; o >>= 1) mx = max_or_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        for (int o = (kThreads / 32) / 2; o > 0; o >>= 1) mx = max_or_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         if (lane < parts) *cluster.map_shared_rank(&s.cta_max[part], lane) = mx;
     }
     meet_behind_first_warps();
@@ -184,15 +185,16 @@ __device__ __forceinline__ float cluster_max(float mx, RowShared& s, cg::cluster
 }
 
 // The cluster's sum, in the order of the CTAs; every thread has it. The warps' sums stay in s.warp_sum, the CTAs' in s.cta_sum[turn].
+template <int kThreads>
 __device__ __forceinline__ double cluster_sum(double v, RowShared& s, int turn, cg::cluster_group& cluster, int part, int parts) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     v = warp_total(v);
     if (lane == 0) s.warp_sum[warp] = v;
     __syncthreads();
     if (warp == 0) {
-        v = s.warp_sum[lane & (kRowWarps - 1)];
+        v = s.warp_sum[lane & ((kThreads / 32) - 1)];
 #pragma unroll
-        for (int o = kRowWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        for (int o = (kThreads / 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (lane < parts) *cluster.map_shared_rank(&s.cta_sum[turn][part], lane) = v;
     }
     meet_behind_first_warps();
@@ -207,7 +209,7 @@ __device__ __forceinline__ void keep_best(float v, int i, float& best, int& at) 
 
 // Index of the largest value of the cluster's row, the lowest among equals (values that are no number are passed over; 0 where there
 // is no other).
-template <typename Each>
+template <int kThreads, typename Each>
 __device__ __forceinline__ int cluster_argmax(const Each& each, RowShared& s, cg::cluster_group& cluster, int part, int parts) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float best = -INFINITY;
@@ -223,7 +225,7 @@ __device__ __forceinline__ int cluster_argmax(const Each& each, RowShared& s, cg
     __syncthreads();
     cluster.barrier_wait();                // (arrived at when the kernel began)
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kRowWarps; ++w) keep_best(s.warp_max[w], s.warp_at[w], best, at);
+        for (int w = 1; w < (kThreads / 32); ++w) keep_best(s.warp_max[w], s.warp_at[w], best, at);
         for (int p = 0; p < parts; ++p) {
             *cluster.map_shared_rank(&s.cta_max[part], p) = best;
             *cluster.map_shared_rank(&s.cta_at[part], p) = at;
@@ -239,9 +241,10 @@ __device__ __forceinline__ int cluster_argmax(const Each& each, RowShared& s, cg
 // Values of a CTA's whole groups: held in registers (kUnits groups of four a thread) or, kUnits = 0, read again in every pass (the cluster's row is then
 // in L2). kOrdered: a warp's groups are neighbours, as a draw wants them; else the block's threads take turns (a little faster). The places
 // in no whole group: one each for the first lanes of the first CTA's first warp and of the last CTA's last warp.
-template <typename T, int kUnits, bool kOrdered> struct Values {
+template <typename T, int kUnits, bool kOrdered, int kThreads> struct Values {
+    static constexpr int kWarps = kThreads / 32;
     static constexpr int kBatch = 4;       // groups whose loads are in flight together
-    static constexpr int kStep = kOrdered ? 32 : kRowThreads;
+    static constexpr int kStep = kOrdered ? 32 : kThreads;
     const Row<T>& r;
     int first, last, edge_at;
     float edge;
@@ -250,13 +253,13 @@ template <typename T, int kUnits, bool kOrdered> struct Values {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         last = min(r.end, r.end_whole);
         if constexpr (kOrdered) {
-            const int share = ((r.end - r.begin + kRowWarps - 1) / kRowWarps + 31) & ~31;
+            const int share = ((r.end - r.begin + kWarps - 1) / kWarps + 31) & ~31;
             first = r.begin + warp * share + lane;
             last = min(last, r.begin + (warp + 1) * share);
         } else {
             first = max(r.begin, r.first_whole) + threadIdx.x;
         }
-        edge_at = part == 0 && warp == 0 && lane < kEdge ? r.head(lane) : part == parts - 1 && warp == kRowWarps - 1 && lane >= kEdge && lane < 2 * kEdge ? r.tail(lane - kEdge) : -1;
+        edge_at = part == 0 && warp == 0 && lane < kEdge ? r.head(lane) : part == parts - 1 && warp == kWarps - 1 && lane >= kEdge && lane < 2 * kEdge ? r.tail(lane - kEdge) : -1;
         edge = edge_at >= 0 ? to_float(r.row[edge_at]) : -INFINITY;
         if constexpr (kUnits > 0) {
 #pragma unroll
@@ -279,7 +282,7 @@ template <typename T, int kUnits, bool kOrdered> struct Values {
             for (int u = 0; u < kUnits; ++u)
                 if (f(first + kStep * u, held[u], none)) return;
         } else {
-            // whole batches of the warp (of the thread, where nothing hangs on the warp) without a look at what is there, the rest one by one
+            // whole batches of the warp (of the thread, where nothing hangs on the warp) without a look at what is there, then what is left
             const int lane = kOrdered ? threadIdx.x & 31 : 0;
             int unit = first;
             for (; unit + (31 - lane) * kOrdered + kStep * (kBatch - 1) < last && (!kOrdered || unit - lane >= r.first_whole); unit += kBatch * kStep) {
@@ -290,11 +293,17 @@ template <typename T, int kUnits, bool kOrdered> struct Values {
                 for (int u = 0; u < kBatch; ++u)
                     if (f(unit + kStep * u, v[u], w[u])) return;
             }
-#pragma unroll 1
-            for (; unit - lane < last; unit += kStep) {
-                float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, w[4] = {0.f, 0.f, 0.f, 0.f};
-                if (there(unit)) { r.load_whole(unit, v); more(unit, w); }
-                if (f(unit, v, w)) return;
+            for (; unit - lane < last; unit += kBatch * kStep) {
+                float v[kBatch][4], w[kBatch][4];
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    v[u][0] = v[u][1] = v[u][2] = v[u][3] = -INFINITY;
+                    w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0.f;
+                    if (there(unit + kStep * u)) { r.load_whole(unit + kStep * u, v[u]); more(unit + kStep * u, w[u]); }
+                }
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u)
+                    if (unit + kStep * u - lane < last && f(unit + kStep * u, v[u], w[u])) return;
             }
         }
     }
@@ -317,7 +326,7 @@ struct RowArgs {
     int* tokens;
     int* accepted;
     float4* work;                          // per row: max, 1 / sum, draft kept (1) or not (0), argmax of a greedy row (an integer's bits)
-    int R, D, place;                       // place: the first of the drafts' places that a launch takes
+    int R, D, skip;                        // skip: rows behind a refusal that is known when they begin are left out
 };
 
 // The request's drafts, or -1 where its rows do not lie in the logits.
@@ -328,7 +337,7 @@ __device__ __forceinline__ int drafts_of(const RowArgs& a, int r) {
 
 // What a draw needs of a row: q's row (or null), the token that a draft without a distribution leaves out, both for refused drafts only.
 template <typename T>
-__device__ __forceinline__ int draw_token(Values<T, 0, true>& values, const ByTemperature& by, float inv, const float* q, int without, float number, int V,
+__device__ __forceinline__ int draw_token(Values<T, 0, true, kRowThreads>& values, const ByTemperature& by, float inv, const float* q, int without, float number, int V,
                                           RowShared& s, cg::cluster_group& cluster, int part, int parts) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool q_wide = q != nullptr && (reinterpret_cast<uintptr_t>(q) / 4 & 3) == static_cast<unsigned>(values.r.off);
@@ -372,7 +381,7 @@ __device__ __forceinline__ int draw_token(Values<T, 0, true>& values, const ByTe
             return false;
         });
         if (turn == 1) cluster.barrier_wait();              // (arrived at when the kernel began)
-        total = cluster_sum(mine, s, turn, cluster, part, parts);
+        total = cluster_sum<kRowThreads>(mine, s, turn, cluster, part, parts);
         if (!subtract || total > 0.0) break;
         subtract = false;                                   // nothing is left of p behind q: the draw is from p (the whole cluster takes this turn)
         __syncthreads();                                    // all have read the warps' sums
@@ -441,8 +450,8 @@ __device__ __forceinline__ int draw_token(Values<T, 0, true>& values, const ByTe
 
 // One cluster per row. kProbs: row i's distribution goes to out; else row j of request r: whether its draft is kept, and if there is none or it is not, the
 // token that a draw at this row gives.
-template <typename T, int kUnits, bool kProbs>
-__global__ void __launch_bounds__(kRowThreads, kUnits ? 2 : 3) row_softmax_kernel(RowArgs a) {
+template <typename T, int kUnits, bool kProbs, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) row_softmax_kernel(RowArgs a) {
     pdl_prologue();
     __shared__ RowShared s;
     cg::cluster_group cluster = cg::this_cluster();
@@ -450,18 +459,28 @@ __global__ void __launch_bounds__(kRowThreads, kUnits ? 2 : 3) row_softmax_kerne
     const int r = blockIdx.x >> a.log_parts;                // the row, or the request
     int row = r, j = 0, d = 0;
     if constexpr (!kProbs) {
-        j = a.place + blockIdx.y;
+        j = blockIdx.y;
         d = drafts_of(a, r);
         if (j > d) return;                 // (the whole cluster)
         row = a.row_start[r] + j;
-        for (int i = 0; i < a.place; ++i)
-            if (a.work[row - j + i].z == 0.f) return;       // a refusal in an earlier launch: nobody asks for this row (the whole cluster)
+        if (a.skip && j > 0) {
+            // A refusal ahead that has been seen: nobody asks for this row. The cluster's CTAs must all go or all stay: who comes first decides.
+            __shared__ int s_decided;
+            if (threadIdx.x == 0) {
+                int* decided = reinterpret_cast<int*>(&a.work[row].w);
+                const int mine = *reinterpret_cast<volatile const int*>(a.accepted + r) < j ? 2 : 1;
+                const int before = atomicCAS(decided, 0, mine);
+                s_decided = before ? before : mine;
+            }
+            __syncthreads();
+            if (s_decided == 2) return;
+        }
     }
     cluster.barrier_arrive();              // every CTA of the cluster runs before another writes into its shared memory
     const T* p = static_cast<const T*>(a.logits) + row * a.stride;
     const Row<T> span(p, a.V, part, a.log_parts);
     if constexpr (kUnits == 0) span.ask();
-    Values<T, kUnits, false> values(span, part, parts);
+    Values<T, kUnits, false, kThreads> values(span, part, parts);
     const float temp = a.temperature[r];
     // the draft, its logit, its probability in q and the number that decides (the same in every thread)
     int x = -1;
@@ -480,7 +499,7 @@ __global__ void __launch_bounds__(kRowThreads, kUnits ? 2 : 3) row_softmax_kerne
         }
     }
     if (!(temp > 0.f)) {
-        const int best = cluster_argmax([&](auto f) {
+        const int best = cluster_argmax<kThreads>([&](auto f) {
             values.groups([&](int unit, float (&v)[4]) {
                 if (values.there(unit))
 #pragma unroll
@@ -492,15 +511,16 @@ __global__ void __launch_bounds__(kRowThreads, kUnits ? 2 : 3) row_softmax_kerne
         if constexpr (kProbs) {
             float* out = a.out + static_cast<size_t>(row) * a.V;
             const int share = ((a.V - 1) >> a.log_parts) + 1, end = static_cast<int>(min(static_cast<long long>(a.V), static_cast<long long>(part + 1) * share));
-            for (int i = part * share + threadIdx.x; i < end; i += kRowThreads) out[i] = i == best ? 1.0f : 0.0f;
+            for (int i = part * share + threadIdx.x; i < end; i += kThreads) out[i] = i == best ? 1.0f : 0.0f;
         } else if (part == 0 && threadIdx.x == 0) {
             a.work[row] = make_float4(0.f, 0.f, x == best ? 1.f : 0.f, __int_as_float(best));
+            if (a.skip && x != best && j < d) atomicMin(a.accepted + r, j);
         }
         return;
     }
     float mx = values.edge;
     values.groups([&](int, float (&v)[4]) { mx = max_or_nan(max_or_nan(mx, v[0], v[1]), v[2], v[3]); return false; });
-    mx = cluster_max(mx, s, cluster, part, parts);
+    mx = cluster_max<kThreads>(mx, s, cluster, part, parts);
     const bool some = mx > -INFINITY && mx < INFINITY;      // else there are no probabilities (a value is none, or infinite, or all are -infinity)
     const ByTemperature by(mx, temp);
     double sum = 0.0;
@@ -512,11 +532,11 @@ __global__ void __launch_bounds__(kRowThreads, kUnits ? 2 : 3) row_softmax_kerne
             if constexpr (kProbs) { v[0] = y[0]; v[1] = y[1]; v[2] = y[2]; v[3] = y[3]; }
             return false;
         });
-        if (threadIdx.x < 32 || threadIdx.x >= kRowThreads - 32) sum += static_cast<double>(by(values.edge));     // (the warps that can have one)
+        if (threadIdx.x < 32 || threadIdx.x >= kThreads - 32) sum += static_cast<double>(by(values.edge));     // (the warps that can have one)
     };
     if (some && !by.plain) weigh([&](float (&y)[4]) { by.usual(y); });
     else if (some) weigh([&](float (&y)[4]) { by.general(y); });
-    sum = cluster_sum(sum, s, 0, cluster, part, parts);
+    sum = cluster_sum<kThreads>(sum, s, 0, cluster, part, parts);
     const float inv = some ? static_cast<float>(1.0 / sum) : NAN;
     if constexpr (kProbs) {
         float* out = a.out + static_cast<size_t>(row) * a.V;
@@ -540,7 +560,17 @@ __global__ void __launch_bounds__(kRowThreads, kUnits ? 2 : 3) row_softmax_kerne
         if (part == 0 && threadIdx.x == 0) {
             const bool kept = some && x >= 0 && __fmul_rn(number, qx) < __fmul_rn(by(lx), inv);
             a.work[row] = make_float4(mx, inv, kept ? 1.f : 0.f, 0.f);
+            if (a.skip && !kept && j < d) atomicMin(a.accepted + r, j);
         }
+    }
+}
+
+// Ahead of rows of which some may be left out: no refusal known, no row decided.
+__global__ void __launch_bounds__(256) draft_begin_kernel(RowArgs a) {
+    pdl_prologue();
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < max(a.N, a.R); i += gridDim.x * 256) {
+        if (i < a.N) a.work[i].w = 0.f;
+        if (i < a.R) a.accepted[i] = INT_MAX;
     }
 }
 
@@ -583,17 +613,17 @@ __global__ void __launch_bounds__(kRowThreads, 2) draft_draw_kernel(RowArgs a) {
     const float* q = stop < d && a.q ? a.q + r * a.q_request + stop * a.q_place : nullptr;
     span.ask();
     if (q) span.ask(q);
-    Values<T, 0, true> values(span, part, parts);
+    Values<T, 0, true, kRowThreads> values(span, part, parts);
     const int without = stop < d && !a.q ? a.drafted[static_cast<size_t>(r) * a.D + stop] : -1;
     const int pick = draw_token<T>(values, ByTemperature(stat.x, temp), stat.y, q, without, a.draw[r], a.V, s, cluster, part, parts);
     if (pick >= 0) tokens[stop] = pick;
 }
 
 template <typename... KArgs, typename... Args>
-inline void launch_row_clusters(void (*kernel)(KArgs...), dim3 grid, int parts, cudaStream_t stream, Args&&... args) {
+inline void launch_row_clusters(void (*kernel)(KArgs...), dim3 grid, int threads, int parts, cudaStream_t stream, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(kRowThreads);
+    cfg.blockDim = dim3(threads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -612,51 +642,57 @@ inline void launch_row_clusters(void (*kernel)(KArgs...), dim3 grid, int parts, 
 // multiprocessor: what a row costs besides its values (the exchanges within warps, block and cluster) is spread over more of them, and rows in flight stay
 // within L2 (742 rows of 128,256: clusters of four 112 us, clusters of eight with rows in registers 168 us). Probabilities (`keeps`) need every
 // exponential twice and keep it in registers wherever those hold the row (512 rows of 151,669: 170 us, 193 us without).
-constexpr int kSlice = 32768;
+constexpr int kSlice = 65536;
 struct RowPlan { int log_parts, units; };
 inline RowPlan row_plan(int V, long long rows, bool keeps = false) {
     const long long groups = (static_cast<long long>(V) + 6) / 4, sms = sm_count();         // with an edge on either side
     int log_parts = 0;
     while ((1 << log_parts) < kRowCtasMost && ((static_cast<long long>(kSlice) << log_parts) < V ||
-                                               ((keeps || (rows << log_parts) * 2 <= 3 * sms) && groups > (2LL * kRowThreads << log_parts)))) ++log_parts;
+                                               ((keeps || (rows << log_parts) * 2 <= 2 * sms) && groups > (2LL * kRowThreads << log_parts)))) ++log_parts;
     const long long per = (((groups - 1) >> log_parts) + 32) & ~31LL, units = (per + kRowThreads - 1) / kRowThreads;
     if (!keeps && rows << log_parts > 2 * sms) return {log_parts, 0};
     return {log_parts, units <= 2 ? 2 : units <= 4 ? 4 : units <= 8 ? 8 : units <= kRowUnitsMost ? kRowUnitsMost : 0};
 }
 
+// Many rows of a small vocabulary: blocks of four warps, eight a multiprocessor, each with a row in registers (2,304 rows of 5,000: 34 us, 49 us with
+// blocks of sixteen warps, whose threads have too few values for what a row costs besides).
+constexpr int kNarrowThreads = 128, kNarrowUnits = 10, kNarrowVocab = 4 * kNarrowThreads * kNarrowUnits - 8;
+
 template <typename T, bool kProbs>
 int launch_rows(RowArgs a, int rows, int places, cudaStream_t st, const char* what) {
-    const RowPlan plan = row_plan(a.V, static_cast<long long>(rows) * places, kProbs);
+    RowPlan plan = row_plan(a.V, static_cast<long long>(rows) * places, kProbs);
+    const bool narrow = a.V <= kNarrowVocab && static_cast<long long>(rows) * places > 2 * sm_count();
+    if (narrow) plan.log_parts = 0;
     a.log_parts = plan.log_parts;
     GI_REQUIRE(rows <= INT_MAX >> plan.log_parts && places <= 65535, "%s: %d rows of %d places exceed the grid limit", what, rows, places);
     const dim3 grid(static_cast<unsigned>(rows) << plan.log_parts, places);
     const int parts = 1 << plan.log_parts;
+    if (narrow) {
+        launch_row_clusters((row_softmax_kernel<T, kNarrowUnits, kProbs, kNarrowThreads>), grid, kNarrowThreads, 1, st, a);
+        return check_launch(what);
+    }
     switch (plan.units) {
-        case 2: launch_row_clusters((row_softmax_kernel<T, 2, kProbs>), grid, parts, st, a); break;
-        case 4: launch_row_clusters((row_softmax_kernel<T, 4, kProbs>), grid, parts, st, a); break;
-        case 8: launch_row_clusters((row_softmax_kernel<T, 8, kProbs>), grid, parts, st, a); break;
-        case kRowUnitsMost: launch_row_clusters((row_softmax_kernel<T, kRowUnitsMost, kProbs>), grid, parts, st, a); break;
-        default: launch_row_clusters((row_softmax_kernel<T, 0, kProbs>), grid, parts, st, a); break;
+        case 2: launch_row_clusters((row_softmax_kernel<T, 2, kProbs, kRowThreads>), grid, kRowThreads, parts, st, a); break;
+        case 4: launch_row_clusters((row_softmax_kernel<T, 4, kProbs, kRowThreads>), grid, kRowThreads, parts, st, a); break;
+        case 8: launch_row_clusters((row_softmax_kernel<T, 8, kProbs, kRowThreads>), grid, kRowThreads, parts, st, a); break;
+        case kRowUnitsMost: launch_row_clusters((row_softmax_kernel<T, kRowUnitsMost, kProbs, kRowThreads>), grid, kRowThreads, parts, st, a); break;
+        default: launch_row_clusters((row_softmax_kernel<T, 0, kProbs, kRowThreads>), grid, kRowThreads, parts, st, a); break;
     }
     return check_launch(what);
 }
 
-// Places of the drafts that a launch takes: all, unless there are kRounds times the rows that the GPU holds at a time, for every launch (128 requests of six
-// drafts, 2.8 kept: two launches 152 us, one 170 us; a launch's last clusters leave SMs idle for about half a round).
-constexpr int kRounds = 4;
-inline int places_of_launch(const RowArgs& a) {
-    const long long rows = static_cast<long long>(a.R) * (a.D + 1), held = 3LL * sm_count() >> row_plan(a.V, rows).log_parts;
-    const long long launches = rows / (kRounds * held);
-    return launches <= 1 ? a.D + 1 : launches > a.D ? 1 : static_cast<int>((a.D + launches) / launches);
-}
-
 template <typename T>
 int launch_verify(RowArgs a, cudaStream_t st) {
-    const int places = places_of_launch(a);
-    for (a.place = 0; a.place <= a.D; a.place += places)
-        if (const int rc = launch_rows<T, false>(a, a.R, a.D + 1 - a.place < places ? a.D + 1 - a.place : places, st, "verify_drafts")) return rc;
+    // From twice the rows that the GPU holds at a time on (128 requests of six drafts, 2.8 kept: 119 us with rows left out, 135 without)
+    const long long rows = static_cast<long long>(a.R) * (a.D + 1);
+    a.skip = rows << row_plan(a.V, rows).log_parts > 4LL * sm_count();
+    if (a.skip) {
+        launch_kernel((draft_begin_kernel), dim3(16), dim3(256), 0, st, a);
+        if (check_launch("verify_drafts")) return 1;
+    }
+    if (const int rc = launch_rows<T, false>(a, a.R, a.D + 1, st, "verify_drafts")) return rc;
     a.log_parts = row_plan(a.V, 1).log_parts;
-    launch_row_clusters((draft_draw_kernel<T>), dim3(static_cast<unsigned>(a.R) << a.log_parts), 1 << a.log_parts, st, a);
+    launch_row_clusters((draft_draw_kernel<T>), dim3(static_cast<unsigned>(a.R) << a.log_parts), kRowThreads, 1 << a.log_parts, st, a);
     return check_launch("verify_drafts");
 }
 

@@ -154,6 +154,18 @@ def test_verification_follows_the_formulas(dtype, R, D, V, masked, probs):
     check_verification(*args, tokens, accepted)
 
 
+@pytest.mark.parametrize("dtype,R,D,V,masked,probs", [("float32", 110, 4, 70001, False, True), ("bfloat16", 130, 5, 66000, True, False),
+                                                      ("float32", 400, 3, 6003, False, True)])
+def test_more_rows_than_the_gpu_holds_at_a_time(dtype, R, D, V, masked, probs):
+    """Rows behind a refusal may be left out, in clusters of two and in blocks of a row each: the answers are the same, in every run."""
+    args = inputs(V, R, D, V, dtype, masked=masked, probs=probs)
+    tokens, accepted = verify(*args)
+    check_verification(*args, tokens, accepted)
+    for _ in range(3):
+        again = verify(*args)
+        assert torch.equal(again[0], tokens) and torch.equal(again[1], accepted)
+
+
 def test_every_count_of_kept_drafts_comes_up():
     args = inputs(3, 300, 4, 50, "float32")
     tokens, accepted = verify(*args)
