@@ -27,6 +27,7 @@ namespace gi {
 namespace cg = cooperative_groups;
 
 constexpr int kRowThreads = 512, kRowWarps = kRowThreads / 32;
+constexpr int kSmallThreads = 256, kNarrowThreads = 128;        // (many rows that registers hold: row_plan)
 constexpr int kRowCtasMost = 8;           // CTAs of a row's cluster
 constexpr int kRowUnitsMost = 10;         // groups of four values that a thread holds: vocabularies of up to 163,840 stay in registers
 constexpr int kEdge = 4;                  // places at either end of a row that may lie in no whole group
@@ -451,7 +452,7 @@ __device__ __forceinline__ int draw_token(Values<T, 0, true, kRowThreads>& value
 // One cluster per row. kProbs: row i's distribution goes to out; else row j of request r: whether its draft is kept, and if there is none or it is not, the
 // token that a draw at this row gives.
 template <typename T, int kUnits, bool kProbs, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads) row_softmax_kernel(RowArgs a) {
+__global__ void __launch_bounds__(kThreads, kThreads != kSmallThreads ? 1024 / kThreads : kUnits > 8 ? 2 : 3) row_softmax_kernel(RowArgs a) {
     pdl_prologue();
     __shared__ RowShared s;
     cg::cluster_group cluster = cg::this_cluster();
@@ -637,46 +638,60 @@ inline void launch_row_clusters(void (*kernel)(KArgs...), dim3 grid, int threads
     counted(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
 }
 
-// CTAs of a row's cluster and groups a thread holds (0: read again in every pass, out of L2). Few rows: as many CTAs as fit the GPU at once, and
-// registers where those hold the row, for the shortest way from first read to answer. Many rows: about kSlice values a CTA and nothing held, three CTAs a
-// multiprocessor: what a row costs besides its values (the exchanges within warps, block and cluster) is spread over more of them, and rows in flight stay
-// within L2 (742 rows of 128,256: clusters of four 112 us, clusters of eight with rows in registers 168 us). Probabilities (`keeps`) need every
-// exponential twice and keep it in registers wherever those hold the row (512 rows of 151,669: 170 us, 193 us without).
+// CTAs of a row's cluster, groups a thread holds (0: read again in every pass, out of L2) and threads of a CTA.
+// Few rows: as many CTAs as fit the GPU at once, and registers where those hold the row, for the shortest way from first read to answer.
+// Many rows: as few CTAs a row as may be, since what a row costs besides its values (the exchanges within warps, block and cluster) grows with them.
+// Probabilities (`keeps`) need every exponential twice and hold it: the fewest CTAs whose registers hold the row (1,000 rows of 32,000: clusters of
+// two 61 us, clusters of eight, where a thread has two groups, 157 us). Verification needs them once: kSlice values a CTA and nothing held, two CTAs a
+// multiprocessor (742 rows of 128,256, the call: 119 us, 159 us in registers), but for rows that one CTA holds (896 of 9,000: 34 us, 37 us).
+// Rows in registers run in CTAs of 256 threads from four a multiprocessor on, whose warps have more to do between two exchanges (300 rows of 32,000:
+// 22.9 us, 24.6 us with 512 threads), and of 512 threads below, whose single round is shorter (64 rows of 151,669: 28.2 us, 31.0 us with 256).
+// Vocabularies of up to 5,112 run in CTAs of 128 threads, eight a multiprocessor, each with a row (2,304 rows of 5,000: 34 us, 49 us with 512).
 constexpr int kSlice = 65536;
-struct RowPlan { int log_parts, units; };
+constexpr int kNarrowUnits = 10;
+struct RowPlan { int log_parts, units, threads; };
 inline RowPlan row_plan(int V, long long rows, bool keeps = false) {
     const long long groups = (static_cast<long long>(V) + 6) / 4, sms = sm_count();         // with an edge on either side
+    constexpr long long kHeld = static_cast<long long>(kRowThreads) * kRowUnitsMost;        // groups that a CTA holds (of 256 threads: twice as many each)
+    if (groups <= kNarrowThreads * kNarrowUnits && rows > 2 * sms) return {0, kNarrowUnits, kNarrowThreads};
     int log_parts = 0;
-    while ((1 << log_parts) < kRowCtasMost && ((static_cast<long long>(kSlice) << log_parts) < V ||
-                                               ((keeps || (rows << log_parts) * 2 <= 2 * sms) && groups > (2LL * kRowThreads << log_parts)))) ++log_parts;
-    const long long per = (((groups - 1) >> log_parts) + 32) & ~31LL, units = (per + kRowThreads - 1) / kRowThreads;
-    if (!keeps && rows << log_parts > 2 * sms) return {log_parts, 0};
-    return {log_parts, units <= 2 ? 2 : units <= 4 ? 4 : units <= 8 ? 8 : units <= kRowUnitsMost ? kRowUnitsMost : 0};
+    while ((1 << log_parts) < kRowCtasMost && (groups > ((keeps ? kHeld : kSlice / 4LL) << log_parts) ||
+                                               ((rows << log_parts) * 2 <= 2 * sms && groups > (2LL * kRowThreads << log_parts)))) ++log_parts;
+    const long long per = (((groups - 1) >> log_parts) + 32) & ~31LL, ctas = rows << log_parts;
+    if (per > kHeld) return {log_parts, 0, kRowThreads};
+    if (ctas > 4 * sms && (keeps || log_parts == 0)) {
+        const long long units = (per + kSmallThreads - 1) / kSmallThreads;
+        return {log_parts, units <= 8 ? 8 : units <= 12 ? 12 : units <= 16 ? 16 : 20, kSmallThreads};
+    }
+    if (!keeps && ctas > 2 * sms) return {log_parts, 0, kRowThreads};
+    const long long units = (per + kRowThreads - 1) / kRowThreads;
+    return {log_parts, units <= 2 ? 2 : units <= 4 ? 4 : units <= 8 ? 8 : kRowUnitsMost, kRowThreads};
 }
-
-// Many rows of a small vocabulary: blocks of four warps, eight a multiprocessor, each with a row in registers (2,304 rows of 5,000: 34 us, 49 us with
-// blocks of sixteen warps, whose threads have too few values for what a row costs besides).
-constexpr int kNarrowThreads = 128, kNarrowUnits = 10, kNarrowVocab = 4 * kNarrowThreads * kNarrowUnits - 8;
 
 template <typename T, bool kProbs>
 int launch_rows(RowArgs a, int rows, int places, cudaStream_t st, const char* what) {
-    RowPlan plan = row_plan(a.V, static_cast<long long>(rows) * places, kProbs);
-    const bool narrow = a.V <= kNarrowVocab && static_cast<long long>(rows) * places > 2 * sm_count();
-    if (narrow) plan.log_parts = 0;
+    const RowPlan plan = row_plan(a.V, static_cast<long long>(rows) * places, kProbs);
     a.log_parts = plan.log_parts;
     GI_REQUIRE(rows <= INT_MAX >> plan.log_parts && places <= 65535, "%s: %d rows of %d places exceed the grid limit", what, rows, places);
     const dim3 grid(static_cast<unsigned>(rows) << plan.log_parts, places);
-    const int parts = 1 << plan.log_parts;
-    if (narrow) {
-        launch_row_clusters((row_softmax_kernel<T, kNarrowUnits, kProbs, kNarrowThreads>), grid, kNarrowThreads, 1, st, a);
-        return check_launch(what);
-    }
-    switch (plan.units) {
-        case 2: launch_row_clusters((row_softmax_kernel<T, 2, kProbs, kRowThreads>), grid, kRowThreads, parts, st, a); break;
-        case 4: launch_row_clusters((row_softmax_kernel<T, 4, kProbs, kRowThreads>), grid, kRowThreads, parts, st, a); break;
-        case 8: launch_row_clusters((row_softmax_kernel<T, 8, kProbs, kRowThreads>), grid, kRowThreads, parts, st, a); break;
-        case kRowUnitsMost: launch_row_clusters((row_softmax_kernel<T, kRowUnitsMost, kProbs, kRowThreads>), grid, kRowThreads, parts, st, a); break;
-        default: launch_row_clusters((row_softmax_kernel<T, 0, kProbs, kRowThreads>), grid, kRowThreads, parts, st, a); break;
+    auto run = [&](auto kernel) { launch_row_clusters(kernel, grid, plan.threads, 1 << plan.log_parts, st, a); };
+    if (plan.threads == kNarrowThreads) {
+        run(row_softmax_kernel<T, kNarrowUnits, kProbs, kNarrowThreads>);
+    } else if (plan.threads == kSmallThreads) {
+        switch (plan.units) {
+            case 8: run(row_softmax_kernel<T, 8, kProbs, kSmallThreads>); break;
+            case 12: run(row_softmax_kernel<T, 12, kProbs, kSmallThreads>); break;
+            case 16: run(row_softmax_kernel<T, 16, kProbs, kSmallThreads>); break;
+            default: run(row_softmax_kernel<T, 20, kProbs, kSmallThreads>); break;
+        }
+    } else {
+        switch (plan.units) {
+            case 2: run(row_softmax_kernel<T, 2, kProbs, kRowThreads>); break;
+            case 4: run(row_softmax_kernel<T, 4, kProbs, kRowThreads>); break;
+            case 8: run(row_softmax_kernel<T, 8, kProbs, kRowThreads>); break;
+            case kRowUnitsMost: run(row_softmax_kernel<T, kRowUnitsMost, kProbs, kRowThreads>); break;
+            default: run(row_softmax_kernel<T, 0, kProbs, kRowThreads>); break;
+        }
     }
     return check_launch(what);
 }

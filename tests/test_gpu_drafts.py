@@ -166,6 +166,14 @@ def test_more_rows_than_the_gpu_holds_at_a_time(dtype, R, D, V, masked, probs):
         assert torch.equal(again[0], tokens) and torch.equal(again[1], accepted)
 
 
+@pytest.mark.parametrize("dtype,V,masked,probs", [("float32", 12001, False, True), ("bfloat16", 16381, True, False), ("float32", 20003, True, True),
+                                                  ("bfloat16", 20480, False, True)])
+def test_many_rows_that_one_block_holds(dtype, V, masked, probs):
+    args = inputs(V, 160, 3, V, dtype, masked=masked, probs=probs)
+    tokens, accepted = verify(*args)
+    check_verification(*args, tokens, accepted)
+
+
 def test_every_count_of_kept_drafts_comes_up():
     args = inputs(3, 300, 4, 50, "float32")
     tokens, accepted = verify(*args)
@@ -337,6 +345,30 @@ def test_token_probabilities(dtype, rows, V):
             want = torch.zeros(V)
             want[argmax_of(logits[r].float())] = 1.0
             assert torch.equal(out[r], want)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,V", [(310, 5113), (620, 8191), (600, 12001), (640, 16380), (601, 20475), (310, 20481), (150, 32003), (320, 40959),
+                                    (160, 50257), (170, 81917), (76, 128256), (77, 163837), (40, 200003)])
+def test_token_probabilities_of_many_rows(dtype, rows, V):
+    """Blocks of a row, clusters of two to eight, each size of block: rows against the formula, all of them against calls of a few rows (whose sum
+    may round the other way: two 32-bit roundings of a value)."""
+    g = torch.Generator().manual_seed(V)
+    logits = (torch.randn(rows, V, generator=g) * 4).to(dt(dtype)).to(DEV)
+    logits[:, V // 2:V // 2 + 9] = -math.inf
+    logits[rows // 2] = -math.inf
+    t = (0.3 + torch.rand(rows, generator=g)).to(DEV)
+    t[rows - 1] = 0.0
+    out = torch.full((rows, V), float("nan"), device=DEV)
+    K().token_probabilities(logits, t, out)
+    for r in (0, 1, rows - 2):
+        p, bound = distribution(logits[r].float().cpu(), float(t[r]))
+        assert bool(((out[r].double().cpu() - p).abs() <= bound).all()), r
+    assert torch.isnan(out[rows // 2]).all()
+    few = torch.empty_like(out)
+    for r in range(0, rows, 5):
+        K().token_probabilities(logits[r:r + 5], t[r:r + 5], few[r:r + 5])
+    torch.testing.assert_close(out, few, rtol=2.0 ** -21, atol=2.0 ** -126, equal_nan=True)
 
 
 def test_token_probabilities_of_rows_without_any_and_of_extreme_temperatures():
