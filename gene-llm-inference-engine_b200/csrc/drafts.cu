@@ -14,7 +14,7 @@
 //
 // What bounds it: few rows the chain of read, exchange, exponentials, exchange (one user's five rows of 128,256: 6.5 us, the draw 9.7 us of which 4.4
 // read p and q); many rows the instructions, 22 a value where the exponential and the quotient alone take 12 (128 requests, 742 rows, of which 550 are
-// looked at: 115 us and 42 us for the draws; 0.48 of the copy bandwidth for what the call cannot do without).
+// looked at: 84 us and 42 us for the draws, 119 us in all; 0.57 of the copy bandwidth for what the call cannot do without).
 #include <climits>
 
 #include <cooperative_groups.h>
@@ -647,16 +647,20 @@ inline void launch_row_clusters(void (*kernel)(KArgs...), dim3 grid, int threads
 // Rows in registers run in CTAs of 256 threads from four a multiprocessor on, whose warps have more to do between two exchanges (300 rows of 32,000:
 // 22.9 us, 24.6 us with 512 threads), and of 512 threads below, whose single round is shorter (64 rows of 151,669: 28.2 us, 31.0 us with 256).
 // Vocabularies of up to 5,112 run in CTAs of 128 threads, eight a multiprocessor, each with a row (2,304 rows of 5,000: 34 us, 49 us with 512).
-constexpr int kSlice = 65536;
+constexpr int kSlice = 65536, kDrawSlice = 32768;
 constexpr int kNarrowUnits = 10;
+// The fewest CTAs a row that have at most `most` groups each (or the most there are); more while all of them still fit the GPU at once.
+inline int fewest_parts(long long groups, long long rows, long long most) {
+    int log_parts = 0;
+    while ((1 << log_parts) < kRowCtasMost && (groups > most << log_parts || (rows << log_parts <= sm_count() && groups > (2LL * kRowThreads << log_parts)))) ++log_parts;
+    return log_parts;
+}
 struct RowPlan { int log_parts, units, threads; };
 inline RowPlan row_plan(int V, long long rows, bool keeps = false) {
     const long long groups = (static_cast<long long>(V) + 6) / 4, sms = sm_count();         // with an edge on either side
     constexpr long long kHeld = static_cast<long long>(kRowThreads) * kRowUnitsMost;        // groups that a CTA holds (of 256 threads: twice as many each)
     if (groups <= kNarrowThreads * kNarrowUnits && rows > 2 * sms) return {0, kNarrowUnits, kNarrowThreads};
-    int log_parts = 0;
-    while ((1 << log_parts) < kRowCtasMost && (groups > ((keeps ? kHeld : kSlice / 4LL) << log_parts) ||
-                                               ((rows << log_parts) * 2 <= 2 * sms && groups > (2LL * kRowThreads << log_parts)))) ++log_parts;
+    const int log_parts = fewest_parts(groups, rows, keeps ? kHeld : kSlice / 4);
     const long long per = (((groups - 1) >> log_parts) + 32) & ~31LL, ctas = rows << log_parts;
     if (per > kHeld) return {log_parts, 0, kRowThreads};
     if (ctas > 4 * sms && (keeps || log_parts == 0)) {
@@ -706,7 +710,9 @@ int launch_verify(RowArgs a, cudaStream_t st) {
         if (check_launch("verify_drafts")) return 1;
     }
     if (const int rc = launch_rows<T, false>(a, a.R, a.D + 1, st, "verify_drafts")) return rc;
-    a.log_parts = row_plan(a.V, 1).log_parts;
+    // the draw, a cluster a request (250 requests of 32,000: 66 us in one CTA each, 99 us in eight; 128 of 128,256: 119 us in four or eight, 128 us in two)
+    a.log_parts = fewest_parts((static_cast<long long>(a.V) + 6) / 4, a.R, kDrawSlice / 4);
+    GI_REQUIRE(a.R <= INT_MAX >> a.log_parts, "verify_drafts: %d requests exceed the grid limit", a.R);
     launch_row_clusters((draft_draw_kernel<T>), dim3(static_cast<unsigned>(a.R) << a.log_parts), kRowThreads, 1 << a.log_parts, st, a);
     return check_launch("verify_drafts");
 }
