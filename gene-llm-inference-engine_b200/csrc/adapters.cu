@@ -10,6 +10,7 @@
 // and out, each in a phase of its own that starts with an exchange (2,048 rows of 4,096 into 6,144, rank 16: 33 us for 18 us of bytes: 8 us for x, 4.5 for the
 // exchanges, 16 for out); high ranks also the tensor cores and what feeds them (8,192 rows of 14,336 into 4,096, rank 64: 63 us for x, 44 us for out).
 #include <climits>
+#include <type_traits>
 
 #include <cooperative_groups.h>
 
@@ -779,12 +780,17 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_many_kernel(Adapte
 }
 
 // ---- 32-bit on the CUDA cores ----
-// 700 rows of 2,048 into 2,048 at rank 12: 15 us (2.7 us of bytes); 2,048 rows of 14,336 into 4,096 at rank 64: 213 us, 0.3 of the multiply-add rate.
+// 700 rows of 2,048 into 2,048 at rank 12: 14 us (2.7 us of bytes), what bounds it the latency of the stages and the exchanges; 2,048 rows of 14,336 into
+// 4,096 at rank 64: 213 us, 0.3 of the multiply-add rate, bound by the reads of shared memory. A tile's own count of rows bounds its work: one row of
+// 4,096 at rank 16 10.6 us (15.9 us with all 32 rows of the tile), 8 rows of 2,048 into 8,192 at rank 32 19 us (30 us).
 // x and `down` pass through a ring of stages of 32 values of K (rows of 128 bytes, 16-byte pieces exchanged by the row's last three bits). Of 16 neighbouring
 // threads each has four columns of `kRows` rows, or with few ranks (S r below 64) a share of every stage's K instead, so that none is idle.
 template <int kRows> struct FloatShape {
     static constexpr int kTile = 16 * kRows, kStageBytes = (kTile + 64) * 128, kStages = kRows == 2 ? 6 : 5;
 };
+// Where a column's first 16-byte piece of a stage lies: the column's last three bits in reverse, so that eight neighbouring threads, whatever their share of
+// columns and of pieces, read eight different ones (42 rows of 14,336 at rank 12, where four threads share K: 33 us, 42 us with the bits as they are).
+__device__ __forceinline__ int piece_of(int col) { return (col & 1) << 2 | (col & 2) | (col >> 2 & 1); }
 template <int kRows>
 __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(AdapterArgs a) {
     pdl_prologue();
@@ -807,7 +813,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(Adapt
     const int stages = (k_end - k_begin + 31) / 32;
     const unsigned ring_at = shared_address(ring);
     const int copy_row = threadIdx.x >> 3, copy_k = 4 * (threadIdx.x & 7);
-    const unsigned copy_to = copy_row * 128 + (((threadIdx.x & 7) ^ (copy_row & 7)) << 4);
+    const unsigned copy_to = copy_row * 128 + (((threadIdx.x & 7) ^ (copy_row & 7)) << 4), copy_col_to = copy_row * 128 + (((threadIdx.x & 7) ^ piece_of(copy_row)) << 4);
     const float* x_rows[M / 32];
     int x_bytes[M / 32];
 #pragma unroll
@@ -817,25 +823,27 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(Adapt
         x_rows[i] = x + max(row, 0) * a.ldx;
     }
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    for (int c0 = 0; c0 < cols; c0 += 64) {
+    // `kThere` of the thread's rows for the columns c0 ..
+    auto pass = [&](int c0, auto rows) {
+        constexpr int kThere = decltype(rows)::value;
         const int some = min(64, cols - c0);
         int log_groups = 0;                    // threads across the columns: 2^log_groups of 16, the others share K
         while ((4 << log_groups) < some) ++log_groups;
         const int groups = 1 << log_groups, across = tx & (groups - 1), split = tx >> log_groups, splits = 16 >> log_groups;
         auto fetch = [&](int stage, int slot) {
-            const unsigned at = ring_at + slot * Shape::kStageBytes + copy_to;
+            const unsigned at = ring_at + slot * Shape::kStageBytes;
             const int k = k_begin + 32 * stage + copy_k;
             const bool in = k < k_end;
 #pragma unroll
-            for (int i = 0; i < M / 32; ++i) copy_16(at + i * 32 * 128, in ? x_rows[i] + k : x, in ? x_bytes[i] : 0);
+            for (int i = 0; i < M / 32; ++i) copy_16(at + copy_to + i * 32 * 128, in ? x_rows[i] + k : x, in ? x_bytes[i] : 0);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 if (copy_row + 32 * i < 4 * groups) {
                     const bool there = in && copy_row + 32 * i < some;
-                    copy_16(at + (M + i * 32) * 128, there ? down + static_cast<size_t>(c0 + copy_row + 32 * i) * a.K + k : down, there ? 16 : 0);
+                    copy_16(at + copy_col_to + (M + i * 32) * 128, there ? down + static_cast<size_t>(c0 + copy_row + 32 * i) * a.K + k : down, there ? 16 : 0);
                 }
         };
-        float acc[kRows][4] = {};
+        float acc[kThere][4] = {};
         __syncthreads();                       // (a further pass: the ring is free again)
 #pragma unroll
         for (int i = 0; i < Shape::kStages - 1; ++i) {
@@ -852,19 +860,19 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(Adapt
             next = slot;
             slot = slot + 1 == Shape::kStages ? 0 : slot + 1;
             for (int q = split; q < 8; q += splits) {
-                float4 xv[kRows], w[4];
+                float4 xv[kThere], w[4];
 #pragma unroll
-                for (int m = 0; m < kRows; ++m) {
+                for (int m = 0; m < kThere; ++m) {
                     const int row = ty + 16 * m;
                     xv[m] = *reinterpret_cast<const float4*>(at + row * 128 + ((q ^ (row & 7)) << 4));
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int col = across + groups * j;
-                    w[j] = *reinterpret_cast<const float4*>(at + (M + col) * 128 + ((q ^ (col & 7)) << 4));
+                    w[j] = *reinterpret_cast<const float4*>(at + (M + col) * 128 + ((q ^ piece_of(col)) << 4));
                 }
 #pragma unroll
-                for (int m = 0; m < kRows; ++m)
+                for (int m = 0; m < kThere; ++m)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         acc[m][j] = fmaf(xv[m].x, w[j].x, acc[m][j]);
@@ -876,7 +884,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(Adapt
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-        for (int m = 0; m < kRows; ++m)
+        for (int m = 0; m < kThere; ++m)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float v = acc[m][j];
@@ -888,10 +896,13 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(Adapt
                 const int col = across + groups * j;
                 if (split == 0 && col < some) h[(ty + 16 * m) * hs + c0 + col] = v;
             }
-    }
+    };
+    for (int c0 = 0; c0 < cols; c0 += 64)
+        if (n <= 16) pass(c0, std::integral_constant<int, 1>{});
+        else pass(c0, std::integral_constant<int, kRows>{});
     cluster.sync();
     // every CTA adds up its share of the tile's sums and gives them to all
-    const int fours = M * cols / 4, four_share = (fours + parts - 1) / parts, fours_end = min(fours, (part + 1) * four_share);
+    const int fours = n * cols / 4, four_share = (fours + parts - 1) / parts, fours_end = min(fours, (part + 1) * four_share);
     for (int i = part * four_share + threadIdx.x; i < fours_end; i += kAdapterThreads) {
         const int row = 4 * i / cols, col = 4 * i % cols;
         const float4 v = cluster_total(h + row * hs + col, scale, cluster, parts);
@@ -900,31 +911,41 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(Adapt
             if (p < parts) *reinterpret_cast<float4*>(cluster.map_shared_rank(sums + row * hs + col, p)) = v;
     }
     cluster.sync();
-    // a column a thread, half of the rows a warp
-    constexpr int kHalf = M / 2;
-    const int row0 = (threadIdx.x >> 7) * kHalf;
     float* out = static_cast<float*>(a.out);
-    const int n_share = (a.N + parts - 1) / parts, n_begin = min(a.N, part * n_share), n_end = row0 < n ? min(a.N, n_begin + n_share) : 0;
-    for (int col = n_begin + (threadIdx.x & 127); col < n_end; col += 128) {
-        int slice = 0;
+    const int n_share = (a.N + parts - 1) / parts, n_begin = min(a.N, part * n_share), n_end = min(a.N, n_begin + n_share);
+    // a column a thread, `kEach` rows from row0 on
+    auto expand = [&](auto rows, int row0, int first, int step) {
+        constexpr int kEach = decltype(rows)::value;
+        for (int col = n_begin + first; col < n_end; col += step) {
+            int slice = 0;
 #pragma unroll
-        for (int s = 0; s < kAdapterSlicesMost - 1; ++s) slice += s < a.S - 1 && col >= a.ends[s];
-        const float* at = sums + row0 * hs + slice * a.r;
-        const float* w_at = up + static_cast<size_t>(col) * a.r;
-        float acc[kHalf] = {};
-        for (int j = 0; j < a.r; j += 4) {
-            const float4 w = __ldg(reinterpret_cast<const float4*>(w_at + j));
+            for (int s = 0; s < kAdapterSlicesMost - 1; ++s) slice += s < a.S - 1 && col >= a.ends[s];
+            const float* at = sums + row0 * hs + slice * a.r;
+            const float* w_at = up + static_cast<size_t>(col) * a.r;
+            float acc[kEach] = {};
+            for (int j = 0; j < a.r; j += 4) {
+                const float4 w = __ldg(reinterpret_cast<const float4*>(w_at + j));
 #pragma unroll
-            for (int i = 0; i < kHalf; ++i) {
-                const float4 v = *reinterpret_cast<const float4*>(at + i * hs + j);
-                acc[i] = fmaf(v.x, w.x, fmaf(v.y, w.y, fmaf(v.z, w.z, fmaf(v.w, w.w, acc[i]))));
+                for (int i = 0; i < kEach; ++i) {
+                    const float4 v = *reinterpret_cast<const float4*>(at + i * hs + j);
+                    acc[i] = fmaf(v.x, w.x, fmaf(v.y, w.y, fmaf(v.z, w.z, fmaf(v.w, w.w, acc[i]))));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int row = s_rows[row0 + i];
+                if (row >= 0) asm volatile("red.global.add.f32 [%0], %1;" :: "l"(out + row * a.ldo + col), "f"(acc[i]) : "memory");
             }
         }
-#pragma unroll
-        for (int i = 0; i < kHalf; ++i) {
-            const int row = s_rows[row0 + i];
-            if (row >= 0) asm volatile("red.global.add.f32 [%0], %1;" :: "l"(out + row * a.ldo + col), "f"(acc[i]) : "memory");
-        }
+    };
+    // (few rows: all threads across the columns; many: half of the rows a thread)
+    if (n <= 4) {
+        expand(std::integral_constant<int, 4>{}, 0, threadIdx.x, kAdapterThreads);
+    } else if (n <= 16) {
+        expand(std::integral_constant<int, 16>{}, 0, threadIdx.x, kAdapterThreads);
+    } else {
+        const int row0 = (threadIdx.x >> 7) * (M / 2);
+        if (row0 < n) expand(std::integral_constant<int, M / 2>{}, row0, threadIdx.x & 127, 128);
     }
 }
 
