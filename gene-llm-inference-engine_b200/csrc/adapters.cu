@@ -786,10 +786,10 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_many_kernel(Adapte
 // x and `down` pass through a ring of stages of 32 values of K (rows of 128 bytes, 16-byte pieces exchanged by the row's last three bits). Of 16 neighbouring
 // threads each has four columns of `kRows` rows, or with few ranks (S r below 64) a share of every stage's K instead, so that none is idle.
 template <int kRows> struct FloatShape {
-    static constexpr int kTile = 16 * kRows, kStageBytes = (kTile + 64) * 128, kStages = kRows == 2 ? 6 : 5;
+    static constexpr int kTile = 16 * kRows, kStageBytes = (kTile + 64) * 128, kStages = kRows == 1 ? 7 : kRows == 2 ? 6 : 5;
 };
 // Where a column's first 16-byte piece of a stage lies: the column's last three bits in reverse, so that eight neighbouring threads, whatever their share of
-// columns and of pieces, read eight different ones (42 rows of 14,336 at rank 12, where four threads share K: 33 us, 42 us with the bits as they are).
+// columns and of pieces, read eight different ones (42 rows of 14,336 at rank 12, where four threads share K, tiles of 32 rows: 33 us, 42 us with the bits as they are).
 __device__ __forceinline__ int piece_of(int col) { return (col & 1) << 2 | (col & 2) | (col >> 2 & 1); }
 template <int kRows>
 __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(AdapterArgs a) {
@@ -814,11 +814,12 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(Adapt
     const unsigned ring_at = shared_address(ring);
     const int copy_row = threadIdx.x >> 3, copy_k = 4 * (threadIdx.x & 7);
     const unsigned copy_to = copy_row * 128 + (((threadIdx.x & 7) ^ (copy_row & 7)) << 4), copy_col_to = copy_row * 128 + (((threadIdx.x & 7) ^ piece_of(copy_row)) << 4);
-    const float* x_rows[M / 32];
-    int x_bytes[M / 32];
+    constexpr int kCopies = (M + 31) / 32;
+    const float* x_rows[kCopies];
+    int x_bytes[kCopies];
 #pragma unroll
-    for (int i = 0; i < M / 32; ++i) {
-        const int row = s_rows[copy_row + 32 * i];
+    for (int i = 0; i < kCopies; ++i) {
+        const int row = copy_row + 32 * i < M ? s_rows[copy_row + 32 * i] : -1;
         x_bytes[i] = row >= 0 ? 16 : 0;
         x_rows[i] = x + max(row, 0) * a.ldx;
     }
@@ -835,7 +836,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(Adapt
             const int k = k_begin + 32 * stage + copy_k;
             const bool in = k < k_end;
 #pragma unroll
-            for (int i = 0; i < M / 32; ++i) copy_16(at + copy_to + i * 32 * 128, in ? x_rows[i] + k : x, in ? x_bytes[i] : 0);
+            for (int i = 0; i < kCopies; ++i)
+                if (copy_row + 32 * i < M) copy_16(at + copy_to + i * 32 * 128, in ? x_rows[i] + k : x, in ? x_bytes[i] : 0);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 if (copy_row + 32 * i < 4 * groups) {
@@ -898,8 +900,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(Adapt
             }
     };
     for (int c0 = 0; c0 < cols; c0 += 64)
-        if (n <= 16) pass(c0, std::integral_constant<int, 1>{});
-        else pass(c0, std::integral_constant<int, kRows>{});
+        if (kRows == 1 || n <= 16) pass(c0, std::integral_constant<int, 1>{});
+        else if constexpr (kRows > 1) pass(c0, std::integral_constant<int, kRows>{});
     cluster.sync();
     // every CTA adds up its share of the tile's sums and gives them to all
     const int fours = n * cols / 4, four_share = (fours + parts - 1) / parts, fours_end = min(fours, (part + 1) * four_share);
@@ -941,9 +943,9 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_float_kernel(Adapt
     // (few rows: all threads across the columns; many: half of the rows a thread)
     if (n <= 4) {
         expand(std::integral_constant<int, 4>{}, 0, threadIdx.x, kAdapterThreads);
-    } else if (n <= 16) {
+    } else if (kRows == 1 || n <= 16) {
         expand(std::integral_constant<int, 16>{}, 0, threadIdx.x, kAdapterThreads);
-    } else {
+    } else if constexpr (kRows > 1) {
         const int row0 = (threadIdx.x >> 7) * (M / 2);
         if (row0 < n) expand(std::integral_constant<int, M / 2>{}, row0, threadIdx.x & 127, 128);
     }
@@ -1041,6 +1043,9 @@ int launch_f32(const AdapterArgs& a, cudaStream_t st) {
     if (!pieces) return launch_plain<float, float>(a, st);
     // (2,048 rows of 14,336 into 4,096 at rank 64: tiles of 64 rows 215 us, of 32 263 us; 1,024 rows of 2,048 at rank 16: 27 and 22 us)
     if (a.plan.T >= 2048 && a.S * a.r <= 256) return launch_float<4>(a, st);
+    // (tiles of 16 rows: 250 rows of 4,096 into 4,096, two adapters of rank 64, 45 us, of 32 66 us, and 42 of
+    // 14,336 at rank 12 26 and 33 us; 150 of 8,192 into 2,048, four of rank 64, 58 and 53 us)
+    if (a.plan.T <= kFewTokens) return launch_float<1>(a, st);
     return launch_float<2>(a, st);
 }
 

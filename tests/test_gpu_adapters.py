@@ -212,3 +212,10 @@ def test_few_of_many_adapters(T):
     got = out.clone()
     K_().adapter_product(x, down, up, scales, K_().adapter_plan(ids, 900, used=5), got)
     compare(x, down, up, scales, out, ids, (72,), got)
+
+
+def test_the_rows_that_need_no_plan_are_the_librarys():
+    from geneinfer_b200.ops import kernels
+    from geneinfer_b200.ops.library import lib
+    assert lib().gi_adapter_direct_rows(kernels.ADAPTER_DIRECT_ADAPTERS) == kernels.ADAPTER_DIRECT_ROWS
+    assert lib().gi_adapter_direct_rows(kernels.ADAPTER_DIRECT_ADAPTERS + 1) == 0
