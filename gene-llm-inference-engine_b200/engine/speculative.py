@@ -42,6 +42,8 @@ class _Side:
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self.row_start = torch.empty(requests + 1, dtype=torch.int32, device=dev)
         self.row_req, self.positions, self.slots = (torch.empty(step_tokens, dtype=torch.int32, device=dev) for _ in range(3))
+        # a step's tokens and counts are copied here: recorded launches name where they lie
+        self.tokens, self.counts = torch.zeros(step_tokens, dtype=torch.int32, device=dev), torch.zeros(requests, dtype=torch.int32, device=dev)
         self.all_rows = torch.arange(max(step_tokens, logit_rows), dtype=torch.int32, device=dev)
         self.no_slots = torch.zeros(requests, dtype=torch.int32, device=dev)
 
@@ -50,10 +52,12 @@ class _Side:
         """A step of ``counts`` tokens a request behind the ``lengths`` cached ones (on the device; ``bounds``: what they are at
         most), with logits at every row or none."""
         T, R = tokens.numel(), self.requests
-        kernels.step_tables(lengths, counts_dev, self.tables, self.held, self.free, self.n_free, self.page_size, self.row_start,
+        self.tokens[:T].copy_(tokens)
+        self.counts.copy_(counts_dev)
+        kernels.step_tables(lengths, self.counts, self.tables, self.held, self.free, self.n_free, self.page_size, self.row_start,
                             self.row_req[:T], self.positions[:T], self.slots[:T], self.status)
-        views = {"tokens": tokens, "positions": self.positions[:T], "row_req": self.row_req[:T], "logit_rows": self.all_rows[:T if logits else 0],
-                 "state_slots": self.no_slots, "seg_start": self.row_start[:R], "seg_len": counts_dev, "tables": [self.tables]}
+        views = {"tokens": self.tokens[:T], "positions": self.positions[:T], "row_req": self.row_req[:T], "logit_rows": self.all_rows[:T if logits else 0],
+                 "state_slots": self.no_slots, "seg_start": self.row_start[:R], "seg_len": self.counts, "tables": [self.tables]}
         if row_adapter is not None:
             views["row_adapter"] = row_adapter
         segments, row = [], 0

@@ -276,3 +276,21 @@ def test_the_command_line_with_an_adapter_and_a_draft_model(tmp_path, capsys):
     assert run("--model", gf.model_dir("a"), "--adapter", folder, "--draft-model", gf.model_dir("a_named"), "--drafts", "3") == want
     assert main([*common, "--model", merged, "--draft-model", merged, "--top-p", "0.9"]) == 2
     assert main([*common, "--model", merged, "--draft-model", merged, "--drafts", "0"]) == 2
+
+
+def test_experts_named_by_token_ids_see_the_steps_own_tokens(tmp_path):
+    """Recorded launches name the place of a step's tokens: portions of prompts of one size, one after another, and the steps of a drafter. One rank for all layers, so
+    that a single group of pages serves the design."""
+    import pinorax_configs as pc
+    from geneinfer_b200 import Engine, SpeculativeEngine
+    layers = [pc.layer(3, 24, 40, 48, 0.2, pc.moe(40, 0.8, 7, 2, shared=(56, 1.7))), pc.layer(5, 8, 16, 48, 0.3, pc.moe(72, 2.5, 5, 1)),
+              pc.layer(2, 16, 24, 48, 0.25, pc.dense(64))]
+    folders = [pc.make_model_dir(pc.model(96, 190, 256, 1e-5, 0.45, 9.0, layers), seed, str(tmp_path / f"model{seed}"), std=0.2) for seed in (3, 4)]
+    prompts = [tc.random_tokens(n, 190, 30 + n) for n in (75, 20, 1, 130)]
+    want = Engine(folders[0], dtype="float32", max_running=2).generate(prompts, max_new_tokens=20)
+    for draft in folders:
+        engine = SpeculativeEngine(folders[0], draft, dtype="float32", max_running=2, max_seq_len=200, step_tokens=16)
+        for _ in range(2):
+            assert engine.generate(prompts, max_new_tokens=20) == want
+        if draft == folders[0]:
+            assert engine.kept >= 0.9 * engine.proposed > 0
