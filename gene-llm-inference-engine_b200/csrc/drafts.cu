@@ -465,10 +465,11 @@ __global__ void __launch_bounds__(kThreads, kThreads != kSmallThreads ? 1024 / k
         if (j > d) return;                 // (the whole cluster)
         row = a.row_start[r] + j;
         if (a.skip && j > 0) {
-            // A refusal ahead that has been seen: nobody asks for this row. The cluster's CTAs must all go or all stay: who comes first decides.
+            // A refusal ahead that has been seen: nobody asks for this row. The cluster's CTAs must all go or all stay: who comes first decides, in the
+            // place of the row's token, which belongs to this cluster alone even where requests share rows (the draw writes it afterwards).
             __shared__ int s_decided;
             if (threadIdx.x == 0) {
-                int* decided = reinterpret_cast<int*>(&a.work[row].w);
+                int* decided = a.tokens + static_cast<size_t>(r) * (a.D + 1) + j;
                 const int mine = *reinterpret_cast<volatile const int*>(a.accepted + r) < j ? 2 : 1;
                 const int before = atomicCAS(decided, 0, mine);
                 s_decided = before ? before : mine;
@@ -569,8 +570,9 @@ __global__ void __launch_bounds__(kThreads, kThreads != kSmallThreads ? 1024 / k
 // Ahead of rows of which some may be left out: no refusal known, no row decided.
 __global__ void __launch_bounds__(256) draft_begin_kernel(RowArgs a) {
     pdl_prologue();
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < max(a.N, a.R); i += gridDim.x * 256) {
-        if (i < a.N) a.work[i].w = 0.f;
+    const long long places = static_cast<long long>(a.R) * (a.D + 1);
+    for (long long i = blockIdx.x * 256 + threadIdx.x; i < places; i += gridDim.x * 256) {
+        a.tokens[i] = 0;
         if (i < a.R) a.accepted[i] = INT_MAX;
     }
 }

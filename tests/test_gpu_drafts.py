@@ -408,3 +408,15 @@ def test_the_quotient_by_the_temperature_is_the_divisions():
     K().token_probabilities(logits, t, out)
     e = torch.exp((logits - logits.amax(1, keepdim=True)) / t[:, None])
     assert torch.equal(out, e * (1.0 / e.double().sum(1, keepdim=True)).float())
+
+
+@pytest.mark.parametrize("dtype,R,D,V", [("float32", 600, 3, 6003), ("bfloat16", 150, 4, 70001), ("float32", 40, 15, 128256)])
+def test_requests_that_share_rows_end(dtype, R, D, V):
+    """Not a use (the rows' results are then anyone's), but every call ends, with tokens of the vocabulary. Rows may be left out here: clusters that decide it for themselves."""
+    logits, row_start, drafted, counts, q, t, accept, draw = inputs(V, R, D, V, dtype, probs=False)
+    counts[:] = D
+    row_start = torch.arange(R, dtype=torch.int32) % 3
+    logits = logits[:D + 4].contiguous()
+    for _ in range(3):
+        tokens, accepted = verify(logits, row_start, drafted, counts, None, t, accept, draw)
+        assert bool(((tokens >= -1) & (tokens < V)).all()) and bool(((accepted >= 0) & (accepted <= D)).all())
