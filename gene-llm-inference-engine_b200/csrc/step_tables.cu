@@ -105,8 +105,8 @@ __global__ void __launch_bounds__(kTableThreads, 1) step_tables_kernel(TableArgs
         count = a.row_start ? a.counts[r] : 0;
         held = a.held[r];
         if (length < 0 || count < 0 || held < 0 || held > a.stride) return false;
-        const long long pages = (static_cast<long long>(length) + count + a.page - 1) / a.page;
-        fits = pages <= a.stride;
+        const long long end = static_cast<long long>(length) + count, pages = (end + a.page - 1) / a.page;
+        fits = pages <= a.stride && end <= INT_MAX;             // (positions are 32-bit, also where a table has room for more)
         need = static_cast<int>(pages < a.stride ? pages : a.stride);
         return true;
     };

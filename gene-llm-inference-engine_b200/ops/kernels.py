@@ -1630,7 +1630,7 @@ def step_tables(lengths: torch.Tensor, counts: torch.Tensor, tables: torch.Tenso
     prefixes are the host manager's business.
 
     ``status`` [1]: 0; else nothing but the status has been written: the number of pages missing, -1 (more rows than places), -2 (a
-    request beyond its table), -3 (a negative number, or more pages held than the table has), -4 (more free pages than the stack holds)."""
+    request beyond its table, or with 2^31 positions or more), -3 (a negative number, or more pages held than the table has), -4 (more free pages than the stack holds)."""
     R, args = _table_args(lengths, tables, held, free_pages, n_free, status)
     rows = row_req.numel()
     if counts.numel() != R or row_start.numel() != R + 1 or positions.numel() != rows or slots.numel() != rows:

@@ -219,3 +219,21 @@ def test_step_tables_refuses_what_does_not_fit():
     K().trim_tables(**trim)
     with pytest.raises(K().KernelError):
         K().trim_tables(**dict(trim, held=ints(4)))
+
+
+def test_positions_beyond_32_bits_are_refused():
+    """A table with room for three pages of 2^30 positions: a request of 2^31 positions is refused, one of 2^31 - 1 is not."""
+    for length, count, status in ((2 ** 31 - 1, 5, -2), (2 ** 31 - 6, 6, -2), (2 ** 31 - 6, 5, 0)):
+        out = [torch.full((n,), 77, dtype=torch.int32, device=DEV) for n in (2, 8, 8, 8)]
+        held, tables = torch.tensor([3], dtype=torch.int32, device=DEV), torch.tensor([[0, 0, 0, -1]], dtype=torch.int32, device=DEV)
+        n, free, word = (torch.tensor([v], dtype=torch.int32, device=DEV) for v in (0, 0, 77))
+        if status == 0:
+            held.fill_(2)
+        to = lambda v: torch.tensor([v], dtype=torch.int32, device=DEV)      # noqa: E731
+        K().step_tables(to(length), to(count), tables, held, free, n, 1 << 30, *out, word)
+        assert int(word) == status
+        if status:
+            assert all(bool((x == 77).all()) for x in out) and int(held) == 3
+        else:
+            last = 2 ** 31 - 2
+            assert out[2].tolist() == list(range(length, last + 1)) + [0] * 3 and out[3].tolist() == [p % (1 << 30) for p in range(length, last + 1)] + [-1] * 3
