@@ -25,7 +25,8 @@ from .step import Segment, StepContext, StepEngine
 class _Side:
     """One of the two models with pages of its own and block tables that live on the device."""
 
-    def __init__(self, model, page_size: int, requests: int, positions: int, step_tokens: int, logit_rows: int):
+    def __init__(self, model, page_size: int, requests: int, positions: int, step_tokens: int, logit_rows: int, status: torch.Tensor):
+        """``status``: a word for every call of the step tables that a round makes (int32, on the device)."""
         stride = (positions + page_size - 1) // page_size
         pool = requests * stride
         self.model, self.page_size, self.requests = model, page_size, requests
@@ -39,7 +40,7 @@ class _Side:
         self.held = torch.zeros(requests, dtype=torch.int32, device=dev)
         self.free = torch.arange(pool, dtype=torch.int32, device=dev)
         self.n_free = torch.full((1,), pool, dtype=torch.int32, device=dev)
-        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.status = status
         self.row_start = torch.empty(requests + 1, dtype=torch.int32, device=dev)
         self.row_req, self.positions, self.slots = (torch.empty(step_tokens, dtype=torch.int32, device=dev) for _ in range(3))
         # a step's tokens and counts are copied here: recorded launches name where they lie
@@ -48,14 +49,18 @@ class _Side:
         self.no_slots = torch.zeros(requests, dtype=torch.int32, device=dev)
 
     def forward(self, tokens: torch.Tensor, counts: Sequence[int], counts_dev: torch.Tensor, lengths: torch.Tensor, bounds: Sequence[int],
-                logits: bool, row_adapter: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                logits: bool, row_adapter: Optional[torch.Tensor] = None, word: int = 0) -> Optional[torch.Tensor]:
         """A step of ``counts`` tokens a request behind the ``lengths`` cached ones (on the device; ``bounds``: what they are at
-        most), with logits at every row or none."""
+        most), with logits at every row or none. ``word``: the status word of the call that makes its tables. A refused call leaves the tables of the
+        step before, on which the model must not run: so it is refused here already where the bounds leave room for it."""
         T, R = tokens.numel(), self.requests
+        pages = [(b + n + self.page_size - 1) // self.page_size for b, n in zip(bounds, counts)]
+        if max(pages) > self.tables.shape[1] or sum(pages) > self.free.numel():
+            raise RuntimeError(f"step tables: {sum(pages)} pages, up to {max(pages)} a request, of {self.free.numel()} and {self.tables.shape[1]}")
         self.tokens[:T].copy_(tokens)
         self.counts.copy_(counts_dev)
         kernels.step_tables(lengths, self.counts, self.tables, self.held, self.free, self.n_free, self.page_size, self.row_start,
-                            self.row_req[:T], self.positions[:T], self.slots[:T], self.status)
+                            self.row_req[:T], self.positions[:T], self.slots[:T], self.status[word:word + 1])
         views = {"tokens": self.tokens[:T], "positions": self.positions[:T], "row_req": self.row_req[:T], "logit_rows": self.all_rows[:T if logits else 0],
                  "state_slots": self.no_slots, "seg_start": self.row_start[:R], "seg_len": self.counts, "tables": [self.tables]}
         if row_adapter is not None:
@@ -76,13 +81,7 @@ class _Side:
         return out
 
     def trim(self, lengths: torch.Tensor) -> None:
-        kernels.trim_tables(lengths, self.tables, self.held, self.free, self.n_free, self.page_size, self.status)
-
-    def check(self) -> None:
-        self.steps.check_status()
-        status = int(self.status)
-        if status:
-            raise RuntimeError(f"step tables were refused (status {status})")
+        kernels.trim_tables(lengths, self.tables, self.held, self.free, self.n_free, self.page_size, self.status[-1:])
 
 
 class SpeculativeEngine:
@@ -105,8 +104,10 @@ class SpeculativeEngine:
         self.vocab, self.device = target.vocab_size, target.device
         R, K, V = max_running, drafts, target.vocab_size
         self.step_tokens = max(step_tokens, R * (K + 1))
-        self.target = _Side(target, page_size, R, self.context + K + 1, self.step_tokens, R * (K + 1))
-        self.draft = _Side(draft, page_size, R, self.context + K + 1, self.step_tokens, R)
+        # how the calls of a round's step tables went (K + 1 steps and the trimming, a row a side), and what is not 0 among those of a batch so far
+        self._status, self._refused = (torch.zeros(2, K + 2, dtype=torch.int32, device=target.device) for _ in range(2))
+        self.target = _Side(target, page_size, R, self.context + K + 1, self.step_tokens, R * (K + 1), self._status[0])
+        self.draft = _Side(draft, page_size, R, self.context + K + 1, self.step_tokens, R, self._status[1])
         if adapter_slots:
             self.target.steps.enable_adapters(adapter_slots, adapter_rank)
         dev = self.device
@@ -128,6 +129,7 @@ class SpeculativeEngine:
         self._numbers_host = [torch.zeros(n).pin_memory() for _ in range(3)]
         self._numbers = [torch.zeros(n, device=dev) for _ in range(3)]
         self._out_host = [torch.zeros(R, K + 2, dtype=torch.int32).pin_memory() for _ in range(3)]
+        self._refused_host = [torch.zeros(2, K + 2, dtype=torch.int32).pin_memory() for _ in range(3)]
         self._done = [None] * 3
         self.rounds = self.proposed = self.kept = 0
 
@@ -168,8 +170,11 @@ class SpeculativeEngine:
             return [[] for _ in prompts]
         fill = lambda t, values, rest: t.copy_(torch.tensor(list(values) + [rest] * (R - n), dtype=t.dtype))      # noqa: E731
         self._lengths.zero_()
+        self._refused.zero_()
+        self._status.zero_()
         for side in (self.target, self.draft):
             side.trim(self._lengths)                           # (whatever an earlier batch held)
+        self._refused |= self._status
         fill(self._temperature, temps, 0.0)
         fill(self._adapters, slots, -1)
         fill(self._current, [p[-1] for p in prompts], 0)
@@ -196,7 +201,7 @@ class SpeculativeEngine:
                 break
             pending = now
         for side in (self.target, self.draft):
-            side.check()
+            side.steps.check_status()
         return results
 
     def _prefill(self, prompts, adapted: bool) -> None:
@@ -221,6 +226,7 @@ class SpeculativeEngine:
                 row_adapter.copy_(self._adapters[torch.tensor(rows).to(dev)])
             self.target.forward(ids, counts, self._counts, self._lengths, fed, False, row_adapter)
             self.draft.forward(ids, counts, self._counts, self._lengths, fed, False)
+            self._refused |= self._status
             self._lengths += self._counts
             fed = [f + c for f, c in zip(fed, counts)]
 
@@ -244,7 +250,7 @@ class SpeculativeEngine:
         ones = [1] * R
         for j in range(K + 1):
             tokens = self._current if j == 0 else self._ids[j - 1]
-            logits = self.draft.forward(tokens, ones, self._ones, self._at[j], [b + j for b in bounds], j < K)
+            logits = self.draft.forward(tokens, ones, self._ones, self._at[j], [b + j for b in bounds], j < K, word=j)
             if j < K:
                 kernels.token_probabilities(logits, self._temperature, self._probs[j])
                 kernels.argmax(logits, self._ids[j])
@@ -265,6 +271,8 @@ class SpeculativeEngine:
         self._lengths.copy_(torch.minimum(self._lengths + self._accepted + 1, self._ends))
         for side in (self.target, self.draft):
             side.trim(self._lengths)
+        self._refused |= self._status
+        self._refused_host[turn].copy_(self._refused, non_blocking=True)
         out = self._out_host[turn]
         out[:, :K + 1].copy_(self._tokens, non_blocking=True)
         out[:, K + 1].copy_(self._accepted, non_blocking=True)
@@ -276,6 +284,9 @@ class SpeculativeEngine:
     def _collect(self, pending, results, alive, max_new: int, stop_ids) -> None:
         turn, event = pending
         event.synchronize()
+        refused = self._refused_host[turn]
+        if refused.any():
+            raise RuntimeError(f"step tables were refused (status {int(refused[refused != 0][0])})")
         out = self._out_host[turn].tolist()
         self.rounds += 1
         for r, result in enumerate(results):

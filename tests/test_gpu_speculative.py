@@ -294,3 +294,43 @@ def test_experts_named_by_token_ids_see_the_steps_own_tokens(tmp_path):
             assert engine.generate(prompts, max_new_tokens=20) == want
         if draft == folders[0]:
             assert engine.kept >= 0.9 * engine.proposed > 0
+
+
+def test_a_refused_call_of_the_step_tables_ends_the_generation(monkeypatch):
+    """One call in the middle of a round, or in a prompt, says that it was refused (its tables are made all the same, so that the model runs on sound ones); the
+    calls behind it are met. The next generation starts from nothing."""
+    from geneinfer_b200.ops import kernels
+    engine = speculative("a", "a_named", "float32", max_running=2, step_tokens=10)
+    prompts = [tc.random_tokens(n, 256, n) for n in (25, 3)]
+    want = engine.generate(prompts, max_new_tokens=12)
+    for name in ("step_tables", "trim_tables"):
+        real = getattr(kernels, name)
+        for at in (0, 1, 5, 8):
+            calls = []
+
+            def some(*args, real=real, at=at, calls=calls):
+                real(*args)
+                calls.append(None)
+                if len(calls) == at + 1:
+                    args[-1].fill_(-2)
+
+            monkeypatch.setattr(kernels, name, some)
+            with pytest.raises(RuntimeError, match="-2"):
+                engine.generate(prompts, max_new_tokens=12)
+            monkeypatch.setattr(kernels, name, real)
+            assert len(calls) > at + 1
+            assert engine.generate(prompts, max_new_tokens=12) == want
+
+
+def test_a_step_that_the_pool_may_not_hold_is_not_run():
+    """Sides whose pool (or whose tables) are smaller than their requests can grow: the step is refused on the host, ahead of any kernel that would run on the tables of another."""
+    for side in ("target", "draft"):
+        for name in ("free", "tables"):
+            engine = speculative("a", "a_named", "float32", max_running=2)
+            some = getattr(engine, side)
+            if name == "free":
+                some.free, some.n_free = some.free[:2].contiguous(), some.n_free.fill_(2)
+            else:
+                some.tables = some.tables[:, :1].contiguous()
+            with pytest.raises(RuntimeError, match="pages"):
+                engine.generate([tc.random_tokens(25, 256, 1), [3]], max_new_tokens=12)
