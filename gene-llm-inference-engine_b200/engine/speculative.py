@@ -70,15 +70,20 @@ class _Side:
             segments.append(Segment(r, row, n, bounds[r], 0, False))
             row += n
         steps = self.steps
-        steps._poll_status(wait=False)
-        failures = kernels.status_failures(steps.device)
         steps._aux_calls = 0
         ctx = StepContext(steps, T, R, T if logits else 0, segments, views)
         with kernels.on_current_stream():
             steps._begin_adapters(ctx)
-            out = self.model.forward(ctx)
-        steps._post_status(failures)
-        return out
+            return self.model.forward(ctx)
+
+    def begin(self) -> None:
+        """Ahead of the steps of a round, or of a portion of prompts: looks at the kernels' status behind those that have finished. ``end``: behind them (once a
+        round: the engine remembers a few places only, and waits for the oldest of them)."""
+        self.steps._poll_status(wait=False)
+        self._failures = kernels.status_failures(self.steps.device)
+
+    def end(self) -> None:
+        self.steps._post_status(self._failures)
 
     def trim(self, lengths: torch.Tensor) -> None:
         kernels.trim_tables(lengths, self.tables, self.held, self.free, self.n_free, self.page_size, self.status[-1:])
@@ -104,8 +109,8 @@ class SpeculativeEngine:
         self.vocab, self.device = target.vocab_size, target.device
         R, K, V = max_running, drafts, target.vocab_size
         self.step_tokens = max(step_tokens, R * (K + 1))
-        # how the calls of a round's step tables went (K + 1 steps and the trimming, a row a side), and what is not 0 among those of a batch so far
-        self._status, self._refused = (torch.zeros(2, K + 2, dtype=torch.int32, device=target.device) for _ in range(2))
+        # how the calls of a round's step tables went (K + 1 steps and the trimming, a row a side)
+        self._status = torch.zeros(2, K + 2, dtype=torch.int32, device=target.device)
         self.target = _Side(target, page_size, R, self.context + K + 1, self.step_tokens, R * (K + 1), self._status[0])
         self.draft = _Side(draft, page_size, R, self.context + K + 1, self.step_tokens, R, self._status[1])
         if adapter_slots:
@@ -117,7 +122,11 @@ class SpeculativeEngine:
         self._ids, self._drafted, self._fed = ints(K, R), ints(R, K), ints(R, K + 1)
         self._ones, self._counts, self._rows = ints(R) + 1, ints(R), ints(R) + (K + 1)
         self._starts = torch.arange(R, dtype=torch.int32, device=dev) * (K + 1)
-        self._tokens, self._accepted = ints(R, K + 1), ints(R)
+        # what a round leaves for the host, in one piece (a copy of columns would wait for the device): the tokens, how many drafts were kept, and which calls of
+        # the step tables were refused in the batch so far
+        self._out = ints((R + 2) * (K + 2))
+        self._tokens, self._accepted, self._refused = self._out.split([R * (K + 1), R, 2 * (K + 2)])
+        self._tokens, self._refused = self._tokens.view(R, K + 1), self._refused.view(2, K + 2)
         self._probs = torch.empty(K, R, V, dtype=torch.float32, device=dev)
         self._scratch = torch.empty(R, V, dtype=torch.float32, device=dev)
         self._work = torch.empty(R * (K + 1), 4, dtype=torch.float32, device=dev)
@@ -128,8 +137,7 @@ class SpeculativeEngine:
         n = R * (2 * K + 1)
         self._numbers_host = [torch.zeros(n).pin_memory() for _ in range(3)]
         self._numbers = [torch.zeros(n, device=dev) for _ in range(3)]
-        self._out_host = [torch.zeros(R, K + 2, dtype=torch.int32).pin_memory() for _ in range(3)]
-        self._refused_host = [torch.zeros(2, K + 2, dtype=torch.int32).pin_memory() for _ in range(3)]
+        self._out_host = [torch.zeros(self._out.numel(), dtype=torch.int32).pin_memory() for _ in range(3)]
         self._done = [None] * 3
         self.rounds = self.proposed = self.kept = 0
 
@@ -224,8 +232,10 @@ class SpeculativeEngine:
             if adapted:
                 row_adapter = self._row_adapter[:len(rows)]
                 row_adapter.copy_(self._adapters[torch.tensor(rows).to(dev)])
-            self.target.forward(ids, counts, self._counts, self._lengths, fed, False, row_adapter)
-            self.draft.forward(ids, counts, self._counts, self._lengths, fed, False)
+            for side, adapter in ((self.target, row_adapter), (self.draft, None)):
+                side.begin()
+                side.forward(ids, counts, self._counts, self._lengths, fed, False, adapter)
+                side.end()
             self._refused |= self._status
             self._lengths += self._counts
             fed = [f + c for f, c in zip(fed, counts)]
@@ -248,6 +258,7 @@ class SpeculativeEngine:
         # the drafts, and one step more that only leaves the last one's keys and values
         torch.add(self._lengths, torch.arange(K + 1, dtype=torch.int32, device=self.device)[:, None], out=self._at)
         ones = [1] * R
+        self.draft.begin()
         for j in range(K + 1):
             tokens = self._current if j == 0 else self._ids[j - 1]
             logits = self.draft.forward(tokens, ones, self._ones, self._at[j], [b + j for b in bounds], j < K, word=j)
@@ -255,6 +266,7 @@ class SpeculativeEngine:
                 kernels.token_probabilities(logits, self._temperature, self._probs[j])
                 kernels.argmax(logits, self._ids[j])
                 kernels.sample(logits, self._scratch, self._temperature, self._no_top_k, self._no_top_p, numbers[j * R:(j + 1) * R], self._ids[j])
+        self.draft.end()
         self._drafted.copy_(self._ids.t())
         self._fed[:, 0].copy_(self._current)
         self._fed[:, 1:].copy_(self._drafted)
@@ -262,7 +274,9 @@ class SpeculativeEngine:
         if adapted:
             row_adapter = self._row_adapter[:R * (K + 1)]
             row_adapter.view(R, K + 1).copy_(self._adapters[:, None].expand(R, K + 1))
+        self.target.begin()
         logits = self.target.forward(self._fed.view(-1), [K + 1] * R, self._rows, self._lengths, bounds, True, row_adapter)
+        self.target.end()
         self._counts.fill_(K)
         kernels.verify_drafts(logits, self._starts, self._drafted, self._counts, self._probs.transpose(0, 1), self._temperature, accept, draw,
                               self._tokens, self._accepted, self._work)
@@ -272,10 +286,7 @@ class SpeculativeEngine:
         for side in (self.target, self.draft):
             side.trim(self._lengths)
         self._refused |= self._status
-        self._refused_host[turn].copy_(self._refused, non_blocking=True)
-        out = self._out_host[turn]
-        out[:, :K + 1].copy_(self._tokens, non_blocking=True)
-        out[:, K + 1].copy_(self._accepted, non_blocking=True)
+        self._out_host[turn].copy_(self._out, non_blocking=True)
         event = torch.cuda.Event()
         event.record()
         self._done[turn] = event
@@ -284,17 +295,19 @@ class SpeculativeEngine:
     def _collect(self, pending, results, alive, max_new: int, stop_ids) -> None:
         turn, event = pending
         event.synchronize()
-        refused = self._refused_host[turn]
-        if refused.any():
-            raise RuntimeError(f"step tables were refused (status {int(refused[refused != 0][0])})")
+        R, K = self.requests, self.drafts
         out = self._out_host[turn].tolist()
+        refused = next((status for status in out[R * (K + 2):] if status), 0)
+        if refused:
+            raise RuntimeError(f"step tables were refused (status {refused})")
+        kept = out[R * (K + 1):R * (K + 2)]
         self.rounds += 1
         for r, result in enumerate(results):
             if not alive[r]:
                 continue
             self.proposed += self.drafts
-            self.kept += out[r][-1]
-            for token in out[r][:out[r][-1] + 1]:
+            self.kept += kept[r]
+            for token in out[r * (K + 1):r * (K + 1) + kept[r] + 1]:
                 result.append(int(token))
                 if token in stop_ids or len(result) == max_new:
                     alive[r] = False

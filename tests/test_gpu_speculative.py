@@ -334,3 +334,24 @@ def test_a_step_that_the_pool_may_not_hold_is_not_run():
                 some.tables = some.tables[:, :1].contiguous()
             with pytest.raises(RuntimeError, match="pages"):
                 engine.generate([tc.random_tokens(25, 256, 1), [3]], max_new_tokens=12)
+
+
+def test_a_round_is_launched_without_a_wait_for_what_runs():
+    """Half a second of earlier work on the stream: the rounds of three requests return while it still runs."""
+    engine = speculative("a", "a_named", "float32", max_running=3)
+    prompts = [tc.random_tokens(n, 256, n) for n in (25, 3, 9)]
+    want = engine.generate(prompts, max_new_tokens=12)
+    real, waited = engine._round, []
+
+    def behind_work(*args):
+        if len(waited) == 1:                   # (the second round: the first is still to be collected)
+            torch.cuda._sleep(1_000_000_000)
+        earlier = torch.cuda.Event()
+        earlier.record()
+        out = real(*args)
+        waited.append(earlier.query())
+        return out
+
+    engine._round = behind_work
+    assert engine.generate(prompts, max_new_tokens=12) == want
+    assert len(waited) > 2 and not waited[1]
