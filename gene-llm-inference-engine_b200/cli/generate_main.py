@@ -152,14 +152,15 @@ def _with_drafts(o: dict, device: str) -> int:
     context = o["max_seq_len"] or read_config(o["model"])[1].max_position_embeddings
     positions = min(o["steps"], context) if o["steps"] > 0 else context
     rank = _adapter_rank(o["adapter"]) if o["adapter"] else 0
-    # (a request's own positions, and those that a refused round may touch)
     engine = SpeculativeEngine(o["model"], o["draft_model"], drafts=o["drafts"], dtype="float32" if o["weights"] == "f32" else "bfloat16", device=device,
-                               max_running=1, max_seq_len=positions + 1, page_size=o["page_size"], adapter_slots=1 if rank else 0, adapter_rank=rank or 16)
+                               max_running=1, max_seq_len=positions, page_size=o["page_size"], adapter_slots=1 if rank else 0, adapter_rank=rank or 16)
     if rank:
         engine.load_adapter(0, o["adapter"])
-    new = min(positions, engine.context - 1) - len(prompt) + 1
+    if engine.context < positions and not o["quiet"]:
+        sys.stderr.write(f"[drafts] the models' contexts end the generation at {engine.context} positions\n")
+    new = engine.context - len(prompt) + 1
     if new < 1:
-        raise ValueError(f"a prompt of {len(prompt)} tokens does not fit in {positions} positions")
+        raise ValueError(f"a prompt of {len(prompt)} tokens does not fit in {engine.context} positions")
     t0 = time.perf_counter()
     out = engine.generate([prompt], new, o["temperature"], o["seed"], o["stop_ids"], [0] if rank else None)[0]
     seconds = time.perf_counter() - t0

@@ -94,39 +94,42 @@ class SpeculativeEngine:
                  max_seq_len: int = 2048, page_size: int = 16, step_tokens: int = 2048, decode_weight_copy: bool = True,
                  adapter_slots: int = 0, adapter_rank: int = 16):
         """``model_dir``, ``draft_dir``: the served and the proposing model, of one vocabulary. ``drafts``: tokens proposed a
-        round. ``max_seq_len``: positions of a request at most (prompt and generated tokens). The other arguments are ``Engine``'s."""
+        round (fewer where a request that runs is nearer to the end of the models' contexts than that). ``max_seq_len``: positions of a request at most, of the
+        prompt and all generated tokens but the last, which is not fed. The other arguments are ``Engine``'s."""
         if drafts < 1 or max_running < 1:
             raise ValueError("drafted tokens: drafts and max_running must be positive")
         self.drafts, self.requests, self.page_size = drafts, max_running, page_size
-        room = max_seq_len + drafts + 1            # positions that a round may write behind the last one that stays
+        room = max_seq_len + drafts                # (positions that a full round may write behind the last one that stays)
         target = load_model(model_dir, dtype=dtype, device=device, max_position=room, weight_tiles=decode_weight_copy)
         draft = load_model(draft_dir, dtype=dtype, device=device, max_position=room, weight_tiles=decode_weight_copy)
         if target.vocab_size != draft.vocab_size:
             raise ValueError(f"drafted tokens: the models' vocabularies differ ({target.vocab_size} and {draft.vocab_size})")
-        self.context = min(target.max_position, draft.max_position) - drafts - 1
-        if self.context < 2:
+        self.positions = min(target.max_position, draft.max_position)
+        self.context = min(max_seq_len, self.positions)
+        if self.context < 1:
             raise ValueError("drafted tokens: the context is too short")
         self.vocab, self.device = target.vocab_size, target.device
         R, K, V = max_running, drafts, target.vocab_size
         self.step_tokens = max(step_tokens, R * (K + 1))
         # how the calls of a round's step tables went (K + 1 steps and the trimming, a row a side)
         self._status = torch.zeros(2, K + 2, dtype=torch.int32, device=target.device)
-        self.target = _Side(target, page_size, R, self.context + K + 1, self.step_tokens, R * (K + 1), self._status[0])
-        self.draft = _Side(draft, page_size, R, self.context + K + 1, self.step_tokens, R, self._status[1])
+        self.target = _Side(target, page_size, R, self.positions, self.step_tokens, R * (K + 1), self._status[0])
+        self.draft = _Side(draft, page_size, R, self.positions, self.step_tokens, R, self._status[1])
         if adapter_slots:
             self.target.steps.enable_adapters(adapter_slots, adapter_rank)
         dev = self.device
         ints = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=dev)      # noqa: E731
         self._lengths, self._current, self._ends = ints(R), ints(R), ints(R)
         self._at = ints(K + 1, R)                                   # lengths of the drafting steps
-        self._ids, self._drafted, self._fed = ints(K, R), ints(R, K), ints(R, K + 1)
-        self._ones, self._counts, self._rows = ints(R) + 1, ints(R), ints(R) + (K + 1)
-        self._starts = torch.arange(R, dtype=torch.int32, device=dev) * (K + 1)
+        self._ids, self._drafted, self._fed = ints(K, R), ints(R * K), ints(R * (K + 1))
+        self._counts = ints(R)
+        # of a round of k drafts: drafts a request, rows a request, its first row
+        self._some = [(ints(R) + k, ints(R) + (k + 1), torch.arange(R, dtype=torch.int32, device=dev) * (k + 1)) for k in range(K + 1)]
         # what a round leaves for the host, in one piece (a copy of columns would wait for the device): the tokens, how many drafts were kept, and which calls of
         # the step tables were refused in the batch so far
         self._out = ints((R + 2) * (K + 2))
         self._tokens, self._accepted, self._refused = self._out.split([R * (K + 1), R, 2 * (K + 2)])
-        self._tokens, self._refused = self._tokens.view(R, K + 1), self._refused.view(2, K + 2)
+        self._refused = self._refused.view(2, K + 2)
         self._probs = torch.empty(K, R, V, dtype=torch.float32, device=dev)
         self._scratch = torch.empty(R, V, dtype=torch.float32, device=dev)
         self._work = torch.empty(R * (K + 1), 4, dtype=torch.float32, device=dev)
@@ -158,7 +161,7 @@ class SpeculativeEngine:
         have = self.target.steps.adapter_step.slots if self.target.steps.adapter_step is not None else 0
         for p, t, a in zip(prompts, temps, slots):
             SamplingParams(temperature=float(t))               # (refuses what is no temperature)
-            if not 1 <= len(p) or len(p) + max_new_tokens > self.context:
+            if not 1 <= len(p) or len(p) + max_new_tokens - 1 > self.context:
                 raise ValueError(f"generate: a prompt of {len(p)} tokens and {max_new_tokens} more do not fit in {self.context} positions")
             if any(not 0 <= int(x) < self.vocab for x in p):
                 raise ValueError("generate: token id out of range")
@@ -186,28 +189,29 @@ class SpeculativeEngine:
         fill(self._temperature, temps, 0.0)
         fill(self._adapters, slots, -1)
         fill(self._current, [p[-1] for p in prompts], 0)
-        # places without a request run along on position 0; a request that has ended stays at its end
+        # places without a request, and those whose request has ended (0 as well), run along from position 0 on
         ends = [len(p) - 1 + max_new for p in prompts] + [0] * (R - n)
         self._ends.copy_(torch.tensor(ends, dtype=torch.int32))
         adapted = any(a >= 0 for a in slots)
         self._prefill(prompts, adapted)
         streams = [RandomStream(s) for s in seeds]
-        lengths = [len(p) - 1 for p in prompts] + [0] * (R - n)
+        lengths = [len(p) - 1 for p in prompts] + [0] * (R - n)          # as of the rounds that have been collected
         results: List[List[int]] = [[] for _ in prompts]
         alive = [True] * n
-        pending = None
+        pending, ahead = None, 0                               # the round that is not collected yet, and the tokens that it may give
         rounds = 0
         while True:
             now = None
             if any(alive) and rounds < max_new:                # (a round gives every request a token at least)
-                bounds = [min(l + rounds * (self.drafts + 1), e) for l, e in zip(lengths, ends)]
-                now = self._round(rounds % 3, streams, temps, bounds, adapted)
+                bounds = [min(l + ahead, e - 1) if e else 0 for l, e in zip(lengths, ends)]
+                drafts = min(self.drafts, self.positions - 1 - max(bounds))          # (a round of k drafts writes k positions behind the length)
+                now = self._round(rounds % 3, drafts, streams, temps, bounds, adapted)
                 rounds += 1
             if pending is not None:
-                self._collect(pending, results, alive, max_new, stop_ids)
+                self._collect(pending, lengths, ends, results, alive, max_new, stop_ids)
             if now is None:
                 break
-            pending = now
+            pending, ahead = now, drafts + 1
         for side in (self.target, self.draft):
             side.steps.check_status()
         return results
@@ -240,9 +244,9 @@ class SpeculativeEngine:
             self._lengths += self._counts
             fed = [f + c for f, c in zip(fed, counts)]
 
-    def _round(self, turn: int, streams, temps, bounds, adapted: bool):
-        """Launches a round; its tokens are on their way to the host behind the returned event."""
-        R, K = self.requests, self.drafts
+    def _round(self, turn: int, K: int, streams, temps, bounds, adapted: bool):
+        """Launches a round of ``K`` drafts; its tokens are on their way to the host behind the returned event."""
+        R = self.requests
         if self._done[turn] is not None:
             self._done[turn].synchronize()
         host, numbers = self._numbers_host[turn], self._numbers[turn]
@@ -254,35 +258,38 @@ class SpeculativeEngine:
                     host[K * R + r * K + j] = stream.next_uniform()              # whether it is kept
                 host[2 * K * R + r] = stream.next_uniform()                      # the token behind the kept ones
         numbers.copy_(host, non_blocking=True)
-        accept, draw = numbers[K * R:2 * K * R].view(R, K), numbers[2 * K * R:]
+        accept, draw = numbers[K * R:2 * K * R].view(R, K), numbers[2 * K * R:2 * K * R + R]
+        drafts, rows, starts = self._some[K]
+        drafted, fed, result = self._drafted[:R * K].view(R, K), self._fed[:R * (K + 1)].view(R, K + 1), self._tokens[:R * (K + 1)].view(R, K + 1)
         # the drafts, and one step more that only leaves the last one's keys and values
-        torch.add(self._lengths, torch.arange(K + 1, dtype=torch.int32, device=self.device)[:, None], out=self._at)
+        torch.add(self._lengths, torch.arange(K + 1, dtype=torch.int32, device=self.device)[:, None], out=self._at[:K + 1])
         ones = [1] * R
         self.draft.begin()
         for j in range(K + 1):
             tokens = self._current if j == 0 else self._ids[j - 1]
-            logits = self.draft.forward(tokens, ones, self._ones, self._at[j], [b + j for b in bounds], j < K, word=j)
+            logits = self.draft.forward(tokens, ones, self._some[0][1], self._at[j], [b + j for b in bounds], j < K, word=j)
             if j < K:
                 kernels.token_probabilities(logits, self._temperature, self._probs[j])
                 kernels.argmax(logits, self._ids[j])
                 kernels.sample(logits, self._scratch, self._temperature, self._no_top_k, self._no_top_p, numbers[j * R:(j + 1) * R], self._ids[j])
         self.draft.end()
-        self._drafted.copy_(self._ids.t())
-        self._fed[:, 0].copy_(self._current)
-        self._fed[:, 1:].copy_(self._drafted)
+        drafted.copy_(self._ids[:K].t())
+        fed[:, 0].copy_(self._current)
+        fed[:, 1:].copy_(drafted)
         row_adapter = None
         if adapted:
             row_adapter = self._row_adapter[:R * (K + 1)]
             row_adapter.view(R, K + 1).copy_(self._adapters[:, None].expand(R, K + 1))
         self.target.begin()
-        logits = self.target.forward(self._fed.view(-1), [K + 1] * R, self._rows, self._lengths, bounds, True, row_adapter)
+        logits = self.target.forward(fed.view(-1), [K + 1] * R, rows, self._lengths, bounds, True, row_adapter)
         self.target.end()
-        self._counts.fill_(K)
-        kernels.verify_drafts(logits, self._starts, self._drafted, self._counts, self._probs.transpose(0, 1), self._temperature, accept, draw,
-                              self._tokens, self._accepted, self._work)
-        # the next round starts behind what was kept
-        self._current.copy_(self._tokens.gather(1, self._accepted.long()[:, None])[:, 0])
-        self._lengths.copy_(torch.minimum(self._lengths + self._accepted + 1, self._ends))
+        kernels.verify_drafts(logits, starts, drafted, drafts, self._probs[:K].transpose(0, 1), self._temperature, accept, draw, result, self._accepted, self._work)
+        # the next round starts behind what was kept; requests that have ended from nothing
+        self._current.copy_(result.gather(1, self._accepted.long()[:, None])[:, 0])
+        self._lengths += self._accepted + 1
+        ended = self._lengths >= self._ends
+        self._lengths.masked_fill_(ended, 0)
+        self._ends.masked_fill_(ended, 0)
         for side in (self.target, self.draft):
             side.trim(self._lengths)
         self._refused |= self._status
@@ -290,22 +297,27 @@ class SpeculativeEngine:
         event = torch.cuda.Event()
         event.record()
         self._done[turn] = event
-        return turn, event
+        return turn, K, event
 
-    def _collect(self, pending, results, alive, max_new: int, stop_ids) -> None:
-        turn, event = pending
+    def _collect(self, pending, lengths, ends, results, alive, max_new: int, stop_ids) -> None:
+        """A round's tokens into ``results``; ``lengths`` and ``ends`` follow those on the device."""
+        turn, K, event = pending
         event.synchronize()
-        R, K = self.requests, self.drafts
+        R = self.requests
         out = self._out_host[turn].tolist()
-        refused = next((status for status in out[R * (K + 2):] if status), 0)
+        kept, statuses = out[R * (self.drafts + 1):R * (self.drafts + 2)], out[R * (self.drafts + 2):]
+        refused = next((status for status in statuses if status), 0)
         if refused:
             raise RuntimeError(f"step tables were refused (status {refused})")
-        kept = out[R * (K + 1):R * (K + 2)]
         self.rounds += 1
+        for r in range(R):
+            lengths[r] += kept[r] + 1
+            if lengths[r] >= ends[r]:
+                lengths[r] = ends[r] = 0
         for r, result in enumerate(results):
             if not alive[r]:
                 continue
-            self.proposed += self.drafts
+            self.proposed += K
             self.kept += kept[r]
             for token in out[r * (K + 1):r * (K + 1) + kept[r] + 1]:
                 result.append(int(token))

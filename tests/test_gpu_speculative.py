@@ -355,3 +355,33 @@ def test_a_round_is_launched_without_a_wait_for_what_runs():
     engine._round = behind_work
     assert engine.generate(prompts, max_new_tokens=12) == want
     assert len(waited) > 2 and not waited[1]
+
+
+@pytest.mark.parametrize("drafts", [1, 4])
+@pytest.mark.parametrize("draft", ["a", "a_named"])
+def test_generation_up_to_the_end_of_the_context(draft, drafts):
+    """128 positions, of which the last token's is the last one fed: rounds near the end propose fewer tokens, down to none. Requests end at different places, one
+    long before the others, one at the context's last position with its prompt."""
+    from geneinfer_b200 import Engine
+    for lengths, new in (((10, 60, 119, 2), 10), ((128, 20), 1), ((126, 125, 30), 3), ((9,), 120)):
+        prompts = [tc.random_tokens(n, 256, 60 + n) for n in lengths]
+        want = Engine(gf.model_dir("a"), dtype="float32", max_running=4).generate(prompts, max_new_tokens=new)
+        engine = speculative("a", draft, "float32", drafts=drafts, max_seq_len=128)
+        assert engine.generate(prompts, max_new_tokens=new) == want
+        for side in (engine.target, engine.draft):
+            held = side.tables[side.tables >= 0].tolist()
+            assert sorted(held + side.free[:int(side.n_free)].tolist()) == list(range(side.free.numel()))
+    sampled = engine.generate([prompts[0]] * 3, max_new_tokens=120, temperature=0.8, seed=3)
+    assert [len(s) for s in sampled] == [120] * 3 and sampled[0] != sampled[1]
+    with pytest.raises(ValueError):
+        engine.generate([tc.random_tokens(10, 256, 1)], max_new_tokens=120)
+
+
+def test_the_command_line_with_a_draft_model_fills_the_context(capsys):
+    from geneinfer_b200.cli.generate_main import main
+    common = ["--model", gf.model_dir("a"), "--prompt-ids", " ".join(map(str, tc.random_tokens(11, 256, 12))), "--temperature", "0", "--dtype", "fp32", "--quiet"]
+    for more in ([], ["--steps", "400"], ["--max-seq-len", "70"], ["--steps", "60"]):
+        assert main([*common, *more]) == 0
+        want = capsys.readouterr().out.split()
+        assert main([*common, *more, "--draft-model", gf.model_dir("a_named")]) == 0
+        assert capsys.readouterr().out.split() == want
