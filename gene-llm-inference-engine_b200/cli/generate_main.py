@@ -24,7 +24,8 @@ USAGE = (
     "  configuration in FILE, a config.json) to DIR, or to a temporary folder when no --model is given.\n"
     "  --adapter DIR: a low-rank adapter (adapter_config.json, adapter_model.safetensors) beside the model's weights.\n"
     "  --draft-model DIR: a model of the same vocabulary proposes N tokens a step (default 4), which the model checks;\n"
-    "  the result is distributed as without it. Top-k and top-p are then off.\n")
+    "  the result is distributed as without it and written once it is whole. Top-k and top-p are then off; --profile\n"
+    "  and --kv-pages (every request has room for the context) do not go with it.\n")
 
 
 class UsageError(Exception):
@@ -126,6 +127,8 @@ def parse(argv: List[str]) -> dict:
         raise UsageError("--device must be cuda: this engine has no CPU or emulated device")
     if o["draft_model"] and (o["top_k"] or (o["top_p"] is not None and o["top_p"] < 1.0)):
         raise UsageError("--draft-model cannot be combined with --top-k or --top-p")
+    if o["draft_model"] and (o["profile"] or o["kv_pages"] is not None):
+        raise UsageError(f"--draft-model cannot be combined with {'--profile' if o['profile'] else '--kv-pages'}")
     if o["draft_model"] and o["drafts"] < 1:
         raise UsageError("--drafts must be positive")
     if o["top_k"] is None:
@@ -149,7 +152,7 @@ def _with_drafts(o: dict, device: str) -> int:
     from ..engine.speculative import SpeculativeEngine
     from ..weights import read_config
     prompt = o["prompt_ids"]
-    context = o["max_seq_len"] or read_config(o["model"])[1].max_position_embeddings
+    context = o["max_seq_len"] or read_config(o["model"])[1].model_spec().max_position
     positions = min(o["steps"], context) if o["steps"] > 0 else context
     rank = _adapter_rank(o["adapter"]) if o["adapter"] else 0
     engine = SpeculativeEngine(o["model"], o["draft_model"], drafts=o["drafts"], dtype="float32" if o["weights"] == "f32" else "bfloat16", device=device,

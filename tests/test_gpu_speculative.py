@@ -385,3 +385,20 @@ def test_the_command_line_with_a_draft_model_fills_the_context(capsys):
         want = capsys.readouterr().out.split()
         assert main([*common, *more, "--draft-model", gf.model_dir("a_named")]) == 0
         assert capsys.readouterr().out.split() == want
+
+
+def test_the_command_line_with_drafts_and_a_design_of_its_own(tmp_path, capsys):
+    """Pinorax names its context ``max_positions``; what does not go with a draft model is refused by name."""
+    import pinorax_configs as pc
+    from geneinfer_b200.cli.generate_main import main
+    config = pc.model(96, 190, 64, 1e-5, 0.45, 9.0, [pc.layer(3, 24, 40, 48, 0.2, pc.dense(136)), pc.layer(5, 8, 16, 48, 0.3, pc.dense(64))])
+    folder = pc.make_model_dir(config, 5, str(tmp_path / "model"), std=0.2)
+    common = ["--model", folder, "--prompt-ids", "5 9 2 100", "--temperature", "0", "--dtype", "fp32", "--quiet"]
+    for more in ([], ["--max-seq-len", "40"], ["--steps", "20"]):
+        assert main([*common, *more]) == 0
+        want = capsys.readouterr().out.split()
+        assert main([*common, *more, "--draft-model", folder]) == 0, capsys.readouterr().err
+        assert capsys.readouterr().out.split() == want
+    for flags in (["--profile"], ["--kv-pages", "64"]):
+        assert main([*common, "--draft-model", folder, *flags]) == 2
+        assert flags[0] in capsys.readouterr().err
