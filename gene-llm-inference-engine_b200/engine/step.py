@@ -394,13 +394,17 @@ class StepEngine:
 
     def put_adapter(self, slot: int, pairs, scale: float) -> None:
         """``pairs``: {(layer, projection): a (down, up) or None for every part stacked in it}; projections that are not
-        named get none. The slot's requests run with it from the next step on."""
+        named get none. The slot's requests run with it from the next step on. Pairs that do not fit leave every slot as it was."""
         if self.adapter_step is None:
             raise RuntimeError("adapters are not enabled")
         known = {(layer, name) for layer, sets in self.adapter_sets.items() for name in sets}
         unknown = sorted(str(k) for k in set(pairs) - known)
         if unknown:
             raise ValueError(f"adapters: no such projection: {', '.join(unknown[:5])}")
+        for layer, sets in self.adapter_sets.items():
+            for name, adapters in sets.items():
+                of = pairs.get((layer, name))
+                adapters.check(slot, [None] * len(adapters.widths) if of is None else of)
         for layer, sets in self.adapter_sets.items():
             for name, adapters in sets.items():
                 if pairs.get((layer, name)) is None:

@@ -48,8 +48,8 @@ class AdapterSet:
         self.up[slot].zero_()
         self.scales[slot] = 0.0
 
-    def put(self, slot: int, pairs: Sequence, scale: float) -> None:
-        """``pairs``: a (down, up) for every part, or None for a part without one."""
+    def check(self, slot: int, pairs: Sequence) -> None:
+        """Raises ``ValueError`` where ``put`` cannot take the pairs."""
         self._check(slot)
         if len(pairs) != len(self.widths):
             raise ValueError(f"adapters: {len(pairs)} pairs for {len(self.widths)} parts")
@@ -62,6 +62,10 @@ class AdapterSet:
                                  f"{self.in_features} inputs and {self.widths[i]} outputs")
             if down.shape[0] > self.rank:
                 raise ValueError(f"adapters: rank {down.shape[0]} exceeds {self.rank}")
+
+    def put(self, slot: int, pairs: Sequence, scale: float) -> None:
+        """``pairs``: a (down, up) for every part, or None for a part without one."""
+        self.check(slot, pairs)
         self.clear(slot)
         at = 0
         for i, (pair, n) in enumerate(zip(pairs, self.widths)):

@@ -402,3 +402,31 @@ def test_the_command_line_with_drafts_and_a_design_of_its_own(tmp_path, capsys):
     for flags in (["--profile"], ["--kv-pages", "64"]):
         assert main([*common, "--draft-model", folder, *flags]) == 2
         assert flags[0] in capsys.readouterr().err
+
+
+def test_an_adapter_that_does_not_fit_leaves_the_slots_as_they_were(tmp_path):
+    from geneinfer_b200.weights.adapters import read_adapter
+    folder, _ = adapter_and_merged("a", 14, tmp_path)
+    steps = engine_of(gf.model_dir("a"), "float32", slots=2)
+    pairs, scale = read_adapter(folder)
+    steps.put_adapter(1, pairs, scale)
+    sets = [s for layer in steps.adapter_sets.values() for s in layer.values()]
+    before = [[t.clone() for t in (s.down, s.up, s.scales)] for s in sets]
+
+    def unchanged():
+        return all(torch.equal(a, b) for s, old in zip(sets, before) for a, b in zip((s.down, s.up, s.scales), old))
+
+    last = max(pairs)
+    for bad in (lambda d, u: (d[:, :-1], u), lambda d, u: (d, u[:-1]), lambda d, u: (d.repeat(3, 1), u.repeat(1, 3)), lambda d, u: (d[0], u)):
+        other = {k: [None if p is None else (p[0] + 1, p[1] + 1) for p in v] for k, v in pairs.items()}
+        other[last] = [bad(*p) if p is not None else None for p in other[last]]
+        with pytest.raises(ValueError):
+            steps.put_adapter(1, other, 2 * scale)
+        assert unchanged()
+    for slot in (-1, 2):
+        with pytest.raises(ValueError):
+            steps.put_adapter(slot, pairs, 2 * scale)
+        assert unchanged()
+    with pytest.raises(ValueError):
+        steps.put_adapter(1, {**pairs, last: pairs[last] + [None]}, 2 * scale)
+    assert unchanged()
