@@ -1077,6 +1077,9 @@ using namespace gi;
 
 // Rows of a step whose products need no plan, with so many adapters.
 extern "C" int gi_adapter_direct_rows(int A) { return A <= kDirectAdapters ? kDirectRows : 0; }
+// Ranks of all slices together, and adapters, at most.
+extern "C" int gi_adapter_ranks_most() { return kAdapterRanksMost; }
+extern "C" int gi_adapter_adapters_most() { return kPlanAdaptersMost; }
 
 static int gi_adapter_plan_impl(const int* row_adapter, int T, int A, int tile_rows, int* plan, void* stream) {
     GI_REQUIRE(T >= 0 && A > 0 && tile_rows > 0, "adapter_plan: sizes must be positive (T=%d, adapters=%d, tile rows=%d)", T, A, tile_rows);

@@ -370,7 +370,7 @@ class StepEngine:
     # ------------------------------------------------------------------ adapters
     def enable_adapters(self, slots: int, rank: int) -> None:
         """Room for ``slots`` low-rank adapters of up to ``rank`` beside the projections of every layer; entries then name a
-        slot each. Before the first step."""
+        slot each. Before the first step. Up to 8,192 slots, and ranks of up to 512 over the parts stacked in a projection (168 for queries, keys and values)."""
         if self.adapter_step is not None:
             raise RuntimeError("adapters are enabled already")
         found = {}
@@ -382,6 +382,9 @@ class StepEngine:
                     raise ValueError(f"adapters: layer {run.layer} has a part ({type(part).__name__}) that takes none")
                 for name, linear, widths in projections:
                     found.setdefault(run.layer, {})[name] = (linear, widths)
+        for projections in found.values():
+            for linear, widths in projections.values():
+                AdapterSet.check_sizes(slots, rank, widths)
         step = AdapterStep(slots, self.max_step_tokens, self.device)
         for layer, projections in found.items():
             for name, (linear, widths) in projections.items():

@@ -32,14 +32,27 @@ class AdapterStep:
 class AdapterSet:
     def __init__(self, slots: int, rank: int, in_features: int, widths: Sequence[int], dtype: torch.dtype, device: torch.device):
         """``widths``: the output columns of the parts stacked in the projection."""
-        if slots < 1 or rank < 1 or not widths:
-            raise ValueError("adapters: slots, rank and parts must be positive")
-        self.slots, self.rank = slots, (rank + 3) // 4 * 4          # (pieces of four ranks are read at once)
+        self.check_sizes(slots, rank, widths)
+        self.slots, self.rank = slots, self.rank_held(rank)
         self.widths = [int(n) for n in widths]
         self.in_features, self.out_features = in_features, sum(self.widths)
         self.down = torch.zeros(slots, len(self.widths) * self.rank, in_features, dtype=dtype, device=device)
         self.up = torch.zeros(slots, self.out_features, self.rank, dtype=dtype, device=device)
         self.scales = torch.zeros(slots, dtype=torch.float32, device=device)
+
+    @staticmethod
+    def rank_held(rank: int) -> int:
+        return (rank + 3) // 4 * 4                                  # (pieces of four ranks are read at once)
+
+    @classmethod
+    def check_sizes(cls, slots: int, rank: int, widths: Sequence[int]) -> None:
+        """Raises ``ValueError`` for sizes that the products do not take."""
+        if slots < 1 or rank < 1 or not widths:
+            raise ValueError("adapters: slots, rank and parts must be positive")
+        if slots > kernels.ADAPTER_ADAPTERS_MOST:
+            raise ValueError(f"adapters: {slots} slots (at most {kernels.ADAPTER_ADAPTERS_MOST})")
+        if len(widths) * cls.rank_held(rank) > kernels.ADAPTER_RANKS_MOST:
+            raise ValueError(f"adapters: rank {rank} in a projection that stacks {len(widths)} (at most {kernels.ADAPTER_RANKS_MOST // len(widths) // 4 * 4})")
 
     def clear(self, slot: int) -> None:
         """The slot's adapter is none: its rows get zeros added."""

@@ -1660,6 +1660,7 @@ class AdapterPlan:
 
 
 ADAPTER_TILE_ROWS = 128
+ADAPTER_RANKS_MOST, ADAPTER_ADAPTERS_MOST = 512, 8192      # ranks of all slices of a projection together, and adapters held, at most (as the library has them)
 ADAPTER_DIRECT_ROWS, ADAPTER_DIRECT_ADAPTERS = 1024, 1024      # steps of up to so many rows (and adapters) need no plan on the device: the products look rows up themselves
 
 
@@ -1674,8 +1675,8 @@ def adapter_plan(row_adapter: torch.Tensor, adapters: int, buffer: Optional[torc
     ``used``: so many different adapters occur at most (default: all), which bounds the blocks that find nothing to do where hundreds
     are loaded. Once a step: every product of the step takes the same plan, which reads ``row_adapter`` when it runs."""
     T = row_adapter.numel()
-    if not 1 <= adapters <= 8192:
-        raise KernelError(f"adapter_plan: {adapters} adapters (1 to 8192)")
+    if not 1 <= adapters <= ADAPTER_ADAPTERS_MOST:
+        raise KernelError(f"adapter_plan: {adapters} adapters (1 to {ADAPTER_ADAPTERS_MOST})")
     used = adapters if used is None else used
     if not 1 <= used <= adapters:
         raise KernelError(f"adapter_plan: {used} of {adapters} adapters used")
@@ -1705,7 +1706,7 @@ def adapter_product(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale
     row's adapter (rows without one are left alone). ``x`` [T, K] and the weights of one dtype, ``down`` [adapters, S * rank, K],
     ``up`` [adapters, N, rank], ``scales`` [adapters] 32-bit; ``out`` [T, N] 32-bit or, with bfloat16 weights, bfloat16 (rounded
     once). ``slices``: the widths of S projections stacked in one output ([q; k; v], [gate; up]), each with ``rank`` rows of
-    ``down`` of its own; None: one. x and out may be columns of wider tensors. Sums in 32 bits."""
+    ``down`` of its own (``ADAPTER_RANKS_MOST`` in all); None: one. x and out may be columns of wider tensors. Sums in 32 bits."""
     T, K = x.shape
     A, N, r = up.shape
     S = 1 if slices is None else len(slices)

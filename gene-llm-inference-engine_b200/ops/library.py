@@ -131,6 +131,8 @@ _SIGNATURES = {
     "gi_argmax": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     "gi_adapter_plan": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p],
     "gi_adapter_direct_rows": [c_int],
+    "gi_adapter_ranks_most": [],
+    "gi_adapter_adapters_most": [],
     "gi_adapter_product": [c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_int,
                            c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
     "gi_step_tables": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,

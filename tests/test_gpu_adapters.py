@@ -219,3 +219,9 @@ def test_the_rows_that_need_no_plan_are_the_librarys():
     from geneinfer_b200.ops.library import lib
     assert lib().gi_adapter_direct_rows(kernels.ADAPTER_DIRECT_ADAPTERS) == kernels.ADAPTER_DIRECT_ROWS
     assert lib().gi_adapter_direct_rows(kernels.ADAPTER_DIRECT_ADAPTERS + 1) == 0
+
+
+def test_the_limits_are_the_librarys():
+    from geneinfer_b200.ops import kernels
+    from geneinfer_b200.ops.library import lib
+    assert lib().gi_adapter_ranks_most() == kernels.ADAPTER_RANKS_MOST and lib().gi_adapter_adapters_most() == kernels.ADAPTER_ADAPTERS_MOST

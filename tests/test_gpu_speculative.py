@@ -430,3 +430,24 @@ def test_an_adapter_that_does_not_fit_leaves_the_slots_as_they_were(tmp_path):
     with pytest.raises(ValueError):
         steps.put_adapter(1, {**pairs, last: pairs[last] + [None]}, 2 * scale)
     assert unchanged()
+
+
+def test_ranks_and_slots_beyond_the_kernels_are_refused_before_anything_is_made():
+    """[q; k; v] stacks three ranks: 168 each at most (512 in all, in steps of four). What the largest gives is what the plain model gives: its adapters are none."""
+    from geneinfer_b200.engine.step import StepEntry
+    for slots, rank in ((1, 169), (1, 172), (1, 512), (8193, 4), (0, 4), (1, 0)):
+        steps = engine_of(gf.model_dir("a"), "float32")
+        with pytest.raises(ValueError):
+            steps.enable_adapters(slots, rank)
+        assert steps.adapter_step is None and not steps.adapter_sets
+        assert all(l.adapters is None for layer in steps.model.layers for _, l, _ in layer.mixer.adaptable() + layer.feed_forward.adaptable())
+    text = tc.random_tokens(30, 256, 5)
+    rows = []
+    for dtype in ("float32", "bfloat16"):
+        for adapter in (-1, 0):
+            steps = engine_of(gf.model_dir("a"), dtype)
+            steps.enable_adapters(1, 168)
+            steps.open(0)
+            rows.append(steps.step([StepEntry(0, text, [29], adapter=adapter)]).cpu().numpy().copy())
+        bound = 2e-5 if dtype == "float32" else 2 * max(gf.bf16_noise("a"), 1e-2)
+        assert np.abs(rows[-1] - rows[-2]).max() <= bound * np.abs(rows[-1]).max()
