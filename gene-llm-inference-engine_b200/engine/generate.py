@@ -63,10 +63,13 @@ class Engine:
     # ------------------------------------------------------------------ the reference's Engine interface
     def submit(self, prompt: Sequence[int], max_positions: int = 0, sampling: Optional[SamplingParams] = None,
                stop_ids: Sequence[int] = (), on_token=None, adapter: int = -1) -> int:
-        if adapter >= 0 and (self.steps.adapter_step is None or adapter >= self.steps.adapter_step.slots):
-            raise ValueError(f"submit: there is no adapter slot {adapter}")
+        self._check_adapter("submit", adapter)
         return self.scheduler.submit(GenerationRequest(list(prompt), max_positions, sampling or SamplingParams(),
                                                        tuple(stop_ids), on_token, adapter))
+
+    def _check_adapter(self, who: str, adapter: int) -> None:
+        if adapter >= 0 and (self.steps.adapter_step is None or adapter >= self.steps.adapter_step.slots):
+            raise ValueError(f"{who}: there is no adapter slot {adapter}")
 
     def load_adapter(self, slot: int, folder: str) -> None:
         """Reads the low-rank adapter in ``folder`` (adapter_config.json, adapter_model.safetensors) into a slot; no request
@@ -115,6 +118,11 @@ class Engine:
         """Generates up to ``max_new_tokens`` for every prompt (all requests run together) and
         returns the generated token ids. Request i samples with seed ``seed + i`` and runs with the adapter in slot ``adapters[i]``
         (-1, or no list: none)."""
+        if adapters is not None:                   # (all of them ahead of the first request: one that is in runs with whoever comes next)
+            if len(adapters) != len(prompts):
+                raise ValueError(f"generate: {len(adapters)} adapters for {len(prompts)} prompts")
+            for adapter in adapters:
+                self._check_adapter("generate", adapter)
         if max_new_tokens <= 0:
             return [[] for _ in prompts]
         ids = []

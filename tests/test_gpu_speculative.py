@@ -451,3 +451,15 @@ def test_ranks_and_slots_beyond_the_kernels_are_refused_before_anything_is_made(
             rows.append(steps.step([StepEntry(0, text, [29], adapter=adapter)]).cpu().numpy().copy())
         bound = 2e-5 if dtype == "float32" else 2 * max(gf.bf16_noise("a"), 1e-2)
         assert np.abs(rows[-1] - rows[-2]).max() <= bound * np.abs(rows[-1]).max()
+
+
+def test_generate_looks_at_every_adapter_before_it_takes_a_request(tmp_path):
+    from geneinfer_b200 import Engine
+    folder, _ = adapter_and_merged("a", 15, tmp_path)
+    engine = Engine(gf.model_dir("a"), dtype="float32", max_running=2, adapter_slots=1, adapter_rank=6)
+    engine.load_adapter(0, folder)
+    prompts = [tc.random_tokens(n, 256, n) for n in (5, 9)]
+    for adapters in ([0], [0, 1], [0, 0, 0], []):
+        with pytest.raises(ValueError):
+            engine.generate(prompts, max_new_tokens=4, adapters=adapters)
+        assert engine.scheduler.idle()
