@@ -526,18 +526,19 @@ __global__ void __launch_bounds__(kThreads, kThreads != kSmallThreads ? 1024 / k
     const bool some = mx > -INFINITY && mx < INFINITY;      // else there are no probabilities (a value is none, or infinite, or all are -infinity)
     const ByTemperature by(mx, temp);
     double sum = 0.0;
-    auto weigh = [&](auto exponentials) {                   // sum += exp of every value; the probabilities keep them
-        values.groups([&](int, float (&v)[4]) {
+    auto weigh = [&](auto exponentials, auto counts) {      // sum += exp of every value; the probabilities keep them
+        values.groups([&](int unit, float (&v)[4]) {
             float y[4] = {v[0], v[1], v[2], v[3]};
             exponentials(y);
-            sum += (static_cast<double>(y[0]) + static_cast<double>(y[1])) + (static_cast<double>(y[2]) + static_cast<double>(y[3]));
+            if (counts(unit)) sum += (static_cast<double>(y[0]) + static_cast<double>(y[1])) + (static_cast<double>(y[2]) + static_cast<double>(y[3]));
             if constexpr (kProbs) { v[0] = y[0]; v[1] = y[1]; v[2] = y[2]; v[3] = y[3]; }
             return false;
         });
-        if (threadIdx.x < 32 || threadIdx.x >= kThreads - 32) sum += static_cast<double>(by(values.edge));     // (the warps that can have one)
+        if (values.edge_at >= 0) sum += static_cast<double>(by(values.edge));
     };
-    if (some && !by.plain) weigh([&](float (&y)[4]) { by.usual(y); });
-    else if (some) weigh([&](float (&y)[4]) { by.general(y); });
+    // (a place that is not there holds -infinity: exp gives 0, but for an infinite temperature, by which it is no number)
+    if (some && !by.plain) weigh([&](float (&y)[4]) { by.usual(y); }, [](int) { return true; });
+    else if (some) weigh([&](float (&y)[4]) { by.general(y); }, [&](int unit) { return values.there(unit); });
     sum = cluster_sum<kThreads>(sum, s, 0, cluster, part, parts);
     const float inv = some ? static_cast<float>(1.0 / sum) : NAN;
     if constexpr (kProbs) {

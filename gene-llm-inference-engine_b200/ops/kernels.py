@@ -1564,7 +1564,7 @@ def sample(logits: torch.Tensor, scratch: torch.Tensor, temperature: torch.Tenso
 def token_probabilities(logits: torch.Tensor, temperature: torch.Tensor, out: torch.Tensor) -> None:
     """out[r, :] = the distribution that ``sample`` draws row r from without filters: exp((l - max l) / T) times the 32-bit
     reciprocal of its sum (taken in 64 bits), T = temperature[r]; one-hot at the argmax for T <= 0 (NaN where a row has no
-    distribution). ``logits`` [rows, vocab] 32-bit or bfloat16, ``out`` 32-bit: what a drafter keeps for ``verify_drafts``."""
+    distribution, as one with a logit of -infinity at an infinite temperature). ``logits`` [rows, vocab] 32-bit or bfloat16, ``out`` 32-bit: what a drafter keeps for ``verify_drafts``."""
     rows, V = logits.shape
     if out.shape != logits.shape or temperature.numel() != rows:
         raise KernelError("token_probabilities: shapes of logits, temperature and out do not agree")

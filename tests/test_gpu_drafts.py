@@ -420,3 +420,29 @@ def test_requests_that_share_rows_end(dtype, R, D, V):
     for _ in range(3):
         tokens, accepted = verify(logits, row_start, drafted, counts, None, t, accept, draw)
         assert bool(((tokens >= -1) & (tokens < V)).all()) and bool(((accepted >= 0) & (accepted <= D)).all())
+
+
+@pytest.mark.parametrize("R,V", [(1, 7), (3, 1000), (400, 33), (5, 50257), (700, 5001), (2, 151669), (100, 70001)])
+def test_an_infinite_temperature_is_the_even_distribution(R, V):
+    """exp((l - m) / inf) = 1 for every finite logit, as the sampler has it; -infinity over infinity is no number, and then neither is any."""
+    g = torch.Generator().manual_seed(V)
+    logits = (torch.randn(R, V, generator=g) * 3).to(DEV)
+    t = torch.full((R,), math.inf, device=DEV)
+    out = torch.empty(R, V, device=DEV)
+    K().token_probabilities(logits, t, out)
+    assert torch.equal(out, torch.full_like(out, float(torch.tensor(1.0 / V))))
+    # drafts: a third of the mass is what a draft of probability 1 / V is kept from; the draw's place is that of the running sum
+    start = torch.arange(R, dtype=torch.int32, device=DEV)
+    none = torch.zeros(R, 0, dtype=torch.int32, device=DEV)
+    draw = ((torch.arange(R) + 0.5) / R).to(DEV)
+    tokens, accepted = verify(logits, start, none, torch.zeros_like(start), None, t, torch.zeros(R, 0, device=DEV), draw)
+    want = (draw.double() * V).floor().int()
+    assert bool(((tokens[:, 0] - want).abs() <= 1).all()) and not accepted.any()
+    scratch, ids = torch.empty_like(logits), torch.zeros(R, dtype=torch.int32, device=DEV)
+    K().sample(logits, scratch, t, torch.zeros_like(ids), torch.ones(R, device=DEV), draw, ids)
+    assert torch.equal(ids, tokens[:, 0])
+    if R > 1 and V > 1:
+        logits[1, V // 2] = -math.inf
+        K().token_probabilities(logits, t, out)
+        assert torch.isnan(out[1]).all() and torch.equal(out[0], torch.full_like(out[0], float(torch.tensor(1.0 / V))))
+        assert int(verify(logits, start, none, torch.zeros_like(start), None, t, torch.zeros(R, 0, device=DEV), draw)[0][1, 0]) == V - 1
