@@ -316,10 +316,9 @@ __global__ void __launch_bounds__(kPlainThreads) adapter_plain_kernel(AdapterArg
 // Rows are the M side in both products, the ranks (then the output's columns) the N side. Lane (g, c) = (lane / 4, lane % 4) holds of A rows g and
 // g + 8, of B column g, and of both the k slots 2c, 2c + 1, 2c + 8, 2c + 9. Which values of k sit in these slots is free as long as A and B agree: reading
 // straight from memory a lane takes neighbours of a row (8 c .. 8 c + 7 for two steps of k, or 4 c .. 4 c + 3 for one), 64 or 32 bytes a row for its four lanes.
-// Between the products a row's r sums are kept as bfloat16 pieces, each what the ones before leave: three for 32-bit outputs hold all 24 bits (two
-// showed as 1.8e-6 of the result against 2e-7), two for bfloat16 outputs (16 bits under a result rounded to 8).
-constexpr int kFewRows = 16, kBlockCols = 32;
-template <typename TO> struct Pieces { static constexpr int n = sizeof(TO) == 4 ? 3 : 2; };
+// Between the products a row's r sums are kept as three bfloat16 pieces, each what the ones before leave, which hold all 24 bits (two showed as 1.8e-6 of a 32-bit
+// result against 2e-7, and as the whole of a bfloat16 one whose terms cancel; 8,192 rows of 14,336 into 4,096 at rank 64 with two 121 us, with three 129 us).
+constexpr int kFewRows = 16, kBlockCols = 32, kPieces = 3;
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -422,7 +421,7 @@ __device__ __forceinline__ void expand(const AdapterArgs& a, UpFragments<kSteps>
                 for (int m = 0; m < MT; ++m) {
                     const unsigned at = ((row0 + 16 * m + (lane & 15)) * ld + k0 + 16 * s + 8 * (lane >> 4)) * 2;
 #pragma unroll
-                    for (int p = 0; p < Pieces<TO>::n; ++p) {
+                    for (int p = 0; p < kPieces; ++p) {
                         unsigned h[4];
                         load_matrices(h, pieces + p * piece_bytes + at);
 #pragma unroll
@@ -508,7 +507,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_few_kernel(Adapter
     __nv_bfloat16* pieces = reinterpret_cast<__nv_bfloat16*>(h + kFewRows * cols);
     const float scale = a.scales[adapter];
     if (rp != a.r)                             // the slots of ranks that are not there
-        for (int i = threadIdx.x; i < kFewRows * ld / 2 * Pieces<TO>::n; i += kAdapterThreads) reinterpret_cast<unsigned*>(pieces)[i] = 0u;
+        for (int i = threadIdx.x; i < kFewRows * ld / 2 * kPieces; i += kAdapterThreads) reinterpret_cast<unsigned*>(pieces)[i] = 0u;
     const int share = ((a.K + parts - 1) / parts + 31) / 32 * 32, k_begin = min(a.K, part * share), k_end = min(a.K, k_begin + share);
     const int row_g = s_rows[g], row_h = s_rows[g + 8];
     const __nv_bfloat16* x_g = static_cast<const __nv_bfloat16*>(a.x) + max(row_g, 0) * a.ldx;
@@ -567,7 +566,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_few_kernel(Adapter
         float4 v = cluster_total(h + row * cols + col, scale, cluster, parts);
         __nv_bfloat16* to = pieces + row * ld + (col / a.r) * rp + rank_slot(col % a.r);
 #pragma unroll
-        for (int p = 0; p < Pieces<TO>::n; ++p, to += kFewRows * ld) {
+        for (int p = 0; p < kPieces; ++p, to += kFewRows * ld) {
             *reinterpret_cast<unsigned*>(to) = next_piece(v.x, v.y);
             *reinterpret_cast<unsigned*>(to + 8) = next_piece(v.z, v.w);
         }
@@ -728,7 +727,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_many_kernel(Adapte
     }
     __syncthreads();
     if (rp != a.r)                             // the slots of ranks that are not there
-        for (int i = threadIdx.x; i < M * ld / 2 * Pieces<TO>::n; i += kAdapterThreads) reinterpret_cast<unsigned*>(pieces)[i] = 0u;
+        for (int i = threadIdx.x; i < M * ld / 2 * kPieces; i += kAdapterThreads) reinterpret_cast<unsigned*>(pieces)[i] = 0u;
     // the warp's first columns of the second product are asked for before the cluster meets
     const int blocks = column_blocks(a), per = (blocks + parts - 1) / parts, first = part * per + warp, last = min(blocks, (part + 1) * per);
     UpFragments<kSteps> f;
@@ -745,7 +744,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_many_kernel(Adapte
         float4 v = cluster_total(h + row * hs + col, scale, cluster, parts);
         __nv_bfloat16* to = pieces + row * ld + (col / a.r) * rp + rank_slot(col % a.r);
 #pragma unroll
-        for (int q = 0; q < Pieces<TO>::n; ++q, to += M * ld) {
+        for (int q = 0; q < kPieces; ++q, to += M * ld) {
             const unsigned p0 = next_piece(v.x, v.y), p1 = next_piece(v.z, v.w);
 #pragma unroll
             for (int p = 0; p < kAdapterClusterMost; ++p)
@@ -1003,21 +1002,21 @@ int launch_plain(const AdapterArgs& a, cudaStream_t st) {
                           2ull * kPlainRows * kAdapterRanksMost * sizeof(float), st);
 }
 
-template <typename TO> inline size_t pieces_bytes(const AdapterArgs& a, int rows) {
-    return 2ull * Pieces<TO>::n * rows * (a.S * ((a.r + 15) / 16 * 16) + 8);
+inline size_t pieces_bytes(const AdapterArgs& a, int rows) {
+    return 2ull * kPieces * rows * (a.S * ((a.r + 15) / 16 * 16) + 8);
 }
 inline size_t sums_bytes(const AdapterArgs& a, int rows) { return 4ull * rows * (a.S * a.r + 8); }
 template <typename Shape> constexpr size_t ring_bytes() { return static_cast<size_t>(Shape::kStages) * Shape::kStageBytes; }
 
 // Whether what lies where the ring was fits there.
-template <int M, bool kOnePass, typename TO> inline bool fits(const AdapterArgs& a) {
-    return (kOnePass ? sums_bytes(a, M) : 0) + pieces_bytes<TO>(a, M) <= ring_bytes<ManyShape<M, kOnePass>>();
+template <int M, bool kOnePass> inline bool fits(const AdapterArgs& a) {
+    return (kOnePass ? sums_bytes(a, M) : 0) + pieces_bytes(a, M) <= ring_bytes<ManyShape<M, kOnePass>>();
 }
 
 template <int kSteps, typename TO>
 int launch_few(const AdapterArgs& a, cudaStream_t st) {
     static SharedLimit limit;
-    return launch_adapter(&adapter_few_kernel<kSteps, TO>, limit, a, kFewRows, 4ull * kFewRows * a.S * a.r + pieces_bytes<TO>(a, kFewRows),
+    return launch_adapter(&adapter_few_kernel<kSteps, TO>, limit, a, kFewRows, 4ull * kFewRows * a.S * a.r + pieces_bytes(a, kFewRows),
                           150 * 1024, st);
 }
 
@@ -1054,11 +1053,11 @@ int launch_steps(const AdapterArgs& a, cudaStream_t st) {
     if (a.plan.T <= kFewTokens) return launch_few<kSteps, TO>(a, st);
     if (a.S * a.r <= kManyCols) {
         // (tiles of 32 rows: 2,048 rows of 4,096 into 6,144 at rank 16 38 us, of 64 48 us; 3,000 of 8,192 into 2,048 35 and 31 us)
-        if (a.plan.T <= 2048 && fits<32, true, TO>(a)) return launch_many<32, true, kSteps, TO>(a, st);
-        if (fits<64, true, TO>(a)) return launch_many<64, true, kSteps, TO>(a, st);
+        if (a.plan.T <= 2048 && fits<32, true>(a)) return launch_many<32, true, kSteps, TO>(a, st);
+        if (fits<64, true>(a)) return launch_many<64, true, kSteps, TO>(a, st);
     }
     // (several passes: tiles of 32 rows leave two blocks a multiprocessor, 1,000 rows into [q; k; v] at rank 64 43 us, of 64 rows 71 us)
-    if (fits<32, false, TO>(a)) return launch_many<32, false, kSteps, TO>(a, st);
+    if (fits<32, false>(a)) return launch_many<32, false, kSteps, TO>(a, st);
     return launch_few<kSteps, TO>(a, st);
 }
 

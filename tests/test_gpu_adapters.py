@@ -225,3 +225,19 @@ def test_the_limits_are_the_librarys():
     from geneinfer_b200.ops import kernels
     from geneinfer_b200.ops.library import lib
     assert lib().gi_adapter_ranks_most() == kernels.ADAPTER_RANKS_MOST and lib().gi_adapter_adapters_most() == kernels.ADAPTER_ADAPTERS_MOST
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES)
+@pytest.mark.parametrize("T", [3, 40, 500, 2500])
+def test_the_values_between_the_products_keep_all_their_bits(dtype, out_dtype, T):
+    """(1 + 2^-9 + 2^-18) - (1 + 2^-9): every product and sum is exact in 32 bits, and so is the answer in either type."""
+    K, N = 64, 40
+    x = torch.zeros(T, K, dtype=dt(dtype), device=DEV)
+    x[:, 0], x[:, 1], x[:, 2] = 1.0, 2.0 ** -9, 2.0 ** -18
+    down = torch.zeros(1, 4, K, dtype=dt(dtype), device=DEV)
+    down[:, 0, :3], down[:, 1, :2] = 1.0, 1.0
+    up = torch.zeros(1, N, 4, dtype=dt(dtype), device=DEV)
+    up[:, :, 0], up[:, :, 1] = 1.0, -1.0
+    out = torch.zeros(T, N, dtype=dt(out_dtype), device=DEV)
+    got = run(x, down, up, torch.ones(1, device=DEV), out, torch.zeros(T, dtype=torch.int32, device=DEV), (N,))
+    assert bool((got == 2.0 ** -18).all())
