@@ -332,13 +332,21 @@ __device__ __forceinline__ unsigned shared_address(const void* p) { return stati
 // The k slot of a rank within its 16: ranks 4 c .. 4 c + 3 sit in slots 2c, 2c + 1, 2c + 8, 2c + 9.
 __device__ __forceinline__ int rank_slot(int j) { return (j & ~15) + 2 * ((j >> 2) & 3) + ((j & 2) << 2) + (j & 1); }
 
-// The next piece of two neighbouring values (an even rank first), which is taken off them.
-__device__ __forceinline__ unsigned next_piece(float& v0, float& v1) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(v0, v1);
-    const float p0 = __bfloat162float(p.x), p1 = __bfloat162float(p.y);
-    v0 = fabsf(p0) < INFINITY ? v0 - p0 : 0.f;             // (an infinity leaves nothing)
-    v1 = fabsf(p1) < INFINITY ? v1 - p1 : 0.f;
-    return *reinterpret_cast<const unsigned*>(&p);
+// The next piece of a value (its bits), which is taken off it. All pieces but the last stay below what is left, so that none of them is zero and all have the value's
+// sign, unless it is zero: with an infinite weight the products then are the infinity that the value's is, and no zero times infinity comes up that the value has not.
+// What is infinite or no number itself is its own piece every time, and none is rounded up to an infinity. (The last piece of a value below 2^-117 may vanish.)
+__device__ __forceinline__ unsigned next_piece(float& v, bool last) {
+    const unsigned u = __float_as_uint(v), size = u & 0x7fffffffu;
+    if (size >= 0x7f800000u) return u >> 16 | (size > 0x7f800000u ? 0x40u : 0u);
+    if (last) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+    const unsigned p = size ? (u - 1) & 0xffff0000u : 0u;
+    v -= __uint_as_float(p);
+    return p >> 16;
+}
+// .. of two neighbouring values (an even rank first).
+__device__ __forceinline__ unsigned next_piece(float& v0, float& v1, bool last) {
+    const unsigned p0 = next_piece(v0, last);
+    return p0 | next_piece(v1, last) << 16;
 }
 
 // kSteps steps of k (16 ranks each) of 32 columns of `up`. Which column is column g of tile q is chosen so that a lane's values of a row are runs
@@ -567,8 +575,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_few_kernel(Adapter
         __nv_bfloat16* to = pieces + row * ld + (col / a.r) * rp + rank_slot(col % a.r);
 #pragma unroll
         for (int p = 0; p < kPieces; ++p, to += kFewRows * ld) {
-            *reinterpret_cast<unsigned*>(to) = next_piece(v.x, v.y);
-            *reinterpret_cast<unsigned*>(to + 8) = next_piece(v.z, v.w);
+            *reinterpret_cast<unsigned*>(to) = next_piece(v.x, v.y, p == kPieces - 1);
+            *reinterpret_cast<unsigned*>(to + 8) = next_piece(v.z, v.w, p == kPieces - 1);
         }
     }
     cluster.barrier_arrive();                  // no CTA leaves while another reads its sums
@@ -745,7 +753,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_many_kernel(Adapte
         __nv_bfloat16* to = pieces + row * ld + (col / a.r) * rp + rank_slot(col % a.r);
 #pragma unroll
         for (int q = 0; q < kPieces; ++q, to += M * ld) {
-            const unsigned p0 = next_piece(v.x, v.y), p1 = next_piece(v.z, v.w);
+            const unsigned p0 = next_piece(v.x, v.y, q == kPieces - 1), p1 = next_piece(v.z, v.w, q == kPieces - 1);
 #pragma unroll
             for (int p = 0; p < kAdapterClusterMost; ++p)
                 if (p < parts) {

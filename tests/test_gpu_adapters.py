@@ -241,3 +241,83 @@ def test_the_values_between_the_products_keep_all_their_bits(dtype, out_dtype, T
     out = torch.zeros(T, N, dtype=dt(out_dtype), device=DEV)
     got = run(x, down, up, torch.ones(1, device=DEV), out, torch.zeros(T, dtype=torch.int32, device=DEV), (N,))
     assert bool((got == 2.0 ** -18).all())
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES)
+@pytest.mark.parametrize("T", [9, 200, 500, 3000])
+@pytest.mark.parametrize("rank", [4, 12, 24, 40, 80])
+def test_infinite_values_of_the_second_matrix(dtype, out_dtype, T, rank):
+    """An infinity times a number that is not zero is infinite, whatever the values between the products are held as; two of opposite signs are no number. Row t's
+    values between the products are all 1 (three bits of a sum) or all 1 + 2^-9 + 2^-18 (no part of it is like another)."""
+    K, N, A = 64, 72, 2
+    x = torch.zeros(T, K)
+    x[:, 0] = 1.0
+    x[1::2, 1], x[1::2, 2] = 2.0 ** -9, 2.0 ** -18
+    x[2::3] *= -1
+    down = torch.zeros(A, rank, K)
+    down[:, :, :3] = 1.0
+    up = torch.full((A, N, rank), 2.0 ** -6)
+    up[0, 5, 1], up[0, 17, rank - 1], up[0, 40, 0] = math.inf, -math.inf, math.inf
+    up[0, 40, rank - 2] = -math.inf
+    up[0, 71] = math.inf
+    up[0, 60, 3] = math.nan
+    x, down, up = (v.to(dt(dtype)).to(DEV) for v in (x, down, up))
+    scales = torch.ones(A, device=DEV)
+    out = torch.zeros(T, N, dtype=dt(out_dtype), device=DEV)
+    ids = torch.arange(T, dtype=torch.int32, device=DEV) % 3 - 1
+    got = run(x, down, up, scales, out, ids, (N,)).float()
+    want, _ = exact(x, down, up, scales, out, ids, (N,))
+    want = want.float()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+    some = torch.isinf(want)
+    assert torch.equal(got[some], want[some])
+    rest = torch.isfinite(want)
+    assert bool(((got - want)[rest].abs() <= 2.0 ** -8 * want[rest].abs()).all())
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES)
+@pytest.mark.parametrize("T", [9, 500])
+def test_sums_between_the_products_near_the_largest_value(dtype, out_dtype, T):
+    """3.3996e38 is finite in 32 bits and rounds to an infinity in bfloat16."""
+    K, N = 64, 40
+    x = torch.zeros(T, K, dtype=dt(dtype), device=DEV)
+    x[:, 0], x[:, 1], x[:, 2] = 2.0 ** 127, 2.0 ** 126, 2.0 ** 119
+    down = torch.zeros(1, 4, K, dtype=dt(dtype), device=DEV)
+    down[:, :, 0], down[:, :, 1], down[:, :, 2] = 1.0, 1.984375, 1.5
+    up = torch.full((1, N, 4), 2.0 ** -70, dtype=dt(dtype), device=DEV)
+    ids = torch.zeros(T, dtype=torch.int32, device=DEV)
+    out = torch.zeros(T, N, dtype=dt(out_dtype), device=DEV)
+    assert 3.39e38 < 2.0 ** 127 + 2.0 ** 126 * 1.984375 + 2.0 ** 119 * 1.5 < float(torch.finfo(torch.float32).max)
+    compare(x, down, up, torch.ones(1, device=DEV), out, ids, (N,), run(x, down, up, torch.ones(1, device=DEV), out, ids, (N,)))
+
+
+@pytest.mark.parametrize("T", [9, 500])
+def test_infinite_values_between_the_products(T):
+    """Infinite inputs times a second matrix of numbers, zeros and infinities: the formula's infinities and its places without a number."""
+    K, N = 64, 40
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T, K, generator=g)
+    x[::2, 7] = math.inf
+    x[1::4, 7] = -math.inf
+    down = torch.zeros(1, 4, K)
+    down[0, :, 7] = torch.tensor([1.0, -1.0, 0.5, 0.0])          # (the last is zero times infinity: no number)
+    down[0, 3, 8] = 1.0
+    up = torch.randn(1, N, 4, generator=g)
+    up[0, :, 3] = 0.0
+    up[0, ::3, 1] = 0.0
+    up[0, 4, 2] = math.inf
+    x, down, up = (v.bfloat16().to(DEV) for v in (x, down, up))
+    ids = torch.zeros(T, dtype=torch.int32, device=DEV)
+    out = torch.zeros(T, N, device=DEV)
+    got = run(x, down, up, torch.ones(1, device=DEV), out, ids, (N,))
+    want = exact(x, down, up, torch.ones(1, device=DEV), out, ids, (N,))[0].float()
+    finite = torch.isfinite(x).all(1)
+    assert torch.isnan(got[~finite]).all() and torch.isnan(want[~finite]).all()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+    # without the row of zeros times infinity: infinities of either sign, and cancelling ones
+    down[0, 3] = 0.25
+    up[0, :, 3] = 0.0078125
+    got = run(x, down, up, torch.ones(1, device=DEV), out, ids, (N,))
+    want = exact(x, down, up, torch.ones(1, device=DEV), out, ids, (N,))[0].float()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+    assert bool(torch.isinf(want).any()) and bool(torch.isnan(want).any())
