@@ -463,3 +463,58 @@ def test_generate_looks_at_every_adapter_before_it_takes_a_request(tmp_path):
         with pytest.raises(ValueError):
             engine.generate(prompts, max_new_tokens=4, adapters=adapters)
         assert engine.scheduler.idle()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_steps_of_more_than_a_thousand_rows_with_adapters(dtype, tmp_path):
+    """1,500 rows of four requests in one step, whose rows the device puts in their adapters' order first; the launches are recorded by the first such step and repeated by
+    the others, with other tokens and other adapters. Against models with the adapters in their weights, one request at a time; bounds as in the test of small steps."""
+    from geneinfer_b200.engine.loading import load_model
+    from geneinfer_b200.engine.step import StepEngine, StepEntry
+    from geneinfer_b200.weights.adapters import read_adapter
+    folders = [adapter_and_merged("c", s, tmp_path, std=0.1 if dtype == "float32" else 0.03) for s in (21, 22)]
+    steps = StepEngine(load_model(gf.model_dir("c"), dtype=dtype), n_pages=160, max_requests=4, max_step_tokens=2048, debug_checks=True)
+    steps.enable_adapters(3, 8)
+    for slot, (folder, _) in zip((2, 0), folders):
+        steps.put_adapter(slot, *read_adapter(folder))
+    plain = {slot: engine_of(m, "float32") for slot, m in ((2, folders[0][1]), (0, folders[1][1]), (-1, gf.model_dir("c")))}
+    bound = 2e-4 if dtype == "float32" else 2 * max(gf.bf16_noise("c"), 1e-2)
+    for turn, slots in enumerate(((2, 0, -1, 2), (-1, 0, 2, 0), (0, 0, 0, 0))):
+        entries = []
+        for r, n in enumerate((400, 300, 420, 380)):
+            steps.open((turn, r))
+            entries.append(StepEntry((turn, r), tc.random_tokens(n, 500, 10 * turn + r), [0, n // 2, n - 1], adapter=slots[r]))
+        got = steps.step(entries).float().cpu().numpy().copy().reshape(4, 3, -1)
+        for r, e in enumerate(entries):
+            engine = plain[slots[r]]
+            engine.open(e.key)
+            want = engine.step([StepEntry(e.key, e.tokens, e.want)]).cpu().numpy()
+            engine.close(e.key)
+            assert np.abs(got[r] - want).max() <= bound * max(1.0, np.abs(want).max()), (turn, r)
+            steps.close(e.key)
+    assert steps.program_runs > 0
+
+
+@pytest.mark.parametrize("case", ["c", "d"])
+def test_drafts_in_bfloat16_follow_the_targets_own_choices(case):
+    """Every token of a greedy generation against the logits that the target itself has behind the tokens before it, in one step: it is the largest there, or nearer to it
+    than the noise that two cuts of the same positions show (the fixture's bound on bfloat16)."""
+    from geneinfer_b200.engine.loading import load_model
+    from geneinfer_b200.engine.step import StepEngine, StepEntry
+    vocab = gf.CASES[case][0]["vocab_size"]
+    prompts = [tc.random_tokens(n, vocab, 190 + n) for n in (17, 40, 3)]
+    engine = speculative(case, case, "bfloat16", max_running=3)
+    got = engine.generate(prompts, max_new_tokens=40)
+    steps = StepEngine(load_model(gf.model_dir(case), dtype="bfloat16"), n_pages=96, max_requests=1, max_step_tokens=512)
+    bound = float(gf.tolerance("bfloat16", case))
+    ties = 0
+    for r, (p, out) in enumerate(zip(prompts, got)):
+        assert len(out) == 40
+        steps.open(r)
+        logits = steps.step([StepEntry(r, p + out[:-1], list(range(len(p) - 1, len(p) + 39)))]).float().cpu().numpy()
+        steps.close(r)
+        for k, t in enumerate(out):
+            row = logits[k]
+            ties += t != int(row.argmax())
+            assert row.max() - row[t] <= 2 * bound * max(1.0, np.abs(row).max()), (r, k)
+    assert ties <= 12
