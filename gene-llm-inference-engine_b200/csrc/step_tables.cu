@@ -13,6 +13,9 @@
 
 #include "common.cuh"
 
+// No kernel behind starts before the tables are written (neither kernel lets its dependents start early): a decode step's attention reads positions, requests
+// and tables ahead of its wait for the kernel ahead, as the step's first kernel never writes them. It could be there while these still ran: only the kernel right
+// behind a kernel waits for that one's end.
 namespace gi {
 
 constexpr int kTableThreads = 1024;            // also the requests of a turn
@@ -90,7 +93,7 @@ __device__ __forceinline__ void write_row(const TableArgs& a, int t, int r, int 
 }
 
 __global__ void __launch_bounds__(kTableThreads, 1) step_tables_kernel(TableArgs a) {
-    pdl_prologue();
+    pdl_wait();
     __shared__ long long scratch[3][32];
     __shared__ int s_row[kTableThreads], s_page[kTableThreads], s_need[kTableThreads];
     __shared__ int s_wrong;
@@ -196,7 +199,10 @@ __global__ void __launch_bounds__(kTableThreads, 1) step_tables_kernel(TableArgs
         *a.status = kTablesDone;
         if (a.row_start) a.row_start[a.R] = static_cast<int>(rows);
     }
-    if (!a.row_start || a.rows > kRowsHere || turns > 1) return;
+    if (!a.row_start || a.rows > kRowsHere || turns > 1) {
+        __threadfence();
+        return;
+    }
     for (int t = threadIdx.x; t < a.rows; t += kTableThreads) {
         if (t < rows) {
             const int r = last_start(s_row, a.R, t);          // (of requests without rows at the same place the last: the one that has them)
@@ -207,11 +213,12 @@ __global__ void __launch_bounds__(kTableThreads, 1) step_tables_kernel(TableArgs
             a.slots[t] = -1;
         }
     }
+    __threadfence();
 }
 
 // A block has neighbouring rows; the starts are searched in shared memory where that holds them.
 __global__ void __launch_bounds__(kRowsThreads) step_rows_kernel(TableArgs a) {
-    pdl_prologue();
+    pdl_wait();
     __shared__ int s_start[kRowsStarts + 1];
     if (*a.status != kTablesDone) return;
     const int rows = a.row_start[a.R];
@@ -233,6 +240,7 @@ __global__ void __launch_bounds__(kRowsThreads) step_rows_kernel(TableArgs a) {
             a.slots[t] = -1;
         }
     }
+    __threadfence();
 }
 
 }  // namespace gi

@@ -57,10 +57,11 @@ class _Side:
         pages = [(b + n + self.page_size - 1) // self.page_size for b, n in zip(bounds, counts)]
         if max(pages) > self.tables.shape[1] or sum(pages) > self.free.numel():
             raise RuntimeError(f"step tables: {sum(pages)} pages, up to {max(pages)} a request, of {self.free.numel()} and {self.tables.shape[1]}")
-        self.tokens[:T].copy_(tokens)
         self.counts.copy_(counts_dev)
         kernels.step_tables(lengths, self.counts, self.tables, self.held, self.free, self.n_free, self.page_size, self.row_start,
                             self.row_req[:T], self.positions[:T], self.slots[:T], self.status[word:word + 1])
+        # (behind the tables: a copy waits for all kernels ahead of it, and the model's first kernel for the copy. Its kernels read the tables early.)
+        self.tokens[:T].copy_(tokens)
         views = {"tokens": self.tokens[:T], "positions": self.positions[:T], "row_req": self.row_req[:T], "logit_rows": self.all_rows[:T if logits else 0],
                  "state_slots": self.no_slots, "seg_start": self.row_start[:R], "seg_len": self.counts, "tables": [self.tables]}
         if row_adapter is not None:

@@ -518,3 +518,39 @@ def test_drafts_in_bfloat16_follow_the_targets_own_choices(case):
             ties += t != int(row.argmax())
             assert row.max() - row[t] <= 2 * bound * max(1.0, np.abs(row).max()), (r, k)
     assert ties <= 12
+
+
+@pytest.mark.parametrize("case,dtype", [("a", "float32"), ("c", "bfloat16"), ("d", "bfloat16"), ("w", "bfloat16")])
+def test_a_drafters_steps_are_the_engines_own_to_the_bit(case, dtype):
+    """Every single-token step of the drafter, over pages' ends and rewinds, against an engine that is fed the same tokens at the same positions: the tables are written by
+    a kernel of the step, ahead of kernels that read them early. And the same generation again gives the same rounds."""
+    from geneinfer_b200.engine.loading import load_model
+    from geneinfer_b200.engine.step import StepEngine, StepEntry
+    vocab = gf.CASES[case][0]["vocab_size"]
+    engine = speculative(case, case, dtype, max_running=1, max_seq_len=120, page_size=8)
+    prompt, seen, rounds = tc.random_tokens(11, vocab, 77), [], []
+    real = engine.draft.forward
+
+    def forward(tokens, counts, counts_dev, lengths, *rest, **more):
+        at = (tokens.clone(), lengths.clone())
+        logits = real(tokens, counts, counts_dev, lengths, *rest, **more)
+        seen.append((*at, None if logits is None else logits.clone()))
+        return logits
+
+    engine.draft.forward = forward
+    for _ in range(4):
+        engine.rounds = engine.kept = 0
+        rounds.append((engine.generate([prompt], max_new_tokens=90), engine.rounds, engine.kept))
+    assert all(r == rounds[0] for r in rounds)
+    steps = StepEngine(load_model(gf.model_dir(case), dtype=dtype, max_position=128), n_pages=32, max_requests=1, page_size=8)
+    steps.open(0)
+    some = 0
+    for tokens, length, logits in seen:
+        tokens, length = tokens.tolist(), int(length)
+        if length == 0 or steps.cache.requests[0].length > length:
+            steps.truncate(0, length)
+        got = steps.step([StepEntry(0, tokens, [len(tokens) - 1])])
+        if logits is not None:
+            assert torch.equal(got, logits), length
+            some += 1
+    assert some >= 4 * 72
