@@ -265,7 +265,7 @@ def main(argv: Optional[List[str]] = None) -> int:
                 f"end token: {'yes' if res.stopped_by_end_token else 'no'}\n")
         if o["profile"]:
             from ..engine.profile import profile_report
-            sys.stderr.write(profile_report(engine, prompt))
+            sys.stderr.write(profile_report(engine, prompt, 0 if rank else -1))
         return 0
     except Exception as e:   # runtime errors: bad model folder, kernels cannot be built, no GPU ...
         sys.stderr.write(f"error: {e}\n")

@@ -34,14 +34,15 @@ OPERATIONS = {
     "causal_conv": ("causal convolution", None),
     "linear_scan": ("recurrence (state update + output)", None),
     "gated_group_norm": ("gated norm", None),
+    "adapter_product": ("low-rank adapters", None),
     "copy_pages": ("page copies", None),
     "argmax": ("sampling", None),
     "sample": ("sampling", None),
 }
 
 
-def profile_report(engine, prompt) -> str:
-    """Feeds ``prompt`` (all but its last token untimed), then times one decode step at that context."""
+def profile_report(engine, prompt, adapter: int = -1) -> str:
+    """Feeds ``prompt`` (all but its last token untimed), then times one decode step at that context, with the adapter in slot ``adapter`` (-1: none)."""
     from ..sampling.params import SamplingParams
     from .step import StepEntry
     records = defaultdict(list)
@@ -66,11 +67,11 @@ def profile_report(engine, prompt) -> str:
     steps.open("profile")
     try:
         if n > 1 or len(prompt) > 1:
-            steps.step([StepEntry("profile", list(prompt[:n]), [])])
+            steps.step([StepEntry("profile", list(prompt[:n]), [], adapter=adapter)])
         steps.use_graphs = steps.use_programs = False      # every launch goes through its (timed) wrapper
         for name in OPERATIONS:
             setattr(kernels, name, timed(name, saved[name]))
-        logits = steps.step([StepEntry("profile", [int(prompt[min(n, len(prompt) - 1)])], [0])])
+        logits = steps.step([StepEntry("profile", [int(prompt[min(n, len(prompt) - 1)])], [0], adapter=adapter)])
         engine.sampler.sample(logits, [SamplingParams(0.0)], [0.0])      # the step's greedy pick belongs to it
         torch.cuda.synchronize()
     finally:

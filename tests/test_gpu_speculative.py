@@ -554,3 +554,14 @@ def test_a_drafters_steps_are_the_engines_own_to_the_bit(case, dtype):
             assert torch.equal(got, logits), length
             some += 1
     assert some >= 4 * 72
+
+
+def test_the_profile_of_a_step_has_the_requests_adapter_in_it(tmp_path, capsys):
+    from geneinfer_b200.cli.generate_main import main
+    folder, _ = adapter_and_merged("a", 16, tmp_path)
+    common = ["--model", gf.model_dir("a"), "--prompt-ids", "5 9 2 100", "--steps", "8", "--temperature", "0", "--dtype", "fp32", "--quiet", "--profile"]
+    assert main(common) == 0
+    assert "low-rank adapters" not in capsys.readouterr().err
+    assert main([*common, "--adapter", folder]) == 0
+    line = next(l for l in capsys.readouterr().err.splitlines() if "low-rank adapters" in l)
+    assert int(line.split("low-rank adapters")[1].split()[0]) == 4 * 2          # four projections of two layers
