@@ -6,9 +6,9 @@
 // adapter_plan). A cluster of CTAs takes a tile: every CTA multiplies its share of K, the partial sums [rows, S r] are added through
 // distributed shared memory, and every CTA writes its share of the columns. x, out and the weights cross memory once; the r values in between never do.
 //
-// What bounds it: single tokens the chain read, sum, exchange, read, add (eight tokens at 2,048 x 2,048, rank 16: 4.4 us); prompts the bytes of x
-// and out, each in a phase of its own that starts with an exchange (2,048 rows of 4,096 into 6,144, rank 16: 33 us for 18 us of bytes: 8 us for x, 4.5 for the
-// exchanges, 16 for out); high ranks also the tensor cores and what feeds them (8,192 rows of 14,336 into 4,096, rank 64: 63 us for x, 44 us for out).
+// What bounds it: single tokens the chain read, sum, exchange, read, add (eight tokens at 2,048 x 2,048, rank 16: 5.3 us); prompts the bytes of x
+// and out, each in a phase of its own that starts with an exchange (2,048 rows of 4,096 into 6,144, rank 16: 33 us for 18 us of bytes: 10 us until x is through, 3 for the
+// exchanges, 20 for out); high ranks also the tensor cores and what feeds them (8,192 rows of 14,336 into 4,096, rank 64: 124 us, 70, 4 and 50 of them so).
 #include <climits>
 #include <type_traits>
 
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kPlainThreads) adapter_plain_kernel(AdapterArg
 // g + 8, of B column g, and of both the k slots 2c, 2c + 1, 2c + 8, 2c + 9. Which values of k sit in these slots is free as long as A and B agree: reading
 // straight from memory a lane takes neighbours of a row (8 c .. 8 c + 7 for two steps of k, or 4 c .. 4 c + 3 for one), 64 or 32 bytes a row for its four lanes.
 // Between the products a row's r sums are kept as three bfloat16 pieces, each what the ones before leave, which hold all 24 bits (two showed as 1.8e-6 of a 32-bit
-// result against 2e-7, and as the whole of a bfloat16 one whose terms cancel; 8,192 rows of 14,336 into 4,096 at rank 64 with two 121 us, with three 129 us).
+// result against 2e-7, and as the whole of a bfloat16 one whose terms cancel; 8,192 rows of 14,336 into 4,096 at rank 64 with two 121 us, with three 128 us).
 constexpr int kFewRows = 16, kBlockCols = 32, kPieces = 3;
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -1048,9 +1048,10 @@ int launch_f32(const AdapterArgs& a, cudaStream_t st) {
     const bool pieces = a.K % 4 == 0 && a.ldx % 4 == 0 && a.r % 4 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
                         reinterpret_cast<uintptr_t>(a.down) % 16 == 0 && reinterpret_cast<uintptr_t>(a.up) % 16 == 0;
     if (!pieces) return launch_plain<float, float>(a, st);
-    // (2,048 rows of 14,336 into 4,096 at rank 64: tiles of 64 rows 215 us, of 32 263 us; 1,024 rows of 2,048 at rank 16: 27 and 22 us)
+    // (tiles of 32 and of 64 rows, four prompts: 14,336 into 4,096 at rank 64, 2,000 rows 266 and 296 us, 2,500 503 and 396; 2,048 into 2,048 at rank 16 28 and 27, 46 and 40:
+    // beyond about 2,100 rows tiles of 32 take a second round. 1,500 rows 265 and 206 us, 28 and 25: there tiles of 64 would be faster)
     if (a.plan.T >= 2048 && a.S * a.r <= 256) return launch_float<4>(a, st);
-    // (tiles of 16 rows: 250 rows of 4,096 into 4,096, two adapters of rank 64, 45 us, of 32 66 us, and 42 of
+    // (tiles of 16 and of 32 rows: 260 rows of 14,336 into 4,096 at rank 64, four adapters, 104 and 123 us, 400 rows of 24 adapters 176 and 132; tiles of 16 rows: 250 rows of 4,096 into 4,096, two adapters of rank 64, 45 us, of 32 66 us, and 42 of
     // 14,336 at rank 12 26 and 33 us; 150 of 8,192 into 2,048, four of rank 64, 58 and 53 us)
     if (a.plan.T <= kFewTokens) return launch_float<1>(a, st);
     return launch_float<2>(a, st);
@@ -1058,9 +1059,12 @@ int launch_f32(const AdapterArgs& a, cudaStream_t st) {
 
 template <int kSteps, typename TO>
 int launch_steps(const AdapterArgs& a, cudaStream_t st) {
+    // (tiles of 16 rows, or of 32 through the ring: 260 rows of four adapters, 2,048 into 16,384 at rank 32, 19 and 25 us, 14,336 into 4,096 at rank 64 21 and 25; 400 rows of 24
+    // adapters 33 and 28, 46 and 29: where each adapter may leave a tile that is not full, small ones are too many)
     if (a.plan.T <= kFewTokens) return launch_few<kSteps, TO>(a, st);
     if (a.S * a.r <= kManyCols) {
-        // (tiles of 32 rows: 2,048 rows of 4,096 into 6,144 at rank 16 38 us, of 64 48 us; 3,000 of 8,192 into 2,048 35 and 31 us)
+        // (tiles of 32 and of 64 rows, four prompts: 4,096 into 6,144 at rank 16, 2,000 rows 38 and 46 us, 2,500 54 and 53, 6,000 107 and 99; 8,192 into 2,048 24 and 24, 36 and
+        // 34, 62 and 54; 14,336 into 4,096 at rank 64 48 and 44, 80 and 68, 148 and 121: up to about 2,100 rows tiles of 32 run in one round of clusters of four)
         if (a.plan.T <= 2048 && fits<32, true>(a)) return launch_many<32, true, kSteps, TO>(a, st);
         if (fits<64, true>(a)) return launch_many<64, true, kSteps, TO>(a, st);
     }

@@ -14,7 +14,7 @@
 //
 // What bounds it: few rows the chain of read, exchange, exponentials, exchange (one user's five rows of 128,256: 6.5 us, the draw 9.7 us of which 4.4
 // read p and q); many rows the instructions, 22 a value where the exponential and the quotient alone take 12 (128 requests, 742 rows, of which 550 are
-// looked at: 84 us and 42 us for the draws, 119 us in all; 0.57 of the copy bandwidth for what the call cannot do without).
+// looked at: 119 us, 82 of them until the rows are through and 37 for the draws behind; 0.57 of the copy bandwidth for what the call cannot do without).
 #include <climits>
 
 #include <cooperative_groups.h>

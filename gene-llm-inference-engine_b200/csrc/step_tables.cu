@@ -8,14 +8,15 @@
 //
 // One block finds the sums over the requests (scans in shared memory) and moves the pages, a page a thread; the rows are written by the
 // same block where they are few, by a second launch where they are many. What bounds it is the chain of dependent steps, not its bytes: 16 requests
-// of up to five tokens 4.8 us, 1,024 of up to 128 (1.6 MB of rows) 6.2 + 6.1 us, with an empty launch at 2.5.
+// of up to five tokens 5.6 us, 1,024 of up to 128 (1.6 MB of rows) 7.3 + 5.0 us, with an empty launch at 2.5.
+//
+// Neither kernel lets the kernels behind it start early. The attention of single tokens reads positions, requests and block tables ahead of its wait (the
+// engine's own steps have them copied in before their first kernel), and a wait is for the kernel right ahead only: a few kernels behind this one, with
+// early starts all the way, it would read the tables of the step before.
 #include <climits>
 
 #include "common.cuh"
 
-// No kernel behind starts before the tables are written (neither kernel lets its dependents start early): a decode step's attention reads positions, requests
-// and tables ahead of its wait for the kernel ahead, as the step's first kernel never writes them. It could be there while these still ran: only the kernel right
-// behind a kernel waits for that one's end.
 namespace gi {
 
 constexpr int kTableThreads = 1024;            // also the requests of a turn
