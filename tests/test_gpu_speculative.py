@@ -565,3 +565,17 @@ def test_the_profile_of_a_step_has_the_requests_adapter_in_it(tmp_path, capsys):
     assert main([*common, "--adapter", folder]) == 0
     line = next(l for l in capsys.readouterr().err.splitlines() if "low-rank adapters" in l)
     assert int(line.split("low-rank adapters")[1].split()[0]) == 4 * 2          # four projections of two layers
+
+
+@pytest.mark.parametrize("drafts", [2, 6])
+def test_generation_with_drafts_over_the_ends_of_the_attentions_chunks(drafts):
+    """Contexts that grow from below 256 positions to the model's 512, beside a short one: the bounds on the lengths, by which launches are sized, run ahead of the lengths."""
+    from geneinfer_b200 import Engine
+    prompts = [tc.random_tokens(n, 500, 300 + n) for n in (250, 312, 5)]
+    want = Engine(gf.model_dir("c"), dtype="float32", max_running=3).generate(prompts, max_new_tokens=200)
+    engine = speculative("c", "c", "float32", drafts=drafts, max_seq_len=512, page_size=8)
+    assert engine.generate(prompts, max_new_tokens=200) == want
+    assert engine.kept >= 0.95 * engine.proposed > 0
+    other = speculative("c", "c", "bfloat16", drafts=drafts, max_seq_len=512)
+    first = other.generate(prompts, max_new_tokens=200)
+    assert other.generate(prompts, max_new_tokens=200) == first and [len(f) for f in first] == [200] * 3
