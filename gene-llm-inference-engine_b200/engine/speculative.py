@@ -42,7 +42,7 @@ class _Side:
         self.n_free = torch.full((1,), pool, dtype=torch.int32, device=dev)
         self.status = status
         self.row_start = torch.empty(requests + 1, dtype=torch.int32, device=dev)
-        self.row_req, self.positions, self.slots = (torch.empty(step_tokens, dtype=torch.int32, device=dev) for _ in range(3))
+        self.row_req, self.positions, self.slots = (torch.zeros(step_tokens, dtype=torch.int32, device=dev) for _ in range(3))
         # a step's tokens and counts are copied here: recorded launches name where they lie
         self.tokens, self.counts = torch.zeros(step_tokens, dtype=torch.int32, device=dev), torch.zeros(requests, dtype=torch.int32, device=dev)
         self.all_rows = torch.arange(max(step_tokens, logit_rows), dtype=torch.int32, device=dev)

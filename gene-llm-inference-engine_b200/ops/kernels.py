@@ -1586,7 +1586,7 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafted: torch.
     distribution (a look-up), q is one at the draft. ``tokens`` [R, D + 1]: the kept drafts, the new token, then -1; ``accepted`` [R]: how many
     drafts were kept (-1, and no token, for a request whose rows do not lie in ``logits``). A row without a distribution (a logit
     that is no number or +infinity, or all of them -infinity) refuses its draft and gives the last token of the vocabulary, as
-    ``sample`` does. No two requests may share a row. ``work`` [N, 4] 32-bit scratch. Two launches, three where there are more rows than the GPU holds twice over."""
+    ``sample`` does. Requests that share a row get either one's results there. ``work`` [N, 4] 32-bit scratch. Two launches, three where there are more rows than the GPU holds twice over."""
     N, V = logits.shape
     R, D = drafted.shape
     if row_start.numel() != R or counts.numel() != R or temperature.numel() != R or draw_uniform.numel() != R or accepted.numel() != R \

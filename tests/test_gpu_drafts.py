@@ -412,7 +412,7 @@ def test_the_quotient_by_the_temperature_is_the_divisions():
 
 @pytest.mark.parametrize("dtype,R,D,V", [("float32", 600, 3, 6003), ("bfloat16", 150, 4, 70001), ("float32", 40, 15, 128256)])
 def test_requests_that_share_rows_end(dtype, R, D, V):
-    """Not a use (the rows' results are then anyone's), but every call ends, with tokens of the vocabulary. Rows may be left out here: clusters that decide it for themselves."""
+    """A shared row's results are either request's, but every call ends, with tokens of the vocabulary. Rows may be left out here: each cluster decides it for itself."""
     logits, row_start, drafted, counts, q, t, accept, draw = inputs(V, R, D, V, dtype, probs=False)
     counts[:] = D
     row_start = torch.arange(R, dtype=torch.int32) % 3
