@@ -112,7 +112,7 @@ def _stream(g, T, D):
 def _in_8_bits(v):
     """q and scale of every row of v; q in 32 bits."""
     m = v.abs().amax(1, keepdim=True)
-    q = torch.round(v * torch.where(m > 0, 127.0 / m, 0.0))
+    q = torch.round(v * torch.where(m > 0, torch.full_like(m, 127.0) / m, 0.0))      # (one quotient: 127.0 / m takes a reciprocal and a product)
     return q, m / 127.0
 
 
