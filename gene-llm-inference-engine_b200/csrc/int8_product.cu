@@ -1,0 +1,857 @@
+// Matrix product in 8-bit integers on the 5th-generation tensor cores, scales for every row and channel:
+//
+//   out[t, n] (+)= scale_a[t] * scale_w[n] * sum over k of a[t, k] * w[n, k]
+//
+// tcgen05.mma kind::i8 adds the products in 32-bit integers in tensor memory. They are exact (K up to 131,056, which the host
+// checks), so a result depends neither on how K is cut nor on which of the two kernels below computed it: every sum is turned
+// into a float once, multiplied by the row's scale, then by the channel's, in that order everywhere.
+//
+// The weights lie in tiles of 128 channels x 128 values of K, 16 KB each, [channel tile][block of K][128][128] with K padded to whole
+// blocks by zeros and every row's eight 16-byte pieces permuted by piece ^ (row % 8): a tile in memory is what tcgen05.mma
+// reads in shared memory (K-major, 128-byte swizzle), so a tile is one stretch of memory and both kernels read the same one copy.
+// Weights of a gated pair lie gate tile, up tile, gate tile, .. (each part padded to whole tiles).
+//
+// Few rows (int8_few_kernel). The weights take the 128-row side and up to 256 rows of activations the narrow side. What bounds it is
+// the stream of the weights: a CTA keeps its share of shared memory full of bulk copies and computes as they land. K is cut over the CTAs of
+// a cluster until the SMs have work; each CTA then collects the sums of its share of the rows from the others' shared memory
+// (integers, so in any order), scales and stores them.
+//
+// Many rows (int8_many_kernel). Pairs of CTAs (cta_group::2) on tiles of 256 rows x 256 channels, persistent, accumulators
+// twice in tensor memory so that the epilogue of a tile runs beside the products of the next. Epilogues: 32-bit store or addition and
+// bfloat16 store by TMA from a staging buffer (or by plain stores, where the output's rows are not whole 16 bytes), and act(gate) * up in
+// bfloat16 for gated weights.
+//
+// Every wait is bounded: where a limit is hit the kernel records a code in the status word, stops issuing work, lets its own copies
+// land, frees its tensor memory and returns.
+#include "common.cuh"
+#include "device_limit.h"
+#include "tma.cuh"
+
+namespace gi {
+namespace {
+
+constexpr int kTileRows = 128;                      // channels of a weight tile
+constexpr int kRowBytes = 128;                      // values of K in a block: one swizzle row
+constexpr int kTileBytes = kTileRows * kRowBytes;
+constexpr unsigned long long kWaitCycles = 4000000000ull;      // about two seconds
+
+enum Int8Error : int { kErrProducer = 41, kErrMma = 42, kErrEpilogue = 43, kErrDrain = 44 };
+
+// ------------------------------------------------------------------------------------------ PTX
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void bar_arrive_remote(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+template <bool CLUSTER>
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    if (CLUSTER)
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Bounded: false where the limit is hit (recorded) or another role of the CTA has given up.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status, int code) {
+    if (bar_try<CLUSTER>(bar, parity)) return true;
+    const unsigned long long t0 = clock64();
+    while (!bar_try<CLUSTER>(bar, parity)) {
+        if (*gave_up) return false;
+        if (clock64() - t0 > kWaitCycles) {
+            *gave_up = 1;
+            atomicCAS(status, 0, code);
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ uint32_t map_to(uint32_t local, uint32_t rank) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+    return remote;
+}
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
+}
+// into this CTA's shared memory, the bytes counted on a barrier of either CTA of the pair
+__device__ __forceinline__ void load_tile_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void load_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy) : "memory");
+}
+__device__ __forceinline__ uint64_t read_once_policy() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ void store_tile(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void add_tile(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];"
+                 ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_allocate(uint32_t dst, uint32_t cols) {
+    if (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+template <bool PAIR>
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// arrives on the barrier (of both CTAs of a pair) once the products issued so far are done
+template <bool PAIR>
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    if (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// K-major tile in shared memory, 128-byte swizzle, groups of 8 rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// D 32-bit integers (2 at bit 4), A and B signed 8-bit (1 at bits 7 and 10), both K-major; N / 8 at bit 17, M / 16 at bit 24
+constexpr uint32_t int8_idesc(int m, int n) { return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24); }
+
+__device__ __forceinline__ float scaled(int sum, float row, float channel) { return __fmul_rn(__fmul_rn(static_cast<float>(sum), row), channel); }
+
+// ------------------------------------------------------------------------------------------ few rows
+struct FewParams {
+    const uint8_t* tiles;
+    const float* a_scales;
+    const float* w_scales;
+    void* out;               // out[t * ldo + n]
+    long long ldo;
+    int out_bf16, accumulate;
+    int T, N;                // N: channels of a part (gated weights: of gate and of up)
+    int gated;
+    int total_kb, kb_per_split, splits;
+    int stages;
+    int* status;
+};
+
+constexpr int kFewThreads = 192;      // producer, MMA, four epilogue warps
+
+template <int BQ>
+struct FewConfig {
+    static constexpr int kKb = BQ <= 64 ? 2 : 1;               // blocks of K to a stage
+    static constexpr int kBlockBytes = kTileBytes + BQ * kRowBytes;
+    static constexpr int kStageBytes = kKb * kBlockBytes;
+    static constexpr int kTmemCols = BQ < 32 ? 32 : BQ;
+    // the sums that the CTAs of a cluster hand each other: up to 8 equal shares of the rows, the last one padded
+    static constexpr int kMeetBytes = (BQ + 7) * kTileRows * 4;
+    static constexpr bool kOwnPlace = BQ <= 64;                // ... behind the stages, or in them once the products are done
+    static constexpr int kSideBytes = 256 + 4 * BQ;            // barriers, flags, the rows' scales
+    static constexpr int smem(int stages, int splits) {
+        return stages * kStageBytes + (kOwnPlace && splits > 1 ? kMeetBytes : 0) + kSideBytes + 1024;
+    }
+};
+
+template <int BQ>
+__global__ void __launch_bounds__(kFewThreads)
+int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const FewParams p) {
+    using Cfg = FewConfig<BQ>;
+    constexpr int kKb = Cfg::kKb;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const int stages = p.stages;
+    uint8_t* behind = smem + stages * Cfg::kStageBytes;
+    int* meet = reinterpret_cast<int*>(Cfg::kOwnPlace ? behind : smem);      // [split][rows of a CTA's share][128]: at most BQ + 7 rows
+    if (Cfg::kOwnPlace && p.splits > 1) behind += Cfg::kMeetBytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(behind);      // [0, 8) full, [8, 16) empty, [16] sums complete
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+    volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* row_scales = reinterpret_cast<float*>(behind + 256);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tile_n = blockIdx.x, tile_t = blockIdx.y, split = blockIdx.z;
+    const int kb_begin = split * p.kb_per_split;
+    const int n_kb = min(p.total_kb, kb_begin + p.kb_per_split) - kb_begin;
+    const int n_steps = (n_kb + kKb - 1) / kKb;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            bar_init(smem_addr(&bars[s]), 1);
+            bar_init(smem_addr(&bars[8 + s]), 1);
+        }
+        bar_init(smem_addr(&bars[16]), 1);
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_allocate<false>(smem_addr(tmem_slot), Cfg::kTmemCols);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint64_t policy = read_once_policy();
+            const uint8_t* src = p.tiles + (static_cast<size_t>(tile_n) * p.total_kb + kb_begin) * kTileBytes;
+            auto blocks_of = [&](int i) { return min(kKb, n_kb - i * kKb); };
+            auto load_w = [&](int i, int s) {
+                load_bulk(smem_addr(smem + s * Cfg::kStageBytes), src + static_cast<size_t>(i) * kKb * kTileBytes, blocks_of(i) * kTileBytes,
+                          smem_addr(&bars[s]), policy);
+            };
+            auto load_a = [&](int i, int s) {
+                for (int j = 0; j < blocks_of(i); ++j)
+                    load_tile(smem_addr(smem + s * Cfg::kStageBytes + kKb * kTileBytes + j * BQ * kRowBytes), &map_a,
+                              (kb_begin + i * kKb + j) * kRowBytes, tile_t * BQ, smem_addr(&bars[s]));
+            };
+            // the weights belong to no earlier kernel: their first tiles are asked for before the wait for the kernels ahead
+            const int early = min(n_steps, stages);
+            for (int i = 0; i < early; ++i) {
+                bar_expect(smem_addr(&bars[i]), blocks_of(i) * Cfg::kBlockBytes);
+                load_w(i, i);
+            }
+            pdl_wait();
+            for (int i = 0; i < early; ++i) load_a(i, i);
+            int issued = early, s = 0, round = 1;
+            if (early == stages) {
+                for (int i = early; i < n_steps; ++i) {
+                    if (!bar_wait(smem_addr(&bars[8 + s]), (round & 1) ^ 1, gave_up, p.status, kErrProducer)) break;
+                    bar_expect(smem_addr(&bars[s]), blocks_of(i) * Cfg::kBlockBytes);
+                    load_w(i, s);
+                    load_a(i, s);
+                    issued = i + 1;
+                    if (++s == stages) { s = 0; ++round; }
+                }
+            }
+            if (*gave_up) {      // every copy must have landed before the CTA leaves
+                for (int i = max(0, issued - stages); i < issued; ++i) {
+                    const unsigned long long t0 = clock64();
+                    while (!bar_try<false>(smem_addr(&bars[i % stages]), (i / stages) & 1))
+                        if (clock64() - t0 > kWaitCycles) { atomicCAS(p.status, 0, kErrDrain); break; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = int8_idesc(kTileRows, BQ);
+            bool ok = true;
+            int s = 0, parity = 0;
+            for (int i = 0; i < n_steps; ++i) {
+                if (!bar_wait(smem_addr(&bars[s]), parity, gave_up, p.status, kErrMma)) { ok = false; break; }
+                fence_after();
+                const uint32_t at = smem_addr(smem + s * Cfg::kStageBytes);
+                const int blocks = min(kKb, n_kb - i * kKb);
+                for (int j = 0; j < blocks; ++j) {
+                    const uint64_t w = tile_desc(at + j * kTileBytes), a = tile_desc(at + kKb * kTileBytes + j * BQ * kRowBytes);
+#pragma unroll
+                    for (int k = 0; k < kRowBytes / 32; ++k)      // 32 values of K to an instruction
+                        mma_i8<false>(tmem, w + 2 * k, a + 2 * k, idesc, (i > 0 || j > 0 || k > 0) ? 1u : 0u);
+                }
+                mma_commit<false>(smem_addr(&bars[8 + s]));
+                if (++s == stages) { s = 0; parity ^= 1; }
+            }
+            if (ok) mma_commit<false>(smem_addr(&bars[16]));
+        }
+    }
+    __syncwarp();
+    // ---------------------------------------------------------------- the sums
+    const int lane_group = warp & 3;
+    const int row = lane_group * 32 + lane;                                  // the channel within the tile = the tensor memory's lane
+    const int rows_here = min(BQ, p.T - tile_t * BQ);
+    const int part_tile = p.gated ? tile_n >> 1 : tile_n;
+    const bool channel_there = part_tile * kTileRows + row < p.N;
+    const int channel = (p.gated && (tile_n & 1) ? p.N : 0) + part_tile * kTileRows + row;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(lane_group * 32) << 16);
+    const bool epilogue = warp >= 2;
+    bool ok = false;
+    float w_scale = 0.f;
+    auto emit = [&](int t, int sum) {      // t: the row within the tile
+        const float v = scaled(sum, row_scales[t], w_scale);
+        const size_t at = static_cast<size_t>(tile_t * BQ + t) * p.ldo + channel;
+        if (p.out_bf16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+        else static_cast<float*>(p.out)[at] = p.accumulate ? __fadd_rn(static_cast<const float*>(p.out)[at], v) : v;
+    };
+    if (epilogue) {
+        if (channel_there) w_scale = __ldg(p.w_scales + channel);
+        pdl_wait();
+        for (int t = threadIdx.x - 64; t < rows_here; t += 128) row_scales[t] = __ldcg(p.a_scales + tile_t * BQ + t);
+        ok = bar_wait(smem_addr(&bars[16]), 0, gave_up, p.status, kErrEpilogue);
+        fence_after();
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+    }
+    if (p.splits == 1) {
+        if (epilogue && __all_sync(0xffffffffu, ok)) {
+#pragma unroll 1
+            for (int c = 0; c < rows_here; c += 16) {
+                uint32_t r[16];
+                tmem_load16(lane_addr + c, r);
+                tmem_load_wait();
+                if (channel_there) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (c + j < rows_here) emit(c + j, static_cast<int>(r[j]));
+                }
+            }
+        }
+    } else {
+        // CTA r of the cluster takes rows r * share .. of the tile
+        const int share = (rows_here + p.splits - 1) / p.splits;
+        if (!Cfg::kOwnPlace) cluster_sync();      // the stages of every CTA are done with
+        if (epilogue) {
+            const bool send = __all_sync(0xffffffffu, ok);
+            int owner = 0, place = 0;
+            uint32_t to = map_to(smem_addr(meet), 0);
+#pragma unroll 1
+            for (int c = 0; c < rows_here; c += 16) {
+                uint32_t r[16];
+                if (send) {
+                    tmem_load16(lane_addr + c, r);
+                    tmem_load_wait();
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    if (c + j < rows_here) {
+                        store_cluster(to + static_cast<uint32_t>(((split * share + place) * kTileRows + row) * 4), send ? r[j] : 0u);
+                        if (++place == share) { place = 0; to = map_to(smem_addr(meet), static_cast<uint32_t>(++owner < p.splits ? owner : 0)); }
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync();                           // everyone's sums have arrived; nobody's memory is written from here on
+        if (epilogue && channel_there) {
+            for (int i = 0; i < share; ++i) {
+                const int t = split * share + i;
+                if (t >= rows_here) break;
+                int sum = 0;
+                for (int s = 0; s < p.splits; ++s) sum += meet[(s * share + i) * kTileRows + row];
+                emit(t, sum);
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after();
+        tmem_free<false>(tmem, Cfg::kTmemCols);
+    }
+}
+
+// ------------------------------------------------------------------------------------------ many rows
+enum ManyEpilogue : int { kStoreF32 = 0, kAddF32 = 1, kStoreBF16 = 2, kGatedBF16 = 3 };
+
+struct ManyParams {
+    const float* a_scales;
+    const float* w_scales;
+    const float* bias;       // gated: [2 N] or null
+    void* out;
+    long long ldo;
+    int plain_stores;        // the output's rows are not whole 16 bytes: no TMA
+    int T, N;                // N: output channels
+    int total_kb;
+    int tiles_t, tiles_n;    // of 256 rows, of BQ channels (gated: 128 of them)
+    int group_t;             // tiles of rows that are walked together
+    int act;
+    float limit;
+    int* status;
+};
+
+constexpr int kManyThreads = 64 + 2 * 128;      // producer, MMA, two epilogue groups of four warps
+
+template <int BQ>
+struct ManyConfig {
+    static constexpr int kWRows = BQ / 2;                                    // channels in this CTA's shared memory
+    static constexpr int kStageBytes = kTileBytes + kWRows * kRowBytes;
+    static constexpr int kStages = BQ == 256 ? 6 : 8;
+    static constexpr int kStagingBytes = kTileRows * 128;                    // 128 rows x 128 bytes, one to a group
+    static constexpr int kTmemCols = 2 * BQ;
+    static constexpr int kSideBytes = 256 + BQ * 4;                          // barriers; the channels' scales of a tile
+    static constexpr int kSmem = kStages * kStageBytes + 2 * kStagingBytes + kSideBytes + 1024;
+    static_assert(kSmem <= 232448, "the pipeline does not fit into an SM's shared memory");
+};
+
+template <int BQ, int EPI>
+__global__ void __launch_bounds__(kManyThreads, 1)
+int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_o,
+                 const ManyParams p) {
+    using Cfg = ManyConfig<BQ>;
+    constexpr int kStages = Cfg::kStages;
+    static_assert(EPI != kGatedBF16 || BQ == 256, "a gated tile is a tile of gates and one of ups");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* staging = smem + kStages * Cfg::kStageBytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 2 * Cfg::kStagingBytes);
+    // [0, S) full, [S, 2S) empty, [2S, 2S + 2) sums complete, [2S + 2, 2S + 4) sums read
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
+    volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* decided = gave_up + 1;
+    float* scales = reinterpret_cast<float*>(staging + 2 * Cfg::kStagingBytes + 256);      // [BQ]
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int worker = blockIdx.x / 2, n_workers = gridDim.x / 2;
+    const int n_tiles = p.tiles_t * p.tiles_n;
+    // Tiles are walked in groups of group_t tiles of rows, through all channels: what the CTAs read at one time is a few tiles of
+    // rows and a few of channels, which L2 holds, instead of all rows again for every few channels.
+    auto tile_of = [&](int i, int& tile_t, int& tile_n) {
+        const int per_group = p.group_t * p.tiles_n, g = i / per_group, in = i - g * per_group;
+        const int here = min(p.group_t, p.tiles_t - g * p.group_t);
+        tile_t = g * p.group_t + in % here;
+        tile_n = in / here;
+    };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            bar_init(smem_addr(&bars[s]), 1);
+            bar_init(smem_addr(&bars[kStages + s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            bar_init(smem_addr(&bars[2 * kStages + b]), 1);
+            bar_init(smem_addr(&bars[2 * kStages + 2 + b]), 2 * (kManyThreads - 64));
+        }
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_allocate<true>(smem_addr(tmem_slot), Cfg::kTmemCols);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();
+    cluster_sync();          // both CTAs' barriers exist before either signals the other's
+    pdl_wait();
+    auto leader_bar = [&](int i) { return map_to(smem_addr(&bars[i]), 0u); };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int i = worker; i < n_tiles && ok; i += n_workers) {
+                int tile_t, tile_n;
+                tile_of(i, tile_t, tile_n);
+                const int t0 = tile_t * 256 + static_cast<int>(rank) * kTileRows;
+                // this CTA's rows of the channels' tile: a tile of its own (256 channels), or half of one (128)
+                const long long w0 = BQ == 256 ? (2ll * tile_n + rank) * p.total_kb * kTileRows
+                                               : static_cast<long long>(tile_n) * p.total_kb * kTileRows + rank * Cfg::kWRows;
+                for (int kb = 0; kb < p.total_kb; ++kb, ++it) {
+                    const int s = it % kStages;
+                    if (!bar_wait(smem_addr(&bars[kStages + s]), ((it / kStages) & 1) ^ 1, gave_up, p.status, kErrProducer)) { ok = false; break; }
+                    const uint32_t stage = smem_addr(smem + s * Cfg::kStageBytes), full = leader_bar(s);
+                    if (rank == 0) bar_expect(smem_addr(&bars[s]), 2 * Cfg::kStageBytes);
+                    load_tile_pair(stage, &map_a, kb * kRowBytes, t0, full);
+                    load_tile_pair(stage + kTileBytes, &map_w, 0, static_cast<int>(w0 + static_cast<long long>(kb) * kTileRows), full);
+                }
+            }
+            if (*gave_up && rank == 0) {
+                for (int i = max(0, it - kStages); i < it; ++i) {
+                    const unsigned long long t0 = clock64();
+                    while (!bar_try<false>(smem_addr(&bars[i % kStages]), (i / kStages) & 1))
+                        if (clock64() - t0 > kWaitCycles) { atomicCAS(p.status, 0, kErrDrain); break; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {      // a pair's products are issued by its first CTA
+            constexpr uint32_t idesc = int8_idesc(256, BQ);
+            int it = 0, n = 0;
+            bool ok = true;
+            for (int i = worker; i < n_tiles && ok; i += n_workers, ++n) {
+                const int buf = n & 1;
+                if (!bar_wait<true>(smem_addr(&bars[2 * kStages + 2 + buf]), ((n >> 1) & 1) ^ 1, gave_up, p.status, kErrMma)) break;
+                fence_after();
+                const uint32_t d = tmem + buf * BQ;
+                for (int kb = 0; kb < p.total_kb; ++kb, ++it) {
+                    const int s = it % kStages;
+                    if (!bar_wait(smem_addr(&bars[s]), (it / kStages) & 1, gave_up, p.status, kErrMma)) { ok = false; break; }
+                    fence_after();
+                    const uint32_t at = smem_addr(smem + s * Cfg::kStageBytes);
+                    const uint64_t a = tile_desc(at), w = tile_desc(at + kTileBytes);
+#pragma unroll
+                    for (int k = 0; k < kRowBytes / 32; ++k) mma_i8<true>(d, a + 2 * k, w + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                    mma_commit<true>(smem_addr(&bars[kStages + s]));
+                }
+                if (ok) mma_commit<true>(smem_addr(&bars[2 * kStages + buf]));
+            }
+        }
+    } else {
+        // Group 0 (warps 2..5) takes the even chunks of a tile's columns, group 1 the odd ones; each has a staging buffer, a
+        // named barrier and a thread that issues its stores. A thread holds one row of the tile.
+        const int group = (warp - 2) >> 2, lane_group = warp & 3;
+        const int row = lane_group * 32 + lane;
+        const int in_group = threadIdx.x - 64 - group * 128;
+        const bool leader = in_group == 0;
+        uint8_t* stg = staging + group * Cfg::kStagingBytes;
+        auto group_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
+        auto both_sync = [&]() { asm volatile("bar.sync 3, 256;" ::: "memory"); };
+        auto sums_read = [&](int buf) {
+            fence_before();
+            if (rank == 0) bar_arrive(smem_addr(&bars[2 * kStages + 2 + buf]));
+            else bar_arrive_remote(leader_bar(2 * kStages + 2 + buf));
+        };
+        int n = 0;
+        for (int i = worker; i < n_tiles; i += n_workers, ++n) {
+            int tile_t, tile_n;
+            tile_of(i, tile_t, tile_n);
+            const int t = tile_t * 256 + static_cast<int>(rank) * kTileRows + row;
+            const int buf = n & 1;
+            const float row_scale = t < p.T ? __ldcg(p.a_scales + t) : 0.f;
+            // the tile's channels: column c of the sums is channel n0 + c (gated: columns 128 .. are the ups)
+            const int n0 = EPI == kGatedBF16 ? tile_n * kTileRows : tile_n * BQ;
+            const int mine = threadIdx.x - 64;
+            const bool up = EPI == kGatedBF16 && mine >= kTileRows;
+            const int ch = n0 + (up ? mine - kTileRows : mine);
+            const float mine_scale = mine < BQ && ch < p.N ? __ldg(p.w_scales + (up ? p.N : 0) + ch) : 0.f;
+            bar_wait(smem_addr(&bars[2 * kStages + buf]), (n >> 1) & 1, gave_up, p.status, kErrEpilogue);
+            both_sync();                               // nobody reads the last tile's scales any more
+            if (mine < BQ) scales[mine] = mine_scale;
+            if (mine == 0) *decided = *gave_up == 0;
+            both_sync();                               // the scales are there, and one decision for all
+            if (!*decided) break;
+            fence_after();
+            const uint32_t d = tmem + buf * BQ + (static_cast<uint32_t>(lane_group * 32) << 16);
+            constexpr int kCols = EPI == kStoreF32 || EPI == kAddF32 ? 32 : 64;      // output columns to a chunk: 128 bytes
+            constexpr int kChunks = EPI == kGatedBF16 ? 2 : BQ / kCols;
+            for (int c = group; c < kChunks; c += 2) {
+                if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the last store has read the staging buffer
+                group_sync();
+                const bool last = c + 2 >= kChunks;
+#pragma unroll
+                for (int half = 0; half < kCols / 32; ++half) {
+                    const int at = c * kCols + half * 32;
+                    uint32_t r[32];
+                    tmem_load16(d + at, r);
+                    tmem_load16(d + at + 16, r + 16);
+                    if constexpr (EPI == kGatedBF16) {
+                        uint32_t u[32];
+                        tmem_load16(d + kTileRows + at, u);
+                        tmem_load16(d + kTileRows + at + 16, u + 16);
+                        tmem_load_wait();
+                        if (last && half == kCols / 32 - 1) sums_read(buf);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            uint32_t packed[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float h[2];
+#pragma unroll
+                                for (int o = 0; o < 2; ++o) {
+                                    const int j = q * 8 + 2 * e + o;
+                                    float g = scaled(static_cast<int>(r[j]), row_scale, scales[at + j]);
+                                    float v = scaled(static_cast<int>(u[j]), row_scale, scales[kTileRows + at + j]);
+                                    if (p.bias != nullptr && n0 + at + j < p.N) {
+                                        g = __fadd_rn(g, __ldg(p.bias + n0 + at + j));
+                                        v = __fadd_rn(v, __ldg(p.bias + p.N + n0 + at + j));
+                                    }
+                                    h[o] = gated_value(g, v, p.act, p.limit);
+                                }
+                                const __nv_bfloat162 hb = __floats2bfloat162_rn(h[0], h[1]);
+                                packed[e] = *reinterpret_cast<const uint32_t*>(&hb);
+                            }
+                            *reinterpret_cast<uint4*>(stg + row * 128 + (((half * 4 + q) ^ (row & 7)) * 16)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+                        }
+                    } else {
+                        tmem_load_wait();
+                        if (last && half == kCols / 32 - 1) sums_read(buf);
+                        if constexpr (EPI == kStoreBF16) {
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                uint32_t packed[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const int j = q * 8 + 2 * e;
+                                    const __nv_bfloat162 vb = __floats2bfloat162_rn(scaled(static_cast<int>(r[j]), row_scale, scales[at + j]),
+                                                                                    scaled(static_cast<int>(r[j + 1]), row_scale, scales[at + j + 1]));
+                                    packed[e] = *reinterpret_cast<const uint32_t*>(&vb);
+                                }
+                                *reinterpret_cast<uint4*>(stg + row * 128 + (((half * 4 + q) ^ (row & 7)) * 16)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) {
+                                float v[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) v[e] = scaled(static_cast<int>(r[q * 4 + e]), row_scale, scales[at + q * 4 + e]);
+                                *reinterpret_cast<float4*>(stg + row * 128 + ((q ^ (row & 7)) * 16)) = make_float4(v[0], v[1], v[2], v[3]);
+                            }
+                        }
+                    }
+                }
+                const int col = n0 + c * kCols, out_row = tile_t * 256 + static_cast<int>(rank) * kTileRows;
+                if (!p.plain_stores) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    group_sync();
+                    if (leader) {
+                        if (EPI == kAddF32) add_tile(&map_o, smem_addr(stg), col, out_row);
+                        else store_tile(&map_o, smem_addr(stg), col, out_row);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                } else {
+                    // a warp stores rows of its quarter of the tile one after the other, the lanes side by side
+                    group_sync();
+                    for (int rr = lane_group * 32; rr < lane_group * 32 + 32; ++rr) {
+                        const int tt = out_row + rr;
+                        if (tt >= p.T) break;
+#pragma unroll
+                        for (int part = 0; part < kCols / 32; ++part) {
+                            const int cc = part * 32 + lane;
+                            if (col + cc >= p.N) continue;
+                            const size_t to = static_cast<size_t>(tt) * p.ldo + col + cc;
+                            if (kCols == 64) {
+                                static_cast<__nv_bfloat16*>(p.out)[to] =
+                                    *reinterpret_cast<const __nv_bfloat16*>(stg + rr * 128 + (((cc >> 3) ^ (rr & 7)) * 16) + (cc & 7) * 2);
+                            } else {
+                                const float v = *reinterpret_cast<const float*>(stg + rr * 128 + (((cc >> 2) ^ (rr & 7)) * 16) + (cc & 3) * 4);
+                                float* o = static_cast<float*>(p.out) + to;
+                                *o = EPI == kAddF32 ? __fadd_rn(*o, v) : v;
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        if (leader) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        fence_before();
+    }
+    __syncthreads();
+    cluster_sync();          // neither CTA leaves while the other may still signal it
+    if (warp == 1) {
+        fence_after();
+        tmem_free<true>(tmem, Cfg::kTmemCols);
+    }
+}
+
+// ------------------------------------------------------------------------------------------ host side
+int encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, unsigned long long rows, unsigned long long cols, unsigned long long row_bytes,
+           int box_rows, int box_cols, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
+    EncodeTiledFn fn = tensor_map_encoder();
+    if (!fn) { set_error("int8_product: cuTensorMapEncodeTiled is not available from the driver"); return 1; }
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {row_bytes};
+    cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+    cuuint32_t elem[2] = {1, 1};
+    const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { set_error("int8_product: cuTensorMapEncodeTiled failed with code %d", static_cast<int>(r)); return 1; }
+    return 0;
+}
+
+int encode_rows(CUtensorMap* map, const void* a, int T, int width, int box_rows) {
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, T, width, width, box_rows, kRowBytes, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+
+template <int BQ>
+int launch_few(const CUtensorMap& map_a, const FewParams& p, dim3 grid, cudaStream_t st) {
+    using Cfg = FewConfig<BQ>;
+    static SharedLimit limit;
+    constexpr int kMost = 232448;
+    const cudaError_t le = limit.allow(reinterpret_cast<const void*>(int8_few_kernel<BQ>), kMost);
+    if (le != cudaSuccess) { set_error("int8_product: cannot reserve %d bytes of shared memory: %s", kMost, cudaGetErrorString(le)); return 1; }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = Cfg::smem(p.stages, p.splits);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = g_pdl_enabled ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = p.splits;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    counted(cudaLaunchKernelEx(&cfg, int8_few_kernel<BQ>, map_a, p));
+    return check_launch("int8_product");
+}
+
+template <int BQ>
+int few_stages(int asked, int steps, int splits) {
+    using Cfg = FewConfig<BQ>;
+    int stages = max(1, min(min(asked, 8), steps));
+    // the sums meet in the stages: there has to be room for them
+    if (!Cfg::kOwnPlace && splits > 1) stages = max(stages, (Cfg::kMeetBytes + Cfg::kStageBytes - 1) / Cfg::kStageBytes);
+    while (stages > 1 && Cfg::smem(stages, splits) > 232448) --stages;
+    return stages;
+}
+
+template <int BQ, int EPI>
+int launch_many(const CUtensorMap& map_a, const CUtensorMap& map_w, const CUtensorMap& map_o, const ManyParams& p, cudaStream_t st) {
+    using Cfg = ManyConfig<BQ>;
+    static SharedLimit limit;
+    const cudaError_t le = limit.allow(reinterpret_cast<const void*>(int8_many_kernel<BQ, EPI>), Cfg::kSmem);
+    if (le != cudaSuccess) { set_error("int8_product: cannot reserve %d bytes of shared memory: %s", Cfg::kSmem, cudaGetErrorString(le)); return 1; }
+    const long long tiles = static_cast<long long>(p.tiles_t) * p.tiles_n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * static_cast<unsigned>(min(tiles, static_cast<long long>(sm_count() / 2))));
+    cfg.blockDim = dim3(kManyThreads);
+    cfg.dynamicSmemBytes = Cfg::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = g_pdl_enabled ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    counted(cudaLaunchKernelEx(&cfg, int8_many_kernel<BQ, EPI>, map_a, map_w, map_o, p));
+    return check_launch("int8_product");
+}
+
+int check_operands(const void* a, int T, int width, const void* tiles, int N, const void* status) {
+    GI_REQUIRE(T > 0 && N > 0 && width > 0, "int8_product: sizes must be positive (rows=%d, channels=%d, width=%d)", T, N, width);
+    GI_REQUIRE(width % 16 == 0 && width <= 131056, "int8_product: a width of %d (multiples of 16, at most 131056: the sums stay within 32 bits)", width);
+    GI_REQUIRE(reinterpret_cast<uintptr_t>(a) % 16 == 0 && reinterpret_cast<uintptr_t>(tiles) % 128 == 0, "int8_product: rows must be 16-byte aligned, weights 128-byte");
+    GI_REQUIRE(status != nullptr, "int8_product: a status word is required");
+    return 0;
+}
+
+int int8_few_impl(const void* a, const float* a_scales, int T, int width, const void* tiles, const float* w_scales, int N, int gated, void* out,
+                  int out_dtype, long long ldo, int accumulate, int bq, int splits, int stages, void* status, void* stream) {
+    if (T == 0) return 0;
+    if (int bad = check_operands(a, T, width, tiles, N, status)) return bad;
+    GI_REQUIRE(out_dtype == kF32 || out_dtype == kBF16, "int8_product: unsupported dtype code %d", out_dtype);
+    GI_REQUIRE(!(accumulate && out_dtype != kF32), "int8_product: accumulation needs a 32-bit output");
+    GI_REQUIRE(splits >= 1 && splits <= 8, "int8_product: %d ranges of K (1 to 8: one cluster)", splits);
+    FewParams p{};
+    p.tiles = static_cast<const uint8_t*>(tiles);
+    p.a_scales = a_scales;
+    p.w_scales = w_scales;
+    p.out = out;
+    p.ldo = ldo;
+    p.out_bf16 = out_dtype == kBF16;
+    p.accumulate = accumulate;
+    p.T = T;
+    p.N = N;
+    p.gated = gated;
+    p.total_kb = (width + kRowBytes - 1) / kRowBytes;
+    p.kb_per_split = (p.total_kb + splits - 1) / splits;
+    p.splits = (p.total_kb + p.kb_per_split - 1) / p.kb_per_split;      // (no range is empty)
+    p.status = static_cast<int*>(status);
+    const int n_tiles = (N + kTileRows - 1) / kTileRows * (gated ? 2 : 1);
+    const dim3 grid(n_tiles, (T + bq - 1) / bq, p.splits);
+    GI_REQUIRE(grid.y <= 65535, "int8_product: too many rows for tiles of %d", bq);
+    CUtensorMap map_a;
+    if (int bad = encode_rows(&map_a, a, T, width, bq)) return bad;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    auto go = [&](auto tile) {
+        constexpr int BQ = decltype(tile)::value;
+        p.stages = few_stages<BQ>(stages, (p.kb_per_split + FewConfig<BQ>::kKb - 1) / FewConfig<BQ>::kKb, p.splits);
+        return launch_few<BQ>(map_a, p, grid, st);
+    };
+    switch (bq) {
+        case 16: return go(std::integral_constant<int, 16>());
+        case 32: return go(std::integral_constant<int, 32>());
+        case 64: return go(std::integral_constant<int, 64>());
+        case 128: return go(std::integral_constant<int, 128>());
+        case 256: return go(std::integral_constant<int, 256>());
+        default: set_error("int8_product: tiles of %d rows (16, 32, 64, 128 or 256)", bq); return 2;
+    }
+}
+
+int int8_many_impl(const void* a, const float* a_scales, int T, int width, const void* tiles, const float* w_scales, int N, int gated, int act, float limit,
+                   const float* bias, void* out, int out_dtype, long long ldo, int accumulate, int bq, int group_t, void* status, void* stream) {
+    if (T == 0) return 0;
+    if (int bad = check_operands(a, T, width, tiles, N, status)) return bad;
+    GI_REQUIRE(out_dtype == kF32 || out_dtype == kBF16, "int8_product: unsupported dtype code %d", out_dtype);
+    GI_REQUIRE(!(accumulate && out_dtype != kF32), "int8_product: accumulation needs a 32-bit output");
+    GI_REQUIRE(!gated || (out_dtype == kBF16 && bq == 256), "int8_product: a gated product has a bfloat16 output");
+    GI_REQUIRE(act >= 0 && act < kActCount, "int8_product: unknown activation %d", act);
+    GI_REQUIRE(bq == 128 || bq == 256, "int8_product: tiles of %d channels (128 or 256)", bq);
+    GI_REQUIRE(group_t >= 1, "int8_product: groups of %d tiles", group_t);
+    ManyParams p{};
+    p.a_scales = a_scales;
+    p.w_scales = w_scales;
+    p.bias = bias;
+    p.out = out;
+    p.ldo = ldo;
+    p.T = T;
+    p.N = N;
+    p.total_kb = (width + kRowBytes - 1) / kRowBytes;
+    p.tiles_t = (T + 255) / 256;
+    p.tiles_n = (N + (gated ? kTileRows : bq) - 1) / (gated ? kTileRows : bq);
+    p.group_t = group_t;
+    p.act = act;
+    p.limit = limit;
+    p.status = static_cast<int*>(status);
+    GI_REQUIRE(static_cast<long long>(p.tiles_t) * p.tiles_n < (1ll << 30), "int8_product: too many tiles");
+    const int elt = out_dtype == kBF16 ? 2 : 4;
+    p.plain_stores = ldo * elt % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0;
+    const long long weight_rows = static_cast<long long>((N + kTileRows - 1) / kTileRows) * (gated ? 2 : 1) * p.total_kb * kTileRows;
+    GI_REQUIRE(weight_rows < (1ll << 31), "int8_product: the weights are too large");
+    CUtensorMap map_a, map_w, map_o{};
+    if (int bad = encode_rows(&map_a, a, T, width, kTileRows)) return bad;
+    if (int bad = encode(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, tiles, weight_rows, kRowBytes, kRowBytes, bq / 2, kRowBytes, CU_TENSOR_MAP_SWIZZLE_NONE,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return bad;
+    if (!p.plain_stores) {
+        if (int bad = encode(&map_o, elt == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, out, T, N, ldo * elt, kTileRows, 128 / elt,
+                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE)) return bad;
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (gated) return launch_many<256, kGatedBF16>(map_a, map_w, map_o, p, st);
+    if (elt == 2) return bq == 256 ? launch_many<256, kStoreBF16>(map_a, map_w, map_o, p, st) : launch_many<128, kStoreBF16>(map_a, map_w, map_o, p, st);
+    if (accumulate) return bq == 256 ? launch_many<256, kAddF32>(map_a, map_w, map_o, p, st) : launch_many<128, kAddF32>(map_a, map_w, map_o, p, st);
+    return bq == 256 ? launch_many<256, kStoreF32>(map_a, map_w, map_o, p, st) : launch_many<128, kStoreF32>(map_a, map_w, map_o, p, st);
+}
+
+}  // namespace
+}  // namespace gi
+
+// Few rows: tiles of bq rows of a [T, width], K in `splits` ranges (one cluster), up to `stages` stages of the pipeline. `gated`: the weights are a gated
+// pair of N channels each, out [T, 2 N] = [gate; up]. out[t, n] at t * ldo + n.
+extern "C" int gi_int8_product_few(const void* a, const float* a_scales, int T, int width, const void* tiles, const float* w_scales, int N, int gated,
+                                   void* out, int out_dtype, long long ldo, int accumulate, int bq, int splits, int stages, void* status, void* stream) {
+    return gi::dispatch(gi::int8_few_impl, a, a_scales, T, width, tiles, w_scales, N, gated, out, out_dtype, ldo, accumulate, bq, splits, stages, status, stream);
+}
+
+// Many rows: tiles of 256 rows x bq channels. `gated`: out [T, N] = act(gate) * up, bfloat16; `bias` [2 N] or null.
+extern "C" int gi_int8_product_many(const void* a, const float* a_scales, int T, int width, const void* tiles, const float* w_scales, int N, int gated,
+                                    int act, float limit, const float* bias, void* out, int out_dtype, long long ldo, int accumulate, int bq, int group_t,
+                                    void* status, void* stream) {
+    return gi::dispatch(gi::int8_many_impl, a, a_scales, T, width, tiles, w_scales, N, gated, act, limit, bias, out, out_dtype, ldo, accumulate, bq, group_t,
+                        status, stream);
+}

@@ -1727,3 +1727,189 @@ def adapter_product(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale
     check(lib().gi_adapter_product(_rows_of(x, "x"), x.stride(0), dtype_code(x.dtype), _dev(down, "down"), _dev(up, "up"),
                                    _dev(scales, "scales", torch.float32), plan.buffer.data_ptr(), T, A, plan.used, plan.tile_rows, _rows_of(out, "out"),
                                    out.stride(0), dtype_code(out.dtype), K, N, r, S, *ends, _stream()), "adapter_product")
+
+
+# ---------------------------------------------------------------------------------------------- 8-bit integers
+# A row of activations and a channel of weights as integers of -127 .. 127 with one 32-bit scale each: value ~ scale * q, with
+# q = rint(v * (127 / m)) and scale = m / 127 for a row v whose largest |v| is m. A row with a NaN or an infinity gets the scale NaN
+# (products with it are NaN), one whose m is below 2^-100 the scale 0. Rows lie in buffers of ``int8_width`` values, zeros behind.
+
+INT8_WIDTH_MOST = 131056      # sums of so many products stay within 32 bits, of -128 times -128 too
+INT8_FEW_ROWS = 256           # up to here products of few rows (weights on the 128-row side)
+
+
+def int8_width(values: int) -> int:
+    """The width of a buffer for rows of so many values in 8 bits: the next multiple of 16."""
+    return (values + 15) // 16 * 16
+
+
+def _here(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """All of them on the current device, on whose stream the kernel runs."""
+    for t in tensors:
+        if t is not None and t.is_cuda and t.get_device() != torch._C._cuda_getDevice():
+            raise KernelError(f"{name}: a tensor is on cuda:{t.get_device()}, the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
+def _rows_int8(name: str, kind: int, x: torch.Tensor, columns: int, out: torch.Tensor, scales: torch.Tensor, add=None, weight=None, eps: float = 0.0,
+               act: int = 0, limit: float = 0.0) -> None:
+    if x.dim() != 2 or out.dim() != 2:
+        raise KernelError(f"{name}: the rows and their integers must be matrices")
+    T = x.shape[0]
+    D = x.shape[1] // columns
+    if D < 1 or x.shape[1] != columns * D or out.shape != (T, int8_width(D)) or scales.numel() != T:
+        raise KernelError(f"{name}: out must be [T, int8_width(D)] and scales [T] for rows of D values")
+    _here(name, x, out, scales, add, weight)
+    check(lib().gi_rows_int8(kind, _rows_of(x, "x"), dtype_code(x.dtype), x.stride(0), 0 if add is None else _dev(add, "add"),
+                             0 if add is None else dtype_code(add.dtype), _opt(weight, "weight", torch.float32), float(eps), act, float(limit),
+                             _dev(out, "out", torch.int8), out.shape[1], _dev(scales, "scales", torch.float32), T, D, _stream()), name)
+
+
+def quantize_rows(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> None:
+    """The rows of ``x`` [T, D] (32-bit or bfloat16; rows may lie apart) in 8 bits: ``out`` [T, int8_width(D)] int8 and ``scales`` [T]."""
+    _rows_int8("quantize_rows", 0, x, 1, out, scales)
+
+
+def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, eps: float,
+                 add: Optional[torch.Tensor] = None) -> None:
+    """x += add (``add`` [T, D] 32-bit or bfloat16, where given), then weight * (x / sqrt(mean(x^2) + eps)) of every row in 8 bits:
+    ``out`` [T, int8_width(D)] int8 and ``scales`` [T]. ``x`` [T, D] is the 32-bit residual stream. The integers are those of
+    x * weight (the norm's factor is the row's: it goes into the scale)."""
+    if x.dim() != 2 or weight.numel() != x.shape[1] or (add is not None and add.shape != x.shape):
+        raise KernelError("rmsnorm_int8: shapes of x, weight and add do not agree")
+    if x.dtype is not torch.float32:
+        raise KernelError(f"rmsnorm_int8: x must be torch.float32, got {x.dtype}")
+    if add is not None and add.data_ptr() == x.data_ptr():
+        raise KernelError("rmsnorm_int8: add must not be x itself")
+    _rows_int8("rmsnorm_int8", 1, x, 1, out, scales, add=add, weight=weight, eps=eps)
+
+
+def gated_act_int8(gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, activation: str = "silu", limit: float = 0.0,
+                   bias: Optional[torch.Tensor] = None) -> None:
+    """act(gate_up[:, :I]) * gate_up[:, I:], rounded to bfloat16, in 8 bits: ``gate_up`` [T, 2I] (32-bit or bfloat16), ``out``
+    [T, int8_width(I)] int8, ``scales`` [T]; ``activation``, ``limit`` and ``bias`` [2I] as ``gated_act`` has them."""
+    if gate_up.dim() != 2 or gate_up.shape[1] % 2 or (bias is not None and bias.numel() != gate_up.shape[1]):
+        raise KernelError("gated_act_int8: gate_up must be [T, 2I] (and the bias [2I])")
+    if activation not in ACTIVATIONS:
+        raise KernelError(f"gated_act_int8: unknown activation '{activation}' (known: {', '.join(sorted(ACTIVATIONS))})")
+    _rows_int8("gated_act_int8", 2, gate_up, 2, out, scales, weight=bias, act=ACTIVATIONS[activation], limit=limit)
+
+
+class Int8Weight:
+    """A weight matrix [N, K] in 8 bits, a scale a channel, laid out as the products read it (``int8_weight``). ``channels`` N (gated: of a
+    part), ``width``: int8_width(K)."""
+
+    __slots__ = ("tiles", "scales", "channels", "width", "gated")
+
+    def __init__(self, tiles: torch.Tensor, scales: torch.Tensor, channels: int, width: int, gated: bool):
+        self.tiles, self.scales, self.channels, self.width, self.gated = tiles, scales, channels, width, gated
+
+
+def int8_weight(q: torch.Tensor, scales: torch.Tensor, gated: bool = False) -> Int8Weight:
+    """Lays out a weight for ``int8_product``: ``q`` [N, K] int8 (or [N, int8_width(K)] from ``quantize_rows``), ``scales`` [N] 32-bit. ``gated``: q is
+    [gate channels; up channels] of a gated feed-forward, for ``int8_gated``. Tiles of 128 channels x 128 values of K in the order
+    [channel tile][block of K], 16 KB each, the 16-byte pieces of row r permuted by piece ^ (r % 8): what the tensor cores read in
+    shared memory. Parts and K are padded to whole tiles with zeros; gate and up tiles alternate."""
+    if q.dim() != 2 or q.dtype is not torch.int8 or scales.numel() != q.shape[0] or scales.dtype is not torch.float32:
+        raise KernelError("int8_weight: q must be int8 [N, K] and scales 32-bit [N]")
+    N, K = q.shape
+    parts = 2 if gated else 1
+    if N < 1 or K < 1 or N % parts:
+        raise KernelError(f"int8_weight: {N} channels of {K} values{' in two parts' if gated else ''}")
+    if int8_width(K) > INT8_WIDTH_MOST:
+        raise KernelError(f"int8_weight: channels of {K} values (at most {INT8_WIDTH_MOST}: their sums stay within 32 bits)")
+    n = N // parts
+    Np, Kp = (n + 127) // 128 * 128, (K + 127) // 128 * 128
+    padded = torch.zeros((parts, Np, Kp), dtype=torch.int8, device=q.device)
+    padded[:, :n, :K] = q.view(parts, n, K)
+    t = padded.view(parts, Np // 128, 128, Kp // 128, 8, 16).permute(1, 0, 3, 2, 4, 5)      # [tile, part, block of K, row, piece, 16]
+    row = torch.arange(128, device=q.device).view(128, 1)
+    source = torch.arange(8, device=q.device).view(1, 8) ^ (row % 8)                      # place p of row r holds piece p ^ (r % 8)
+    tiles = t[:, :, :, row, source].contiguous().view(-1)
+    return Int8Weight(tiles, scales.reshape(-1).contiguous(), n, int8_width(K), gated)
+
+
+def _few_plan(T: int, n_tiles: int, blocks: int):
+    """(rows of a tile, ranges of K, stages) of a product of few rows."""
+    bq = next(b for b in (16, 32, 64, 128, 256) if b >= min(T, 256))
+    tiles = n_tiles * ((T + bq - 1) // bq)
+    splits = max(1, min(8, sm_count() // max(1, tiles), blocks))
+    return bq, splits, 3 if bq <= 64 else 4
+
+
+def _few(a, a_scales, w, out, accumulate, plan=None) -> None:
+    bq, splits, stages = plan or _few_plan(a.shape[0], (w.channels + 127) // 128 * (2 if w.gated else 1), (w.width + 127) // 128)
+    check(lib().gi_int8_product_few(_dev(a, "a", torch.int8), _dev(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
+                                    w.scales.data_ptr(), w.channels, int(w.gated), _rows_of(out, "out"), dtype_code(out.dtype), out.stride(0),
+                                    int(bool(accumulate)), bq, splits, stages, _tc_state(a.device).status.data_ptr(), _stream()), "int8_product")
+
+
+def _many_plan(T: int, N: int):
+    """(channels of a tile, tiles of rows walked together) of a product of many rows."""
+    return (256 if N > 128 else 128), 8
+
+
+def _many(a, a_scales, w, out, out_stride, accumulate, act=0, limit=0.0, bias=None, plan=None) -> None:
+    bq, group = plan or _many_plan(a.shape[0], w.channels)
+    check(lib().gi_int8_product_many(_dev(a, "a", torch.int8), _dev(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
+                                     w.scales.data_ptr(), w.channels, int(w.gated), act, float(limit), _opt(bias, "bias", torch.float32), out.data_ptr(),
+                                     dtype_code(out.dtype), out_stride, int(bool(accumulate)), 256 if w.gated else bq, group,
+                                     _tc_state(a.device).status.data_ptr(), _stream()), "int8_product")
+
+
+def _int8_operands(name: str, a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, *more: Optional[torch.Tensor]) -> int:
+    if a.dim() != 2 or a.shape[1] != w.width or a_scales.numel() != a.shape[0]:
+        raise KernelError(f"{name}: a must be [T, {w.width}] (the weight's width) and a_scales [T]")
+    _here(name, a, a_scales, w.tiles, *more)
+    return a.shape[0]
+
+
+def int8_product(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: torch.Tensor, accumulate: bool = False, plan=None) -> None:
+    """out[t, n] (+)= a_scales[t] * w.scales[n] * sum over k of a[t, k] * w[n, k]: ``a`` [T, w.width] int8 with ``a_scales`` [T], ``out``
+    [T, N] 32-bit (``accumulate``: added to) or bfloat16; its rows may lie apart. The sums are exact integers: a row's result does
+    not depend on the other rows of the call."""
+    T = _int8_operands("int8_product", a, a_scales, w, out)
+    if w.gated:
+        raise KernelError("int8_product: the weight is laid out for int8_gated")
+    if out.shape != (T, w.channels):
+        raise KernelError(f"int8_product: out must be [T, {w.channels}]")
+    if accumulate and out.dtype is not torch.float32:
+        raise KernelError("int8_product: accumulation needs a 32-bit output")
+    if (len(plan) == 3) if plan else T <= INT8_FEW_ROWS:
+        _few(a, a_scales, w, out, accumulate, plan)
+    else:
+        _rows_of(out, "out")
+        _many(a, a_scales, w, out, out.stride(0), accumulate, plan=plan)
+
+
+def int8_gated_work(rows: int, w: Int8Weight) -> int:
+    """32-bit values of the scratch that ``int8_gated`` needs for up to ``rows`` rows."""
+    return rows * max(2 * w.channels, 4)
+
+
+def int8_gated(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: torch.Tensor, out_scales: torch.Tensor, work: torch.Tensor,
+               activation: str = "silu", limit: float = 0.0, bias: Optional[torch.Tensor] = None) -> None:
+    """The first half of a gated feed-forward in 8 bits: h = act(gate) * up rounded to bfloat16, of the products of ``a`` [T, w.width]
+    with both parts of ``w`` (``int8_weight`` with ``gated``), and h in 8 bits to ``out`` [T, int8_width(I)] and ``out_scales`` [T]. ``work``: 32-bit scratch of
+    ``int8_gated_work`` values. ``activation``, ``limit``, ``bias`` [2I]: see ``gated_act``. Two launches: few rows leave the products in 32 bits for
+    ``gated_act_int8``; with many the activation is the product's epilogue."""
+    T = _int8_operands("int8_gated", a, a_scales, w, out, out_scales, work, bias)
+    I = w.channels
+    if not w.gated:
+        raise KernelError("int8_gated: the weight is not laid out as a gated pair")
+    if out.shape != (T, int8_width(I)) or out_scales.numel() != T or (bias is not None and bias.numel() != 2 * I):
+        raise KernelError(f"int8_gated: out must be [T, {int8_width(I)}] and out_scales [T] (and the bias [{2 * I}])")
+    if activation not in ACTIVATIONS:
+        raise KernelError(f"int8_gated: unknown activation '{activation}' (known: {', '.join(sorted(ACTIVATIONS))})")
+    _dev(work, "work", torch.float32)
+    if work.numel() < int8_gated_work(T, w):
+        raise KernelError(f"int8_gated: work must hold {int8_gated_work(T, w)} values")
+    work = work.view(-1)
+    if T <= INT8_FEW_ROWS:
+        both = work[:T * 2 * I].view(T, 2 * I)
+        _few(a, a_scales, w, both, False)
+        gated_act_int8(both, out, out_scales, activation, limit, bias)
+        return
+    stride = (I + 7) // 8 * 8                 # whole 16 bytes
+    h = work.view(torch.bfloat16)[:T * stride].view(T, stride)[:, :I]
+    _many(a, a_scales, w, h, stride, False, ACTIVATIONS[activation], limit, bias)
+    quantize_rows(h, out, out_scales)
