@@ -13,6 +13,7 @@
 #include <cstdio>
 #include <functional>
 #include <tuple>
+#include <type_traits>
 #include <vector>
 
 namespace gi {
@@ -81,8 +82,9 @@ __device__ __forceinline__ void timeline_record(int, int) {}
 #define GI_TIMELINE_SETTER(name) extern "C" int name(void*) { return 2; }
 #endif
 enum TimelineKernel : int {
-    kTlRmsNorm = 1, kTlSwiGLU = 2, kTlAttentionDecode = 3, kTlAddRanges = 4, kTlRopeStore = 5, kTlAttentionPrefill = 6,
+    kTlRmsNorm = 1, kTlSwiGLU = 2, kTlAttentionDecode = 3, kTlAddRanges = 4, kTlRopeStore = 5, kTlAttentionPrefill = 6, kTlInt8Rows = 7,
     kTlProduct = 100,            // + the form (TcSpecKind) of the few-token product
+    kTlInt8ProductFew = 121, kTlInt8ProductMany = 221,
     kTlProductManyTokens = 200,  // + 2 * epilogue (TcEpilogue) + (1 on pairs of CTAs)
 };
 
@@ -125,6 +127,35 @@ __device__ __forceinline__ float gated_value(float g, float u, int act, float li
         return g * (1.0f / (1.0f + expf(-1.702f * g))) * (u + 1.0f);
     }
     return g * (1.0f / (1.0f + expf(-g))) * u;
+}
+
+// The same for a result that is rounded to bfloat16 (half a step 2^-9): exponential and quotient with the hardware's approximations, whose errors
+// stay below 2^-16 of the result (the exponent z log2 e, up to 128, is rounded to 24 bits), and tanh-GELU as g * sigmoid(2 z), which does
+// not cancel. What is below 2^-126 counts as zero.
+__device__ __forceinline__ float sigmoid_times(float z, float g) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return g * r;
+}
+template <int ACT>
+__device__ __forceinline__ float gated_value_bf16(float g, float u, float limit) {
+    if (ACT == kActRelu) return fmaxf(g, 0.f) * u;
+    if (ACT == kActGeluTanh) return sigmoid_times(1.5957691216057308f * (g + 0.044715f * g * g * g), g) * u;
+    if (ACT == kActCappedSwish) {
+        g = fminf(g, limit);
+        u = fminf(fmaxf(u, -limit), limit);
+        return sigmoid_times(1.702f * g, g) * (u + 1.0f);
+    }
+    return sigmoid_times(g, g) * u;
+}
+// f(std::integral_constant<int, ACT>()) with the activation as a constant: one branch outside a loop over values instead of one in each.
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F f) {
+    if (act == kActRelu) f(std::integral_constant<int, kActRelu>());
+    else if (act == kActGeluTanh) f(std::integral_constant<int, kActGeluTanh>());
+    else if (act == kActCappedSwish) f(std::integral_constant<int, kActCappedSwish>());
+    else f(std::integral_constant<int, kActSilu>());
 }
 
 // What an ungated feed-forward applies to its first product, 32-bit: 0 nothing, 1 the square of ReLU.

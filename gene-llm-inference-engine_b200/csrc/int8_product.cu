@@ -11,7 +11,7 @@
 // reads in shared memory (K-major, 128-byte swizzle), so a tile is one stretch of memory and both kernels read the same one copy.
 // Weights of a gated pair lie gate tile, up tile, gate tile, .. (each part padded to whole tiles).
 //
-// Few rows (int8_few_kernel). The weights take the 128-row side and up to 256 rows of activations the narrow side. What bounds it is
+// Few rows (int8_few_kernel). The weights take the 128-row side and up to 64 rows of activations the narrow side. What bounds it is
 // the stream of the weights: a CTA keeps its share of shared memory full of bulk copies and computes as they land. K is cut over the CTAs of
 // a cluster until the SMs have work; each CTA then collects the sums of its share of the rows from the others' shared memory
 // (integers, so in any order), scales and stores them.
@@ -137,20 +137,23 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint3
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
                      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-// arrives on the barrier (of both CTAs of a pair) once the products issued so far are done
-template <bool PAIR>
+// arrives on the barrier once the products issued so far are done; of a pair's products on the barriers at this place in both CTAs
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-    if (PAIR)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                     ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
-    else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
 }
 __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
                    "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load8(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr));
 }
 __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
@@ -170,7 +173,6 @@ struct FewParams {
     const float* w_scales;
     void* out;               // out[t * ldo + n]
     long long ldo;
-    int out_bf16, accumulate;
     int T, N;                // N: channels of a part (gated weights: of gate and of up)
     int gated;
     int total_kb, kb_per_split, splits;
@@ -178,46 +180,48 @@ struct FewParams {
     int* status;
 };
 
-constexpr int kFewThreads = 192;      // producer, MMA, four epilogue warps
+enum Epilogue : int { kStoreF32 = 0, kAddF32 = 1, kStoreBF16 = 2, kGatedBF16 = 3 };
 
+// Tiles of BQ rows. Tiles of 8 have one group of four epilogue warps, larger ones two that take turns (one token through 8192 -> 2048 with 16 rows to a
+// tile: 5.9 us with one group, 6.4 with two; 64 rows through 4096 -> 4096: 8.8 and 8.0).
 template <int BQ>
 struct FewConfig {
-    static constexpr int kKb = BQ <= 64 ? 2 : 1;               // blocks of K to a stage
+    static constexpr int kGroups = BQ <= 8 ? 1 : 2;
+    static constexpr int kThreads = 64 + 128 * kGroups;        // producer, MMA, epilogue
+    static constexpr int kKb = BQ <= 8 ? 2 : 1;                // blocks of K to a stage
     static constexpr int kBlockBytes = kTileBytes + BQ * kRowBytes;
     static constexpr int kStageBytes = kKb * kBlockBytes;
     static constexpr int kTmemCols = BQ < 32 ? 32 : BQ;
-    // the sums that the CTAs of a cluster hand each other: up to 8 equal shares of the rows, the last one padded
-    static constexpr int kMeetBytes = (BQ + 7) * kTileRows * 4;
-    static constexpr bool kOwnPlace = BQ <= 64;                // ... behind the stages, or in them once the products are done
     static constexpr int kSideBytes = 256 + 4 * BQ;            // barriers, flags, the rows' scales
-    static constexpr int smem(int stages, int splits) {
-        return stages * kStageBytes + (kOwnPlace && splits > 1 ? kMeetBytes : 0) + kSideBytes + 1024;
-    }
+    // the sums that the CTAs of a cluster hand each other: equal shares of a tile's rows, the last one padded
+    static constexpr int meet(int rows, int splits) { return splits > 1 ? (rows + splits - 1) / splits * splits * kTileRows * 4 : 0; }
+    static constexpr int smem(int stages, int rows, int splits) { return stages * kStageBytes + meet(rows, splits) + kSideBytes; }
 };
 
-template <int BQ>
-__global__ void __launch_bounds__(kFewThreads)
+// A kernel for each epilogue, with and without a cluster: a short kernel pays for every instruction that it has to fetch.
+template <int BQ, int EPI, bool CLUSTER>
+__global__ void __launch_bounds__(FewConfig<BQ>::kThreads)
 int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const FewParams p) {
     using Cfg = FewConfig<BQ>;
     constexpr int kKb = Cfg::kKb;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    const int stages = p.stages;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int stages = p.stages, splits = CLUSTER ? p.splits : 1;
     uint8_t* behind = smem + stages * Cfg::kStageBytes;
-    int* meet = reinterpret_cast<int*>(Cfg::kOwnPlace ? behind : smem);      // [split][rows of a CTA's share][128]: at most BQ + 7 rows
-    if (Cfg::kOwnPlace && p.splits > 1) behind += Cfg::kMeetBytes;
+    int* meet = reinterpret_cast<int*>(behind);                // [split][rows of a CTA's share][128]
+    if (CLUSTER) behind += Cfg::meet(min(BQ, p.T), splits);
     uint64_t* bars = reinterpret_cast<uint64_t*>(behind);      // [0, 8) full, [8, 16) empty, [16] sums complete
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* row_scales = reinterpret_cast<float*>(behind + 256);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tile_n = blockIdx.x, tile_t = blockIdx.y, split = blockIdx.z;
+    const int tile_n = blockIdx.x, tile_t = blockIdx.y, split = CLUSTER ? blockIdx.z : 0;
     const int kb_begin = split * p.kb_per_split;
     const int n_kb = min(p.total_kb, kb_begin + p.kb_per_split) - kb_begin;
     const int n_steps = (n_kb + kKb - 1) / kKb;
 
     if (threadIdx.x == 0) {
+        timeline_record(kTlInt8ProductFew, 0);
         for (int s = 0; s < stages; ++s) {
             bar_init(smem_addr(&bars[s]), 1);
             bar_init(smem_addr(&bars[8 + s]), 1);
@@ -239,6 +243,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const FewParams p) {
             const uint8_t* src = p.tiles + (static_cast<size_t>(tile_n) * p.total_kb + kb_begin) * kTileBytes;
             auto blocks_of = [&](int i) { return min(kKb, n_kb - i * kKb); };
             auto load_w = [&](int i, int s) {
+                bar_expect(smem_addr(&bars[s]), blocks_of(i) * Cfg::kBlockBytes);
                 load_bulk(smem_addr(smem + s * Cfg::kStageBytes), src + static_cast<size_t>(i) * kKb * kTileBytes, blocks_of(i) * kTileBytes,
                           smem_addr(&bars[s]), policy);
             };
@@ -249,22 +254,17 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const FewParams p) {
             };
             // the weights belong to no earlier kernel: their first tiles are asked for before the wait for the kernels ahead
             const int early = min(n_steps, stages);
-            for (int i = 0; i < early; ++i) {
-                bar_expect(smem_addr(&bars[i]), blocks_of(i) * Cfg::kBlockBytes);
-                load_w(i, i);
-            }
+            for (int i = 0; i < early; ++i) load_w(i, i);
             pdl_wait();
+            timeline_record(kTlInt8ProductFew, 1);
             for (int i = 0; i < early; ++i) load_a(i, i);
-            int issued = early, s = 0, round = 1;
-            if (early == stages) {
-                for (int i = early; i < n_steps; ++i) {
-                    if (!bar_wait(smem_addr(&bars[8 + s]), (round & 1) ^ 1, gave_up, p.status, kErrProducer)) break;
-                    bar_expect(smem_addr(&bars[s]), blocks_of(i) * Cfg::kBlockBytes);
-                    load_w(i, s);
-                    load_a(i, s);
-                    issued = i + 1;
-                    if (++s == stages) { s = 0; ++round; }
-                }
+            int issued = early, s = 0, parity = 0;
+            for (int i = early; i < n_steps; ++i) {      // (early == stages, where there are more steps)
+                if (!bar_wait(smem_addr(&bars[8 + s]), parity, gave_up, p.status, kErrProducer)) break;
+                load_w(i, s);
+                load_a(i, s);
+                issued = i + 1;
+                if (++s == stages) { s = 0; parity ^= 1; }
             }
             if (*gave_up) {      // every copy must have landed before the CTA leaves
                 for (int i = max(0, issued - stages); i < issued; ++i) {
@@ -282,18 +282,21 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const FewParams p) {
             for (int i = 0; i < n_steps; ++i) {
                 if (!bar_wait(smem_addr(&bars[s]), parity, gave_up, p.status, kErrMma)) { ok = false; break; }
                 fence_after();
+                if (i == 0) timeline_record(kTlInt8ProductFew, 2);
                 const uint32_t at = smem_addr(smem + s * Cfg::kStageBytes);
                 const int blocks = min(kKb, n_kb - i * kKb);
+#pragma unroll 1
                 for (int j = 0; j < blocks; ++j) {
                     const uint64_t w = tile_desc(at + j * kTileBytes), a = tile_desc(at + kKb * kTileBytes + j * BQ * kRowBytes);
 #pragma unroll
                     for (int k = 0; k < kRowBytes / 32; ++k)      // 32 values of K to an instruction
                         mma_i8<false>(tmem, w + 2 * k, a + 2 * k, idesc, (i > 0 || j > 0 || k > 0) ? 1u : 0u);
                 }
-                mma_commit<false>(smem_addr(&bars[8 + s]));
+                mma_commit(smem_addr(&bars[8 + s]));
                 if (++s == stages) { s = 0; parity ^= 1; }
             }
-            if (ok) mma_commit<false>(smem_addr(&bars[16]));
+            if (ok) mma_commit(smem_addr(&bars[16]));
+            timeline_record(kTlInt8ProductFew, 3);
         }
     }
     __syncwarp();
@@ -306,74 +309,105 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const FewParams p) {
     const int channel = (p.gated && (tile_n & 1) ? p.N : 0) + part_tile * kTileRows + row;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(lane_group * 32) << 16);
     const bool epilogue = warp >= 2;
+    // CTA r of the cluster ends rows r * share .. of the tile (share: all of them without a cluster)
+    const int share = (rows_here + splits - 1) / splits, first = split * share, n_mine = min(share, rows_here - first);
     bool ok = false;
     float w_scale = 0.f;
-    auto emit = [&](int t, int sum) {      // t: the row within the tile
-        const float v = scaled(sum, row_scales[t], w_scale);
-        const size_t at = static_cast<size_t>(tile_t * BQ + t) * p.ldo + channel;
-        if (p.out_bf16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-        else static_cast<float*>(p.out)[at] = p.accumulate ? __fadd_rn(static_cast<const float*>(p.out)[at], v) : v;
+    constexpr int kBytes = EPI == kStoreBF16 ? 2 : 4;
+    char* out = static_cast<char*>(p.out) + (static_cast<size_t>(tile_t * BQ) * p.ldo + channel) * kBytes;
+    const size_t out_step = static_cast<size_t>(p.ldo) * kBytes;
+    // Rows t .. t + kGroup - 1 (n of them there) of this thread's channel. All loads stand before the first store: nothing tells the compiler that they do
+    // not overlap, and one load behind each store costs a row 100 cycles (128 rows one by one: 7 us).
+    constexpr int kGroup = 8;
+    const int group_first = Cfg::kGroups == 1 ? 0 : ((warp - 2) >> 2) * kGroup;
+    auto load_old = [&](int t, int n, float* old) {
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) old[j] = j < n ? __ldcg(reinterpret_cast<const float*>(out + (t + j) * out_step)) : 0.f;
     };
+    auto put = [&](int t, int n, const int* sum, const float* old) {
+        float v[kGroup];
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) v[j] = scaled(sum[j], row_scales[min(t + j, BQ - 1)], w_scale);
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) {
+            if (j >= n) continue;
+            if (EPI == kStoreBF16) *reinterpret_cast<__nv_bfloat16*>(out + (t + j) * out_step) = __float2bfloat16_rn(v[j]);
+            else *reinterpret_cast<float*>(out + (t + j) * out_step) = EPI == kAddF32 ? __fadd_rn(old[j], v[j]) : v[j];
+        }
+    };
+    float old[kGroup];
+    const bool adds = EPI == kAddF32 && epilogue && channel_there;
     if (epilogue) {
         if (channel_there) w_scale = __ldg(p.w_scales + channel);
         pdl_wait();
-        for (int t = threadIdx.x - 64; t < rows_here; t += 128) row_scales[t] = __ldcg(p.a_scales + tile_t * BQ + t);
+        for (int t = threadIdx.x - 64; t < rows_here; t += 128 * Cfg::kGroups) row_scales[t] = __ldcg(p.a_scales + tile_t * BQ + t);
+        if (adds) load_old(first + group_first, n_mine - group_first, old);          // while the products run
         ok = bar_wait(smem_addr(&bars[16]), 0, gave_up, p.status, kErrEpilogue);
         fence_after();
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(128 * Cfg::kGroups) : "memory");
+        if (threadIdx.x == 64) timeline_record(kTlInt8ProductFew, 4);
     }
-    if (p.splits == 1) {
-        if (epilogue && __all_sync(0xffffffffu, ok)) {
+    const bool whole = epilogue && __all_sync(0xffffffffu, ok);
+    if constexpr (!CLUSTER) {
+        if (whole) {
 #pragma unroll 1
-            for (int c = 0; c < rows_here; c += 16) {
-                uint32_t r[16];
-                tmem_load16(lane_addr + c, r);
+            for (int c = group_first; c < rows_here; c += Cfg::kGroups * kGroup) {
+                uint32_t r[kGroup];
+                tmem_load8(lane_addr + c, r);
+                if (adds && c > group_first) load_old(c, rows_here - c, old);
                 tmem_load_wait();
-                if (channel_there) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (c + j < rows_here) emit(c + j, static_cast<int>(r[j]));
-                }
+                if (channel_there) put(c, rows_here - c, reinterpret_cast<const int*>(r), old);
             }
         }
     } else {
-        // CTA r of the cluster takes rows r * share .. of the tile
-        const int share = (rows_here + p.splits - 1) / p.splits;
-        if (!Cfg::kOwnPlace) cluster_sync();      // the stages of every CTA are done with
         if (epilogue) {
-            const bool send = __all_sync(0xffffffffu, ok);
-            int owner = 0, place = 0;
-            uint32_t to = map_to(smem_addr(meet), 0);
 #pragma unroll 1
-            for (int c = 0; c < rows_here; c += 16) {
-                uint32_t r[16];
-                if (send) {
-                    tmem_load16(lane_addr + c, r);
+            for (int c = group_first; c < rows_here; c += Cfg::kGroups * kGroup) {
+                uint32_t r[kGroup];
+                if (whole) {
+                    tmem_load8(lane_addr + c, r);
                     tmem_load_wait();
                 }
+                int owner = c / share, place = c - owner * share;
+                uint32_t to = map_to(smem_addr(meet + (split * share) * kTileRows + row), static_cast<uint32_t>(owner));
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
+                for (int j = 0; j < kGroup; ++j) {
                     if (c + j < rows_here) {
-                        store_cluster(to + static_cast<uint32_t>(((split * share + place) * kTileRows + row) * 4), send ? r[j] : 0u);
-                        if (++place == share) { place = 0; to = map_to(smem_addr(meet), static_cast<uint32_t>(++owner < p.splits ? owner : 0)); }
+                        store_cluster(to + static_cast<uint32_t>(place * kTileRows * 4), whole ? r[j] : 0u);
+                        if (++place == share) {
+                            place = 0;
+                            ++owner;
+                            to = map_to(smem_addr(meet + (split * share) * kTileRows + row), static_cast<uint32_t>(min(owner, splits - 1)));
+                        }
                     }
                 }
             }
         }
         __syncwarp();
         cluster_sync();                           // everyone's sums have arrived; nobody's memory is written from here on
+        if (threadIdx.x == 64) timeline_record(kTlInt8ProductFew, 7);
         if (epilogue && channel_there) {
-            for (int i = 0; i < share; ++i) {
-                const int t = split * share + i;
-                if (t >= rows_here) break;
-                int sum = 0;
-                for (int s = 0; s < p.splits; ++s) sum += meet[(s * share + i) * kTileRows + row];
-                emit(t, sum);
+#pragma unroll 1
+            for (int i = group_first; i < n_mine; i += Cfg::kGroups * kGroup) {
+                int sum[kGroup];
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j) sum[j] = 0;
+                if (adds && i > group_first) load_old(first + i, n_mine - i, old);
+#pragma unroll 1
+                for (int s = 0; s < splits; ++s) {
+                    const int* from = meet + (s * share + i) * kTileRows + row;
+#pragma unroll
+                    for (int j = 0; j < kGroup; ++j)
+                        if (i + j < n_mine) sum[j] += from[j * kTileRows];
+                }
+                put(first + i, n_mine - i, sum, old);
             }
         }
+        if (threadIdx.x == 64) timeline_record(kTlInt8ProductFew, 5);
     }
     fence_before();
     __syncthreads();
+    if (threadIdx.x == 0) timeline_record(kTlInt8ProductFew, 6);
     if (warp == 1) {
         fence_after();
         tmem_free<false>(tmem, Cfg::kTmemCols);
@@ -381,8 +415,6 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const FewParams p) {
 }
 
 // ------------------------------------------------------------------------------------------ many rows
-enum ManyEpilogue : int { kStoreF32 = 0, kAddF32 = 1, kStoreBF16 = 2, kGatedBF16 = 3 };
-
 struct ManyParams {
     const float* a_scales;
     const float* w_scales;
@@ -392,7 +424,7 @@ struct ManyParams {
     int plain_stores;        // the output's rows are not whole 16 bytes: no TMA
     int T, N;                // N: output channels
     int total_kb;
-    int tiles_t, tiles_n;    // of 256 rows, of BQ channels (gated: 128 of them)
+    int tiles_t, tiles_n;    // of 256 rows, of 256 channels (gated: 128 gates and their ups)
     int group_t;             // tiles of rows that are walked together
     int act;
     float limit;
@@ -401,41 +433,59 @@ struct ManyParams {
 
 constexpr int kManyThreads = 64 + 2 * 128;      // producer, MMA, two epilogue groups of four warps
 
-template <int BQ>
-struct ManyConfig {
-    static constexpr int kWRows = BQ / 2;                                    // channels in this CTA's shared memory
-    static constexpr int kStageBytes = kTileBytes + kWRows * kRowBytes;
-    static constexpr int kStages = BQ == 256 ? 6 : 8;
-    static constexpr int kStagingBytes = kTileRows * 128;                    // 128 rows x 128 bytes, one to a group
-    static constexpr int kTmemCols = 2 * BQ;
-    static constexpr int kSideBytes = 256 + BQ * 4;                          // barriers; the channels' scales of a tile
-    static constexpr int kSmem = kStages * kStageBytes + 2 * kStagingBytes + kSideBytes + 1024;
-    static_assert(kSmem <= 232448, "the pipeline does not fit into an SM's shared memory");
-};
+constexpr int kTileN = 256;                                                  // channels of a tile: 128 in each CTA's shared memory
+constexpr int kManyStageBytes = 2 * kTileBytes;
+constexpr int kManyStages = 6;
+constexpr int kStagingBytes = kTileRows * 128;                               // 128 rows x 128 bytes, one to a group
+constexpr int kManySmem = kManyStages * kManyStageBytes + 2 * kStagingBytes + 256 + 4 * kTileN + 1024;      // barriers; the channels' scales of a tile
+static_assert(kManySmem <= 232448, "the pipeline does not fit into an SM's shared memory");
 
-template <int BQ, int EPI>
+// act(gate) * up of 32 channels, packed to bfloat16; n0: the first one's number.
+__device__ __forceinline__ void gated32(uint32_t* r, uint32_t* u, const float* gate_scales, const float* up_scales, float row_scale, int n0, const ManyParams& p,
+                                        uint32_t* packed) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        r[j] = __float_as_uint(scaled(static_cast<int>(r[j]), row_scale, gate_scales[j]));
+        u[j] = __float_as_uint(scaled(static_cast<int>(u[j]), row_scale, up_scales[j]));
+    }
+    if (p.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            const float bg = n0 + j < p.N ? __ldg(p.bias + n0 + j) : 0.f, bu = n0 + j < p.N ? __ldg(p.bias + p.N + n0 + j) : 0.f;
+            r[j] = __float_as_uint(__fadd_rn(__uint_as_float(r[j]), bg));
+            u[j] = __float_as_uint(__fadd_rn(__uint_as_float(u[j]), bu));
+        }
+    }
+    with_activation(p.act, [&](auto act) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+            const __nv_bfloat162 hb = __floats2bfloat162_rn(gated_value_bf16<decltype(act)::value>(__uint_as_float(r[j]), __uint_as_float(u[j]), p.limit),
+                                                            gated_value_bf16<decltype(act)::value>(__uint_as_float(r[j + 1]), __uint_as_float(u[j + 1]), p.limit));
+            packed[j / 2] = *reinterpret_cast<const uint32_t*>(&hb);
+        }
+    });
+}
+
+template <int EPI>
 __global__ void __launch_bounds__(kManyThreads, 1)
 int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_o,
                  const ManyParams p) {
-    using Cfg = ManyConfig<BQ>;
-    constexpr int kStages = Cfg::kStages;
-    static_assert(EPI != kGatedBF16 || BQ == 256, "a gated tile is a tile of gates and one of ups");
+    constexpr int kStages = kManyStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint8_t* staging = smem + kStages * Cfg::kStageBytes;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 2 * Cfg::kStagingBytes);
+    uint8_t* staging = smem + kStages * kManyStageBytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 2 * kStagingBytes);
     // [0, S) full, [S, 2S) empty, [2S, 2S + 2) sums complete, [2S + 2, 2S + 4) sums read
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* decided = gave_up + 1;
-    float* scales = reinterpret_cast<float*>(staging + 2 * Cfg::kStagingBytes + 256);      // [BQ]
+    float* scales = reinterpret_cast<float*>(staging + 2 * kStagingBytes + 256);      // [256]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int worker = blockIdx.x / 2, n_workers = gridDim.x / 2;
     const int n_tiles = p.tiles_t * p.tiles_n;
-    // Tiles are walked in groups of group_t tiles of rows, through all channels: what the CTAs read at one time is a few tiles of
-    // rows and a few of channels, which L2 holds, instead of all rows again for every few channels.
+    // Tiles are walked in groups of group_t tiles of rows, through all channels.
     auto tile_of = [&](int i, int& tile_t, int& tile_n) {
         const int per_group = p.group_t * p.tiles_n, g = i / per_group, in = i - g * per_group;
         const int here = min(p.group_t, p.tiles_t - g * p.group_t);
@@ -444,6 +494,7 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     };
 
     if (threadIdx.x == 0) {
+        timeline_record(kTlInt8ProductMany, 0);
         for (int s = 0; s < kStages; ++s) {
             bar_init(smem_addr(&bars[s]), 1);
             bar_init(smem_addr(&bars[kStages + s]), 1);
@@ -455,7 +506,7 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) tmem_allocate<true>(smem_addr(tmem_slot), Cfg::kTmemCols);
+    if (warp == 1) tmem_allocate<true>(smem_addr(tmem_slot), 2 * kTileN);
     fence_before();
     __syncthreads();
     fence_after();
@@ -463,6 +514,7 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     pdl_launch_dependents();
     cluster_sync();          // both CTAs' barriers exist before either signals the other's
     pdl_wait();
+    if (threadIdx.x == 0) timeline_record(kTlInt8ProductMany, 1);
     auto leader_bar = [&](int i) { return map_to(smem_addr(&bars[i]), 0u); };
 
     if (warp == 0) {
@@ -473,16 +525,14 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 int tile_t, tile_n;
                 tile_of(i, tile_t, tile_n);
                 const int t0 = tile_t * 256 + static_cast<int>(rank) * kTileRows;
-                // this CTA's rows of the channels' tile: a tile of its own (256 channels), or half of one (128)
-                const long long w0 = BQ == 256 ? (2ll * tile_n + rank) * p.total_kb * kTileRows
-                                               : static_cast<long long>(tile_n) * p.total_kb * kTileRows + rank * Cfg::kWRows;
+                const int w0 = (2 * tile_n + static_cast<int>(rank)) * p.total_kb * kTileRows;      // this CTA's tile of the channels
                 for (int kb = 0; kb < p.total_kb; ++kb, ++it) {
                     const int s = it % kStages;
                     if (!bar_wait(smem_addr(&bars[kStages + s]), ((it / kStages) & 1) ^ 1, gave_up, p.status, kErrProducer)) { ok = false; break; }
-                    const uint32_t stage = smem_addr(smem + s * Cfg::kStageBytes), full = leader_bar(s);
-                    if (rank == 0) bar_expect(smem_addr(&bars[s]), 2 * Cfg::kStageBytes);
+                    const uint32_t stage = smem_addr(smem + s * kManyStageBytes), full = leader_bar(s);
+                    if (rank == 0) bar_expect(smem_addr(&bars[s]), 2 * kManyStageBytes);
                     load_tile_pair(stage, &map_a, kb * kRowBytes, t0, full);
-                    load_tile_pair(stage + kTileBytes, &map_w, 0, static_cast<int>(w0 + static_cast<long long>(kb) * kTileRows), full);
+                    load_tile_pair(stage + kTileBytes, &map_w, 0, w0 + kb * kTileRows, full);
                 }
             }
             if (*gave_up && rank == 0) {
@@ -495,35 +545,37 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {      // a pair's products are issued by its first CTA
-            constexpr uint32_t idesc = int8_idesc(256, BQ);
+            constexpr uint32_t idesc = int8_idesc(256, kTileN);
             int it = 0, n = 0;
             bool ok = true;
             for (int i = worker; i < n_tiles && ok; i += n_workers, ++n) {
                 const int buf = n & 1;
                 if (!bar_wait<true>(smem_addr(&bars[2 * kStages + 2 + buf]), ((n >> 1) & 1) ^ 1, gave_up, p.status, kErrMma)) break;
                 fence_after();
-                const uint32_t d = tmem + buf * BQ;
+                const uint32_t d = tmem + buf * kTileN;
                 for (int kb = 0; kb < p.total_kb; ++kb, ++it) {
                     const int s = it % kStages;
                     if (!bar_wait(smem_addr(&bars[s]), (it / kStages) & 1, gave_up, p.status, kErrMma)) { ok = false; break; }
                     fence_after();
-                    const uint32_t at = smem_addr(smem + s * Cfg::kStageBytes);
+                    if (it == 0) timeline_record(kTlInt8ProductMany, 2);
+                    const uint32_t at = smem_addr(smem + s * kManyStageBytes);
                     const uint64_t a = tile_desc(at), w = tile_desc(at + kTileBytes);
 #pragma unroll
                     for (int k = 0; k < kRowBytes / 32; ++k) mma_i8<true>(d, a + 2 * k, w + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
-                    mma_commit<true>(smem_addr(&bars[kStages + s]));
+                    mma_commit_pair(smem_addr(&bars[kStages + s]));
                 }
-                if (ok) mma_commit<true>(smem_addr(&bars[2 * kStages + buf]));
+                if (ok) mma_commit_pair(smem_addr(&bars[2 * kStages + buf]));
             }
+            timeline_record(kTlInt8ProductMany, 3);
         }
     } else {
         // Group 0 (warps 2..5) takes the even chunks of a tile's columns, group 1 the odd ones; each has a staging buffer, a
         // named barrier and a thread that issues its stores. A thread holds one row of the tile.
         const int group = (warp - 2) >> 2, lane_group = warp & 3;
         const int row = lane_group * 32 + lane;
-        const int in_group = threadIdx.x - 64 - group * 128;
-        const bool leader = in_group == 0;
-        uint8_t* stg = staging + group * Cfg::kStagingBytes;
+        const int mine = static_cast<int>(threadIdx.x) - 64;
+        const bool leader = (mine & 127) == 0;
+        uint8_t* stg = staging + group * kStagingBytes;
         auto group_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
         auto both_sync = [&]() { asm volatile("bar.sync 3, 256;" ::: "memory"); };
         auto sums_read = [&](int buf) {
@@ -539,21 +591,21 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             const int buf = n & 1;
             const float row_scale = t < p.T ? __ldcg(p.a_scales + t) : 0.f;
             // the tile's channels: column c of the sums is channel n0 + c (gated: columns 128 .. are the ups)
-            const int n0 = EPI == kGatedBF16 ? tile_n * kTileRows : tile_n * BQ;
-            const int mine = threadIdx.x - 64;
+            const int n0 = EPI == kGatedBF16 ? tile_n * kTileRows : tile_n * kTileN;
             const bool up = EPI == kGatedBF16 && mine >= kTileRows;
             const int ch = n0 + (up ? mine - kTileRows : mine);
-            const float mine_scale = mine < BQ && ch < p.N ? __ldg(p.w_scales + (up ? p.N : 0) + ch) : 0.f;
+            const float mine_scale = ch < p.N ? __ldg(p.w_scales + (up ? p.N : 0) + ch) : 0.f;
             bar_wait(smem_addr(&bars[2 * kStages + buf]), (n >> 1) & 1, gave_up, p.status, kErrEpilogue);
             both_sync();                               // nobody reads the last tile's scales any more
-            if (mine < BQ) scales[mine] = mine_scale;
+            scales[mine] = mine_scale;
             if (mine == 0) *decided = *gave_up == 0;
             both_sync();                               // the scales are there, and one decision for all
             if (!*decided) break;
             fence_after();
-            const uint32_t d = tmem + buf * BQ + (static_cast<uint32_t>(lane_group * 32) << 16);
+            if (n == 0 && mine == 0) timeline_record(kTlInt8ProductMany, 4);
+            const uint32_t d = tmem + buf * kTileN + (static_cast<uint32_t>(lane_group * 32) << 16);
             constexpr int kCols = EPI == kStoreF32 || EPI == kAddF32 ? 32 : 64;      // output columns to a chunk: 128 bytes
-            constexpr int kChunks = EPI == kGatedBF16 ? 2 : BQ / kCols;
+            constexpr int kChunks = EPI == kGatedBF16 ? 2 : kTileN / kCols;
             for (int c = group; c < kChunks; c += 2) {
                 if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the last store has read the staging buffer
                 group_sync();
@@ -565,57 +617,36 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     tmem_load16(d + at, r);
                     tmem_load16(d + at + 16, r + 16);
                     if constexpr (EPI == kGatedBF16) {
-                        uint32_t u[32];
+                        uint32_t u[32], packed[16];
                         tmem_load16(d + kTileRows + at, u);
                         tmem_load16(d + kTileRows + at + 16, u + 16);
                         tmem_load_wait();
                         if (last && half == kCols / 32 - 1) sums_read(buf);
+                        gated32(r, u, scales + at, scales + kTileRows + at, row_scale, n0 + at, p, packed);
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            uint32_t packed[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                float h[2];
-#pragma unroll
-                                for (int o = 0; o < 2; ++o) {
-                                    const int j = q * 8 + 2 * e + o;
-                                    float g = scaled(static_cast<int>(r[j]), row_scale, scales[at + j]);
-                                    float v = scaled(static_cast<int>(u[j]), row_scale, scales[kTileRows + at + j]);
-                                    if (p.bias != nullptr && n0 + at + j < p.N) {
-                                        g = __fadd_rn(g, __ldg(p.bias + n0 + at + j));
-                                        v = __fadd_rn(v, __ldg(p.bias + p.N + n0 + at + j));
-                                    }
-                                    h[o] = gated_value(g, v, p.act, p.limit);
-                                }
-                                const __nv_bfloat162 hb = __floats2bfloat162_rn(h[0], h[1]);
-                                packed[e] = *reinterpret_cast<const uint32_t*>(&hb);
-                            }
-                            *reinterpret_cast<uint4*>(stg + row * 128 + (((half * 4 + q) ^ (row & 7)) * 16)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-                        }
+                        for (int q = 0; q < 4; ++q)
+                            *reinterpret_cast<uint4*>(stg + row * 128 + (((half * 4 + q) ^ (row & 7)) * 16)) =
+                                make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
                     } else {
                         tmem_load_wait();
                         if (last && half == kCols / 32 - 1) sums_read(buf);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(scaled(static_cast<int>(r[j]), row_scale, scales[at + j]));
                         if constexpr (EPI == kStoreBF16) {
 #pragma unroll
                             for (int q = 0; q < 4; ++q) {
                                 uint32_t packed[4];
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    const int j = q * 8 + 2 * e;
-                                    const __nv_bfloat162 vb = __floats2bfloat162_rn(scaled(static_cast<int>(r[j]), row_scale, scales[at + j]),
-                                                                                    scaled(static_cast<int>(r[j + 1]), row_scale, scales[at + j + 1]));
+                                    const __nv_bfloat162 vb = __floats2bfloat162_rn(__uint_as_float(r[q * 8 + 2 * e]), __uint_as_float(r[q * 8 + 2 * e + 1]));
                                     packed[e] = *reinterpret_cast<const uint32_t*>(&vb);
                                 }
                                 *reinterpret_cast<uint4*>(stg + row * 128 + (((half * 4 + q) ^ (row & 7)) * 16)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
                             }
                         } else {
 #pragma unroll
-                            for (int q = 0; q < 8; ++q) {
-                                float v[4];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) v[e] = scaled(static_cast<int>(r[q * 4 + e]), row_scale, scales[at + q * 4 + e]);
-                                *reinterpret_cast<float4*>(stg + row * 128 + ((q ^ (row & 7)) * 16)) = make_float4(v[0], v[1], v[2], v[3]);
-                            }
+                            for (int q = 0; q < 8; ++q)
+                                *reinterpret_cast<uint4*>(stg + row * 128 + ((q ^ (row & 7)) * 16)) = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
                         }
                     }
                 }
@@ -653,13 +684,15 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
         }
         if (leader) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (mine == 0) timeline_record(kTlInt8ProductMany, 5);
         fence_before();
     }
     __syncthreads();
+    if (threadIdx.x == 0) timeline_record(kTlInt8ProductMany, 6);
     cluster_sync();          // neither CTA leaves while the other may still signal it
     if (warp == 1) {
         fence_after();
-        tmem_free<true>(tmem, Cfg::kTmemCols);
+        tmem_free<true>(tmem, 2 * kTileN);
     }
 }
 
@@ -682,17 +715,17 @@ int encode_rows(CUtensorMap* map, const void* a, int T, int width, int box_rows)
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, T, width, width, box_rows, kRowBytes, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
-template <int BQ>
+template <int BQ, int EPI, bool CLUSTER>
 int launch_few(const CUtensorMap& map_a, const FewParams& p, dim3 grid, cudaStream_t st) {
     using Cfg = FewConfig<BQ>;
     static SharedLimit limit;
     constexpr int kMost = 232448;
-    const cudaError_t le = limit.allow(reinterpret_cast<const void*>(int8_few_kernel<BQ>), kMost);
+    const cudaError_t le = limit.allow(reinterpret_cast<const void*>(int8_few_kernel<BQ, EPI, CLUSTER>), kMost);
     if (le != cudaSuccess) { set_error("int8_product: cannot reserve %d bytes of shared memory: %s", kMost, cudaGetErrorString(le)); return 1; }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(kFewThreads);
-    cfg.dynamicSmemBytes = Cfg::smem(p.stages, p.splits);
+    cfg.blockDim = dim3(Cfg::kThreads);
+    cfg.dynamicSmemBytes = Cfg::smem(p.stages, min(BQ, p.T), p.splits);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -702,32 +735,32 @@ int launch_few(const CUtensorMap& map_a, const FewParams& p, dim3 grid, cudaStre
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = p.splits;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    counted(cudaLaunchKernelEx(&cfg, int8_few_kernel<BQ>, map_a, p));
+    cfg.numAttrs = CLUSTER ? 2 : 1;
+    counted(cudaLaunchKernelEx(&cfg, int8_few_kernel<BQ, EPI, CLUSTER>, map_a, p));
     return check_launch("int8_product");
 }
 
+// Stages of the pipeline: `asked`, or as many as let two CTAs share an SM (twice the copies under way, and the CTAs of the next product fetch their first weights
+// while this one ends); no more than there are steps.
 template <int BQ>
-int few_stages(int asked, int steps, int splits) {
+int few_stages(int asked, int steps, int rows, int splits) {
     using Cfg = FewConfig<BQ>;
-    int stages = max(1, min(min(asked, 8), steps));
-    // the sums meet in the stages: there has to be room for them
-    if (!Cfg::kOwnPlace && splits > 1) stages = max(stages, (Cfg::kMeetBytes + Cfg::kStageBytes - 1) / Cfg::kStageBytes);
-    while (stages > 1 && Cfg::smem(stages, splits) > 232448) --stages;
+    constexpr int kTwoToAnSm = 233472 / 2 - 1024;
+    int stages = max(1, min(asked > 0 ? min(asked, 8) : 8, steps));
+    while (stages > 1 && Cfg::smem(stages, rows, splits) > (asked > 0 ? 232448 : kTwoToAnSm)) --stages;
     return stages;
 }
 
-template <int BQ, int EPI>
+template <int EPI>
 int launch_many(const CUtensorMap& map_a, const CUtensorMap& map_w, const CUtensorMap& map_o, const ManyParams& p, cudaStream_t st) {
-    using Cfg = ManyConfig<BQ>;
     static SharedLimit limit;
-    const cudaError_t le = limit.allow(reinterpret_cast<const void*>(int8_many_kernel<BQ, EPI>), Cfg::kSmem);
-    if (le != cudaSuccess) { set_error("int8_product: cannot reserve %d bytes of shared memory: %s", Cfg::kSmem, cudaGetErrorString(le)); return 1; }
+    const cudaError_t le = limit.allow(reinterpret_cast<const void*>(int8_many_kernel<EPI>), kManySmem);
+    if (le != cudaSuccess) { set_error("int8_product: cannot reserve %d bytes of shared memory: %s", kManySmem, cudaGetErrorString(le)); return 1; }
     const long long tiles = static_cast<long long>(p.tiles_t) * p.tiles_n;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * static_cast<unsigned>(min(tiles, static_cast<long long>(sm_count() / 2))));
+    cfg.gridDim = dim3(2 * static_cast<unsigned>(min(tiles, static_cast<long long>(max(1, sm_count() / 2)))));
     cfg.blockDim = dim3(kManyThreads);
-    cfg.dynamicSmemBytes = Cfg::kSmem;
+    cfg.dynamicSmemBytes = kManySmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -738,7 +771,7 @@ int launch_many(const CUtensorMap& map_a, const CUtensorMap& map_w, const CUtens
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    counted(cudaLaunchKernelEx(&cfg, int8_many_kernel<BQ, EPI>, map_a, map_w, map_o, p));
+    counted(cudaLaunchKernelEx(&cfg, int8_many_kernel<EPI>, map_a, map_w, map_o, p));
     return check_launch("int8_product");
 }
 
@@ -763,8 +796,6 @@ int int8_few_impl(const void* a, const float* a_scales, int T, int width, const 
     p.w_scales = w_scales;
     p.out = out;
     p.ldo = ldo;
-    p.out_bf16 = out_dtype == kBF16;
-    p.accumulate = accumulate;
     p.T = T;
     p.N = N;
     p.gated = gated;
@@ -780,28 +811,30 @@ int int8_few_impl(const void* a, const float* a_scales, int T, int width, const 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     auto go = [&](auto tile) {
         constexpr int BQ = decltype(tile)::value;
-        p.stages = few_stages<BQ>(stages, (p.kb_per_split + FewConfig<BQ>::kKb - 1) / FewConfig<BQ>::kKb, p.splits);
-        return launch_few<BQ>(map_a, p, grid, st);
+        p.stages = few_stages<BQ>(stages, (p.kb_per_split + FewConfig<BQ>::kKb - 1) / FewConfig<BQ>::kKb, min(BQ, T), p.splits);
+        if (p.splits > 1) {
+            if (out_dtype == kBF16) return launch_few<BQ, kStoreBF16, true>(map_a, p, grid, st);
+            return accumulate ? launch_few<BQ, kAddF32, true>(map_a, p, grid, st) : launch_few<BQ, kStoreF32, true>(map_a, p, grid, st);
+        }
+        if (out_dtype == kBF16) return launch_few<BQ, kStoreBF16, false>(map_a, p, grid, st);
+        return accumulate ? launch_few<BQ, kAddF32, false>(map_a, p, grid, st) : launch_few<BQ, kStoreF32, false>(map_a, p, grid, st);
     };
     switch (bq) {
-        case 16: return go(std::integral_constant<int, 16>());
+        case 8: return go(std::integral_constant<int, 8>());
         case 32: return go(std::integral_constant<int, 32>());
         case 64: return go(std::integral_constant<int, 64>());
-        case 128: return go(std::integral_constant<int, 128>());
-        case 256: return go(std::integral_constant<int, 256>());
-        default: set_error("int8_product: tiles of %d rows (16, 32, 64, 128 or 256)", bq); return 2;
+        default: set_error("int8_product: tiles of %d rows (8, 32 or 64)", bq); return 2;
     }
 }
 
 int int8_many_impl(const void* a, const float* a_scales, int T, int width, const void* tiles, const float* w_scales, int N, int gated, int act, float limit,
-                   const float* bias, void* out, int out_dtype, long long ldo, int accumulate, int bq, int group_t, void* status, void* stream) {
+                   const float* bias, void* out, int out_dtype, long long ldo, int accumulate, int group_t, void* status, void* stream) {
     if (T == 0) return 0;
     if (int bad = check_operands(a, T, width, tiles, N, status)) return bad;
     GI_REQUIRE(out_dtype == kF32 || out_dtype == kBF16, "int8_product: unsupported dtype code %d", out_dtype);
     GI_REQUIRE(!(accumulate && out_dtype != kF32), "int8_product: accumulation needs a 32-bit output");
-    GI_REQUIRE(!gated || (out_dtype == kBF16 && bq == 256), "int8_product: a gated product has a bfloat16 output");
+    GI_REQUIRE(!gated || out_dtype == kBF16, "int8_product: a gated product has a bfloat16 output");
     GI_REQUIRE(act >= 0 && act < kActCount, "int8_product: unknown activation %d", act);
-    GI_REQUIRE(bq == 128 || bq == 256, "int8_product: tiles of %d channels (128 or 256)", bq);
     GI_REQUIRE(group_t >= 1, "int8_product: groups of %d tiles", group_t);
     ManyParams p{};
     p.a_scales = a_scales;
@@ -813,7 +846,7 @@ int int8_many_impl(const void* a, const float* a_scales, int T, int width, const
     p.N = N;
     p.total_kb = (width + kRowBytes - 1) / kRowBytes;
     p.tiles_t = (T + 255) / 256;
-    p.tiles_n = (N + (gated ? kTileRows : bq) - 1) / (gated ? kTileRows : bq);
+    p.tiles_n = (N + (gated ? kTileRows : kTileN) - 1) / (gated ? kTileRows : kTileN);
     p.group_t = group_t;
     p.act = act;
     p.limit = limit;
@@ -825,33 +858,33 @@ int int8_many_impl(const void* a, const float* a_scales, int T, int width, const
     GI_REQUIRE(weight_rows < (1ll << 31), "int8_product: the weights are too large");
     CUtensorMap map_a, map_w, map_o{};
     if (int bad = encode_rows(&map_a, a, T, width, kTileRows)) return bad;
-    if (int bad = encode(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, tiles, weight_rows, kRowBytes, kRowBytes, bq / 2, kRowBytes, CU_TENSOR_MAP_SWIZZLE_NONE,
+    if (int bad = encode(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, tiles, weight_rows, kRowBytes, kRowBytes, kTileRows, kRowBytes, CU_TENSOR_MAP_SWIZZLE_NONE,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return bad;
     if (!p.plain_stores) {
         if (int bad = encode(&map_o, elt == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, out, T, N, ldo * elt, kTileRows, 128 / elt,
                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE)) return bad;
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (gated) return launch_many<256, kGatedBF16>(map_a, map_w, map_o, p, st);
-    if (elt == 2) return bq == 256 ? launch_many<256, kStoreBF16>(map_a, map_w, map_o, p, st) : launch_many<128, kStoreBF16>(map_a, map_w, map_o, p, st);
-    if (accumulate) return bq == 256 ? launch_many<256, kAddF32>(map_a, map_w, map_o, p, st) : launch_many<128, kAddF32>(map_a, map_w, map_o, p, st);
-    return bq == 256 ? launch_many<256, kStoreF32>(map_a, map_w, map_o, p, st) : launch_many<128, kStoreF32>(map_a, map_w, map_o, p, st);
+    if (gated) return launch_many<kGatedBF16>(map_a, map_w, map_o, p, st);
+    if (elt == 2) return launch_many<kStoreBF16>(map_a, map_w, map_o, p, st);
+    return accumulate ? launch_many<kAddF32>(map_a, map_w, map_o, p, st) : launch_many<kStoreF32>(map_a, map_w, map_o, p, st);
 }
 
 }  // namespace
 }  // namespace gi
+GI_TIMELINE_SETTER(gi_timeline_set_int8_product)
 
-// Few rows: tiles of bq rows of a [T, width], K in `splits` ranges (one cluster), up to `stages` stages of the pipeline. `gated`: the weights are a gated
+// Few rows: tiles of bq rows of a [T, width], K in `splits` ranges (one cluster), `stages` stages of the pipeline (0: chosen). `gated`: the weights are a gated
 // pair of N channels each, out [T, 2 N] = [gate; up]. out[t, n] at t * ldo + n.
 extern "C" int gi_int8_product_few(const void* a, const float* a_scales, int T, int width, const void* tiles, const float* w_scales, int N, int gated,
                                    void* out, int out_dtype, long long ldo, int accumulate, int bq, int splits, int stages, void* status, void* stream) {
     return gi::dispatch(gi::int8_few_impl, a, a_scales, T, width, tiles, w_scales, N, gated, out, out_dtype, ldo, accumulate, bq, splits, stages, status, stream);
 }
 
-// Many rows: tiles of 256 rows x bq channels. `gated`: out [T, N] = act(gate) * up, bfloat16; `bias` [2 N] or null.
+// Many rows: tiles of 256 rows x 256 channels, `group_t` tiles of rows walked together. `gated`: out [T, N] = act(gate) * up, bfloat16; `bias` [2 N] or null.
 extern "C" int gi_int8_product_many(const void* a, const float* a_scales, int T, int width, const void* tiles, const float* w_scales, int N, int gated,
-                                    int act, float limit, const float* bias, void* out, int out_dtype, long long ldo, int accumulate, int bq, int group_t,
+                                    int act, float limit, const float* bias, void* out, int out_dtype, long long ldo, int accumulate, int group_t,
                                     void* status, void* stream) {
-    return gi::dispatch(gi::int8_many_impl, a, a_scales, T, width, tiles, w_scales, N, gated, act, limit, bias, out, out_dtype, ldo, accumulate, bq, group_t,
+    return gi::dispatch(gi::int8_many_impl, a, a_scales, T, width, tiles, w_scales, N, gated, act, limit, bias, out, out_dtype, ldo, accumulate, group_t,
                         status, stream);
 }

@@ -36,79 +36,123 @@ struct RowsParams {
 constexpr unsigned kInfBits = 0x7f800000u, kLeastBits = 0x0d800000u;      // 2^-100
 constexpr float kDown = 8.271806125530277e-25f;                           // 2^-80
 
-template <bool VEC>
-__device__ __forceinline__ float4 load4(const float* p, int c, int D) {
-    if (VEC) return c < D ? *reinterpret_cast<const float4*>(p + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-    return make_float4(c < D ? p[c] : 0.f, c + 1 < D ? p[c + 1] : 0.f, c + 2 < D ? p[c + 2] : 0.f, c + 3 < D ? p[c + 3] : 0.f);
+// Four values of a row to a thread. VEC: neighbours, at 4 i, one access of 16 (8) bytes; rows of any width and alignment: at i, i + G, i + 2 G,
+// i + 3 G, so that the lanes of a warp stay side by side (2048 rows of 2050: 43 us with four neighbours one by one, 21 with these).
+template <bool VEC, int G>
+__device__ __forceinline__ int column(int i, int j) { return VEC ? 4 * i + j : (i / G) * 4 * G + i % G + j * G; }
+
+template <bool VEC, int G>
+__device__ __forceinline__ float4 load4(const float* p, int i, int D) {
+    if constexpr (VEC) {
+        return 4 * i < D ? *reinterpret_cast<const float4*>(p + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = column<VEC, G>(i, j) < D ? p[column<VEC, G>(i, j)] : 0.f;
+        return make_float4(v[0], v[1], v[2], v[3]);
+    }
 }
-template <bool VEC>
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p, int c, int D) {
-    if (VEC) {
-        if (c >= D) return make_float4(0.f, 0.f, 0.f, 0.f);
-        const uint2 raw = *reinterpret_cast<const uint2*>(p + c);
+template <bool VEC, int G>
+__device__ __forceinline__ float4 load4(const __nv_bfloat16* p, int i, int D) {
+    if constexpr (VEC) {
+        if (4 * i >= D) return make_float4(0.f, 0.f, 0.f, 0.f);
+        const uint2 raw = *reinterpret_cast<const uint2*>(p + 4 * i);
         return make_float4(__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16),
                            __uint_as_float(raw.y & 0xffff0000u));
+    } else {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = column<VEC, G>(i, j) < D ? to_float(p[column<VEC, G>(i, j)]) : 0.f;
+        return make_float4(v[0], v[1], v[2], v[3]);
     }
-    return make_float4(c < D ? to_float(p[c]) : 0.f, c + 1 < D ? to_float(p[c + 1]) : 0.f, c + 2 < D ? to_float(p[c + 2]) : 0.f,
-                       c + 3 < D ? to_float(p[c + 3]) : 0.f);
 }
-template <bool VEC>
-__device__ __forceinline__ void store4(float* p, int c, int D, const float4 v) {
-    if (VEC) {
-        if (c < D) *reinterpret_cast<float4*>(p + c) = v;
-        return;
+template <bool VEC, int G>
+__device__ __forceinline__ void store4(float* p, int i, int D, const float4 v) {
+    if constexpr (VEC) {
+        if (4 * i < D) *reinterpret_cast<float4*>(p + 4 * i) = v;
+    } else {
+        const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (column<VEC, G>(i, j) < D) p[column<VEC, G>(i, j)] = e[j];
     }
-    if (c < D) p[c] = v.x;
-    if (c + 1 < D) p[c + 1] = v.y;
-    if (c + 2 < D) p[c + 2] = v.z;
-    if (c + 3 < D) p[c + 3] = v.w;
 }
 
 struct NoAdd {};        // a norm without an addition
 
-__device__ __forceinline__ float gated_bf16(float g, float u, int act, float limit) {
-    return __bfloat162float(__float2bfloat16_rn(gated_value(g, u, act, limit)));
+__device__ __forceinline__ float4 plus(const float4 a, const float4 b) {
+    return make_float4(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y), __fadd_rn(a.z, b.z), __fadd_rn(a.w, b.w));
 }
 
-// Columns c .. c + 3 of a row: v, and what its squares add to ss. `first`: the norm's addition is done and written back.
-template <int KIND, typename TX, typename TA, bool VEC>
-__device__ __forceinline__ float4 values4(const RowsParams& p, long long row, int c, const float4 w, float factor, bool first, float& ss) {
+// N groups of four values of a row, i0, i0 + G, ..: v of each, and what the squares add to ss. All loads stand before the first
+// store of a row that is written back (nothing tells the compiler that they do not overlap). `first`: the norm's addition is done.
+template <int KIND, typename TX, typename TA, bool VEC, int G, int N>
+__device__ __forceinline__ void values(const RowsParams& p, long long row, int i0, const float4* w, float factor, bool first, float& ss, float4* v) {
     const TX* x = static_cast<const TX*>(p.x) + row * p.ldx;
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = load4<VEC, G>(x, i0 + k * G, p.D);
     if constexpr (KIND == kRowsGated) {
-        float4 g = load4<VEC>(x, c, p.D), u = load4<VEC>(x + p.D, c, p.D);
+        float4 u[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) u[k] = load4<VEC, G>(x + p.D, i0 + k * G, p.D);
         if (p.weight != nullptr) {
-            const float4 bg = load4<VEC>(p.weight, c, p.D), bu = load4<VEC>(p.weight + p.D, c, p.D);
-            g = make_float4(__fadd_rn(g.x, bg.x), __fadd_rn(g.y, bg.y), __fadd_rn(g.z, bg.z), __fadd_rn(g.w, bg.w));
-            u = make_float4(__fadd_rn(u.x, bu.x), __fadd_rn(u.y, bu.y), __fadd_rn(u.z, bu.z), __fadd_rn(u.w, bu.w));
-        }
-        return make_float4(gated_bf16(g.x, u.x, p.act, p.limit), gated_bf16(g.y, u.y, p.act, p.limit),
-                           gated_bf16(g.z, u.z, p.act, p.limit), gated_bf16(g.w, u.w, p.act, p.limit));
-    } else if constexpr (KIND == kRowsNorm) {
-        float4 v = load4<VEC>(x, c, p.D);
-        if constexpr (!std::is_same<TA, NoAdd>::value) {
-            if (first) {
-                const float4 a = load4<VEC>(static_cast<const TA*>(p.add) + row * p.D, c, p.D);
-                v = make_float4(__fadd_rn(v.x, a.x), __fadd_rn(v.y, a.y), __fadd_rn(v.z, a.z), __fadd_rn(v.w, a.w));
-                store4<VEC>(static_cast<float*>(const_cast<void*>(p.x)) + row * p.ldx, c, p.D, v);
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                v[k] = plus(v[k], load4<VEC, G>(p.weight, i0 + k * G, p.D));
+                u[k] = plus(u[k], load4<VEC, G>(p.weight + p.D, i0 + k * G, p.D));
             }
         }
-        v = make_float4(v.x * factor, v.y * factor, v.z * factor, v.w * factor);
-        ss = fmaf(v.x, v.x, ss); ss = fmaf(v.y, v.y, ss); ss = fmaf(v.z, v.z, ss); ss = fmaf(v.w, v.w, ss);
-        return make_float4(__fmul_rn(v.x, w.x), __fmul_rn(v.y, w.y), __fmul_rn(v.z, w.z), __fmul_rn(v.w, w.w));
+        with_activation(p.act, [&](auto act) {
+            auto h = [&](float g, float up) { return gated_value_bf16<decltype(act)::value>(g, up, p.limit); };
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(h(v[k].x, u[k].x), h(v[k].y, u[k].y));
+                const __nv_bfloat162 hi = __floats2bfloat162_rn(h(v[k].z, u[k].z), h(v[k].w, u[k].w));
+                const uint32_t a = *reinterpret_cast<const uint32_t*>(&lo), b = *reinterpret_cast<const uint32_t*>(&hi);
+                v[k] = make_float4(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u), __uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u));
+            }
+        });
+    } else if constexpr (KIND == kRowsNorm) {
+        if constexpr (!std::is_same<TA, NoAdd>::value) {
+            if (first) {
+                float4 a[N];
+#pragma unroll
+                for (int k = 0; k < N; ++k) a[k] = load4<VEC, G>(static_cast<const TA*>(p.add) + row * p.D, i0 + k * G, p.D);
+#pragma unroll
+                for (int k = 0; k < N; ++k) v[k] = plus(v[k], a[k]);
+#pragma unroll
+                for (int k = 0; k < N; ++k) store4<VEC, G>(static_cast<float*>(const_cast<void*>(p.x)) + row * p.ldx, i0 + k * G, p.D, v[k]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const float4 e = make_float4(v[k].x * factor, v[k].y * factor, v[k].z * factor, v[k].w * factor);
+            ss = fmaf(e.x, e.x, ss); ss = fmaf(e.y, e.y, ss); ss = fmaf(e.z, e.z, ss); ss = fmaf(e.w, e.w, ss);
+            v[k] = make_float4(__fmul_rn(e.x, w[k].x), __fmul_rn(e.y, w[k].y), __fmul_rn(e.z, w[k].z), __fmul_rn(e.w, w[k].w));
+        }
+    }
+}
+
+// rint(v * inv) of |v * inv| <= 127.5 in the low byte: the sum with 1.5 * 2^23 is rounded to a whole number, to the even one of two (an addition, where
+// the conversion to an integer takes the unit that exponentials take, a quarter as wide).
+__device__ __forceinline__ uint32_t int_of(float v, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.f)); }
+
+template <bool VEC, int G>
+__device__ __forceinline__ void put4(int8_t* q, int i, int width, const float4 v, float inv, bool none) {
+    const uint32_t a = int_of(v.x, inv), b = int_of(v.y, inv), c = int_of(v.z, inv), d = int_of(v.w, inv);
+    if constexpr (VEC) {
+        if (4 * i < width) reinterpret_cast<uint32_t*>(q)[i] = none ? 0u : __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
     } else {
-        return load4<VEC>(x, c, p.D);
+        const uint32_t e[4] = {a, b, c, d};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (column<VEC, G>(i, j) < width) q[column<VEC, G>(i, j)] = none ? 0 : static_cast<int8_t>(e[j] & 0xffu);
     }
 }
 
 __device__ __forceinline__ unsigned top_bits(const float4 v, unsigned m) {
     m = max(m, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
     return max(m, max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
-}
-
-__device__ __forceinline__ uint32_t four_ints(const float4 v, float inv) {
-    const int a = __float2int_rn(__fmul_rn(v.x, inv)), b = __float2int_rn(__fmul_rn(v.y, inv));
-    const int c = __float2int_rn(__fmul_rn(v.z, inv)), d = __float2int_rn(__fmul_rn(v.w, inv));
-    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 // The row's largest |v| and sum of squares over the G threads that share it.
@@ -139,28 +183,36 @@ __device__ __forceinline__ float2 row_factors(unsigned m_bits, float ss, const R
     return make_float2(__fdiv_rn(127.f, m), scale);
 }
 
-// G threads to a row, V groups of four values each in registers.
+// G threads to a row, V groups of four values each in registers, read in batches.
 template <int KIND, typename TX, typename TA, int G, int V, bool VEC>
-__global__ void __launch_bounds__(G < 128 ? 128 : G)
+__global__ void __launch_bounds__(G < 128 ? 128 : G, G <= 512 ? 1024 / (G < 128 ? 128 : G) : 1)
 rows_int8_kernel(const RowsParams p) {
     constexpr int kRows = G < 128 ? 128 / G : 1;
+    constexpr int kBatch = V <= 4 ? V : 2;
+    constexpr bool kEarly = V <= 4;      // the norm's weights are read before the wait for the kernel ahead, where registers hold them
     __shared__ unsigned part_m[2][32];
     __shared__ float part_s[2][32];
     const int t = threadIdx.x % G;
     const long long row = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / G;
+    if (threadIdx.x == 0) timeline_record(kTlInt8Rows, 0);
     pdl_launch_dependents();
-    float4 w[KIND == kRowsNorm ? V : 1];
-    if (KIND == kRowsNorm) {      // the weights belong to no earlier kernel
+    float4 w[kBatch];
+    auto weights = [&](int k0) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) w[k] = load4<VEC>(p.weight, 4 * (t + k * G), p.D);
-    }
+        for (int k = 0; k < kBatch; ++k) w[k] = KIND == kRowsNorm ? load4<VEC, G>(p.weight, t + (k0 + k) * G, p.D) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    if (kEarly) weights(0);
     pdl_wait();
+    if (threadIdx.x == 0) timeline_record(kTlInt8Rows, 1);
     if (row >= p.T) return;       // (whole warps: rows of several to a block have a warp each)
     float4 v[V];
     unsigned m = 0;
     float ss = 0.f, factor = 1.f;
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = values4<KIND, TX, TA, VEC>(p, row, 4 * (t + k * G), w[KIND == kRowsNorm ? k : 0], 1.f, true, ss);
+    for (int k = 0; k < V; k += kBatch) {
+        if (!kEarly) weights(k);
+        values<KIND, TX, TA, VEC, G, kBatch>(p, row, t + k * G, w, 1.f, true, ss, v + k);
+    }
 #pragma unroll
     for (int k = 0; k < V; ++k) m = top_bits(v[k], m);
     meet<G, KIND>(m, ss, part_m[0], part_s[0]);
@@ -168,25 +220,21 @@ rows_int8_kernel(const RowsParams p) {
         factor = kDown;
         m = 0;
         ss = 0.f;
-#pragma unroll 1
-        for (int k = 0; k < V; ++k) {
-            const float4 wk = load4<VEC>(p.weight, 4 * (t + k * G), p.D);
-            m = top_bits(values4<KIND, TX, TA, VEC>(p, row, 4 * (t + k * G), wk, factor, false, ss), m);
-        }
-        meet<G, KIND>(m, ss, part_m[1], part_s[1]);
-        float unused = 0.f;
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = values4<KIND, TX, TA, VEC>(p, row, 4 * (t + k * G), w[KIND == kRowsNorm ? k : 0], factor, false, unused);
+        for (int k = 0; k < V; k += kBatch) {
+            if (!kEarly) weights(k);
+            values<KIND, TX, TA, VEC, G, kBatch>(p, row, t + k * G, w, factor, false, ss, v + k);
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) m = top_bits(v[k], m);
+        meet<G, KIND>(m, ss, part_m[1], part_s[1]);
     }
     const float2 f = row_factors<KIND>(m, ss, p, factor);
     const bool none = f.x == 0.f;        // (0 * infinity would not be 0)
-    uint32_t* q = reinterpret_cast<uint32_t*>(p.q + row * p.width);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int c = t + k * G;
-        if (4 * c < p.width) q[c] = none ? 0u : four_ints(v[k], f.x);
-    }
+    for (int k = 0; k < V; ++k) put4<VEC, G>(p.q + row * p.width, t + k * G, p.width, v[k], f.x, none);
     if (t == 0) p.scales[row] = f.y;
+    if (threadIdx.x == 0) timeline_record(kTlInt8Rows, 6);
 }
 
 // Rows wider than a block's registers: the same twice over memory.
@@ -199,22 +247,28 @@ wide_rows_int8_kernel(const RowsParams p) {
     pdl_prologue();
     unsigned m = 0;
     float ss = 0.f, factor = 1.f;
-    auto weight = [&](int c) { return KIND == kRowsNorm ? load4<false>(p.weight, c, p.D) : make_float4(0.f, 0.f, 0.f, 0.f); };
-    for (int c = 4 * threadIdx.x; c < p.D; c += 4096) m = top_bits(values4<KIND, TX, TA, false>(p, row, c, weight(c), 1.f, true, ss), m);
+    float4 v[1], w[1];
+    auto pass = [&](int i, bool first, float& squares) {
+        w[0] = KIND == kRowsNorm ? load4<false, 1024>(p.weight, i, p.D) : make_float4(0.f, 0.f, 0.f, 0.f);
+        values<KIND, TX, TA, false, 1024, 1>(p, row, i, w, factor, first, squares, v);
+    };
+    const int groups = (p.width + 4095) / 4096 * 1024;
+    for (int i = threadIdx.x; i < groups; i += 1024) { pass(i, true, ss); m = top_bits(v[0], m); }
     meet<1024, KIND>(m, ss, part_m[0], part_s[0]);
     if (KIND == kRowsNorm && (m >= kInfBits || !(ss < __uint_as_float(kInfBits)))) {
         factor = kDown;
         m = 0;
         ss = 0.f;
-        for (int c = 4 * threadIdx.x; c < p.D; c += 4096) m = top_bits(values4<KIND, TX, TA, false>(p, row, c, weight(c), factor, false, ss), m);
+        for (int i = threadIdx.x; i < groups; i += 1024) { pass(i, false, ss); m = top_bits(v[0], m); }
         meet<1024, KIND>(m, ss, part_m[1], part_s[1]);
     }
     const float2 f = row_factors<KIND>(m, ss, p, factor);
     const bool none = f.x == 0.f;
-    uint32_t* q = reinterpret_cast<uint32_t*>(p.q + row * p.width);
     float unused = 0.f;
-    for (int c = 4 * threadIdx.x; c < p.width; c += 4096)
-        q[c / 4] = none ? 0u : four_ints(values4<KIND, TX, TA, false>(p, row, c, weight(c), factor, false, unused), f.x);
+    for (int i = threadIdx.x; i < groups; i += 1024) {
+        pass(i, false, unused);
+        put4<false, 1024>(p.q + row * p.width, i, p.width, v[0], f.x, none);
+    }
     if (threadIdx.x == 0) p.scales[row] = f.y;
 }
 
@@ -227,7 +281,10 @@ void launch_rows(const RowsParams& p, cudaStream_t st) {
     else if (p.width <= 2048) go(rows_int8_kernel<KIND, TX, TA, 128, 4, VEC>, 128, 1);
     else if (p.width <= 4096) go(rows_int8_kernel<KIND, TX, TA, 256, 4, VEC>, 256, 1);
     else if (p.width <= 8192) go(rows_int8_kernel<KIND, TX, TA, 512, 4, VEC>, 512, 1);
-    else if (p.width <= 16384) go(rows_int8_kernel<KIND, TX, TA, 512, 8, VEC>, 512, 1);
+    else if (p.width <= 16384) {
+        if (VEC) go(rows_int8_kernel<KIND, TX, TA, 512, 8, true>, 512, 1);      // two rows to an SM: one is read while the other is written
+        else go(rows_int8_kernel<KIND, TX, TA, 1024, 4, false>, 1024, 1);       // (512 threads lack the registers)
+    }
     else if (p.width <= 32768) go(rows_int8_kernel<KIND, TX, TA, 1024, 8, VEC>, 1024, 1);
     else go(wide_rows_int8_kernel<KIND, TX, TA>, 1024, 1);
 }
@@ -270,6 +327,7 @@ int rows_int8_impl(int kind, const void* x, int x_dtype, long long ldx, const vo
 
 }  // namespace
 }  // namespace gi
+GI_TIMELINE_SETTER(gi_timeline_set_int8_rows)
 
 // q [T, width] and scales [T] of T rows: kind 0 of x [T, D], 1 of the norm of x (32-bit; x += add [T, D] first where add is given), 2 of
 // act(g) * u with x [T, 2 D] = [g; u] and `weight` its bias (may be null). Rows of x lie ldx values apart.

@@ -1735,7 +1735,7 @@ def adapter_product(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale
 # (products with it are NaN), one whose m is below 2^-100 the scale 0. Rows lie in buffers of ``int8_width`` values, zeros behind.
 
 INT8_WIDTH_MOST = 131056      # sums of so many products stay within 32 bits, of -128 times -128 too
-INT8_FEW_ROWS = 256           # up to here products of few rows (weights on the 128-row side)
+_FEW_CTAS = 264               # CTAs of a product of few rows that a B200 holds at once, two to an SM, in clusters of up to eight
 
 
 def int8_width(values: int) -> int:
@@ -1828,31 +1828,36 @@ def int8_weight(q: torch.Tensor, scales: torch.Tensor, gated: bool = False) -> I
     return Int8Weight(tiles, scales.reshape(-1).contiguous(), n, int8_width(K), gated)
 
 
-def _few_plan(T: int, n_tiles: int, blocks: int):
-    """(rows of a tile, ranges of K, stages) of a product of few rows."""
-    bq = next(b for b in (16, 32, 64, 128, 256) if b >= min(T, 256))
-    tiles = n_tiles * ((T + bq - 1) // bq)
-    splits = max(1, min(8, sm_count() // max(1, tiles), blocks))
-    return bq, splits, 3 if bq <= 64 else 4
+def _int8_plan(T: int, w: Int8Weight):
+    """("few", rows of a tile, ranges of K, stages) or ("many", tiles of rows walked together). Measured on B200 (us).
+
+    Few rows: tiles of 8, 32 or 64 rows; tiles of 32 as long as they all fit at once (64 rows, 2048 -> 2048: 4.9 with tiles of 32 and 5.6 with 64; 4096 ->
+    28672: 34.6 and 21.2) and K is short (160 rows, 8192 -> 2048: 13.2 and 10.8). K is cut while all CTAs fit at once and a range has four blocks (8
+    rows, 4096 -> 4096: 5.4 with 8 ranges, 5.7 with 4, 6.8 with 2), from a hundred tiles on sixteen (8 rows, 2048 -> 16384: 7.2 with one range, 7.6 with
+    two; 1000 rows, 8192 -> 1024: 22.4 and 17.9).
+    Many rows, from where the tiles of 64 rows no longer fit at once: 400 rows, 4096 -> 4096 (224 tiles): few 14.4, many 17.2; 333 rows, 2048 -> 16384
+    (768 tiles): 26.8 and 19.2. The longer side is walked once, so that the shorter stays in L2: 8192 rows, 14336 -> 4096: 0.31 ms with one tile of
+    rows at a time, 0.35 with all; 4096 -> 28672: 0.86 and 0.63."""
+    n_tiles, blocks = (w.channels + 127) // 128 * (2 if w.gated else 1), (w.width + 127) // 128
+    tiles_32 = n_tiles * ((T + 31) // 32)
+    bq = 8 if T <= 8 else 32 if (tiles_32 <= _FEW_CTAS if T <= 64 else tiles_32 <= 128 and blocks <= 32) else 64
+    tiles = n_tiles * max(1, (T + bq - 1) // bq)
+    if T <= 64 or tiles <= 2 * sm_count():
+        return "few", bq, max(1, min(8, blocks // (16 if tiles > 96 else 4), _FEW_CTAS // tiles)), 0
+    return "many", 1 if T >= w.channels else (T + 255) // 256
 
 
-def _few(a, a_scales, w, out, accumulate, plan=None) -> None:
-    bq, splits, stages = plan or _few_plan(a.shape[0], (w.channels + 127) // 128 * (2 if w.gated else 1), (w.width + 127) // 128)
+def _few(a, a_scales, w, out, accumulate, plan) -> None:
+    _, bq, splits, stages = plan
     check(lib().gi_int8_product_few(_dev(a, "a", torch.int8), _dev(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
                                     w.scales.data_ptr(), w.channels, int(w.gated), _rows_of(out, "out"), dtype_code(out.dtype), out.stride(0),
                                     int(bool(accumulate)), bq, splits, stages, _tc_state(a.device).status.data_ptr(), _stream()), "int8_product")
 
 
-def _many_plan(T: int, N: int):
-    """(channels of a tile, tiles of rows walked together) of a product of many rows."""
-    return (256 if N > 128 else 128), 8
-
-
-def _many(a, a_scales, w, out, out_stride, accumulate, act=0, limit=0.0, bias=None, plan=None) -> None:
-    bq, group = plan or _many_plan(a.shape[0], w.channels)
+def _many(a, a_scales, w, out, out_stride, accumulate, plan, act=0, limit=0.0, bias=None) -> None:
     check(lib().gi_int8_product_many(_dev(a, "a", torch.int8), _dev(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
                                      w.scales.data_ptr(), w.channels, int(w.gated), act, float(limit), _opt(bias, "bias", torch.float32), out.data_ptr(),
-                                     dtype_code(out.dtype), out_stride, int(bool(accumulate)), 256 if w.gated else bq, group,
+                                     dtype_code(out.dtype), out_stride, int(bool(accumulate)), plan[1],
                                      _tc_state(a.device).status.data_ptr(), _stream()), "int8_product")
 
 
@@ -1874,11 +1879,12 @@ def int8_product(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: to
         raise KernelError(f"int8_product: out must be [T, {w.channels}]")
     if accumulate and out.dtype is not torch.float32:
         raise KernelError("int8_product: accumulation needs a 32-bit output")
-    if (len(plan) == 3) if plan else T <= INT8_FEW_ROWS:
+    plan = plan or _int8_plan(T, w)
+    if plan[0] == "few":
         _few(a, a_scales, w, out, accumulate, plan)
     else:
         _rows_of(out, "out")
-        _many(a, a_scales, w, out, out.stride(0), accumulate, plan=plan)
+        _many(a, a_scales, w, out, out.stride(0), accumulate, plan)
 
 
 def int8_gated_work(rows: int, w: Int8Weight) -> int:
@@ -1903,13 +1909,13 @@ def int8_gated(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: torc
     _dev(work, "work", torch.float32)
     if work.numel() < int8_gated_work(T, w):
         raise KernelError(f"int8_gated: work must hold {int8_gated_work(T, w)} values")
-    work = work.view(-1)
-    if T <= INT8_FEW_ROWS:
+    work, plan = work.view(-1), _int8_plan(T, w)
+    if plan[0] == "few":
         both = work[:T * 2 * I].view(T, 2 * I)
-        _few(a, a_scales, w, both, False)
+        _few(a, a_scales, w, both, False, plan)
         gated_act_int8(both, out, out_scales, activation, limit, bias)
         return
     stride = (I + 7) // 8 * 8                 # whole 16 bytes
     h = work.view(torch.bfloat16)[:T * stride].view(T, stride)[:, :I]
-    _many(a, a_scales, w, h, stride, False, ACTIVATIONS[activation], limit, bias)
+    _many(a, a_scales, w, h, stride, False, plan, ACTIVATIONS[activation], limit, bias)
     quantize_rows(h, out, out_scales)

@@ -16,15 +16,16 @@ import torch
 
 from .library import lib
 
-KERNELS = {1: "rmsnorm", 2: "swiglu", 3: "attention_decode", 4: "add ranges", 5: "rope_store", 6: "attention_prefill",
+KERNELS = {1: "rmsnorm", 2: "swiglu", 3: "attention_decode", 4: "add ranges", 5: "rope_store", 6: "attention_prefill", 7: "int8 rows",
            101: "product qkv+rope", 102: "product add", 103: "product store",
            111: "product qkv+rope (general)", 112: "product add (general)", 113: "product store (general)",
+           121: "product int8", 221: "products int8 (pairs)",
            200: "products store", 201: "products store (pairs)", 202: "products add", 203: "products add (pairs)",
            204: "products swiglu", 205: "products swiglu (pairs)", 206: "products rope", 207: "products rope (pairs)"}
 EVENTS = {"rmsnorm": {0: "enter", 1: "waited", 6: "leave"}, "swiglu": {0: "enter", 1: "waited", 6: "leave"},
           "attention_decode": {0: "enter", 1: "waited", 2: "queries loaded", 3: "first tile done", 4: "last tile done", 6: "leave"},
           "add ranges": {0: "enter", 1: "waited", 6: "leave"}, "rope_store": {0: "enter", 1: "waited"},
-          "attention_prefill": {0: "enter", 1: "waited", 6: "leave"},
+          "attention_prefill": {0: "enter", 1: "waited", 6: "leave"}, "int8 rows": {0: "enter", 1: "waited", 6: "leave"},
           "product": {0: "enter", 1: "waited", 2: "first operands", 3: "last MMA issued", 4: "accumulator ready",
                       7: "partial tiles arrived", 8: "sums complete", 5: "results stored", 6: "leave"},
           "products": {0: "enter", 1: "waited", 2: "first operands", 3: "last MMA issued", 4: "first accumulator ready",
@@ -38,7 +39,7 @@ class Recorder:
         self.buffer = torch.zeros(2 + 2 * capacity, dtype=torch.int64, device=device)
         self.buffer[1] = capacity
         for setter in ("gi_timeline_set_gemm", "gi_timeline_set_elementwise", "gi_timeline_set_attention",
-                       "gi_timeline_set_attention_tc"):
+                       "gi_timeline_set_attention_tc", "gi_timeline_set_int8_rows", "gi_timeline_set_int8_product"):
             code = getattr(lib(), setter)(self.buffer.data_ptr())
             if code == 2:
                 raise RuntimeError("this library was built without time stamps: call library.use_timeline_build() first")

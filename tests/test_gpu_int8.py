@@ -235,10 +235,15 @@ def test_every_cut_of_a_product_gives_the_same(T, K, N):
     a, s = _a(k, g, T, K)
     w = k.int8_weight(q, ws)
     want = _scaled(_sums(a, q, K), s, ws)
-    for plan in [(bq, splits, stages) for bq in (16, 32, 64, 128, 256) for splits in (1, 2, 3, 5, 8) for stages in (1, 2, 4)] + [(128, 1), (128, 3), (256, 1), (256, 8)]:
+    for plan in [("few", bq, splits, stages) for bq in (8, 32, 64) for splits in (1, 2, 3, 5, 8) for stages in (1, 2, 4)] + [("many", group) for group in (1, 3, 8)]:
         out = torch.full((T, N), math.nan, device=DEV)
         k.int8_product(a, s, w, out, plan=plan)
         assert torch.equal(out, want), plan
+        half = torch.full((T, N), math.nan, dtype=torch.bfloat16, device=DEV)
+        k.int8_product(a, s, w, half, plan=plan)
+        assert torch.equal(half, want.to(torch.bfloat16)), plan
+        k.int8_product(a, s, w, out, accumulate=True, plan=plan)
+        assert torch.equal(out, want + want), plan
 
 
 def test_the_largest_sums_stay_exact():
