@@ -14,12 +14,14 @@ from typing import List, Optional
 
 USAGE = (
     "usage: gi_generate --model DIR (--prompt-ids \"1 2 3\" | --prompt-ids-file FILE) [--steps N] [--max-seq-len N]\n"
-    "                   [--weights native|f32 | --dtype bf16|fp32] [--device cuda] [--profile] [--temperature F]\n"
+    "                   [--weights native|f32|int8 | --dtype bf16|fp32] [--device cuda] [--profile] [--temperature F]\n"
     "                   [--top-k N] [--top-p F] [--seed N] [--stop-ids \"2 7\"] [--page-size N] [--kv-pages N]\n"
     "                   [--no-echo] [--quiet] [--dump-tokens FILE] [--random-weights SEED --config FILE]\n"
     "                   [--adapter DIR] [--draft-model DIR [--drafts N]]\n"
     "  DIR holds config.json and model.safetensors. --steps is the maximum number of positions including the\n"
-    "  prompt (default: the context length). --weights f32 (= --dtype fp32) runs the whole model in true 32-bit.\n"
+    "  prompt (default: the context length). --weights f32 (= --dtype fp32) runs the whole model in true 32-bit;\n"
+    "  int8: the layers' projections in 8-bit integers with a scale a channel, rounded when the model is loaded, and their inputs\n"
+    "  with a scale a row (with --draft-model: of the model of --model). It does not go with --adapter.\n"
     "  --random-weights SEED --config FILE first writes such a folder (random bfloat16 weights from the seed, for the\n"
     "  configuration in FILE, a config.json) to DIR, or to a temporary folder when no --model is given.\n"
     "  --adapter DIR: a low-rank adapter (adapter_config.json, adapter_model.safetensors) beside the model's weights.\n"
@@ -91,7 +93,10 @@ def parse(argv: List[str]) -> dict:
             name = value().lower()
             if name not in ("bf16", "bfloat16", "fp32", "f32", "float32"):
                 raise UsageError("--dtype must be bf16 or fp32")
-            o["weights"] = "native" if name in ("bf16", "bfloat16") else "f32"
+            if name not in ("bf16", "bfloat16"):
+                o["weights"] = "f32"
+            elif o["weights"] != "int8":            # (which computes in bfloat16 besides)
+                o["weights"] = "native"
         elif flag == "--random-weights": o["random_weights"] = _int(flag, value())
         elif flag == "--config": o["config"] = value()
         elif flag in ("--help", "-h"): o["help"] = True
@@ -121,8 +126,10 @@ def parse(argv: List[str]) -> dict:
         raise UsageError("--model is required")
     if not o["prompt_ids"]:
         raise UsageError("--prompt-ids or --prompt-ids-file is required (at least one token id)")
-    if o["weights"] not in ("native", "f32"):
-        raise UsageError("--weights must be native or f32 (int8 is not built)")
+    if o["weights"] not in ("native", "f32", "int8"):
+        raise UsageError("--weights must be native, f32 or int8")
+    if o["weights"] == "int8" and o["adapter"]:
+        raise UsageError("--weights int8 cannot be combined with --adapter")
     if not o["device"].startswith("cuda"):
         raise UsageError("--device must be cuda: this engine has no CPU or emulated device")
     if o["draft_model"] and (o["top_k"] or (o["top_p"] is not None and o["top_p"] < 1.0)):
@@ -156,7 +163,8 @@ def _with_drafts(o: dict, device: str) -> int:
     positions = min(o["steps"], context) if o["steps"] > 0 else context
     rank = _adapter_rank(o["adapter"]) if o["adapter"] else 0
     engine = SpeculativeEngine(o["model"], o["draft_model"], drafts=o["drafts"], dtype="float32" if o["weights"] == "f32" else "bfloat16", device=device,
-                               max_running=1, max_seq_len=positions, page_size=o["page_size"], adapter_slots=1 if rank else 0, adapter_rank=rank or 16)
+                               max_running=1, max_seq_len=positions, page_size=o["page_size"], adapter_slots=1 if rank else 0, adapter_rank=rank or 16,
+                               weights="int8" if o["weights"] == "int8" else "native")
     if rank:
         engine.load_adapter(0, o["adapter"])
     if engine.context < positions and not o["quiet"]:
@@ -220,7 +228,8 @@ def main(argv: Optional[List[str]] = None) -> int:
         rank = _adapter_rank(o["adapter"]) if o["adapter"] else 0
         engine = Engine(o["model"], dtype="float32" if o["weights"] == "f32" else "bfloat16", device=device,
                         max_seq_len=o["max_seq_len"] or None, page_size=o["page_size"], kv_pages=o["kv_pages"],
-                        max_running=1, prefix_cache=False, adapter_slots=1 if rank else 0, adapter_rank=rank or 16)
+                        max_running=1, prefix_cache=False, adapter_slots=1 if rank else 0, adapter_rank=rank or 16,
+                        weights="int8" if o["weights"] == "int8" else "native")
         if rank:
             engine.load_adapter(0, o["adapter"])
         load_s = time.perf_counter() - t0

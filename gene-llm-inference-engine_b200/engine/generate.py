@@ -24,7 +24,7 @@ class Engine:
                  max_seq_len: Optional[int] = None, page_size: int = 16, kv_pages: Optional[int] = None,
                  max_running: int = 8, step_tokens: int = 2048, prefill_chunk: int = 0, prefix_cache: bool = True,
                  decode_weight_copy: bool = True, nvtx: bool = False, debug_checks: bool = False,
-                 adapter_slots: int = 0, adapter_rank: int = 16):
+                 adapter_slots: int = 0, adapter_rank: int = 16, weights: str = "native"):
         """``model_dir``: folder with config.json and model.safetensors. ``dtype``: "bfloat16"
         (serving kernels) or "float32" (everything in true 32-bit). ``max_seq_len`` lowers the
         context length. ``kv_pages``: pages of ``page_size`` positions in the pool (default: room
@@ -32,9 +32,13 @@ class Engine:
         ``decode_weight_copy`` (bfloat16): a second copy of the matrices laid out for decode steps, which
         then stream the weights faster; False saves that memory. ``nvtx`` wraps steps, layers and the head in NVTX
         ranges; ``debug_checks`` validates every step's descriptor (positions, page ids) on the host before launch.
-        ``adapter_slots``: how many low-rank adapters of up to ``adapter_rank`` can be held (``load_adapter``); every request names its own."""
+        ``adapter_slots``: how many low-rank adapters of up to ``adapter_rank`` can be held (``load_adapter``); every request names its own.
+        ``weights`` "int8": the layers' projections in 8-bit integers (a scale a channel, and a scale for every row that goes into one), for designs whose
+        layers are norm, attention, norm, gated feed-forward; half the bytes of a decode step's projections. No adapters beside it."""
+        if adapter_slots and weights != "native":
+            raise ValueError("Engine: adapters go with native weights")
         self.model = load_model(model_dir, dtype=dtype, device=device, max_position=max_seq_len,
-                                weight_tiles=decode_weight_copy)
+                                weight_tiles=decode_weight_copy, weights=weights)
         context = self.model.max_position
         if kv_pages is None:
             per_request = (context + page_size - 1) // page_size

@@ -35,6 +35,10 @@ OPERATIONS = {
     "linear_scan": ("recurrence (state update + output)", None),
     "gated_group_norm": ("gated norm", None),
     "adapter_product": ("low-rank adapters", None),
+    "rmsnorm_int8": ("rmsnorm, rows in 8 bits", None),
+    "quantize_rows": ("rows in 8 bits", None),
+    "int8_product": ("matrix products (8-bit integers)", 2),
+    "int8_gated": ("ffn gate+up with act(gate) * up, 8-bit integers", 2),
     "copy_pages": ("page copies", None),
     "argmax": ("sampling", None),
     "sample": ("sampling", None),
@@ -57,6 +61,7 @@ def profile_report(engine, prompt, adapter: int = -1) -> str:
             out = fn(*a, **k)
             e.record()
             w = a[weight_arg] if weight_arg is not None and len(a) > weight_arg else None
+            w = getattr(w, "tiles", w)              # (a weight in 8 bits)
             records[label].append((s, e, w.numel() * w.element_size() if w is not None else 0))
             return out
         return wrapper

@@ -93,15 +93,17 @@ class _Side:
 class SpeculativeEngine:
     def __init__(self, model_dir: str, draft_dir: str, drafts: int = 4, dtype: str = "bfloat16", device: str = "cuda:0", max_running: int = 8,
                  max_seq_len: int = 2048, page_size: int = 16, step_tokens: int = 2048, decode_weight_copy: bool = True,
-                 adapter_slots: int = 0, adapter_rank: int = 16):
+                 adapter_slots: int = 0, adapter_rank: int = 16, weights: str = "native"):
         """``model_dir``, ``draft_dir``: the served and the proposing model, of one vocabulary. ``drafts``: tokens proposed a
         round (fewer where a request that runs is nearer to the end of the models' contexts than that). ``max_seq_len``: positions of a request at most, of the
-        prompt and all generated tokens but the last, which is not fed. The other arguments are ``Engine``'s."""
+        prompt and all generated tokens but the last, which is not fed. ``weights``: of the served model (the draft's are native). The other arguments are ``Engine``'s."""
+        if adapter_slots and weights != "native":
+            raise ValueError("drafted tokens: adapters go with native weights")
         if drafts < 1 or max_running < 1:
             raise ValueError("drafted tokens: drafts and max_running must be positive")
         self.drafts, self.requests, self.page_size = drafts, max_running, page_size
         room = max_seq_len + drafts                # (positions that a full round may write behind the last one that stays)
-        target = load_model(model_dir, dtype=dtype, device=device, max_position=room, weight_tiles=decode_weight_copy)
+        target = load_model(model_dir, dtype=dtype, device=device, max_position=room, weight_tiles=decode_weight_copy, weights=weights)
         draft = load_model(draft_dir, dtype=dtype, device=device, max_position=room, weight_tiles=decode_weight_copy)
         if target.vocab_size != draft.vocab_size:
             raise ValueError(f"drafted tokens: the models' vocabularies differ ({target.vocab_size} and {draft.vocab_size})")

@@ -1794,11 +1794,16 @@ def gated_act_int8(gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tenso
     _rows_int8("gated_act_int8", 2, gate_up, 2, out, scales, weight=bias, act=ACTIVATIONS[activation], limit=limit)
 
 
+class Int8Rows:
+    """Rows in 8 bits as one thing: ``q`` [T, int8_width(D)] int8 and ``scales`` [T] of rows of D values."""
+
+    def __init__(self, q: torch.Tensor, scales: torch.Tensor, values: int):
+        self.q, self.scales, self.shape = q, scales, (q.shape[0], values)
+
+
 class Int8Weight:
     """A weight matrix [N, K] in 8 bits, a scale a channel, laid out as the products read it (``int8_weight``). ``channels`` N (gated: of a
     part), ``width``: int8_width(K)."""
-
-    __slots__ = ("tiles", "scales", "channels", "width", "gated")
 
     def __init__(self, tiles: torch.Tensor, scales: torch.Tensor, channels: int, width: int, gated: bool):
         self.tiles, self.scales, self.channels, self.width, self.gated = tiles, scales, channels, width, gated
@@ -1828,6 +1833,15 @@ def int8_weight(q: torch.Tensor, scales: torch.Tensor, gated: bool = False) -> I
     return Int8Weight(tiles, scales.reshape(-1).contiguous(), n, int8_width(K), gated)
 
 
+def _int8_tiles(w: Int8Weight) -> int:
+    return (w.channels + 127) // 128 * (2 if w.gated else 1)
+
+
+def _few_most(n_tiles: int) -> int:
+    """The most rows that count as few: tiles of 64 of them that an SM holds two of at once."""
+    return 64 * max(1, 2 * sm_count() // n_tiles)
+
+
 def _int8_plan(T: int, w: Int8Weight):
     """("few", rows of a tile, ranges of K, stages) or ("many", tiles of rows walked together). Measured on B200 (us).
 
@@ -1838,11 +1852,11 @@ def _int8_plan(T: int, w: Int8Weight):
     Many rows, from where the tiles of 64 rows no longer fit at once: 400 rows, 4096 -> 4096 (224 tiles): few 14.4, many 17.2; 333 rows, 2048 -> 16384
     (768 tiles): 26.8 and 19.2. The longer side is walked once, so that the shorter stays in L2: 8192 rows, 14336 -> 4096: 0.31 ms with one tile of
     rows at a time, 0.35 with all; 4096 -> 28672: 0.86 and 0.63."""
-    n_tiles, blocks = (w.channels + 127) // 128 * (2 if w.gated else 1), (w.width + 127) // 128
+    n_tiles, blocks = _int8_tiles(w), (w.width + 127) // 128
     tiles_32 = n_tiles * ((T + 31) // 32)
     bq = 8 if T <= 8 else 32 if (tiles_32 <= _FEW_CTAS if T <= 64 else tiles_32 <= 128 and blocks <= 32) else 64
     tiles = n_tiles * max(1, (T + bq - 1) // bq)
-    if T <= 64 or tiles <= 2 * sm_count():
+    if T <= _few_most(n_tiles):
         return "few", bq, max(1, min(8, blocks // (16 if tiles > 96 else 4), _FEW_CTAS // tiles)), 0
     return "many", 1 if T >= w.channels else (T + 255) // 256
 
@@ -1888,8 +1902,8 @@ def int8_product(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: to
 
 
 def int8_gated_work(rows: int, w: Int8Weight) -> int:
-    """32-bit values of the scratch that ``int8_gated`` needs for up to ``rows`` rows."""
-    return rows * max(2 * w.channels, 4)
+    """32-bit values of the scratch that ``int8_gated`` needs for up to ``rows`` rows: both products of few rows, or h of all in bfloat16."""
+    return max(2 * w.channels * min(rows, _few_most(_int8_tiles(w))), rows * ((w.channels + 7) // 8 * 4))
 
 
 def int8_gated(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: torch.Tensor, out_scales: torch.Tensor, work: torch.Tensor,

@@ -20,6 +20,37 @@ import torch
 from . import kernels
 
 
+class Int8Linear:
+    """A weight in 8-bit integers with a scale a channel, for rows in 8 bits (``kernels.Int8Rows``): half the bytes of a decode step's weights and twice the
+    products a cycle of a prompt's. Every channel is rounded on the device when the model is built: q = rint(w * (127 / m)), m its largest |w|. One copy
+    of the weight serves few rows and many. ``gated``: [gate; up] of a gated feed-forward, for ``kernels.int8_gated``."""
+
+    def __init__(self, weight: torch.Tensor, device: torch.device, gated: bool = False):
+        if weight.dim() != 2:
+            raise ValueError("Linear: the weight must be a matrix")
+        self.out_features, self.in_features = weight.shape
+        w = weight.to(device=device)
+        w = (w if w.dtype in (torch.float32, torch.bfloat16) else w.float()).contiguous()
+        q = torch.empty(self.out_features, kernels.int8_width(self.in_features), dtype=torch.int8, device=device)
+        scales = torch.empty(self.out_features, device=device)
+        kernels.quantize_rows(w, q, scales)
+        self.weight = kernels.int8_weight(q, scales, gated=gated)
+
+    def forward(self, a: kernels.Int8Rows, out: torch.Tensor, accumulate: bool = False, norm=None, added=None) -> torch.Tensor:
+        """``norm`` = (weight, eps, rows): the norm of out's rows goes to ``rows`` (Int8Rows) once the product is added; ``added`` [T, N] 32-bit:
+        where the product waits for that addition, which the norm does on its way."""
+        if norm is None:
+            kernels.int8_product(a.q, a.scales, self.weight, out, accumulate)
+            return out
+        weight, eps, rows = norm
+        if accumulate:
+            kernels.int8_product(a.q, a.scales, self.weight, added)
+        else:
+            kernels.int8_product(a.q, a.scales, self.weight, out)
+        kernels.rmsnorm_int8(out, weight, rows.q, rows.scales, eps, add=added if accumulate else None)
+        return out
+
+
 class Linear:
     # not counted among a model's weight bytes: a second layout of the same weights, and adapters that rows may have beside them
     not_weights = ("weight_tiles", "adapters", "adapter_step")

@@ -6,8 +6,8 @@ import torch
 from ..cache import CacheNeed, StateNeed
 from ..config import PartSpec
 from ..ops import kernels
-from ..ops.linear import Linear
-from .registry import POSITION_ENCODINGS, build_part, register_mixer
+from ..ops.linear import Int8Linear, Linear
+from .registry import POSITION_ENCODINGS, build_part, int8_rows, register_mixer
 
 
 @register_mixer("attention")
@@ -180,8 +180,14 @@ class AttentionMixer:
                 raise ValueError(f"attention: conv has shape {tuple(weights['conv'].shape)}, expected ({qkv_rows}, {self.conv_taps})")
             self.conv = weights["conv"].to(device=build.device, dtype=torch.float32).contiguous()
             self.conv_channels = qkv_rows
-        self.w_qkv = Linear(weights["w_qkv"], build.compute_dtype, build.device, tiles=build.weight_tiles)
-        self.w_o = Linear(weights["w_o"], build.compute_dtype, build.device, tiles=build.weight_tiles)
+        self.int8 = build.weights == "int8"
+        if self.int8:
+            if self.extended:
+                raise ValueError("attention: weights in 8 bits go with none of the options")
+            self.w_qkv, self.w_o = Int8Linear(weights["w_qkv"], build.device), Int8Linear(weights["w_o"], build.device)
+        else:
+            self.w_qkv = Linear(weights["w_qkv"], build.compute_dtype, build.device, tiles=build.weight_tiles)
+            self.w_o = Linear(weights["w_o"], build.compute_dtype, build.device, tiles=build.weight_tiles)
         self.dtype = build.compute_dtype
         # bfloat16 with a head size the tensor-core kernels are built for; else the general kernel
         self.fast = self.dtype is torch.bfloat16 and not self.row_form and kernels.attention_fast_supported(
@@ -224,8 +230,8 @@ class AttentionMixer:
 
     def adaptable(self):
         """[(name of the projection, its Linear, widths of the parts stacked in it)]: where adapters can be (none with the options,
-        whose projections stack more than queries, keys and values)."""
-        if self.extended:
+        whose projections stack more than queries, keys and values, or with weights in 8 bits)."""
+        if self.extended or self.int8:
             return []
         H, Hkv, hd = self.num_heads, self.num_kv_heads, self.head_dim
         return [("w_qkv", self.w_qkv, (H * hd, Hkv * hd, Hkv * hd)), ("w_o", self.w_o, (self.hidden_size,))]
@@ -323,7 +329,8 @@ class AttentionMixer:
         """``xn``: normalised input [T, hidden] in the compute dtype; ``x``: the 32-bit residual
         stream, to which the mixer's output is added. ``run`` names whose cache to use. ``then``: the Linear
         of the large product that follows this mixer (the feed-forward's first), for the last product here to
-        ask the start of its weights into L2. ``norm`` = (weight, eps, out): the norm of x when the output is added."""
+        ask the start of its weights into L2. ``norm`` = (weight, eps, out): the norm of x when the output is added. With weights
+        in 8 bits ``xn`` and the norm's output are rows in 8 bits."""
         T = xn.shape[0]
         H, Hkv, hd = self.num_heads, self.num_kv_heads, self.head_dim
         k_cache, v_cache = ctx.pages(run.cache_layer)
@@ -332,7 +339,7 @@ class AttentionMixer:
         if self.extended:
             self._forward_extended(ctx, run, xn, x, q, k_cache, v_cache, tables, then)
             return
-        if self.dtype is torch.bfloat16 and not self.w_qkv.adapted and kernels.gemm_rope_store_supported(
+        if not self.int8 and self.dtype is torch.bfloat16 and not self.w_qkv.adapted and kernels.gemm_rope_store_supported(
                 T, self.hidden_size, H, Hkv, hd, self.position.cos, self.position.interleaved):
             # rotation and page store in the epilogue of the product
             kernels.gemm_rope_store(xn, self.w_qkv.weight, ctx.positions, ctx.row_req, tables, self.position.cos,
@@ -346,6 +353,12 @@ class AttentionMixer:
                                write_kv=run.writes_cache)
         att = ctx.scratch("att", (T, H * hd), self.dtype)
         self._attend(ctx, q, k_cache, v_cache, att, tables)
+        if self.int8:
+            rows = int8_rows(ctx, "att", T, H * hd)
+            kernels.quantize_rows(att, rows.q, rows.scales)
+            added = None if norm is None else ctx.scratch("int8_added", (T, self.hidden_size), torch.float32)
+            self.w_o.forward(rows, x, accumulate=True, norm=norm, added=added)
+            return
         self.w_o.forward(att, x, accumulate=True, then=then, norm=norm)
 
     def _forward_extended(self, ctx, run, xn, x, q, k_cache, v_cache, tables, then) -> None:

@@ -4,7 +4,7 @@ from __future__ import annotations
 import torch
 
 from .norm import LayerNorm, RMSNorm, ScalarRMSNorm
-from .registry import FEED_FORWARDS, MIXERS, NORMS, build_part, register_block, sub_weights
+from .registry import FEED_FORWARDS, MIXERS, NORMS, build_part, int8_rows, register_block, sub_weights
 from .stream import EmbeddingAdd, EmbeddingMix
 
 
@@ -25,14 +25,22 @@ class PreNormBlock:
         self.feed_forward = build_part(FEED_FORWARDS, "feed-forward", layer_spec.feed_forward,
                                        sub_weights(weights, "feed_forward."), build)
         self.dtype = build.compute_dtype
+        self.int8 = build.weights == "int8"      # the sublayers read rows in 8 bits
+        if self.int8:
+            for part in (self.mixer, self.feed_forward):
+                if not getattr(part, "int8", False):
+                    raise ValueError(f"weights in 8 bits: {type(part).__name__} has no such form")
+            for norm in (self.mixer_norm, self.feed_forward_norm):
+                if type(norm) not in (RMSNorm, ScalarRMSNorm):
+                    raise ValueError(f"weights in 8 bits: {type(norm).__name__} has no output in 8 bits")
         self._next = {}             # run -> the norm of the next run's block where that reads the stream as this one leaves it
 
     def followed_in_run(self, run, block, stream_input) -> None:
-        after = block.mixer_norm if stream_input is None and isinstance(block, PreNormBlock) else None
+        after = block.mixer_norm if stream_input is None and isinstance(block, PreNormBlock) and block.int8 == self.int8 else None
         self._next[run] = after if self._next.get(run, after) is after else None      # (a run that comes twice, before different blocks)
 
     def forward(self, ctx, run, x: torch.Tensor) -> None:
-        xn = ctx.scratch("normed", tuple(x.shape), self.dtype)
+        xn = int8_rows(ctx, "normed", *x.shape) if self.int8 else ctx.scratch("normed", tuple(x.shape), self.dtype)
         T = x.shape[0]
         carry = getattr(ctx, "carry", None)
         tapped = getattr(ctx, "tapping", False)

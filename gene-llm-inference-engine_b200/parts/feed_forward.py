@@ -4,8 +4,8 @@ from __future__ import annotations
 import torch
 
 from ..ops import kernels
-from ..ops.linear import Linear
-from .registry import register_feed_forward, sub_weights
+from ..ops.linear import Int8Linear, Linear
+from .registry import int8_rows, register_feed_forward, sub_weights
 
 
 @register_feed_forward("swiglu")
@@ -16,7 +16,9 @@ class SwiGLUFeedForward:
     Params: ``hidden_size``, ``intermediate_size`` and optionally ``activation`` (one of ``kernels.ACTIVATIONS``: "silu", the
     default; "relu"; "gelu_tanh"; "capped_swish", which is not of the form act(gate) * up, with its bound
     ``activation_limit``) and ``bias`` (every projection has one: z = W u + b). Weights: ``w_gate_up`` [2I, hidden] (gate
-    rows first, then up rows) and ``w_down`` [hidden, I]; with ``bias`` also ``b_gate_up`` [2I] and ``b_down`` [hidden]."""
+    rows first, then up rows) and ``w_down`` [hidden, I]; with ``bias`` also ``b_gate_up`` [2I] and ``b_down`` [hidden].
+
+    Weights in 8 bits (``BuildContext.weights``): ``xn`` comes as rows in 8 bits and the activated rows go to the down projection in 8 bits too."""
 
     graph_safe = True      # launches depend only on the step's shape: decode steps may be captured in a CUDA graph
 
@@ -35,8 +37,12 @@ class SwiGLUFeedForward:
             raise ValueError(f"swiglu: w_gate_up has shape {tuple(weights['w_gate_up'].shape)}, expected ({2 * I}, {D})")
         if tuple(weights["w_down"].shape) != (D, I):
             raise ValueError(f"swiglu: w_down has shape {tuple(weights['w_down'].shape)}, expected ({D}, {I})")
-        self.w_gate_up = Linear(weights["w_gate_up"], build.compute_dtype, build.device, tiles=build.weight_tiles)
-        self.w_down = Linear(weights["w_down"], build.compute_dtype, build.device, tiles=build.weight_tiles)
+        self.int8 = build.weights == "int8"
+        if self.int8:
+            self.w_gate_up, self.w_down = Int8Linear(weights["w_gate_up"], build.device, gated=True), Int8Linear(weights["w_down"], build.device)
+        else:
+            self.w_gate_up = Linear(weights["w_gate_up"], build.compute_dtype, build.device, tiles=build.weight_tiles)
+            self.w_down = Linear(weights["w_down"], build.compute_dtype, build.device, tiles=build.weight_tiles)
         self.b_gate_up = self.b_down = None
         if params.get("bias"):
             for name, n in (("b_gate_up", 2 * I), ("b_down", D)):
@@ -56,10 +62,12 @@ class SwiGLUFeedForward:
     @property
     def first_product(self):
         """The Linear of the first product (a block hands it to the mixer that runs before, see AttentionMixer.forward)."""
-        return self.w_gate_up
+        return None if self.int8 else self.w_gate_up
 
     def adaptable(self):
-        """[(name of the projection, its Linear, widths of the parts stacked in it)]: where adapters can be."""
+        """[(name of the projection, its Linear, widths of the parts stacked in it)]: where adapters can be (none beside weights in 8 bits)."""
+        if self.int8:
+            return []
         return [("w_gate_up", self.w_gate_up, (self.intermediate_size, self.intermediate_size)), ("w_down", self.w_down, (self.hidden_size,))]
 
     def launch_key(self, ctx):
@@ -74,6 +82,16 @@ class SwiGLUFeedForward:
     def forward(self, ctx, xn: torch.Tensor, x: torch.Tensor, accumulate: bool = True, norm=None) -> None:
         """``accumulate`` False: x is set to the output instead of being added to. ``norm`` = (weight, eps, out): the norm of x then."""
         T = xn.shape[0]
+        if self.int8:
+            h = int8_rows(ctx, "ffn_hidden", T, self.intermediate_size)
+            need = kernels.int8_gated_work(ctx.max_step_tokens, self.w_gate_up.weight)
+            kernels.int8_gated(xn.q, xn.scales, self.w_gate_up.weight, h.q, h.scales, ctx.scratch("int8_gated_work", (need,), torch.float32, capacity=need),
+                               self.activation, self.limit, self.b_gate_up)
+            added = None if norm is None else ctx.scratch("int8_added", (T, self.hidden_size), torch.float32)
+            self.w_down.forward(h, x, accumulate=accumulate, norm=norm, added=added)
+            if self.b_down is not None and not self.output_bias_left:
+                kernels.add_bias(x, self.b_down)
+            return
         h = ctx.scratch("ffn_hidden", (T, self.intermediate_size), self.dtype)
         if self.dtype is torch.bfloat16 and not self.w_gate_up.adapted and kernels.gemm_swiglu_supported(T, self.intermediate_size, self.hidden_size):
             # activation (and bias) in the product's epilogue

@@ -27,10 +27,17 @@ class LayerRun:
 
 class DecoderModel:
     def __init__(self, spec: ModelSpec, params: Dict[str, torch.Tensor], compute_dtype: torch.dtype,
-                 device: torch.device, max_position: Optional[int] = None, weight_tiles: bool = True):
+                 device: torch.device, max_position: Optional[int] = None, weight_tiles: bool = True, weights: str = "native"):
+        """``weights`` "int8": the layers' projections in 8-bit integers (embedding, norms and head stay as they are); for designs whose layers are
+        norm, attention, norm, gated feed-forward."""
         spec.validate()
         if compute_dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("compute dtype must be float32 or bfloat16")
+        if weights not in ("native", "int8"):
+            raise ValueError(f"unknown form of the weights '{weights}' (native or int8)")
+        for layer_spec in spec.layers:
+            if weights == "int8" and layer_spec.block != "pre_norm":
+                raise ValueError(f"weights in 8 bits: layers of the arrangement '{layer_spec.block}' have no such form")
         self.spec = spec
         self.dtype = compute_dtype
         self.device = device
@@ -41,7 +48,7 @@ class DecoderModel:
         else:
             self.max_position = min(spec.max_position, max_position) if max_position else spec.max_position
         build = BuildContext(device=device, compute_dtype=compute_dtype, max_position=self.max_position,
-                             weight_tiles=weight_tiles)
+                             weight_tiles=weight_tiles, weights=weights)
 
         emb = params["embedding.weight"]
         if tuple(emb.shape) != (spec.vocab_size, spec.hidden_size):

@@ -32,8 +32,12 @@ class RMSNorm:
         """Its one launch depends on the number of rows only (which the caller's key holds)."""
         return ()
 
-    def forward(self, x: torch.Tensor, out: torch.Tensor, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
-        kernels.rmsnorm(x, self.weight, out, self.eps, rows)
+    def forward(self, x: torch.Tensor, out, rows: Optional[torch.Tensor] = None):
+        """``out``: a tensor, or rows in 8 bits (``kernels.Int8Rows``)."""
+        if isinstance(out, kernels.Int8Rows):
+            kernels.rmsnorm_int8(x, self.weight, out.q, out.scales, self.eps)
+        else:
+            kernels.rmsnorm(x, self.weight, out, self.eps, rows)
         return out
 
     def join_stream(self, y: torch.Tensor, x: torch.Tensor, more=None, next_norm=None, xn_out=None) -> None:

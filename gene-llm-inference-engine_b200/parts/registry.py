@@ -27,6 +27,7 @@ class BuildContext:
     compute_dtype: torch.dtype       # torch.float32 (true 32-bit path) or torch.bfloat16
     max_position: int                # context length the engine is built for
     weight_tiles: bool = True        # bfloat16: keep a second, tile-by-tile copy of each matrix for few-token products
+    weights: str = "native"          # "int8": the projections in 8-bit integers, of parts that have that form
 
 
 def _register(table: Dict[str, Callable], kind: str):
@@ -62,6 +63,13 @@ def register_logit_transform(kind: str):
 
 def register_stream_input(kind: str):
     return _register(STREAM_INPUTS, kind)
+
+
+def int8_rows(ctx, name: str, rows: int, values: int):
+    """Scratch for rows in 8 bits."""
+    from ..ops import kernels
+    return kernels.Int8Rows(ctx.scratch(f"int8_{name}", (rows, kernels.int8_width(values)), torch.int8),
+                            ctx.scratch(f"int8_{name}_scales", (rows,), torch.float32), values)
 
 
 def build_part(table: Dict[str, Callable], what: str, spec, weights, build: BuildContext):

@@ -1,0 +1,119 @@
+"""Weights and rows in 8-bit integers without a GPU: layouts, plans, scratch sizes, and what is refused before a kernel runs."""
+import pytest
+import torch
+
+import kidarax_configs
+import nipadra_configs
+import tiny_configs as tc
+from geneinfer_b200.ops import kernels as k
+
+
+def _unlaid(w, K):
+    """[parts, channels, K] from the tiles: the definition of the layout, read backwards."""
+    parts = 2 if w.gated else 1
+    blocks = (w.width + 127) // 128
+    t = w.tiles.view(-1, parts, blocks, 128, 8, 16)
+    out = torch.zeros(parts, t.shape[0] * 128, blocks * 128, dtype=torch.int8)
+    for tile in range(t.shape[0]):
+        for part in range(parts):
+            for b in range(blocks):
+                for piece in range(8):
+                    for r in range(128):
+                        out[part, tile * 128 + r, b * 128 + piece * 16:b * 128 + piece * 16 + 16] = t[tile, part, b, r, piece ^ (r % 8)]
+    return out
+
+
+@pytest.mark.parametrize("N,K,gated", [(1, 1, False), (130, 200, False), (256, 128, False), (6, 33, True), (300, 129, True)])
+def test_the_layout_of_a_weight(N, K, gated):
+    g = torch.Generator().manual_seed(N + K)
+    q = torch.randint(-127, 128, (N, K), generator=g, dtype=torch.int8)
+    w = k.int8_weight(q, torch.ones(N), gated=gated)
+    parts = 2 if gated else 1
+    assert (w.channels, w.width, w.gated) == (N // parts, k.int8_width(K), gated) and w.width % 16 == 0 and 0 <= w.width - K < 16
+    back = _unlaid(w, K)
+    assert torch.equal(back[:, :N // parts, :K], q.view(parts, N // parts, K))
+    assert not back[:, N // parts:].any() and not back[:, :, K:].any()
+
+
+def test_plans_fit_the_kernels():
+    """Every plan names a tile that exists, ranges of K that are not empty, and few rows' CTAs that fit on the GPU at once."""
+    w = k.int8_weight(torch.zeros(1, 1, dtype=torch.int8), torch.ones(1))
+    for channels in (1, 128, 300, 2048, 6144, 16384, 128256):
+        for width in (16, 128, 2048, 14336, k.INT8_WIDTH_MOST):
+            for gated in (False, True):
+                w.channels, w.width, w.gated = channels, width, gated
+                few_ended = False
+                for T in list(range(0, 70)) + [96, 128, 200, 256, 300, 512, 1000, 4096, 100000]:
+                    plan = k._int8_plan(T, w)
+                    if plan[0] == "few":
+                        _, bq, splits, stages = plan
+                        assert bq in (8, 32, 64) and 1 <= splits <= 8 and stages == 0 and not few_ended
+                        assert splits == 1 or splits * ((channels + 127) // 128) * (2 if gated else 1) * ((T + bq - 1) // bq) <= 264
+                        assert splits <= (width + 127) // 128
+                        assert not gated or 2 * channels * T <= k.int8_gated_work(T, w)
+                    else:
+                        few_ended = True
+                        assert T > 64 and 1 <= plan[1] <= (T + 255) // 256
+                        assert not gated or (channels + 7) // 8 * 8 * T <= 2 * k.int8_gated_work(T, w)
+                    assert not gated or k.int8_gated_work(T, w) <= k.int8_gated_work(T + 1, w)
+
+
+def test_weights_that_do_not_fit_are_refused():
+    q, s = torch.zeros(4, 8, dtype=torch.int8), torch.ones(4)
+    for bad in ((q.float(), s), (q, s[:3]), (q, s.double()), (q[0], s), (q[:, :0], s), (torch.zeros(1, k.INT8_WIDTH_MOST + 1, dtype=torch.int8), s[:1])):
+        with pytest.raises(k.KernelError):
+            k.int8_weight(*bad)
+    with pytest.raises(k.KernelError, match="two parts"):
+        k.int8_weight(q[:3], s[:3], gated=True)
+
+
+def test_calls_that_do_not_fit_are_refused():
+    """Shapes first, so that a wrong call is told what is wrong with it on any machine; then that there is no CPU path."""
+    x, w, s = torch.zeros(3, 20), torch.ones(20), torch.zeros(3)
+    q = torch.zeros(3, 32, dtype=torch.int8)
+    for call in (lambda: k.quantize_rows(x, q[:, :16], s), lambda: k.quantize_rows(x, q[:2], s), lambda: k.quantize_rows(x, q, s[:2]),
+                 lambda: k.quantize_rows(x[0], q, s), lambda: k.quantize_rows(x[:, :0], q, s),
+                 lambda: k.rmsnorm_int8(x, w[:19], q, s, 1e-5), lambda: k.rmsnorm_int8(x, w, q, s, 1e-5, add=x[:2]),
+                 lambda: k.rmsnorm_int8(x.bfloat16(), w, q, s, 1e-5), lambda: k.rmsnorm_int8(x, w, q, s, 1e-5, add=x),
+                 lambda: k.gated_act_int8(x[:, :19], q, s), lambda: k.gated_act_int8(torch.zeros(3, 40), q, s, "tanh"),
+                 lambda: k.gated_act_int8(torch.zeros(3, 40), q, s, bias=torch.zeros(20)),
+                 lambda: k.quantize_rows(x, q, s), lambda: k.quantize_rows(x.double(), q, s)):
+        with pytest.raises(k.KernelError):
+            call()
+    plain, pair = k.int8_weight(torch.zeros(8, 20, dtype=torch.int8), torch.ones(8)), k.int8_weight(torch.zeros(8, 20, dtype=torch.int8), torch.ones(8), gated=True)
+    out, wide = torch.zeros(3, 8), torch.zeros(100)
+    for call in (lambda: k.int8_product(q[:, :16], s, plain, out), lambda: k.int8_product(q, s[:2], plain, out), lambda: k.int8_product(q, s, pair, out),
+                 lambda: k.int8_product(q, s, plain, out[:, :7]), lambda: k.int8_product(q, s, plain, out.bfloat16(), accumulate=True),
+                 lambda: k.int8_gated(q, s, plain, q[:, :16], s, wide), lambda: k.int8_gated(q, s, pair, q, s, wide),
+                 lambda: k.int8_gated(q, s, pair, q[:, :16].contiguous(), s, wide, "tanh"), lambda: k.int8_gated(q, s, pair, q[:, :16].contiguous(), s, wide[:4]),
+                 lambda: k.int8_gated(q, s, pair, q[:, :16].contiguous(), s, wide, bias=torch.zeros(4))):
+        with pytest.raises(k.KernelError):
+            call()
+
+
+def test_models_without_such_a_form_are_refused():
+    from geneinfer_b200 import Engine, SpeculativeEngine
+    from geneinfer_b200.config import parse_config
+    from geneinfer_b200.parts import DecoderModel
+    with pytest.raises(ValueError, match="adapters"):
+        Engine("nowhere", adapter_slots=1, weights="int8")
+    with pytest.raises(ValueError, match="adapters"):
+        SpeculativeEngine("nowhere", "nowhere", adapter_slots=1, weights="int8")
+    for config in (nipadra_configs.NIP_P, kidarax_configs.KID_A):
+        with pytest.raises(ValueError, match="8 bits"):
+            DecoderModel(parse_config(config)[1].model_spec(), {}, torch.bfloat16, torch.device("cpu"), weights="int8")
+    llama = parse_config(tc.TINY_A)[1].model_spec()
+    with pytest.raises(ValueError, match="int4"):
+        DecoderModel(llama, {}, torch.bfloat16, torch.device("cpu"), weights="int4")
+
+
+def test_command_line():
+    from geneinfer_b200.cli.generate_main import UsageError, parse
+    base = ["--model", "m", "--prompt-ids", "1 2"]
+    assert parse(base + ["--weights", "int8"])["weights"] == "int8"
+    assert parse(base + ["--weights", "int8", "--dtype", "bf16"])["weights"] == "int8"
+    assert parse(base + ["--weights", "int8", "--dtype", "fp32"])["weights"] == "f32"
+    assert parse(base + ["--dtype", "bf16"])["weights"] == "native"
+    for bad in (["--weights", "int4"], ["--weights", "int8", "--adapter", "a"]):
+        with pytest.raises(UsageError):
+            parse(base + bad)
