@@ -188,7 +188,7 @@ template <int KIND, typename TX, typename TA, int G, int V, bool VEC>
 __global__ void __launch_bounds__(G < 128 ? 128 : G, G <= 512 ? 1024 / (G < 128 ? 128 : G) : 1)
 rows_int8_kernel(const RowsParams p) {
     constexpr int kRows = G < 128 ? 128 / G : 1;
-    constexpr int kBatch = V <= 4 ? V : 2;
+    constexpr int kBatch = V <= 4 ? V : sizeof(TX) == 2 ? 4 : 2;      // (16-bit values wait in half the registers)
     constexpr bool kEarly = V <= 4;      // the norm's weights are read before the wait for the kernel ahead, where registers hold them
     __shared__ unsigned part_m[2][32];
     __shared__ float part_s[2][32];

@@ -1743,29 +1743,35 @@ def int8_width(values: int) -> int:
     return (values + 15) // 16 * 16
 
 
-def _here(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    """All of them on the current device, on whose stream the kernel runs."""
-    for t in tensors:
-        if t is not None and t.is_cuda and t.get_device() != torch._C._cuda_getDevice():
-            raise KernelError(f"{name}: a tensor is on cuda:{t.get_device()}, the current device is cuda:{torch._C._cuda_getDevice()}")
+def _here(name: str, first: torch.Tensor, *more: Optional[torch.Tensor]) -> None:
+    """All of them on the current device, on whose stream the kernel runs. (What is not on a device at all is refused by the checks of each.)"""
+    device = first.get_device()
+    if device >= 0 and device != torch._C._cuda_getDevice():
+        raise KernelError(f"{name}: a tensor is on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    for t in more:
+        if t is not None and t.get_device() != device:
+            raise KernelError(f"{name}: the tensors must be on one device (cuda:{device} and {t.device})")
 
 
 def _rows_int8(name: str, kind: int, x: torch.Tensor, columns: int, out: torch.Tensor, scales: torch.Tensor, add=None, weight=None, eps: float = 0.0,
                act: int = 0, limit: float = 0.0) -> None:
-    if x.dim() != 2 or out.dim() != 2:
-        raise KernelError(f"{name}: the rows and their integers must be matrices")
-    T = x.shape[0]
-    D = x.shape[1] // columns
-    if D < 1 or x.shape[1] != columns * D or out.shape != (T, int8_width(D)) or scales.numel() != T:
+    T, D = x.shape
+    D //= columns
+    width = (D + 15) // 16 * 16
+    if D < 1 or out.shape != (T, width) or scales.numel() != T:
         raise KernelError(f"{name}: out must be [T, int8_width(D)] and scales [T] for rows of D values")
     _here(name, x, out, scales, add, weight)
-    check(lib().gi_rows_int8(kind, _rows_of(x, "x"), dtype_code(x.dtype), x.stride(0), 0 if add is None else _dev(add, "add"),
-                             0 if add is None else dtype_code(add.dtype), _opt(weight, "weight", torch.float32), float(eps), act, float(limit),
-                             _dev(out, "out", torch.int8), out.shape[1], _dev(scales, "scales", torch.float32), T, D, _stream()), name)
+    code = lib().gi_rows_int8(kind, _rows_of(x, "x"), dtype_code(x.dtype), x.stride(0), 0 if add is None else _dev(add, "add"),
+                              0 if add is None else dtype_code(add.dtype), 0 if weight is None else _dev(weight, "weight", torch.float32), eps, act, limit,
+                              _dev(out, "out", torch.int8), width, _dev(scales, "scales", torch.float32), T, D, _stream())
+    if code:
+        check(code, name)
 
 
 def quantize_rows(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> None:
     """The rows of ``x`` [T, D] (32-bit or bfloat16; rows may lie apart) in 8 bits: ``out`` [T, int8_width(D)] int8 and ``scales`` [T]."""
+    if x.dim() != 2:
+        raise KernelError("quantize_rows: x must be a matrix")
     _rows_int8("quantize_rows", 0, x, 1, out, scales)
 
 
@@ -1778,9 +1784,9 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, scale
         raise KernelError("rmsnorm_int8: shapes of x, weight and add do not agree")
     if x.dtype is not torch.float32:
         raise KernelError(f"rmsnorm_int8: x must be torch.float32, got {x.dtype}")
-    if add is not None and add.data_ptr() == x.data_ptr():
+    if add is not None and add.data_ptr() == x.data_ptr() and x.numel():
         raise KernelError("rmsnorm_int8: add must not be x itself")
-    _rows_int8("rmsnorm_int8", 1, x, 1, out, scales, add=add, weight=weight, eps=eps)
+    _rows_int8("rmsnorm_int8", 1, x, 1, out, scales, add, weight, eps)
 
 
 def gated_act_int8(gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, activation: str = "silu", limit: float = 0.0,
@@ -1791,7 +1797,7 @@ def gated_act_int8(gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tenso
         raise KernelError("gated_act_int8: gate_up must be [T, 2I] (and the bias [2I])")
     if activation not in ACTIVATIONS:
         raise KernelError(f"gated_act_int8: unknown activation '{activation}' (known: {', '.join(sorted(ACTIVATIONS))})")
-    _rows_int8("gated_act_int8", 2, gate_up, 2, out, scales, weight=bias, act=ACTIVATIONS[activation], limit=limit)
+    _rows_int8("gated_act_int8", 2, gate_up, 2, out, scales, None, bias, 0.0, ACTIVATIONS[activation], limit)
 
 
 class Int8Rows:
@@ -1807,6 +1813,7 @@ class Int8Weight:
 
     def __init__(self, tiles: torch.Tensor, scales: torch.Tensor, channels: int, width: int, gated: bool):
         self.tiles, self.scales, self.channels, self.width, self.gated = tiles, scales, channels, width, gated
+        self.plans = {}      # rows -> the plan of a product of so many: sizes decide, once
 
 
 def int8_weight(q: torch.Tensor, scales: torch.Tensor, gated: bool = False) -> Int8Weight:
@@ -1843,6 +1850,15 @@ def _few_most(n_tiles: int) -> int:
 
 
 def _int8_plan(T: int, w: Int8Weight):
+    plan = w.plans.get(T)
+    if plan is None:
+        if len(w.plans) >= 4096:
+            w.plans.clear()
+        plan = w.plans[T] = _int8_plan_of(T, w)
+    return plan
+
+
+def _int8_plan_of(T: int, w: Int8Weight):
     """("few", rows of a tile, ranges of K, stages) or ("many", tiles of rows walked together). Measured on B200 (us).
 
     Few rows: tiles of 8, 32 or 64 rows; tiles of 32 as long as they all fit at once (64 rows, 2048 -> 2048: 4.9 with tiles of 32 and 5.6 with 64; 4096 ->
@@ -1861,24 +1877,26 @@ def _int8_plan(T: int, w: Int8Weight):
     return "many", 1 if T >= w.channels else (T + 255) // 256
 
 
-def _few(a, a_scales, w, out, accumulate, plan) -> None:
-    _, bq, splits, stages = plan
-    check(lib().gi_int8_product_few(_dev(a, "a", torch.int8), _dev(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
-                                    w.scales.data_ptr(), w.channels, int(w.gated), _rows_of(out, "out"), dtype_code(out.dtype), out.stride(0),
-                                    int(bool(accumulate)), bq, splits, stages, _tc_state(a.device).status.data_ptr(), _stream()), "int8_product")
+def _few(a, a_scales, w, out, out_dtype, out_stride, accumulate, plan) -> None:
+    code = lib().gi_int8_product_few(_dev(a, "a", torch.int8), _dev(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
+                                     w.scales.data_ptr(), w.channels, int(w.gated), out, out_dtype, out_stride, int(bool(accumulate)), plan[1], plan[2], plan[3],
+                                     _tc_state(a.device).status.data_ptr(), _stream())
+    if code:
+        check(code, "int8_product")
 
 
-def _many(a, a_scales, w, out, out_stride, accumulate, plan, act=0, limit=0.0, bias=None) -> None:
-    check(lib().gi_int8_product_many(_dev(a, "a", torch.int8), _dev(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
-                                     w.scales.data_ptr(), w.channels, int(w.gated), act, float(limit), _opt(bias, "bias", torch.float32), out.data_ptr(),
-                                     dtype_code(out.dtype), out_stride, int(bool(accumulate)), plan[1],
-                                     _tc_state(a.device).status.data_ptr(), _stream()), "int8_product")
+def _many(a, a_scales, w, out, out_dtype, out_stride, accumulate, plan, act=0, limit=0.0, bias=0) -> None:
+    code = lib().gi_int8_product_many(_dev(a, "a", torch.int8), _dev(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
+                                      w.scales.data_ptr(), w.channels, int(w.gated), act, limit, bias, out, out_dtype, out_stride, int(bool(accumulate)), plan[1],
+                                      _tc_state(a.device).status.data_ptr(), _stream())
+    if code:
+        check(code, "int8_product")
 
 
 def _int8_operands(name: str, a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, *more: Optional[torch.Tensor]) -> int:
     if a.dim() != 2 or a.shape[1] != w.width or a_scales.numel() != a.shape[0]:
         raise KernelError(f"{name}: a must be [T, {w.width}] (the weight's width) and a_scales [T]")
-    _here(name, a, a_scales, w.tiles, *more)
+    _here(name, a, a_scales, w.tiles, w.scales, *more)
     return a.shape[0]
 
 
@@ -1894,11 +1912,7 @@ def int8_product(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: to
     if accumulate and out.dtype is not torch.float32:
         raise KernelError("int8_product: accumulation needs a 32-bit output")
     plan = plan or _int8_plan(T, w)
-    if plan[0] == "few":
-        _few(a, a_scales, w, out, accumulate, plan)
-    else:
-        _rows_of(out, "out")
-        _many(a, a_scales, w, out, out.stride(0), accumulate, plan)
+    (_few if plan[0] == "few" else _many)(a, a_scales, w, _rows_of(out, "out"), dtype_code(out.dtype), out.stride(0), accumulate, plan)
 
 
 def int8_gated_work(rows: int, w: Int8Weight) -> int:
@@ -1913,23 +1927,24 @@ def int8_gated(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: torc
     ``int8_gated_work`` values. ``activation``, ``limit``, ``bias`` [2I]: see ``gated_act``. Two launches: few rows leave the products in 32 bits for
     ``gated_act_int8``; with many the activation is the product's epilogue."""
     T = _int8_operands("int8_gated", a, a_scales, w, out, out_scales, work, bias)
-    I = w.channels
+    I, width = w.channels, int8_width(w.channels)
     if not w.gated:
         raise KernelError("int8_gated: the weight is not laid out as a gated pair")
-    if out.shape != (T, int8_width(I)) or out_scales.numel() != T or (bias is not None and bias.numel() != 2 * I):
-        raise KernelError(f"int8_gated: out must be [T, {int8_width(I)}] and out_scales [T] (and the bias [{2 * I}])")
+    if out.shape != (T, width) or out_scales.numel() != T or (bias is not None and bias.numel() != 2 * I):
+        raise KernelError(f"int8_gated: out must be [T, {width}] and out_scales [T] (and the bias [{2 * I}])")
     if activation not in ACTIVATIONS:
         raise KernelError(f"int8_gated: unknown activation '{activation}' (known: {', '.join(sorted(ACTIVATIONS))})")
-    _dev(work, "work", torch.float32)
     if work.numel() < int8_gated_work(T, w):
         raise KernelError(f"int8_gated: work must hold {int8_gated_work(T, w)} values")
-    work, plan = work.view(-1), _int8_plan(T, w)
-    if plan[0] == "few":
-        both = work[:T * 2 * I].view(T, 2 * I)
-        _few(a, a_scales, w, both, False, plan)
-        gated_act_int8(both, out, out_scales, activation, limit, bias)
-        return
-    stride = (I + 7) // 8 * 8                 # whole 16 bytes
-    h = work.view(torch.bfloat16)[:T * stride].view(T, stride)[:, :I]
-    _many(a, a_scales, w, h, stride, False, plan, ACTIVATIONS[activation], limit, bias)
-    quantize_rows(h, out, out_scales)
+    act, plan = ACTIVATIONS[activation], _int8_plan(T, w)
+    scratch, bias = _dev(work, "work", torch.float32), 0 if bias is None else _dev(bias, "bias", torch.float32)
+    q, scales = _dev(out, "out", torch.int8), _dev(out_scales, "out_scales", torch.float32)
+    if plan[0] == "few":                      # [gate; up] in 32 bits, then the activation with the rows
+        _few(a, a_scales, w, scratch, F32, 2 * I, False, plan)
+        code = lib().gi_rows_int8(2, scratch, F32, 2 * I, 0, 0, bias, 0.0, act, limit, q, width, scales, T, I, _stream())
+    else:
+        stride = (I + 7) // 8 * 8             # whole 16 bytes
+        _many(a, a_scales, w, scratch, BF16, stride, False, plan, act, limit, bias)
+        code = lib().gi_rows_int8(0, scratch, BF16, stride, 0, 0, 0, 0.0, 0, 0.0, q, width, scales, T, I, _stream())
+    if code:
+        check(code, "int8_gated")

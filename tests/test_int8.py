@@ -44,7 +44,7 @@ def test_plans_fit_the_kernels():
                 w.channels, w.width, w.gated = channels, width, gated
                 few_ended = False
                 for T in list(range(0, 70)) + [96, 128, 200, 256, 300, 512, 1000, 4096, 100000]:
-                    plan = k._int8_plan(T, w)
+                    plan = k._int8_plan_of(T, w)
                     if plan[0] == "few":
                         _, bq, splits, stages = plan
                         assert bq in (8, 32, 64) and 1 <= splits <= 8 and stages == 0 and not few_ended
