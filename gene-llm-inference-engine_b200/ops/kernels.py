@@ -1845,8 +1845,8 @@ def _int8_tiles(w: Int8Weight) -> int:
 
 
 def _few_most(n_tiles: int) -> int:
-    """The most rows that count as few: tiles of 64 of them that an SM holds two of at once."""
-    return 64 * max(1, 2 * sm_count() // n_tiles)
+    """The most rows that count as few: tiles of 64 of them of which all fit at once, two to an SM; one of 128 where that is all that fits."""
+    return 64 * max(2 if n_tiles <= 2 * sm_count() else 1, 2 * sm_count() // n_tiles)
 
 
 def _int8_plan(T: int, w: Int8Weight):
@@ -1862,7 +1862,8 @@ def _int8_plan_of(T: int, w: Int8Weight):
     """("few", rows of a tile, ranges of K, stages) or ("many", tiles of rows walked together). Measured on B200 (us).
 
     Few rows: tiles of 8, 32 or 64 rows; tiles of 32 as long as they all fit at once (64 rows, 2048 -> 2048: 4.9 with tiles of 32 and 5.6 with 64; 4096 ->
-    28672: 34.6 and 21.2) and K is short (160 rows, 8192 -> 2048: 13.2 and 10.8). K is cut while all CTAs fit at once and a range has four blocks (8
+    28672: 34.6 and 21.2) and K is short (160 rows, 8192 -> 2048: 13.2 and 10.8); of 128 rows where there are too many tiles of 64 and too few for pairs of
+    CTAs to be busy (128 rows, 4096 -> 28672: 24.9, with tiles of 64 38.7, as many rows 31.4). K is cut while all CTAs fit at once and a range has four blocks (8
     rows, 4096 -> 4096: 5.4 with 8 ranges, 5.7 with 4, 6.8 with 2), from a hundred tiles on sixteen (8 rows, 2048 -> 16384: 7.2 with one range, 7.6 with
     two; 1000 rows, 8192 -> 1024: 22.4 and 17.9).
     Many rows, from where the tiles of 64 rows no longer fit at once: 400 rows, 4096 -> 4096 (224 tiles): few 14.4, many 17.2; 333 rows, 2048 -> 16384
@@ -1870,10 +1871,13 @@ def _int8_plan_of(T: int, w: Int8Weight):
     rows at a time, 0.35 with all; 4096 -> 28672: 0.86 and 0.63."""
     n_tiles, blocks = _int8_tiles(w), (w.width + 127) // 128
     tiles_32 = n_tiles * ((T + 31) // 32)
-    bq = 8 if T <= 8 else 32 if (tiles_32 <= _FEW_CTAS if T <= 64 else tiles_32 <= 128 and blocks <= 32) else 64
+    if T <= 64:
+        bq = 8 if T <= 8 else 32 if tiles_32 <= _FEW_CTAS else 64
+    else:
+        bq = 128 if n_tiles > sm_count() else 32 if tiles_32 <= 128 and blocks <= 32 else 64
     tiles = n_tiles * max(1, (T + bq - 1) // bq)
     if T <= _few_most(n_tiles):
-        return "few", bq, max(1, min(8, blocks // (16 if tiles > 96 else 4), _FEW_CTAS // tiles)), 0
+        return "few", bq, 1 if bq == 128 else max(1, min(8, blocks // (16 if tiles > 96 else 4), _FEW_CTAS // tiles)), 0
     return "many", 1 if T >= w.channels else (T + 255) // 256
 
 

@@ -200,7 +200,7 @@ def _scaled(sums, a_scales, w_scales):
 
 
 SHAPES = [(1, 16, 1), (1, 2048, 2048), (3, 100, 130), (16, 8192, 256), (17, 4096, 333), (33, 1000, 64), (64, 4096, 1000), (65, 129, 2049),
-          (128, 2064, 700), (200, 5000, 513), (256, 2048, 4096), (257, 512, 300), (300, 4096, 1024), (511, 1040, 129), (1000, 777, 1001), (2049, 2048, 512)]
+          (128, 2064, 700), (100, 300, 19100), (200, 5000, 513), (256, 2048, 4096), (257, 512, 300), (300, 4096, 1024), (511, 1040, 129), (1000, 777, 1001), (2049, 2048, 512)]
 
 
 @pytest.mark.parametrize("T,K,N", SHAPES)
@@ -225,6 +225,10 @@ def test_product(T, K, N):
     wide = torch.full((T, N + 5), 7.0, device=DEV)                      # rows that lie apart, at an odd place
     k.int8_product(a, s, w, wide[:, 3:3 + N])
     assert torch.equal(wide[:, 3:3 + N], want) and (wide[:, :3] == 7).all() and (wide[:, 3 + N:] == 7).all()
+    for dtype in (torch.float32, torch.bfloat16):                       # rows behind the last one stay as they were
+        more = torch.full((T + 300, N), 7.0, device=DEV, dtype=dtype)
+        k.int8_product(a, s, w, more[:T])
+        assert torch.equal(more[:T], want.to(dtype)) and (more[T:] == 7).all()
 
 
 @pytest.mark.parametrize("T,K,N", [(1, 8192, 2048), (40, 2048, 1500), (100, 1300, 640), (256, 4096, 512), (700, 900, 700)])
@@ -235,7 +239,8 @@ def test_every_cut_of_a_product_gives_the_same(T, K, N):
     a, s = _a(k, g, T, K)
     w = k.int8_weight(q, ws)
     want = _scaled(_sums(a, q, K), s, ws)
-    for plan in [("few", bq, splits, stages) for bq in (8, 32, 64) for splits in (1, 2, 3, 5, 8) for stages in (1, 2, 4)] + [("many", group) for group in (1, 3, 8)]:
+    for plan in [("few", bq, splits, stages) for bq in (8, 32, 64) for splits in (1, 2, 3, 5, 8) for stages in (1, 2, 4)] + \
+            [("few", 128, 1, stages) for stages in (1, 2, 4)] + [("many", group) for group in (1, 3, 8)]:
         out = torch.full((T, N), math.nan, device=DEV)
         k.int8_product(a, s, w, out, plan=plan)
         assert torch.equal(out, want), plan
@@ -327,6 +332,17 @@ def test_no_rows():
     k.int8_product(q, s, w, torch.empty(0, 64, device=DEV))
     k.int8_gated(q, s, gated, q, s, torch.empty(0, device=DEV))
     torch.cuda.synchronize()
+
+
+def test_tensors_of_two_devices_are_refused():
+    k = _kernels()
+    a, s = _a(k, _gen(1), 3, 64)
+    x, one = torch.ones(3, 64, device=DEV), torch.ones(64, device=DEV)
+    w = k.int8_weight(torch.ones(8, 64, dtype=torch.int8), torch.ones(8))
+    for call in (lambda: k.int8_product(a, s, w, torch.empty(3, 8, device=DEV)), lambda: k.quantize_rows(x, a, s.cpu()), lambda: k.rmsnorm_int8(x, one.cpu(), a, s, EPS),
+                 lambda: k.rmsnorm_int8(x, one, a.cpu(), s, EPS), lambda: k.gated_act_int8(x, a[:, :32].cpu(), s)):
+        with pytest.raises(k.KernelError, match="one device"):
+            call()
 
 
 def test_in_a_captured_graph_and_on_another_stream():

@@ -47,7 +47,7 @@ def test_plans_fit_the_kernels():
                     plan = k._int8_plan_of(T, w)
                     if plan[0] == "few":
                         _, bq, splits, stages = plan
-                        assert bq in (8, 32, 64) and 1 <= splits <= 8 and stages == 0 and not few_ended
+                        assert bq in (8, 32, 64, 128) and 1 <= splits <= (1 if bq == 128 else 8) and stages == 0 and not few_ended
                         assert splits == 1 or splits * ((channels + 127) // 128) * (2 if gated else 1) * ((T + bq - 1) // bq) <= 264
                         assert splits <= (width + 127) // 128
                         assert not gated or 2 * channels * T <= k.int8_gated_work(T, w)
