@@ -439,6 +439,7 @@ constexpr int kManyStages = 6;
 constexpr int kStagingBytes = kTileRows * 128;                               // 128 rows x 128 bytes, one to a group
 constexpr int kManySmem = kManyStages * kManyStageBytes + 2 * kStagingBytes + 256 + 4 * kTileN + 1024;      // barriers; the channels' scales of a tile
 static_assert(kManySmem <= 232448, "the pipeline does not fit into an SM's shared memory");
+static_assert(kTileN / 32 * kStagingBytes <= kManyStages * kManyStageBytes, "the last tile's chunks do not fit into the stages");
 
 // act(gate) * up of 32 channels, packed to bfloat16; n0: the first one's number.
 __device__ __forceinline__ void gated32(uint32_t* r, uint32_t* u, const float* gate_scales, const float* up_scales, float row_scale, int n0, const ManyParams& p,
@@ -575,7 +576,6 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         const int row = lane_group * 32 + lane;
         const int mine = static_cast<int>(threadIdx.x) - 64;
         const bool leader = (mine & 127) == 0;
-        uint8_t* stg = staging + group * kStagingBytes;
         auto group_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
         auto both_sync = [&]() { asm volatile("bar.sync 3, 256;" ::: "memory"); };
         auto sums_read = [&](int buf) {
@@ -606,9 +606,15 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             const uint32_t d = tmem + buf * kTileN + (static_cast<uint32_t>(lane_group * 32) << 16);
             constexpr int kCols = EPI == kStoreF32 || EPI == kAddF32 ? 32 : 64;      // output columns to a chunk: 128 bytes
             constexpr int kChunks = EPI == kGatedBF16 ? 2 : kTileN / kCols;
+            // The pipeline's stages are free once the sums of this CTA's last tile are complete: each chunk then has a place of its own there and waits for no
+            // earlier store.
+            const bool free_stages = i + n_workers >= n_tiles;
             for (int c = group; c < kChunks; c += 2) {
-                if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the last store has read the staging buffer
-                group_sync();
+                uint8_t* stg = free_stages ? smem + c * kStagingBytes : staging + group * kStagingBytes;
+                if (!free_stages) {
+                    if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the last store has read the staging buffer
+                    group_sync();
+                }
                 const bool last = c + 2 >= kChunks;
 #pragma unroll
                 for (int half = 0; half < kCols / 32; ++half) {
