@@ -84,6 +84,9 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+// the two halves of a barrier over the cluster's threads
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
@@ -236,6 +239,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const FewParams p) {
     fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_launch_dependents();
+    if (CLUSTER) cluster_arrive();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -360,6 +364,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const FewParams p) {
             }
         }
     } else {
+        cluster_wait();                           // every CTA of the cluster has begun: its shared memory may be written
         if (epilogue) {
 #pragma unroll 1
             for (int c = group_first; c < rows_here; c += Cfg::kGroups * kGroup) {

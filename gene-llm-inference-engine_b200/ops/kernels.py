@@ -1813,7 +1813,7 @@ class Int8Weight:
 
     def __init__(self, tiles: torch.Tensor, scales: torch.Tensor, channels: int, width: int, gated: bool):
         self.tiles, self.scales, self.channels, self.width, self.gated = tiles, scales, channels, width, gated
-        self.plans = {}      # rows -> the plan of a product of so many: sizes decide, once
+        self.plans, self.works = {}, {}      # rows -> the plan of a product of so many, and the scratch: sizes decide, once
 
 
 def int8_weight(q: torch.Tensor, scales: torch.Tensor, gated: bool = False) -> Int8Weight:
@@ -1921,7 +1921,12 @@ def int8_product(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: to
 
 def int8_gated_work(rows: int, w: Int8Weight) -> int:
     """32-bit values of the scratch that ``int8_gated`` needs for up to ``rows`` rows: both products of few rows, or h of all in bfloat16."""
-    return max(2 * w.channels * min(rows, _few_most(_int8_tiles(w))), rows * ((w.channels + 7) // 8 * 4))
+    need = w.works.get(rows)
+    if need is None:
+        if len(w.works) >= 4096:
+            w.works.clear()
+        need = w.works[rows] = max(2 * w.channels * min(rows, _few_most(_int8_tiles(w))), rows * ((w.channels + 7) // 8 * 4))
+    return need
 
 
 def int8_gated(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: torch.Tensor, out_scales: torch.Tensor, work: torch.Tensor,

@@ -69,6 +69,21 @@ def test_rows_that_lie_apart():
             _check_rows(q, s, want, m.double() / 127, D)
 
 
+def test_normed_and_activated_rows_that_lie_apart():
+    k = _kernels()
+    for D, ld in ((256, 260), (100, 333), (2048, 4096)):
+        g = _gen(D)
+        wide, w, more = _normal(g, 6, ld), torch.ones(D, device=DEV), _normal(g, 6, D)
+        keep, after = wide[:, D:].clone(), wide[:, :D] + more
+        q, s = _buffers(k, 6, D)
+        k.rmsnorm_int8(wide[:, :D], w, q, s, EPS, add=more)
+        assert torch.equal(wide[:, :D], after) and torch.equal(wide[:, D:], keep)
+        assert torch.equal(q[:, :D], _ints(after)[0]) and not q[:, D:].any()
+        both = _normal(g, 6, 2 * ld)[:, 3:3 + 2 * D]
+        k.gated_act_int8(both, q, s, "relu")
+        _near_ints(q, s, _act64(both[:, :D], both[:, D:], "relu", 0.0), 2 * 2.0 ** -9 + 2.0 ** -18)
+
+
 @pytest.mark.parametrize("add", [None, torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("D", WIDTHS)
 def test_normed_rows(D, add):

@@ -41,7 +41,7 @@ def test_plans_fit_the_kernels():
     for channels in (1, 128, 300, 2048, 6144, 16384, 128256):
         for width in (16, 128, 2048, 14336, k.INT8_WIDTH_MOST):
             for gated in (False, True):
-                w.channels, w.width, w.gated = channels, width, gated
+                w.channels, w.width, w.gated, w.works = channels, width, gated, {}
                 few_ended = False
                 for T in list(range(0, 70)) + [96, 128, 200, 256, 300, 512, 1000, 4096, 100000]:
                     plan = k._int8_plan_of(T, w)
