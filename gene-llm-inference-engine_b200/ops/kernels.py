@@ -1744,13 +1744,22 @@ def int8_width(values: int) -> int:
 
 
 def _here(name: str, first: torch.Tensor, *more: Optional[torch.Tensor]) -> None:
-    """All of them on the current device, on whose stream the kernel runs. (What is not on a device at all is refused by the checks of each.)"""
+    """All of them on the current device, on whose stream the kernel runs."""
     device = first.get_device()
-    if device >= 0 and device != torch._C._cuda_getDevice():
-        raise KernelError(f"{name}: a tensor is on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
     for t in more:
         if t is not None and t.get_device() != device:
-            raise KernelError(f"{name}: the tensors must be on one device (cuda:{device} and {t.device})")
+            raise KernelError(f"{name}: the tensors must be on one device ({first.device} and {t.device})")
+    if device < 0:
+        raise KernelError(f"{name}: the tensors must be on a CUDA device (there is no CPU path)")
+    if device != torch._C._cuda_getDevice():
+        raise KernelError(f"{name}: the tensors are on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
+def _ptr(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
+    """``_dev`` of a tensor that ``_here`` has looked at."""
+    if t.dtype is dtype and t.is_contiguous():
+        return t.data_ptr()
+    return _dev(t, name, dtype)
 
 
 def _rows_int8(name: str, kind: int, x: torch.Tensor, columns: int, out: torch.Tensor, scales: torch.Tensor, add=None, weight=None, eps: float = 0.0,
@@ -1762,8 +1771,8 @@ def _rows_int8(name: str, kind: int, x: torch.Tensor, columns: int, out: torch.T
         raise KernelError(f"{name}: out must be [T, int8_width(D)] and scales [T] for rows of D values")
     _here(name, x, out, scales, add, weight)
     code = lib().gi_rows_int8(kind, _rows_of(x, "x"), dtype_code(x.dtype), x.stride(0), 0 if add is None else _dev(add, "add"),
-                              0 if add is None else dtype_code(add.dtype), 0 if weight is None else _dev(weight, "weight", torch.float32), eps, act, limit,
-                              _dev(out, "out", torch.int8), width, _dev(scales, "scales", torch.float32), T, D, _stream())
+                              0 if add is None else dtype_code(add.dtype), 0 if weight is None else _ptr(weight, "weight", torch.float32), eps, act, limit,
+                              _ptr(out, "out", torch.int8), width, _ptr(scales, "scales", torch.float32), T, D, _stream())
     if code:
         check(code, name)
 
@@ -1882,7 +1891,7 @@ def _int8_plan_of(T: int, w: Int8Weight):
 
 
 def _few(a, a_scales, w, out, out_dtype, out_stride, accumulate, plan) -> None:
-    code = lib().gi_int8_product_few(_dev(a, "a", torch.int8), _dev(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
+    code = lib().gi_int8_product_few(_ptr(a, "a", torch.int8), _ptr(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
                                      w.scales.data_ptr(), w.channels, int(w.gated), out, out_dtype, out_stride, int(bool(accumulate)), plan[1], plan[2], plan[3],
                                      _tc_state(a.device).status.data_ptr(), _stream())
     if code:
@@ -1890,7 +1899,7 @@ def _few(a, a_scales, w, out, out_dtype, out_stride, accumulate, plan) -> None:
 
 
 def _many(a, a_scales, w, out, out_dtype, out_stride, accumulate, plan, act=0, limit=0.0, bias=0) -> None:
-    code = lib().gi_int8_product_many(_dev(a, "a", torch.int8), _dev(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
+    code = lib().gi_int8_product_many(_ptr(a, "a", torch.int8), _ptr(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
                                       w.scales.data_ptr(), w.channels, int(w.gated), act, limit, bias, out, out_dtype, out_stride, int(bool(accumulate)), plan[1],
                                       _tc_state(a.device).status.data_ptr(), _stream())
     if code:
@@ -1946,8 +1955,8 @@ def int8_gated(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: torc
     if work.numel() < int8_gated_work(T, w):
         raise KernelError(f"int8_gated: work must hold {int8_gated_work(T, w)} values")
     act, plan = ACTIVATIONS[activation], _int8_plan(T, w)
-    scratch, bias = _dev(work, "work", torch.float32), 0 if bias is None else _dev(bias, "bias", torch.float32)
-    q, scales = _dev(out, "out", torch.int8), _dev(out_scales, "out_scales", torch.float32)
+    scratch, bias = _ptr(work, "work", torch.float32), 0 if bias is None else _ptr(bias, "bias", torch.float32)
+    q, scales = _ptr(out, "out", torch.int8), _ptr(out_scales, "out_scales", torch.float32)
     if plan[0] == "few":                      # [gate; up] in 32 bits, then the activation with the rows
         _few(a, a_scales, w, scratch, F32, 2 * I, False, plan)
         code = lib().gi_rows_int8(2, scratch, F32, 2 * I, 0, 0, bias, 0.0, act, limit, q, width, scales, T, I, _stream())

@@ -101,7 +101,7 @@ def test_requests_do_not_see_each_other(case):
     assert all(len(g) == 20 for g in got)
 
 
-@pytest.mark.parametrize("case", ["c", "d", "w"])
+@pytest.mark.parametrize("case", ["c", "d", "w", "w3"])
 def test_generation_in_bfloat16(case):
     """The serving path: prompts in portions, decoded steps from graphs; twice the same, no wait gave up, and half the projections' bytes."""
     from geneinfer_b200 import Engine
@@ -145,3 +145,7 @@ def test_command_line():
     want = engine.generate([prompt], max_new_tokens=20 - len(prompt) + 1, temperature=0.0)[0]
     assert [int(t) for t in run.stdout.split()] == want
     assert "8-bit integers" in run.stderr
+    drafted = subprocess.run([sys.executable, os.path.join(ROOT, "bin", "gi_generate"), "--model", gf.model_dir("c"), "--weights", "int8", "--draft-model",
+                              gf.model_dir("c"), "--temperature", "0", "--steps", "20", "--no-echo", "--prompt-ids", " ".join(map(str, prompt))],
+                             stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
+    assert drafted.returncode == 0 and len(drafted.stdout.split()) == len(want), drafted.stderr
