@@ -185,6 +185,8 @@ struct FewParams {
 
 enum Epilogue : int { kStoreF32 = 0, kAddF32 = 1, kStoreBF16 = 2, kGatedBF16 = 3 };
 
+// Measured on B200 in a stream of launches, weights from memory: 8 rows 4096 -> 28672 18.4 us (6.4 TB/s), 64 rows 21.2; one token 8192 -> 2048 5.4 us, 2048 ->
+// 2048 3.5 (the hand-over from launch to launch, first operands and the cluster's exchange, about 3 us); 400 rows 4096 -> 4096 14.4.
 // Tiles of BQ rows. Tiles of 8 have one group of four epilogue warps, larger ones two that take turns (one token through 8192 -> 2048 with 16 rows to a
 // tile: 5.9 us with one group, 6.4 with two; 64 rows through 4096 -> 4096: 8.8 and 8.0).
 template <int BQ>
@@ -436,6 +438,8 @@ struct ManyParams {
     int* status;
 };
 
+// Measured on B200: 8192 x 14336 -> 4096 305 us (3,160 TOP/s), 4096 x 4096 -> 4096 48 to 52 (2,650 to 2,850: 256 tiles are 3.46 rounds of 74 pairs), 2048 x 2048 -> 2 x
+// 8192 with its activation 49. A CTA takes in 32 KB and its tensor core works 512 cycles for every 128 values of K: both are near their limits.
 constexpr int kManyThreads = 64 + 2 * 128;      // producer, MMA, two epilogue groups of four warps
 
 constexpr int kTileN = 256;                                                  // channels of a tile: 128 in each CTA's shared memory

@@ -1787,7 +1787,7 @@ def quantize_rows(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> N
 def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, eps: float,
                  add: Optional[torch.Tensor] = None) -> None:
     """x += add (``add`` [T, D] 32-bit or bfloat16, where given), then weight * (x / sqrt(mean(x^2) + eps)) of every row in 8 bits:
-    ``out`` [T, int8_width(D)] int8 and ``scales`` [T]. ``x`` [T, D] is the 32-bit residual stream. The integers are those of
+    ``out`` [T, int8_width(D)] int8 and ``scales`` [T]. ``x`` [T, D] is the 32-bit residual stream (its rows may lie apart). The integers are those of
     x * weight (the norm's factor is the row's: it goes into the scale)."""
     if x.dim() != 2 or weight.numel() != x.shape[1] or (add is not None and add.shape != x.shape):
         raise KernelError("rmsnorm_int8: shapes of x, weight and add do not agree")
@@ -1800,7 +1800,7 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, scale
 
 def gated_act_int8(gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, activation: str = "silu", limit: float = 0.0,
                    bias: Optional[torch.Tensor] = None) -> None:
-    """act(gate_up[:, :I]) * gate_up[:, I:], rounded to bfloat16, in 8 bits: ``gate_up`` [T, 2I] (32-bit or bfloat16), ``out``
+    """act(gate_up[:, :I]) * gate_up[:, I:], rounded to bfloat16, in 8 bits: ``gate_up`` [T, 2I] (32-bit or bfloat16; rows may lie apart), ``out``
     [T, int8_width(I)] int8, ``scales`` [T]; ``activation``, ``limit`` and ``bias`` [2I] as ``gated_act`` has them."""
     if gate_up.dim() != 2 or gate_up.shape[1] % 2 or (bias is not None and bias.numel() != gate_up.shape[1]):
         raise KernelError("gated_act_int8: gate_up must be [T, 2I] (and the bias [2I])")

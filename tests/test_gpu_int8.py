@@ -335,6 +335,36 @@ def test_a_feed_forward_of_them():
         assert torch.equal(out, stream + _scaled(_sums(hq, down[0], I), hs, down[1]))
 
 
+def test_offsets_beyond_32_bits():
+    """More than 2^31 values in rows, integers and results: the last rows come out as they do alone."""
+    k = _kernels()
+    g = _gen(12)
+    T, D = 131100, 16400                                                # rows: 2.15e9 values
+    x = torch.zeros(T, D, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = _normal(g, 3, D)
+    q, s = torch.empty(T, D, dtype=torch.int8, device=DEV), torch.empty(T, device=DEV)
+    k.quantize_rows(x, q, s)
+    want, m = _ints(x[-3:].float())
+    _check_rows(q[-3:], s[-3:], want, m.double() / 127, D)
+    assert (s[:-3] == 0).all() and not q[:4].any()
+    del x
+    w = k.int8_weight(*_weight(g, 130, D))
+    out = torch.empty(T, 130, device=DEV)
+    k.int8_product(q, s, w, out)
+    few = torch.empty(3, 130, device=DEV)
+    k.int8_product(q[-3:], s[-3:], w, few)
+    assert torch.equal(out[-3:], few) and (out[:-3] == 0).all()
+    del q, out
+    T, N = 70000, 32768                                                 # results: 2.29e9 values
+    a, s = _a(k, g, T, 64)
+    w = k.int8_weight(*_weight(g, N, 64))
+    out = torch.empty(T, N, dtype=torch.bfloat16, device=DEV)
+    k.int8_product(a, s, w, out)
+    few = torch.empty(5, N, dtype=torch.bfloat16, device=DEV)
+    k.int8_product(a[-5:], s[-5:], w, few)
+    assert torch.equal(out[-5:], few)
+
+
 def test_no_rows():
     k = _kernels()
     g = _gen(2)
