@@ -85,9 +85,11 @@ __device__ __forceinline__ float4 plus(const float4 a, const float4 b) {
 }
 
 // N groups of four values of a row, i0, i0 + G, ..: v of each, and what the squares add to ss. All loads stand before the first
-// store of a row that is written back (nothing tells the compiler that they do not overlap). `first`: the norm's addition is done.
+// store of a row that is written back (nothing tells the compiler that they do not overlap). `first`: the norm's addition is done. Only the first
+// `live` groups have columns for any thread: activations of the others are skipped, by all threads at once (14,336 values in 512 x 8 groups of four: an
+// eighth). Their loads are not: they are masked anyway, and a branch between loads keeps them from being under way together.
 template <int KIND, typename TX, typename TA, bool VEC, int G, int N>
-__device__ __forceinline__ void values(const RowsParams& p, long long row, int i0, const float4* w, float factor, bool first, float& ss, float4* v) {
+__device__ __forceinline__ void values(const RowsParams& p, long long row, int i0, int live, const float4* w, float factor, bool first, float& ss, float4* v) {
     const TX* x = static_cast<const TX*>(p.x) + row * p.ldx;
 #pragma unroll
     for (int k = 0; k < N; ++k) v[k] = load4<VEC, G>(x, i0 + k * G, p.D);
@@ -106,6 +108,7 @@ __device__ __forceinline__ void values(const RowsParams& p, long long row, int i
             auto h = [&](float g, float up) { return gated_value_bf16<decltype(act)::value>(g, up, p.limit); };
 #pragma unroll
             for (int k = 0; k < N; ++k) {
+                if (k >= live) continue;
                 const __nv_bfloat162 lo = __floats2bfloat162_rn(h(v[k].x, u[k].x), h(v[k].y, u[k].y));
                 const __nv_bfloat162 hi = __floats2bfloat162_rn(h(v[k].z, u[k].z), h(v[k].w, u[k].w));
                 const uint32_t a = *reinterpret_cast<const uint32_t*>(&lo), b = *reinterpret_cast<const uint32_t*>(&hi);
@@ -197,6 +200,7 @@ rows_int8_kernel(const RowsParams p) {
     __shared__ float part_s[2][32];
     const int t = threadIdx.x % G;
     const long long row = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / G;
+    const int live = (p.width + 4 * G - 1) / (4 * G);
     if (threadIdx.x == 0) timeline_record(kTlInt8Rows, 0);
     pdl_launch_dependents();
     float4 w[kBatch];
@@ -214,7 +218,7 @@ rows_int8_kernel(const RowsParams p) {
 #pragma unroll
     for (int k = 0; k < V; k += kBatch) {
         if (!kEarly) weights(k);
-        values<KIND, TX, TA, VEC, G, kBatch>(p, row, t + k * G, w, 1.f, true, ss, v + k);
+        values<KIND, TX, TA, VEC, G, kBatch>(p, row, t + k * G, live - k, w, 1.f, true, ss, v + k);
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) m = top_bits(v[k], m);
@@ -226,7 +230,7 @@ rows_int8_kernel(const RowsParams p) {
 #pragma unroll
         for (int k = 0; k < V; k += kBatch) {
             if (!kEarly) weights(k);
-            values<KIND, TX, TA, VEC, G, kBatch>(p, row, t + k * G, w, factor, false, ss, v + k);
+            values<KIND, TX, TA, VEC, G, kBatch>(p, row, t + k * G, live - k, w, factor, false, ss, v + k);
         }
 #pragma unroll
         for (int k = 0; k < V; ++k) m = top_bits(v[k], m);
@@ -253,7 +257,7 @@ wide_rows_int8_kernel(const RowsParams p) {
     float4 v[1], w[1];
     auto pass = [&](int i, bool first, float& squares) {
         w[0] = KIND == kRowsNorm ? load4<false, 1024>(p.weight, i, p.D) : make_float4(0.f, 0.f, 0.f, 0.f);
-        values<KIND, TX, TA, false, 1024, 1>(p, row, i, w, factor, first, squares, v);
+        values<KIND, TX, TA, false, 1024, 1>(p, row, i, 1, w, factor, first, squares, v);
     };
     const int groups = (p.width + 4095) / 4096 * 1024;
     for (int i = threadIdx.x; i < groups; i += 1024) { pass(i, true, ss); m = top_bits(v[0], m); }

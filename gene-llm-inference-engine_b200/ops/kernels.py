@@ -1762,17 +1762,25 @@ def _ptr(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
     return _dev(t, name, dtype)
 
 
+def _strided(t: torch.Tensor, name: str, row: int) -> Tuple[int, int]:
+    """Address of a matrix whose rows may lie apart, and how far (rows of ``row`` values)."""
+    if t.is_contiguous():
+        return t.data_ptr(), row
+    return _rows_of(t, name), t.stride(0)
+
+
 def _rows_int8(name: str, kind: int, x: torch.Tensor, columns: int, out: torch.Tensor, scales: torch.Tensor, add=None, weight=None, eps: float = 0.0,
                act: int = 0, limit: float = 0.0) -> None:
-    T, D = x.shape
-    D //= columns
+    T, row = x.shape
+    D = row // columns
     width = (D + 15) // 16 * 16
     if D < 1 or out.shape != (T, width) or scales.numel() != T:
         raise KernelError(f"{name}: out must be [T, int8_width(D)] and scales [T] for rows of D values")
     _here(name, x, out, scales, add, weight)
-    code = lib().gi_rows_int8(kind, _rows_of(x, "x"), dtype_code(x.dtype), x.stride(0), 0 if add is None else _dev(add, "add"),
-                              0 if add is None else dtype_code(add.dtype), 0 if weight is None else _ptr(weight, "weight", torch.float32), eps, act, limit,
-                              _ptr(out, "out", torch.int8), width, _ptr(scales, "scales", torch.float32), T, D, _stream())
+    at, stride = _strided(x, "x", row)
+    extra, extra_type = (0, 0) if add is None else (_dev(add, "add"), dtype_code(add.dtype))
+    code = lib().gi_rows_int8(kind, at, dtype_code(x.dtype), stride, extra, extra_type, 0 if weight is None else _ptr(weight, "weight", torch.float32),
+                              eps, act, limit, _ptr(out, "out", torch.int8), width, _ptr(scales, "scales", torch.float32), T, D, _stream())
     if code:
         check(code, name)
 
@@ -1925,7 +1933,8 @@ def int8_product(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: to
     if accumulate and out.dtype is not torch.float32:
         raise KernelError("int8_product: accumulation needs a 32-bit output")
     plan = plan or _int8_plan(T, w)
-    (_few if plan[0] == "few" else _many)(a, a_scales, w, _rows_of(out, "out"), dtype_code(out.dtype), out.stride(0), accumulate, plan)
+    at, stride = _strided(out, "out", w.channels)
+    (_few if plan[0] == "few" else _many)(a, a_scales, w, at, dtype_code(out.dtype), stride, accumulate, plan)
 
 
 def int8_gated_work(rows: int, w: Int8Weight) -> int:
