@@ -42,7 +42,7 @@ def _check_rows(q, scales, want_q, want_scales, D):
     assert torch.allclose(scales.double(), want_scales, rtol=8 * 2.0 ** -24, atol=0)
 
 
-WIDTHS = [1, 3, 16, 127, 512, 513, 2048, 2050, 4096, 5000, 8192, 9001, 16384, 20480, 32768, 40001]
+WIDTHS = [1, 3, 8, 16, 20, 127, 512, 513, 1000, 2048, 2050, 4096, 4100, 5000, 8192, 9001, 16384, 20480, 32768, 40001]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -388,6 +388,42 @@ def test_tensors_of_two_devices_are_refused():
                  lambda: k.rmsnorm_int8(x, one, a.cpu(), s, EPS), lambda: k.gated_act_int8(x, a[:, :32].cpu(), s)):
         with pytest.raises(k.KernelError, match="one device"):
             call()
+
+
+def test_two_streams_at_once():
+    """Nothing is shared between calls: products, rows and gated halves of two streams beside each other give what they give alone."""
+    k = _kernels()
+    g = _gen(21)
+    jobs = []
+    for T, K, N in ((5, 4096, 1024), (700, 1024, 1500), (64, 2048, 4096), (300, 512, 8000)):
+        w, pair = k.int8_weight(*_weight(g, N, K)), k.int8_weight(*_weight(g, 2 * N, K), gated=True)
+        x = _normal(g, T, K)
+        a, s = _buffers(k, T, K)
+        h, hs = _buffers(k, T, N)
+        jobs.append((x, a, s, w, pair, h, hs, torch.empty(k.int8_gated_work(T, pair), device=DEV), torch.empty(T, N, device=DEV)))
+
+    def go(x, a, s, w, pair, h, hs, work, out):
+        k.rmsnorm_int8(x, torch.ones(x.shape[1], device=DEV), a, s, EPS)
+        k.int8_product(a, s, w, out)
+        k.int8_gated(a, s, pair, h, hs, work)
+
+    alone = []
+    for job in jobs:
+        go(*job)
+        torch.cuda.synchronize()
+        alone.append([t.clone() for t in (job[1], job[2], job[5], job[6], job[8])])
+    for job in jobs:
+        for t in (job[1], job[2], job[5], job[6], job[8]):
+            t.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for i, job in enumerate(jobs):
+            with torch.cuda.stream(streams[i % 2]):
+                go(*job)
+    torch.cuda.synchronize()
+    for job, want in zip(jobs, alone):
+        assert all(torch.equal(t, u) for t, u in zip((job[1], job[2], job[5], job[6], job[8]), want))
 
 
 def test_in_a_captured_graph_and_on_another_stream():
