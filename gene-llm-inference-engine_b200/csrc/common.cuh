@@ -138,13 +138,16 @@ __device__ __forceinline__ float sigmoid_times(float z, float g) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
     return g * r;
 }
+// (a NaN stays one, where fminf and fmaxf would take the other value)
+__device__ __forceinline__ float no_more_than(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float no_less_than(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 template <int ACT>
 __device__ __forceinline__ float gated_value_bf16(float g, float u, float limit) {
-    if (ACT == kActRelu) return fmaxf(g, 0.f) * u;
+    if (ACT == kActRelu) return no_less_than(g, 0.f) * u;
     if (ACT == kActGeluTanh) return sigmoid_times(1.5957691216057308f * (g + 0.044715f * g * g * g), g) * u;
     if (ACT == kActCappedSwish) {
-        g = fminf(g, limit);
-        u = fminf(fmaxf(u, -limit), limit);
+        g = no_more_than(g, limit);
+        u = no_more_than(no_less_than(u, -limit), limit);
         return sigmoid_times(1.702f * g, g) * (u + 1.0f);
     }
     return sigmoid_times(g, g) * u;

@@ -12,7 +12,8 @@
 //
 // What is not finite: the largest |v| is kept as the bits of its absolute value, an integer that orders infinities and NaN above
 // every number, so that one of them anywhere in a row shows: such a row gets the scale NaN and zeros, and every product with it is
-// NaN. A norm whose squares (or products with the weights) leave the range of 32 bits is taken again from values 2^-80 times as large.
+// NaN. A norm whose squares (or products with the weights) leave the range of 32 bits is taken again from values 2^-80 times as large, one whose squares
+// vanish beside an eps that is as small from values 2^80 times as large.
 // Rows whose largest |v| is below 2^-100 count as zero (scale 0): 127 / m would leave that range at the other end.
 #include "common.cuh"
 
@@ -34,7 +35,8 @@ struct RowsParams {
 };
 
 constexpr unsigned kInfBits = 0x7f800000u, kLeastBits = 0x0d800000u;      // 2^-100
-constexpr float kDown = 8.271806125530277e-25f;                           // 2^-80
+constexpr float kDown = 8.271806125530277e-25f, kUp = 1.2089258196146292e24f;      // 2^-80, 2^80
+constexpr float kLeastSquares = 7.888609052210118e-31f, kLeastEps = 7.52316384526264e-37f;      // 2^-100, 2^-120
 
 // Four values of a row to a thread. VEC: neighbours, at 4 i, one access of 16 (8) bytes; rows of any width and alignment: at i, i + G, i + 2 G,
 // i + 3 G, so that the lanes of a warp stay side by side (2048 rows of 2050: 43 us with four neighbours one by one, 15.7 with these; of 2048: 9).
@@ -158,6 +160,12 @@ __device__ __forceinline__ unsigned top_bits(const float4 v, unsigned m) {
     return max(m, max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
 }
 
+// What the values of a norm have to be multiplied by before it is taken again; 1: nothing.
+__device__ __forceinline__ float other_factor(unsigned m, float ss, float eps) {
+    if (m >= kInfBits || !(ss < __uint_as_float(kInfBits))) return kDown;
+    return ss < kLeastSquares && eps < kLeastEps && m > 0 ? kUp : 1.f;
+}
+
 // The row's largest |v| and sum of squares over the G threads that share it.
 template <int G, int KIND>
 __device__ __forceinline__ void meet(unsigned& m, float& ss, unsigned* part_m, float* part_s) {
@@ -223,8 +231,7 @@ rows_int8_kernel(const RowsParams p) {
 #pragma unroll
     for (int k = 0; k < V; ++k) m = top_bits(v[k], m);
     meet<G, KIND>(m, ss, part_m[0], part_s[0]);
-    if (KIND == kRowsNorm && (m >= kInfBits || !(ss < __uint_as_float(kInfBits)))) {
-        factor = kDown;
+    if (KIND == kRowsNorm && (factor = other_factor(m, ss, p.eps)) != 1.f) {
         m = 0;
         ss = 0.f;
 #pragma unroll
@@ -262,8 +269,7 @@ wide_rows_int8_kernel(const RowsParams p) {
     const int groups = (p.width + 4095) / 4096 * 1024;
     for (int i = threadIdx.x; i < groups; i += 1024) { pass(i, true, ss); m = top_bits(v[0], m); }
     meet<1024, KIND>(m, ss, part_m[0], part_s[0]);
-    if (KIND == kRowsNorm && (m >= kInfBits || !(ss < __uint_as_float(kInfBits)))) {
-        factor = kDown;
+    if (KIND == kRowsNorm && (factor = other_factor(m, ss, p.eps)) != 1.f) {
         m = 0;
         ss = 0.f;
         for (int i = threadIdx.x; i < groups; i += 1024) { pass(i, false, ss); m = top_bits(v[0], m); }

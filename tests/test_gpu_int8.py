@@ -133,6 +133,23 @@ def test_normed_rows_of_extreme_values():
             assert float((got - want).abs().max()) <= float(want.abs().max()) / 127 * 0.5001, row
 
 
+def test_normed_rows_without_an_eps():
+    """Rows whose squares vanish in 32 bits, with nothing beside them under the root."""
+    k = _kernels()
+    for D in (64, 2048, 33000):
+        g = _gen(D)
+        w = 0.5 + torch.rand(D, generator=g, device=DEV)
+        for eps in (0.0, 1e-38):
+            x = _normal(g, 4, D) * torch.tensor([[1.0], [1e-18], [1e-24], [0.0]], device=DEV)
+            q, s = _buffers(k, 4, D)
+            k.rmsnorm_int8(x, w, q, s, eps)
+            for row in range(3):
+                want = x[row].double() * w.double() / (x[row].double().square().mean() + eps).sqrt()
+                got = q[row, :D].double() * s[row].double()
+                assert float((got - want).abs().max()) <= float(want.abs().max()) / 127 * 0.501, (D, eps, row)
+            assert float(s[3]) == 0 and not q[3].any()
+
+
 def test_rows_of_extreme_values():
     k = _kernels()
     for dtype in (torch.float32, torch.bfloat16):
@@ -192,6 +209,12 @@ def test_activated_rows_of_extreme_values():
     q, s = _buffers(k, 4, 640)
     k.gated_act_int8(x, q, s, "silu")
     assert torch.isnan(s[:2]).all() and not q[:3].any() and float(s[2]) == 0 and float(s[3]) > 0
+    for activation in ("silu", "relu", "gelu_tanh", "capped_swish"):      # a NaN in either half, and none is lost to a bound
+        for at in (9, 640 + 9):
+            x = _normal(_gen(4), 2, 2 * 640)
+            x[0, at] = math.nan
+            k.gated_act_int8(x, q[:2], s[:2], activation, 2.0)
+            assert math.isnan(float(s[0])) and not q[0].any() and float(s[1]) > 0, (activation, at)
 
 
 def _weight(g, N, K):
