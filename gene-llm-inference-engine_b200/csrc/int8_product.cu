@@ -918,3 +918,19 @@ extern "C" int gi_int8_product_many(const void* a, const float* a_scales, int T,
     return gi::dispatch(gi::int8_many_impl, a, a_scales, T, width, tiles, w_scales, N, gated, act, limit, bias, out, out_dtype, ldo, accumulate, group_t,
                         status, stream);
 }
+
+extern "C" int gi_rows_int8(int kind, const void* x, int x_dtype, long long ldx, const void* add, int add_dtype, const float* weight, float eps, int act,
+                            float limit, void* q, int width, float* scales, int T, int D, void* stream);
+
+// act(gate) * up of a gated pair of N channels each, in 8 bits: q [T, out_width] and scales [T]. Few rows (bq > 0: see gi_int8_product_few) leave [gate; up] in `work`
+// as 32-bit [T, 2 N] for the activation with the rows; many (bq 0, `splits` the tiles of rows walked together) act(gate) * up as bfloat16, rows of whole 16 bytes.
+extern "C" int gi_int8_gated(const void* a, const float* a_scales, int T, int width, const void* tiles, const float* w_scales, int N, int act, float limit,
+                             const float* bias, void* work, void* q, int out_width, float* scales, int bq, int splits, int stages, void* status, void* stream) {
+    if (bq > 0) {
+        const int code = gi_int8_product_few(a, a_scales, T, width, tiles, w_scales, N, 1, work, gi::kF32, 2ll * N, 0, bq, splits, stages, status, stream);
+        return code ? code : gi_rows_int8(2, work, gi::kF32, 2ll * N, nullptr, 0, bias, 0.f, act, limit, q, out_width, scales, T, N, stream);
+    }
+    const long long row = (N + 7ll) / 8 * 8;
+    const int code = gi_int8_product_many(a, a_scales, T, width, tiles, w_scales, N, 1, act, limit, bias, work, gi::kBF16, row, 0, splits, status, stream);
+    return code ? code : gi_rows_int8(0, work, gi::kBF16, row, nullptr, 0, nullptr, 0.f, 0, 0.f, q, out_width, scales, T, N, stream);
+}

@@ -1900,15 +1900,15 @@ def _int8_plan_of(T: int, w: Int8Weight):
 
 def _few(a, a_scales, w, out, out_dtype, out_stride, accumulate, plan) -> None:
     code = lib().gi_int8_product_few(_ptr(a, "a", torch.int8), _ptr(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
-                                     w.scales.data_ptr(), w.channels, int(w.gated), out, out_dtype, out_stride, int(bool(accumulate)), plan[1], plan[2], plan[3],
+                                     w.scales.data_ptr(), w.channels, 0, out, out_dtype, out_stride, int(bool(accumulate)), plan[1], plan[2], plan[3],
                                      _tc_state(a.device).status.data_ptr(), _stream())
     if code:
         check(code, "int8_product")
 
 
-def _many(a, a_scales, w, out, out_dtype, out_stride, accumulate, plan, act=0, limit=0.0, bias=0) -> None:
+def _many(a, a_scales, w, out, out_dtype, out_stride, accumulate, plan) -> None:
     code = lib().gi_int8_product_many(_ptr(a, "a", torch.int8), _ptr(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
-                                      w.scales.data_ptr(), w.channels, int(w.gated), act, limit, bias, out, out_dtype, out_stride, int(bool(accumulate)), plan[1],
+                                      w.scales.data_ptr(), w.channels, 0, 0, 0.0, 0, out, out_dtype, out_stride, int(bool(accumulate)), plan[1],
                                       _tc_state(a.device).status.data_ptr(), _stream())
     if code:
         check(code, "int8_product")
@@ -1963,15 +1963,11 @@ def int8_gated(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: torc
         raise KernelError(f"int8_gated: unknown activation '{activation}' (known: {', '.join(sorted(ACTIVATIONS))})")
     if work.numel() < int8_gated_work(T, w):
         raise KernelError(f"int8_gated: work must hold {int8_gated_work(T, w)} values")
-    act, plan = ACTIVATIONS[activation], _int8_plan(T, w)
-    scratch, bias = _ptr(work, "work", torch.float32), 0 if bias is None else _ptr(bias, "bias", torch.float32)
-    q, scales = _ptr(out, "out", torch.int8), _ptr(out_scales, "out_scales", torch.float32)
-    if plan[0] == "few":                      # [gate; up] in 32 bits, then the activation with the rows
-        _few(a, a_scales, w, scratch, F32, 2 * I, False, plan)
-        code = lib().gi_rows_int8(2, scratch, F32, 2 * I, 0, 0, bias, 0.0, act, limit, q, width, scales, T, I, _stream())
-    else:
-        stride = (I + 7) // 8 * 8             # whole 16 bytes
-        _many(a, a_scales, w, scratch, BF16, stride, False, plan, act, limit, bias)
-        code = lib().gi_rows_int8(0, scratch, BF16, stride, 0, 0, 0, 0.0, 0, 0.0, q, width, scales, T, I, _stream())
+    plan = _int8_plan(T, w)
+    few = plan[0] == "few"
+    code = lib().gi_int8_gated(_ptr(a, "a", torch.int8), _ptr(a_scales, "a_scales", torch.float32), T, w.width, w.tiles.data_ptr(), w.scales.data_ptr(), I,
+                               ACTIVATIONS[activation], limit, 0 if bias is None else _ptr(bias, "bias", torch.float32), _ptr(work, "work", torch.float32),
+                               _ptr(out, "out", torch.int8), width, _ptr(out_scales, "out_scales", torch.float32), plan[1] if few else 0,
+                               plan[2] if few else plan[1], plan[3] if few else 0, _tc_state(a.device).status.data_ptr(), _stream())
     if code:
         check(code, "int8_gated")

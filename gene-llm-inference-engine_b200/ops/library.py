@@ -146,6 +146,8 @@ _SIGNATURES = {
                             c_int, c_void_p, c_void_p],
     "gi_int8_product_many": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_int,
                              c_longlong, c_int, c_int, c_void_p, c_void_p],
+    "gi_int8_gated": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                      c_int, c_int, c_int, c_void_p, c_void_p],
     "gi_sample": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
 }
 
