@@ -428,7 +428,7 @@ struct ManyParams {
     const float* bias;       // gated: [2 N] or null
     void* out;
     long long ldo;
-    int plain_stores;        // the output's rows are not whole 16 bytes: no TMA
+    int plain_stores;        // the output's rows do not start on or do not end with whole 16 bytes: no TMA
     int T, N;                // N: output channels
     int total_kb;
     int tiles_t, tiles_n;    // of 256 rows, of 256 channels (gated: 128 gates and their ups)
@@ -883,7 +883,8 @@ int int8_many_impl(const void* a, const float* a_scales, int T, int width, const
     p.status = static_cast<int*>(status);
     GI_REQUIRE(static_cast<long long>(p.tiles_t) * p.tiles_n < (1ll << 30), "int8_product: too many tiles");
     const int elt = out_dtype == kBF16 ? 2 : 4;
-    p.plain_stores = ldo * elt % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0;
+    // (a TMA store writes whole 16 bytes: it would reach into what lies behind a row's last channel. Behind a gated row there is scratch.)
+    p.plain_stores = ldo * elt % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0 || (!gated && static_cast<long long>(N) * elt % 16 != 0);
     const long long weight_rows = static_cast<long long>((N + kTileRows - 1) / kTileRows) * (gated ? 2 : 1) * p.total_kb * kTileRows;
     GI_REQUIRE(weight_rows < (1ll << 31), "int8_product: the weights are too large");
     CUtensorMap map_a, map_w, map_o{};

@@ -269,6 +269,28 @@ def test_product(T, K, N):
         assert torch.equal(more[:T], want.to(dtype)) and (more[T:] == 7).all()
 
 
+@pytest.mark.parametrize("T", [5, 100, 1000])
+def test_nothing_behind_a_rows_last_channel_is_written(T):
+    """Rows that lie whole 16 bytes apart and end within them: a store of whole pieces would reach into what lies behind."""
+    k = _kernels()
+    g = _gen(T)
+    for N in (333, 334, 335, 336, 1001, 2049):
+        q, ws = _weight(g, N, 200)
+        a, s = _a(k, g, T, 200)
+        w = k.int8_weight(q, ws)
+        want = _scaled(_sums(a, q, 200), s, ws)
+        for dtype in (torch.float32, torch.bfloat16):
+            wide = torch.full((T, (N + 15) // 16 * 16), 7.0, device=DEV, dtype=dtype)
+            for plan in (None, ("many", 1)):
+                k.int8_product(a, s, w, wide[:, :N], plan=plan)
+                assert torch.equal(wide[:, :N], want.to(dtype)) and (wide[:, N:] == 7).all(), (N, dtype, plan)
+        wide = torch.full((T, (N + 15) // 16 * 16), 7.0, device=DEV)
+        for plan in (None, ("many", 1)):
+            before = wide[:, :N].clone()
+            k.int8_product(a, s, w, wide[:, :N], accumulate=True, plan=plan)
+            assert torch.equal(wide[:, :N], before + want) and (wide[:, N:] == 7).all(), (N, plan)
+
+
 @pytest.mark.parametrize("T,K,N", [(1, 8192, 2048), (40, 2048, 1500), (100, 1300, 640), (256, 4096, 512), (700, 900, 700)])
 def test_every_cut_of_a_product_gives_the_same(T, K, N):
     k = _kernels()
