@@ -180,6 +180,7 @@ struct FewParams {
     int gated;
     int total_kb, kb_per_split, splits;
     int stages;
+    int w_constant;          // no kernel that may still be running writes the tiles: the first ones may be asked for before the wait
     int* status;
 };
 
@@ -258,12 +259,16 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const FewParams p) {
                     load_tile(smem_addr(smem + s * Cfg::kStageBytes + kKb * kTileBytes + j * BQ * kRowBytes), &map_a,
                               (kb_begin + i * kKb + j) * kRowBytes, tile_t * BQ, smem_addr(&bars[s]));
             };
-            // the weights belong to no earlier kernel: their first tiles are asked for before the wait for the kernels ahead
+            // constant weights: their first tiles are asked for before the wait for the kernels ahead
             const int early = min(n_steps, stages);
-            for (int i = 0; i < early; ++i) load_w(i, i);
+            if (p.w_constant)
+                for (int i = 0; i < early; ++i) load_w(i, i);
             pdl_wait();
             timeline_record(kTlInt8ProductFew, 1);
-            for (int i = 0; i < early; ++i) load_a(i, i);
+            for (int i = 0; i < early; ++i) {
+                if (!p.w_constant) load_w(i, i);
+                load_a(i, i);
+            }
             int issued = early, s = 0, parity = 0;
             for (int i = early; i < n_steps; ++i) {      // (early == stages, where there are more steps)
                 if (!bar_wait(smem_addr(&bars[8 + s]), parity, gave_up, p.status, kErrProducer)) break;
@@ -345,7 +350,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const FewParams p) {
     const bool adds = EPI == kAddF32 && epilogue && channel_there;
     if (epilogue) {
         pdl_wait();
-        if (channel_there) w_scale = __ldg(p.w_scales + channel);
+        if (channel_there) w_scale = __ldcg(p.w_scales + channel);
         for (int t = threadIdx.x - 64; t < rows_here; t += 128 * Cfg::kGroups) row_scales[t] = __ldcg(p.a_scales + tile_t * BQ + t);
         if (adds) load_old(first + group_first, n_mine - group_first, old);          // while the products run
         ok = bar_wait(smem_addr(&bars[16]), 0, gave_up, p.status, kErrEpilogue);
@@ -461,7 +466,7 @@ __device__ __forceinline__ void gated32(uint32_t* r, uint32_t* u, const float* g
     if (p.bias != nullptr) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-            const float bg = n0 + j < p.N ? __ldg(p.bias + n0 + j) : 0.f, bu = n0 + j < p.N ? __ldg(p.bias + p.N + n0 + j) : 0.f;
+            const float bg = n0 + j < p.N ? p.bias[n0 + j] : 0.f, bu = n0 + j < p.N ? p.bias[p.N + n0 + j] : 0.f;
             r[j] = __float_as_uint(__fadd_rn(__uint_as_float(r[j]), bg));
             u[j] = __float_as_uint(__fadd_rn(__uint_as_float(u[j]), bu));
         }
@@ -603,7 +608,7 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             const int n0 = EPI == kGatedBF16 ? tile_n * kTileRows : tile_n * kTileN;
             const bool up = EPI == kGatedBF16 && mine >= kTileRows;
             const int ch = n0 + (up ? mine - kTileRows : mine);
-            const float mine_scale = ch < p.N ? __ldg(p.w_scales + (up ? p.N : 0) + ch) : 0.f;
+            const float mine_scale = ch < p.N ? __ldcg(p.w_scales + (up ? p.N : 0) + ch) : 0.f;
             bar_wait(smem_addr(&bars[2 * kStages + buf]), (n >> 1) & 1, gave_up, p.status, kErrEpilogue);
             both_sync();                               // nobody reads the last tile's scales any more
             scales[mine] = mine_scale;
@@ -811,7 +816,7 @@ int check_operands(const void* a, int T, int width, const void* tiles, int N, co
 }
 
 int int8_few_impl(const void* a, const float* a_scales, int T, int width, const void* tiles, const float* w_scales, int N, int gated, void* out,
-                  int out_dtype, long long ldo, int accumulate, int bq, int splits, int stages, void* status, void* stream) {
+                  int out_dtype, long long ldo, int accumulate, int bq, int splits, int stages, int w_constant, void* status, void* stream) {
     if (T == 0) return 0;
     if (int bad = check_operands(a, T, width, tiles, N, status)) return bad;
     GI_REQUIRE(out_dtype == kF32 || out_dtype == kBF16, "int8_product: unsupported dtype code %d", out_dtype);
@@ -826,6 +831,7 @@ int int8_few_impl(const void* a, const float* a_scales, int T, int width, const 
     p.T = T;
     p.N = N;
     p.gated = gated;
+    p.w_constant = w_constant;
     p.total_kb = (width + kRowBytes - 1) / kRowBytes;
     p.kb_per_split = (p.total_kb + splits - 1) / splits;
     p.splits = (p.total_kb + p.kb_per_split - 1) / p.kb_per_split;      // (no range is empty)
@@ -906,10 +912,13 @@ int int8_many_impl(const void* a, const float* a_scales, int T, int width, const
 GI_TIMELINE_SETTER(gi_timeline_set_int8_product)
 
 // Few rows: tiles of bq rows of a [T, width], K in `splits` ranges (one cluster), `stages` stages of the pipeline (0: chosen). `gated`: the weights are a gated
-// pair of N channels each, out [T, 2 N] = [gate; up]. out[t, n] at t * ldo + n.
+// pair of N channels each, out [T, 2 N] = [gate; up]. out[t, n] at t * ldo + n. w_constant: no launch before this one that may still be running writes the
+// tiles, so that the first ones may be asked for before the wait for them.
 extern "C" int gi_int8_product_few(const void* a, const float* a_scales, int T, int width, const void* tiles, const float* w_scales, int N, int gated,
-                                   void* out, int out_dtype, long long ldo, int accumulate, int bq, int splits, int stages, void* status, void* stream) {
-    return gi::dispatch(gi::int8_few_impl, a, a_scales, T, width, tiles, w_scales, N, gated, out, out_dtype, ldo, accumulate, bq, splits, stages, status, stream);
+                                   void* out, int out_dtype, long long ldo, int accumulate, int bq, int splits, int stages, int w_constant, void* status,
+                                   void* stream) {
+    return gi::dispatch(gi::int8_few_impl, a, a_scales, T, width, tiles, w_scales, N, gated, out, out_dtype, ldo, accumulate, bq, splits, stages, w_constant,
+                        status, stream);
 }
 
 // Many rows: tiles of 256 rows x 256 channels, `group_t` tiles of rows walked together. `gated`: out [T, N] = act(gate) * up, bfloat16; `bias` [2 N] or null.
@@ -921,17 +930,18 @@ extern "C" int gi_int8_product_many(const void* a, const float* a_scales, int T,
 }
 
 extern "C" int gi_rows_int8(int kind, const void* x, int x_dtype, long long ldx, const void* add, int add_dtype, const float* weight, float eps, int act,
-                            float limit, void* q, int width, float* scales, int T, int D, void* stream);
+                            float limit, void* q, int width, float* scales, int T, int D, int w_constant, void* stream);
 
 // act(gate) * up of a gated pair of N channels each, in 8 bits: q [T, out_width] and scales [T]. Few rows (bq > 0: see gi_int8_product_few) leave [gate; up] in `work`
 // as 32-bit [T, 2 N] for the activation with the rows; many (bq 0, `splits` the tiles of rows walked together) act(gate) * up as bfloat16, rows of whole 16 bytes.
 extern "C" int gi_int8_gated(const void* a, const float* a_scales, int T, int width, const void* tiles, const float* w_scales, int N, int act, float limit,
-                             const float* bias, void* work, void* q, int out_width, float* scales, int bq, int splits, int stages, void* status, void* stream) {
+                             const float* bias, void* work, void* q, int out_width, float* scales, int bq, int splits, int stages, int w_constant, void* status,
+                             void* stream) {
     if (bq > 0) {
-        const int code = gi_int8_product_few(a, a_scales, T, width, tiles, w_scales, N, 1, work, gi::kF32, 2ll * N, 0, bq, splits, stages, status, stream);
-        return code ? code : gi_rows_int8(2, work, gi::kF32, 2ll * N, nullptr, 0, bias, 0.f, act, limit, q, out_width, scales, T, N, stream);
+        const int code = gi_int8_product_few(a, a_scales, T, width, tiles, w_scales, N, 1, work, gi::kF32, 2ll * N, 0, bq, splits, stages, w_constant, status, stream);
+        return code ? code : gi_rows_int8(2, work, gi::kF32, 2ll * N, nullptr, 0, bias, 0.f, act, limit, q, out_width, scales, T, N, 0, stream);
     }
     const long long row = (N + 7ll) / 8 * 8;
     const int code = gi_int8_product_many(a, a_scales, T, width, tiles, w_scales, N, 1, act, limit, bias, work, gi::kBF16, row, 0, splits, status, stream);
-    return code ? code : gi_rows_int8(0, work, gi::kBF16, row, nullptr, 0, nullptr, 0.f, 0, 0.f, q, out_width, scales, T, N, stream);
+    return code ? code : gi_rows_int8(0, work, gi::kBF16, row, nullptr, 0, nullptr, 0.f, 0, 0.f, q, out_width, scales, T, N, 0, stream);
 }

@@ -32,6 +32,7 @@ struct RowsParams {
     int T, D, width;        // width: D or more, a multiple of 16; zeros behind D
     int act;
     float limit, eps;
+    int w_constant;         // norm: no kernel that may still be running writes weight: it may be read before the wait
 };
 
 constexpr unsigned kInfBits = 0x7f800000u, kLeastBits = 0x0d800000u;      // 2^-100
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G <= 512 ? 1024 / (G < 128 
 rows_int8_kernel(const RowsParams p) {
     constexpr int kRows = G < 128 ? 128 / G : 1;
     constexpr int kBatch = V <= 4 ? V : sizeof(TX) == 2 ? 4 : 2;      // (16-bit values wait in half the registers)
-    constexpr bool kEarly = V <= 4;      // the norm's weights are read before the wait for the kernel ahead, where registers hold them
+    constexpr bool kHeld = V <= 4;       // registers hold all of a thread's weights of a norm: constant ones are read before the wait for the kernel ahead
     __shared__ unsigned part_m[2][32];
     __shared__ float part_s[2][32];
     const int t = threadIdx.x % G;
@@ -216,16 +217,17 @@ rows_int8_kernel(const RowsParams p) {
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) w[k] = KIND == kRowsNorm ? load4<VEC, G>(p.weight, t + (k0 + k) * G, p.D) : make_float4(0.f, 0.f, 0.f, 0.f);
     };
-    if (kEarly) weights(0);
+    if (kHeld && p.w_constant) weights(0);
     pdl_wait();
     if (threadIdx.x == 0) timeline_record(kTlInt8Rows, 1);
     if (row >= p.T) return;       // (whole warps: rows of several to a block have a warp each)
+    if (kHeld && !p.w_constant) weights(0);
     float4 v[V];
     unsigned m = 0;
     float ss = 0.f, factor = 1.f;
 #pragma unroll
     for (int k = 0; k < V; k += kBatch) {
-        if (!kEarly) weights(k);
+        if (!kHeld) weights(k);
         values<KIND, TX, TA, VEC, G, kBatch>(p, row, t + k * G, live - k, w, 1.f, true, ss, v + k);
     }
 #pragma unroll
@@ -236,7 +238,7 @@ rows_int8_kernel(const RowsParams p) {
         ss = 0.f;
 #pragma unroll
         for (int k = 0; k < V; k += kBatch) {
-            if (!kEarly) weights(k);
+            if (!kHeld) weights(k);
             values<KIND, TX, TA, VEC, G, kBatch>(p, row, t + k * G, live - k, w, factor, false, ss, v + k);
         }
 #pragma unroll
@@ -313,7 +315,7 @@ int run_rows(const RowsParams& p, bool vec, cudaStream_t st) {
 bool aligned4(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == kF32 ? 16 : 8) == 0; }
 
 int rows_int8_impl(int kind, const void* x, int x_dtype, long long ldx, const void* add, int add_dtype, const float* weight, float eps, int act,
-                   float limit, void* q, int width, float* scales, int T, int D, void* stream) {
+                   float limit, void* q, int width, float* scales, int T, int D, int w_constant, void* stream) {
     if (T == 0) return 0;
     GI_REQUIRE(T > 0 && D > 0, "rows_int8: sizes must be positive (rows=%d, D=%d)", T, D);
     GI_REQUIRE(D <= (1 << 30), "rows_int8: rows of %d values (at most 2^30)", D);
@@ -322,7 +324,7 @@ int rows_int8_impl(int kind, const void* x, int x_dtype, long long ldx, const vo
     GI_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0, "rows_int8: the output must be 16-byte aligned");
     GI_REQUIRE(act >= 0 && act < kActCount, "rows_int8: unknown activation %d", act);
     GI_REQUIRE(ldx >= (kind == kRowsGated ? 2ll : 1ll) * D || T == 1, "rows_int8: rows of x overlap");
-    const RowsParams p{x, add, weight, static_cast<int8_t*>(q), scales, ldx, T, D, width, act, limit, eps};
+    const RowsParams p{x, add, weight, static_cast<int8_t*>(q), scales, ldx, T, D, width, act, limit, eps, w_constant};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     bool vec = D % 4 == 0 && (ldx % 4 == 0 || T == 1) && aligned4(x, x_dtype) && (weight == nullptr || aligned4(weight, kF32));
     if (kind == kRowsNorm) {
@@ -343,8 +345,9 @@ int rows_int8_impl(int kind, const void* x, int x_dtype, long long ldx, const vo
 GI_TIMELINE_SETTER(gi_timeline_set_int8_rows)
 
 // q [T, width] and scales [T] of T rows: kind 0 of x [T, D], 1 of the norm of x (32-bit; x += add [T, D] first where add is given), 2 of
-// act(g) * u with x [T, 2 D] = [g; u] and `weight` its bias (may be null). Rows of x lie ldx values apart.
+// act(g) * u with x [T, 2 D] = [g; u] and `weight` its bias (may be null). Rows of x lie ldx values apart. w_constant: no launch before this one that may
+// still be running writes the norm's `weight`, so that it may be read before the wait for them.
 extern "C" int gi_rows_int8(int kind, const void* x, int x_dtype, long long ldx, const void* add, int add_dtype, const float* weight, float eps,
-                            int act, float limit, void* q, int width, float* scales, int T, int D, void* stream) {
-    return gi::dispatch(gi::rows_int8_impl, kind, x, x_dtype, ldx, add, add_dtype, weight, eps, act, limit, q, width, scales, T, D, stream);
+                            int act, float limit, void* q, int width, float* scales, int T, int D, int w_constant, void* stream) {
+    return gi::dispatch(gi::rows_int8_impl, kind, x, x_dtype, ldx, add, add_dtype, weight, eps, act, limit, q, width, scales, T, D, w_constant, stream);
 }

@@ -1770,7 +1770,7 @@ def _strided(t: torch.Tensor, name: str, row: int) -> Tuple[int, int]:
 
 
 def _rows_int8(name: str, kind: int, x: torch.Tensor, columns: int, out: torch.Tensor, scales: torch.Tensor, add=None, weight=None, eps: float = 0.0,
-               act: int = 0, limit: float = 0.0) -> None:
+               act: int = 0, limit: float = 0.0, w_constant: bool = False) -> None:
     T, row = x.shape
     D = row // columns
     width = (D + 15) // 16 * 16
@@ -1780,7 +1780,7 @@ def _rows_int8(name: str, kind: int, x: torch.Tensor, columns: int, out: torch.T
     at, stride = _strided(x, "x", row)
     extra, extra_type = (0, 0) if add is None else (_dev(add, "add"), dtype_code(add.dtype))
     code = lib().gi_rows_int8(kind, at, dtype_code(x.dtype), stride, extra, extra_type, 0 if weight is None else _ptr(weight, "weight", torch.float32),
-                              eps, act, limit, _ptr(out, "out", torch.int8), width, _ptr(scales, "scales", torch.float32), T, D, _stream())
+                              eps, act, limit, _ptr(out, "out", torch.int8), width, _ptr(scales, "scales", torch.float32), T, D, int(w_constant), _stream())
     if code:
         check(code, name)
 
@@ -1793,17 +1793,18 @@ def quantize_rows(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> N
 
 
 def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, eps: float,
-                 add: Optional[torch.Tensor] = None) -> None:
+                 add: Optional[torch.Tensor] = None, w_constant: bool = False) -> None:
     """x += add (``add`` [T, D] 32-bit or bfloat16, where given), then weight * (x / sqrt(mean(x^2) + eps)) of every row in 8 bits:
     ``out`` [T, int8_width(D)] int8 and ``scales`` [T]. ``x`` [T, D] is the 32-bit residual stream (its rows may lie apart). The integers are those of
-    x * weight (the norm's factor is the row's: it goes into the scale)."""
+    x * weight (the norm's factor is the row's: it goes into the scale). ``w_constant``: no launch of this library that may still be running writes ``weight``
+    (a model's weights, all written long before), which is then read before the launches ahead have ended; otherwise it may be their output."""
     if x.dim() != 2 or weight.numel() != x.shape[1] or (add is not None and add.shape != x.shape):
         raise KernelError("rmsnorm_int8: shapes of x, weight and add do not agree")
     if x.dtype is not torch.float32:
         raise KernelError(f"rmsnorm_int8: x must be torch.float32, got {x.dtype}")
     if add is not None and add.data_ptr() == x.data_ptr() and x.numel():
         raise KernelError("rmsnorm_int8: add must not be x itself")
-    _rows_int8("rmsnorm_int8", 1, x, 1, out, scales, add, weight, eps)
+    _rows_int8("rmsnorm_int8", 1, x, 1, out, scales, add, weight, eps, w_constant=w_constant)
 
 
 def gated_act_int8(gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, activation: str = "silu", limit: float = 0.0,
@@ -1826,10 +1827,12 @@ class Int8Rows:
 
 class Int8Weight:
     """A weight matrix [N, K] in 8 bits, a scale a channel, laid out as the products read it (``int8_weight``). ``channels`` N (gated: of a
-    part), ``width``: int8_width(K)."""
+    part), ``width``: int8_width(K). ``constant``: no launch of this library that may still be running writes ``tiles``; products of few rows then ask for the
+    first ones before the launches ahead have ended. It holds for what ``int8_weight`` lays out: the tiles are a copy of their own that torch writes (whose launches let
+    none behind them start early). Who writes them by other means sets it to False. ``scales`` are read behind the wait and may be the launch's before."""
 
-    def __init__(self, tiles: torch.Tensor, scales: torch.Tensor, channels: int, width: int, gated: bool):
-        self.tiles, self.scales, self.channels, self.width, self.gated = tiles, scales, channels, width, gated
+    def __init__(self, tiles: torch.Tensor, scales: torch.Tensor, channels: int, width: int, gated: bool, constant: bool = False):
+        self.tiles, self.scales, self.channels, self.width, self.gated, self.constant = tiles, scales, channels, width, gated, constant
         self.plans, self.works = {}, {}      # rows -> the plan of a product of so many, and the scratch: sizes decide, once
 
 
@@ -1854,7 +1857,7 @@ def int8_weight(q: torch.Tensor, scales: torch.Tensor, gated: bool = False) -> I
     row = torch.arange(128, device=q.device).view(128, 1)
     source = torch.arange(8, device=q.device).view(1, 8) ^ (row % 8)                      # place p of row r holds piece p ^ (r % 8)
     tiles = t[:, :, :, row, source].contiguous().view(-1)
-    return Int8Weight(tiles, scales.reshape(-1).contiguous(), n, int8_width(K), gated)
+    return Int8Weight(tiles, scales.reshape(-1).contiguous(), n, int8_width(K), gated, constant=True)
 
 
 def _int8_tiles(w: Int8Weight) -> int:
@@ -1901,7 +1904,7 @@ def _int8_plan_of(T: int, w: Int8Weight):
 def _few(a, a_scales, w, out, out_dtype, out_stride, accumulate, plan) -> None:
     code = lib().gi_int8_product_few(_ptr(a, "a", torch.int8), _ptr(a_scales, "a_scales", torch.float32), a.shape[0], w.width, w.tiles.data_ptr(),
                                      w.scales.data_ptr(), w.channels, 0, out, out_dtype, out_stride, int(bool(accumulate)), plan[1], plan[2], plan[3],
-                                     _tc_state(a.device).status.data_ptr(), _stream())
+                                     int(w.constant), _tc_state(a.device).status.data_ptr(), _stream())
     if code:
         check(code, "int8_product")
 
@@ -1968,6 +1971,6 @@ def int8_gated(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: torc
     code = lib().gi_int8_gated(_ptr(a, "a", torch.int8), _ptr(a_scales, "a_scales", torch.float32), T, w.width, w.tiles.data_ptr(), w.scales.data_ptr(), I,
                                ACTIVATIONS[activation], limit, 0 if bias is None else _ptr(bias, "bias", torch.float32), _ptr(work, "work", torch.float32),
                                _ptr(out, "out", torch.int8), width, _ptr(out_scales, "out_scales", torch.float32), plan[1] if few else 0,
-                               plan[2] if few else plan[1], plan[3] if few else 0, _tc_state(a.device).status.data_ptr(), _stream())
+                               plan[2] if few else plan[1], plan[3] if few else 0, int(w.constant), _tc_state(a.device).status.data_ptr(), _stream())
     if code:
         check(code, "int8_gated")

@@ -141,13 +141,13 @@ _SIGNATURES = {
     "gi_verify_drafts": [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong,
                          c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "gi_rows_int8": [c_int, c_void_p, c_int, c_longlong, c_void_p, c_int, c_void_p, c_float, c_int, c_float, c_void_p, c_int, c_void_p, c_int,
-                     c_int, c_void_p],
+                     c_int, c_int, c_void_p],
     "gi_int8_product_few": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_longlong, c_int, c_int, c_int,
-                            c_int, c_void_p, c_void_p],
+                            c_int, c_int, c_void_p, c_void_p],
     "gi_int8_product_many": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_int,
                              c_longlong, c_int, c_int, c_void_p, c_void_p],
     "gi_int8_gated": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
-                      c_int, c_int, c_int, c_void_p, c_void_p],
+                      c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "gi_sample": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
 }
 

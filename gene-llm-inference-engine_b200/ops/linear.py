@@ -47,7 +47,7 @@ class Int8Linear:
             kernels.int8_product(a.q, a.scales, self.weight, added)
         else:
             kernels.int8_product(a.q, a.scales, self.weight, out)
-        kernels.rmsnorm_int8(out, weight, rows.q, rows.scales, eps, add=added if accumulate else None)
+        kernels.rmsnorm_int8(out, weight, rows.q, rows.scales, eps, add=added if accumulate else None, w_constant=True)
         return out
 
 

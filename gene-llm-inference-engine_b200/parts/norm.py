@@ -35,7 +35,7 @@ class RMSNorm:
     def forward(self, x: torch.Tensor, out, rows: Optional[torch.Tensor] = None):
         """``out``: a tensor, or rows in 8 bits (``kernels.Int8Rows``)."""
         if isinstance(out, kernels.Int8Rows):
-            kernels.rmsnorm_int8(x, self.weight, out.q, out.scales, self.eps)
+            kernels.rmsnorm_int8(x, self.weight, out.q, out.scales, self.eps, w_constant=True)
         else:
             kernels.rmsnorm(x, self.weight, out, self.eps, rows)
         return out

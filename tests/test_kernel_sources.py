@@ -84,3 +84,21 @@ def test_a_kernels_shared_memory_limit_is_set_on_every_device(tmp_path):
 def test_no_launcher_remembers_for_the_process_what_belongs_to_a_device(name):
     """What the 32-bit path launches: it runs on whichever device is current, of several in a process."""
     assert not re.search(r"static (?:const )?(?:bool|cudaError_t) \w+\s*=", _source(name))
+
+
+def _kernel_body(text, name):
+    """From the kernel's name to the end of its function (a closing brace in the first column)."""
+    return re.search(r"\n" + name + r"\(.*?\n\}", text, re.S).group(0)
+
+
+def test_weights_in_8_bits_are_read_ahead_of_the_wait_only_where_they_are_constant():
+    """A kernel that reads weights before its wait for the launches ahead has old values where one of those writes them."""
+    rows = _kernel_body(_source("int8_rows.cu"), "rows_int8_kernel")
+    ahead = rows[:rows.index("pdl_wait();")]
+    assert re.findall(r"if \((.*?)\) weights\(", ahead) == ["kHeld && p.w_constant"] and len(re.findall(r"\bweights\(", ahead)) == 1
+    assert "if (kHeld && !p.w_constant) weights(0);" in rows[rows.index("pdl_wait();"):]
+    few = _kernel_body(_source("int8_product.cu"), "int8_few_kernel")
+    ahead = few[:few.index("pdl_wait();")]
+    assert re.findall(r"if \(p.w_constant\)\s*for \(.*?\) load_w\(", ahead) and len(re.findall(r"(?<!auto )\bload_w\(", ahead)) == 1
+    for name in ("int8_rows.cu", "int8_product.cu"):        # and never by a load that must not see what is written while the kernel is resident
+        assert "__ldg" not in _source(name) and "ld.global.nc" not in _source(name)
