@@ -288,6 +288,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const FewParams p) {
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc = int8_idesc(kTileRows, BQ);
+            pdl_wait();          // the rows come with the kernels ahead: the waits' limit counts from their end, and this kernel's copies alone
             bool ok = true;
             int s = 0, parity = 0;
             for (int i = 0; i < n_steps; ++i) {

@@ -102,3 +102,14 @@ def test_weights_in_8_bits_are_read_ahead_of_the_wait_only_where_they_are_consta
     assert re.findall(r"if \(p.w_constant\)\s*for \(.*?\) load_w\(", ahead) and len(re.findall(r"(?<!auto )\bload_w\(", ahead)) == 1
     for name in ("int8_rows.cu", "int8_product.cu"):        # and never by a load that must not see what is written while the kernel is resident
         assert "__ldg" not in _source(name) and "ld.global.nc" not in _source(name)
+
+
+def test_the_limit_of_a_wait_for_8_bit_operands_does_not_count_the_launches_ahead():
+    """Every role of the product waits for the launches ahead (however long they take) before its first bounded wait for this launch's own copies."""
+    few = _kernel_body(_source("int8_product.cu"), "int8_few_kernel")
+    producer, rest = few[few.index("if (warp == 0) {"):].split("} else if (warp == 1) {", 1)
+    mma, epilogue = rest.split("const int lane_group", 1)
+    for role in (producer, mma, epilogue):
+        assert 0 < role.index("pdl_wait();") < role.index("bar_wait(")
+    many = _kernel_body(_source("int8_product.cu"), "int8_many_kernel")
+    assert many.index("\n    pdl_wait();") < many.index("bar_wait")
