@@ -1769,6 +1769,19 @@ def _strided(t: torch.Tensor, name: str, row: int) -> Tuple[int, int]:
     return _rows_of(t, name), t.stride(0)
 
 
+def _overlap(x: torch.Tensor, other: torch.Tensor) -> bool:
+    """Whether ``other``, values side by side, shares memory with a row of the matrix ``x`` (between rows that lie apart it may lie)."""
+    T, size = x.shape[0], x.element_size()
+    row, stride = x.shape[1] * size, x.stride(0) * size
+    first, length = other.data_ptr() - x.data_ptr(), other.numel() * other.element_size()
+    if length == 0 or first + length <= 0 or first >= (T - 1) * stride + row:
+        return False
+    if first < 0 or T == 1 or stride == 0:
+        return True
+    at, behind = divmod(first, stride)
+    return behind < row or (behind + length > stride and at + 1 < T)
+
+
 def _rows_int8(name: str, kind: int, x: torch.Tensor, columns: int, out: torch.Tensor, scales: torch.Tensor, add=None, weight=None, eps: float = 0.0,
                act: int = 0, limit: float = 0.0, w_constant: bool = False) -> None:
     T, row = x.shape
@@ -1796,14 +1809,14 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, scale
                  add: Optional[torch.Tensor] = None, w_constant: bool = False) -> None:
     """x += add (``add`` [T, D] 32-bit or bfloat16, where given), then weight * (x / sqrt(mean(x^2) + eps)) of every row in 8 bits:
     ``out`` [T, int8_width(D)] int8 and ``scales`` [T]. ``x`` [T, D] is the 32-bit residual stream (its rows may lie apart). The integers are those of
-    x * weight (the norm's factor is the row's: it goes into the scale). ``w_constant``: no launch of this library that may still be running writes ``weight``
+    x * weight (the norm's factor is the row's: it goes into the scale). ``add`` and ``x`` must not overlap. ``w_constant``: no launch of this library that may still be running writes ``weight``
     (a model's weights, all written long before), which is then read before the launches ahead have ended; otherwise it may be their output."""
     if x.dim() != 2 or weight.numel() != x.shape[1] or (add is not None and add.shape != x.shape):
         raise KernelError("rmsnorm_int8: shapes of x, weight and add do not agree")
     if x.dtype is not torch.float32:
         raise KernelError(f"rmsnorm_int8: x must be torch.float32, got {x.dtype}")
-    if add is not None and add.data_ptr() == x.data_ptr() and x.numel():
-        raise KernelError("rmsnorm_int8: add must not be x itself")
+    if add is not None and x.numel() and _overlap(x, add):
+        raise KernelError("rmsnorm_int8: add must not overlap x, which is written")
     _rows_int8("rmsnorm_int8", 1, x, 1, out, scales, add, weight, eps, w_constant=w_constant)
 
 

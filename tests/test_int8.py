@@ -117,3 +117,24 @@ def test_command_line():
     for bad in (["--weights", "int4"], ["--weights", "int8", "--adapter", "a"]):
         with pytest.raises(UsageError):
             parse(base + bad)
+
+
+def test_an_addition_that_overlaps_the_stream_is_refused():
+    """The stream is written while the addition is read, by other blocks: any shared value is a race. Between rows that lie apart nothing is shared."""
+    D = 20
+    flat, w = torch.zeros(40 * D), torch.ones(D)
+
+    def call(x, add):
+        T = x.shape[0]
+        return lambda: k.rmsnorm_int8(x, w, torch.zeros(T, 32, dtype=torch.int8), torch.zeros(T), 1e-5, add=add)
+
+    rows = flat.view(-1, D)
+    apart = flat.view(-1, 4 * D)[:, :D]
+    for x, add in ((rows[1:], rows[:-1]), (rows[:-1], rows[1:]), (rows[:5], rows[:5]), (rows[:5], rows[4:9]), (flat[:3 * D].view(3, D), flat[1:3 * D + 1].view(3, D)),
+                   (apart[:2], rows[3:5]), (apart[:2], rows[4:6]), (apart[1:3], rows[3:5]), (apart[:1], rows[:1]), (rows[1:3], flat.view(torch.bfloat16)[2 * D:4 * D].view(2, D))):
+        with pytest.raises(k.KernelError, match="overlap"):
+            call(x, add)()
+    for x, add in ((rows[:5], rows[5:10]), (rows[5:10], rows[:5]), (apart[:2], rows[1:3]), (apart[:2], rows[2:4]), (apart[:1], rows[1:2]), (apart[8:], rows[38:40][:2]),
+                   (rows[2:3], flat.view(torch.bfloat16)[:D].view(1, D))):
+        with pytest.raises(k.KernelError, match="no CPU path"):      # taken, up to there
+            call(x, add)()
