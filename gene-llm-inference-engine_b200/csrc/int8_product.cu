@@ -822,6 +822,8 @@ int int8_few_impl(const void* a, const float* a_scales, int T, int width, const 
     if (int bad = check_operands(a, T, width, tiles, N, status)) return bad;
     GI_REQUIRE(out_dtype == kF32 || out_dtype == kBF16, "int8_product: unsupported dtype code %d", out_dtype);
     GI_REQUIRE(!(accumulate && out_dtype != kF32), "int8_product: accumulation needs a 32-bit output");
+    GI_REQUIRE(T == 1 || ldo >= (gated ? 2ll : 1ll) * N, "int8_product: rows of the output overlap");
+    GI_REQUIRE(bq == 8 || bq == 32 || bq == 64 || bq == 128, "int8_product: tiles of %d rows (8, 32, 64 or 128)", bq);
     GI_REQUIRE(splits >= 1 && splits <= (bq == 128 ? 1 : 8), "int8_product: %d ranges of K with tiles of %d rows (1 to 8: one cluster; one with 128)", splits, bq);
     FewParams p{};
     p.tiles = static_cast<const uint8_t*>(tiles);
@@ -859,8 +861,7 @@ int int8_few_impl(const void* a, const float* a_scales, int T, int width, const 
         case 8: return go(std::integral_constant<int, 8>());
         case 32: return go(std::integral_constant<int, 32>());
         case 64: return go(std::integral_constant<int, 64>());
-        case 128: return go(std::integral_constant<int, 128>());
-        default: set_error("int8_product: tiles of %d rows (8, 32, 64 or 128)", bq); return 2;
+        default: return go(std::integral_constant<int, 128>());
     }
 }
 
@@ -870,6 +871,7 @@ int int8_many_impl(const void* a, const float* a_scales, int T, int width, const
     if (int bad = check_operands(a, T, width, tiles, N, status)) return bad;
     GI_REQUIRE(out_dtype == kF32 || out_dtype == kBF16, "int8_product: unsupported dtype code %d", out_dtype);
     GI_REQUIRE(!(accumulate && out_dtype != kF32), "int8_product: accumulation needs a 32-bit output");
+    GI_REQUIRE(T == 1 || ldo >= N, "int8_product: rows of the output overlap");
     GI_REQUIRE(!gated || out_dtype == kBF16, "int8_product: a gated product has a bfloat16 output");
     GI_REQUIRE(act >= 0 && act < kActCount, "int8_product: unknown activation %d", act);
     GI_REQUIRE(group_t >= 1, "int8_product: groups of %d tiles", group_t);
@@ -884,7 +886,7 @@ int int8_many_impl(const void* a, const float* a_scales, int T, int width, const
     p.total_kb = (width + kRowBytes - 1) / kRowBytes;
     p.tiles_t = (T + 255) / 256;
     p.tiles_n = (N + (gated ? kTileRows : kTileN) - 1) / (gated ? kTileRows : kTileN);
-    p.group_t = group_t;
+    p.group_t = min(group_t, p.tiles_t);
     p.act = act;
     p.limit = limit;
     p.status = static_cast<int*>(status);

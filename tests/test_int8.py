@@ -138,3 +138,26 @@ def test_an_addition_that_overlaps_the_stream_is_refused():
                    (rows[2:3], flat.view(torch.bfloat16)[:D].view(1, D))):
         with pytest.raises(k.KernelError, match="no CPU path"):      # taken, up to there
             call(x, add)()
+
+
+def test_plans_that_do_not_exist_are_refused():
+    """By an error code of the library, before anything is divided by a tile's height or launched (no GPU needed)."""
+    a, scales, out = torch.zeros(16, 16, dtype=torch.int8), torch.ones(16), torch.zeros(16, 4)
+    w = k.int8_weight(torch.zeros(4, 16, dtype=torch.int8), torch.ones(4))
+    room = torch.zeros(w.tiles.numel() + 128, dtype=torch.int8)
+    tiles = room.data_ptr() + -room.data_ptr() % 128
+    status = torch.zeros(1, dtype=torch.int32)
+
+    def few(bq, splits, ldo=4, gated=0):
+        return k.lib().gi_int8_product_few(a.data_ptr(), scales.data_ptr(), 16, 16, tiles, scales.data_ptr(), 4, gated, out.data_ptr(), k.F32, ldo, 0, bq, splits, 0, 0,
+                                           status.data_ptr(), 0)
+
+    def many(group, ldo=4):
+        return k.lib().gi_int8_product_many(a.data_ptr(), scales.data_ptr(), 16, 16, tiles, scales.data_ptr(), 4, 0, 0, 0.0, 0, out.data_ptr(), k.F32, ldo, 0, group,
+                                            status.data_ptr(), 0)
+
+    for code, message in ((lambda: few(0, 1), "tiles of 0 rows"), (lambda: few(-8, 1), "tiles of -8 rows"), (lambda: few(16, 1), "tiles of 16 rows"), (lambda: few(8, 0), "ranges of K"),
+                          (lambda: few(8, 9), "ranges of K"), (lambda: few(128, 2), "ranges of K"), (lambda: few(8, 1, ldo=3), "overlap"), (lambda: few(8, 1, ldo=7, gated=1), "overlap"),
+                          (lambda: many(0), "groups of 0"), (lambda: many(1, ldo=0), "overlap")):
+        with pytest.raises(k.KernelError, match=message):
+            k.check(code(), "int8_product")
