@@ -12,8 +12,9 @@
 //
 // What is not finite: the largest |v| is kept as the bits of its absolute value, an integer that orders infinities and NaN above
 // every number, so that one of them anywhere in a row shows: such a row gets the scale NaN and zeros, and every product with it is
-// NaN. A norm whose squares (or products with the weights) leave the range of 32 bits is taken again from values 2^-80 times as large, one whose squares
-// vanish beside an eps that is as small from values 2^80 times as large.
+// NaN. A norm whose squares or products with the weights leave the range of 32 bits is taken again: the squares from values 2^-80 times as large, or
+// 2^80 times where they vanish beside an eps that is as small, and the products with the weights likewise, each by a factor of its own (values near 1 with weights
+// near 2^127 have squares as they should be).
 // Rows whose largest |v| is below 2^-100 count as zero (scale 0): 127 / m would leave that range at the other end.
 #include "common.cuh"
 
@@ -35,7 +36,7 @@ struct RowsParams {
     int w_constant;         // norm: no kernel that may still be running writes weight: it may be read before the wait
 };
 
-constexpr unsigned kInfBits = 0x7f800000u, kLeastBits = 0x0d800000u;      // 2^-100
+constexpr unsigned kInfBits = 0x7f800000u, kLeastBits = 0x0d800000u, kSmallBits = 0x35800000u;      // 2^-100, 2^-20
 constexpr float kDown = 8.271806125530277e-25f, kUp = 1.2089258196146292e24f;      // 2^-80, 2^80
 constexpr float kLeastSquares = 7.888609052210118e-31f, kLeastEps = 7.52316384526264e-37f;      // 2^-100, 2^-120
 
@@ -83,6 +84,9 @@ __device__ __forceinline__ void store4(float* p, int i, int D, const float4 v) {
 
 struct NoAdd {};        // a norm without an addition
 
+// What a norm's values are multiplied by ahead of their squares and ahead of the weights.
+struct Factors { float squares = 1.f, values = 1.f; };
+
 __device__ __forceinline__ float4 plus(const float4 a, const float4 b) {
     return make_float4(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y), __fadd_rn(a.z, b.z), __fadd_rn(a.w, b.w));
 }
@@ -92,7 +96,7 @@ __device__ __forceinline__ float4 plus(const float4 a, const float4 b) {
 // `live` groups have columns for any thread: activations of the others are skipped, by all threads at once (14,336 values in 512 x 8 groups of four: an
 // eighth). Their loads are not: they are masked anyway, and a branch between loads keeps them from being under way together.
 template <int KIND, typename TX, typename TA, bool VEC, int G, int N>
-__device__ __forceinline__ void values(const RowsParams& p, long long row, int i0, int live, const float4* w, float factor, bool first, float& ss, float4* v) {
+__device__ __forceinline__ void values(const RowsParams& p, long long row, int i0, int live, const float4* w, const Factors factor, bool first, float& ss, float4* v) {
     const TX* x = static_cast<const TX*>(p.x) + row * p.ldx;
 #pragma unroll
     for (int k = 0; k < N; ++k) v[k] = load4<VEC, G>(x, i0 + k * G, p.D);
@@ -132,9 +136,10 @@ __device__ __forceinline__ void values(const RowsParams& p, long long row, int i
         }
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const float4 e = make_float4(v[k].x * factor, v[k].y * factor, v[k].z * factor, v[k].w * factor);
+            auto times = [&](float f) { return make_float4(v[k].x * f, v[k].y * f, v[k].z * f, v[k].w * f); };
+            const float4 e = times(factor.squares), x = times(factor.values);
             ss = fmaf(e.x, e.x, ss); ss = fmaf(e.y, e.y, ss); ss = fmaf(e.z, e.z, ss); ss = fmaf(e.w, e.w, ss);
-            v[k] = make_float4(__fmul_rn(e.x, w[k].x), __fmul_rn(e.y, w[k].y), __fmul_rn(e.z, w[k].z), __fmul_rn(e.w, w[k].w));
+            v[k] = make_float4(__fmul_rn(x.x, w[k].x), __fmul_rn(x.y, w[k].y), __fmul_rn(x.z, w[k].z), __fmul_rn(x.w, w[k].w));
         }
     }
 }
@@ -161,10 +166,14 @@ __device__ __forceinline__ unsigned top_bits(const float4 v, unsigned m) {
     return max(m, max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
 }
 
-// What the values of a norm have to be multiplied by before it is taken again; 1: nothing.
-__device__ __forceinline__ float other_factor(unsigned m, float ss, float eps) {
-    if (m >= kInfBits || !(ss < __uint_as_float(kInfBits))) return kDown;
-    return ss < kLeastSquares && eps < kLeastEps && m > 0 ? kUp : 1.f;
+// The factors that a norm has to be taken again with; false: it is right as it is. (Products below 2^-20 of values that are small enough for kUp: none above
+// 2^60 then.)
+__device__ __forceinline__ bool other_factors(unsigned m, float ss, float eps, Factors& f) {
+    if (!(ss < __uint_as_float(kInfBits))) f.squares = kDown;
+    else if (ss < kLeastSquares && eps < kLeastEps && m > 0) f.squares = kUp;
+    if (m >= kInfBits) f.values = kDown;
+    else if (f.squares == kUp && m < kSmallBits) f.values = kUp;
+    return f.squares != 1.f || f.values != 1.f;
 }
 
 // The row's largest |v| and sum of squares over the G threads that share it.
@@ -185,13 +194,17 @@ __device__ __forceinline__ void meet(unsigned& m, float& ss, unsigned* part_m, f
 
 // 127 / m and the scale of a row; a row that is not finite: 0 and NaN.
 template <int KIND>
-__device__ __forceinline__ float2 row_factors(unsigned m_bits, float ss, const RowsParams& p, float factor) {
+__device__ __forceinline__ float2 row_factors(unsigned m_bits, float ss, const RowsParams& p, const Factors factor) {
     if (m_bits >= kInfBits || (KIND == kRowsNorm && !(ss < __uint_as_float(kInfBits)))) return make_float2(0.f, __uint_as_float(0x7fc00000u));
     if (m_bits < kLeastBits) return make_float2(0.f, 0.f);
     const float m = __uint_as_float(m_bits);
     float scale = __fdiv_rn(m, 127.f);
-    // (of values `factor` times as large: their mean square and eps are both factor^2 times as large, and the factors cancel)
-    if (KIND == kRowsNorm) scale = __fdiv_rn(scale, sqrtf(__fdiv_rn(ss, static_cast<float>(p.D)) + p.eps * factor * factor));
+    // (squares of values f times as large: their mean and eps are both f^2 times as large, the root f times; powers of two are exact)
+    if (KIND == kRowsNorm) {
+        const float f = factor.squares, root = sqrtf(__fdiv_rn(ss, static_cast<float>(p.D)) + p.eps * f * f);
+        scale = __fdiv_rn(scale, root);
+        if (f != factor.values) scale *= f > factor.values ? kUp : kDown;      // f / values: 2^80 or 2^-80, as they never lie further apart
+    }
     return make_float2(__fdiv_rn(127.f, m), scale);
 }
 
@@ -224,16 +237,17 @@ rows_int8_kernel(const RowsParams p) {
     if (kHeld && !p.w_constant) weights(0);
     float4 v[V];
     unsigned m = 0;
-    float ss = 0.f, factor = 1.f;
+    float ss = 0.f;
+    Factors factor;
 #pragma unroll
     for (int k = 0; k < V; k += kBatch) {
         if (!kHeld) weights(k);
-        values<KIND, TX, TA, VEC, G, kBatch>(p, row, t + k * G, live - k, w, 1.f, true, ss, v + k);
+        values<KIND, TX, TA, VEC, G, kBatch>(p, row, t + k * G, live - k, w, factor, true, ss, v + k);
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) m = top_bits(v[k], m);
     meet<G, KIND>(m, ss, part_m[0], part_s[0]);
-    if (KIND == kRowsNorm && (factor = other_factor(m, ss, p.eps)) != 1.f) {
+    if (KIND == kRowsNorm && other_factors(m, ss, p.eps, factor)) {
         m = 0;
         ss = 0.f;
 #pragma unroll
@@ -262,7 +276,8 @@ wide_rows_int8_kernel(const RowsParams p) {
     const long long row = blockIdx.x;
     pdl_prologue();
     unsigned m = 0;
-    float ss = 0.f, factor = 1.f;
+    float ss = 0.f;
+    Factors factor;
     float4 v[1], w[1];
     auto pass = [&](int i, bool first, float& squares) {
         w[0] = KIND == kRowsNorm ? load4<false, 1024>(p.weight, i, p.D) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -271,7 +286,7 @@ wide_rows_int8_kernel(const RowsParams p) {
     const int groups = (p.width + 4095) / 4096 * 1024;
     for (int i = threadIdx.x; i < groups; i += 1024) { pass(i, true, ss); m = top_bits(v[0], m); }
     meet<1024, KIND>(m, ss, part_m[0], part_s[0]);
-    if (KIND == kRowsNorm && (factor = other_factor(m, ss, p.eps)) != 1.f) {
+    if (KIND == kRowsNorm && other_factors(m, ss, p.eps, factor)) {
         m = 0;
         ss = 0.f;
         for (int i = threadIdx.x; i < groups; i += 1024) { pass(i, false, ss); m = top_bits(v[0], m); }

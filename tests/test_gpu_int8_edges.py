@@ -29,3 +29,24 @@ def test_more_tiles_walked_together_than_there_are():
         out = torch.full((700, 1000), math.nan, device=DEV)
         k.int8_product(a, s, w, out, plan=("many", group))
         assert torch.equal(out, want), group
+
+
+@pytest.mark.parametrize("D", [300, 2048, 9001, 16384, 33000])
+def test_norms_with_weights_near_the_ends_of_32_bits(D):
+    """Ordinary rows whose products with the weights overflow, small rows without an eps with weights as large, large rows with small weights: a norm's squares and
+    its products with the weights leave the range each by itself."""
+    k = _kernels()
+    g = torch.Generator(device=DEV).manual_seed(D)
+    for size, weight, eps in ((3.0, 1.5e38, 1e-5), (3.0, 1.5e38, 0.0), (1e-20, 1e36, 0.0), (1e-24, 1e-12, 0.0), (1e-20, 1.0, 0.0), (1e25, 1e-30, 1e-5), (1e25, 1.0, 1e-5), (1e25, 1e20, 1e-5)):
+        x = torch.randn(3, D, generator=g, device=DEV) * size
+        x[1] = 0
+        w = (0.5 + 0.5 * torch.rand(D, generator=g, device=DEV)) * weight
+        more = torch.zeros_like(x)
+        q, s = torch.empty(3, k.int8_width(D), dtype=torch.int8, device=DEV), torch.empty(3, device=DEV)
+        k.rmsnorm_int8(x, w, q, s, eps, add=more)
+        assert float(s[1]) == 0 and not q[1].any()
+        for row in (0, 2):
+            want = x[row].double() / (x[row].double().square().mean() + eps).sqrt() * w.double()
+            got = q[row, :D].double() * s[row].double()
+            # half a step of the integers and, far below it, the 32-bit scale's and borders' roundings (a scale below 2^-126 has steps of 2^-149)
+            assert float((got - want).abs().max()) <= float(want.abs().max()) / 127 * 0.501, (size, weight, eps, row)
