@@ -184,7 +184,7 @@ struct FewParams {
     int* status;
 };
 
-enum Epilogue : int { kStoreF32 = 0, kAddF32 = 1, kStoreBF16 = 2, kGatedBF16 = 3 };
+enum Epilogue : int { kStoreF32 = 0, kAddF32 = 1, kStoreBF16 = 2, kGatedBF16 = 3, kAddLanesF32 = 4 };      // (the last: many rows whose outputs TMA cannot address)
 
 // Measured on B200 in a stream of launches, weights from memory: 8 rows 4096 -> 28672 18.4 us (6.4 TB/s), 64 rows 21.2; one token 8192 -> 2048 5.4 us, 2048 ->
 // 2048 3.5 (the hand-over from launch to launch, first operands and the cluster's exchange, about 3 us); 400 rows 4096 -> 4096 14.4.
@@ -598,6 +598,17 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             if (rank == 0) bar_arrive(smem_addr(&bars[2 * kStages + 2 + buf]));
             else bar_arrive_remote(leader_bar(2 * kStages + 2 + buf));
         };
+        // kAddLanesF32: what is added to is read by the lanes, side by side in a row, 32 rows of a chunk at once and a chunk ahead of its use. (Additions in L2, atomicAdd,
+        // take 49 us for 4000 x 2000 -> 4097 and this 61; but they count values below 2^-126 as zeros, which neither the TMA form nor the kernel of few rows does.
+        // Asked for into L2 a tile ahead 60.)
+        constexpr bool kLanes = EPI == kAddLanesF32;
+        float old[kLanes ? 32 : 1];
+        auto load_old = [&](float* dst, int tile_t, int col) {
+            const int first = tile_t * 256 + static_cast<int>(rank) * kTileRows + lane_group * 32, rows = p.T - first;
+            const float* o = static_cast<const float*>(p.out) + static_cast<size_t>(first) * p.ldo + col + lane;
+#pragma unroll
+            for (int j = 0; j < (kLanes ? 32 : 0); ++j) dst[j] = col + lane < p.N && j < rows ? __ldcg(o + j * p.ldo) : 0.f;
+        };
         int n = 0;
         for (int i = worker; i < n_tiles; i += n_workers, ++n) {
             int tile_t, tile_n;
@@ -610,6 +621,7 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             const bool up = EPI == kGatedBF16 && mine >= kTileRows;
             const int ch = n0 + (up ? mine - kTileRows : mine);
             const float mine_scale = ch < p.N ? __ldcg(p.w_scales + (up ? p.N : 0) + ch) : 0.f;
+            if (kLanes) load_old(old, tile_t, n0 + group * 32);
             bar_wait(smem_addr(&bars[2 * kStages + buf]), (n >> 1) & 1, gave_up, p.status, kErrEpilogue);
             both_sync();                               // nobody reads the last tile's scales any more
             scales[mine] = mine_scale;
@@ -619,7 +631,7 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             fence_after();
             if (n == 0 && mine == 0) timeline_record(kTlInt8ProductMany, 4);
             const uint32_t d = tmem + buf * kTileN + (static_cast<uint32_t>(lane_group * 32) << 16);
-            constexpr int kCols = EPI == kStoreF32 || EPI == kAddF32 ? 32 : 64;      // output columns to a chunk: 128 bytes
+            constexpr int kCols = EPI == kStoreBF16 || EPI == kGatedBF16 ? 64 : 32;      // output columns to a chunk: 128 bytes
             constexpr int kChunks = EPI == kGatedBF16 ? 2 : kTileN / kCols;
             // The pipeline's stages are free once the sums of this CTA's last tile are complete: each chunk then has a place of its own there and waits for no
             // earlier store.
@@ -631,6 +643,7 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     group_sync();
                 }
                 const bool last = c + 2 >= kChunks;
+                const int col = n0 + c * kCols, out_row = tile_t * 256 + static_cast<int>(rank) * kTileRows;
 #pragma unroll
                 for (int half = 0; half < kCols / 32; ++half) {
                     const int at = c * kCols + half * 32;
@@ -671,8 +684,20 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         }
                     }
                 }
-                const int col = n0 + c * kCols, out_row = tile_t * 256 + static_cast<int>(rank) * kTileRows;
-                if (!p.plain_stores) {
+                if constexpr (kLanes) {
+                    float next[32];
+                    if (c + 2 < kChunks) load_old(next, tile_t, col + 2 * kCols);
+                    group_sync();
+                    const int rows = min(32, p.T - (out_row + lane_group * 32));
+                    float* o = static_cast<float*>(p.out) + static_cast<size_t>(out_row + lane_group * 32) * p.ldo + col + lane;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float v = *reinterpret_cast<const float*>(stg + (lane_group * 32 + j) * 128 + (((lane >> 2) ^ (j & 7)) * 16) + (lane & 3) * 4);
+                        if (col + lane < p.N && j < rows) o[j * p.ldo] = __fadd_rn(old[j], v);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) old[j] = next[j];
+                } else if (!p.plain_stores) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     group_sync();
                     if (leader) {
@@ -681,9 +706,7 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
                 } else {
-                    // A warp stores the rows of its quarter of the tile, the lanes side by side, eight rows at a time. What is added to is added
-                    // where it lies, once a value, as the TMA form does (read first, a row after the other: 4000 x 2000 -> 4097 277 us, eight at a
-                    // time 90, this 49).
+                    // A warp stores the rows of its quarter of the tile, the lanes side by side, eight rows at a time.
                     group_sync();
 #pragma unroll 1
                     for (int r0 = lane_group * 32; r0 < lane_group * 32 + 32 && out_row + r0 < p.T; r0 += 8) {
@@ -705,11 +728,8 @@ int8_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                                 for (int j = 0; j < 8; ++j)
                                     v[j] = *reinterpret_cast<const float*>(stg + (r0 + j) * 128 + (((cc >> 2) ^ ((r0 + j) & 7)) * 16) + (cc & 3) * 4);
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    if (!there || out_row + r0 + j >= p.T) continue;
-                                    if (EPI == kAddF32) atomicAdd(o + j * p.ldo, v[j]);
-                                    else o[j * p.ldo] = v[j];
-                                }
+                                for (int j = 0; j < 8; ++j)
+                                    if (there && out_row + r0 + j < p.T) o[j * p.ldo] = v[j];
                             }
                         }
                     }
@@ -907,6 +927,7 @@ int int8_many_impl(const void* a, const float* a_scales, int T, int width, const
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (gated) return launch_many<kGatedBF16>(map_a, map_w, map_o, p, st);
     if (elt == 2) return launch_many<kStoreBF16>(map_a, map_w, map_o, p, st);
+    if (accumulate && p.plain_stores) return launch_many<kAddLanesF32>(map_a, map_w, map_o, p, st);
     return accumulate ? launch_many<kAddF32>(map_a, map_w, map_o, p, st) : launch_many<kStoreF32>(map_a, map_w, map_o, p, st);
 }
 

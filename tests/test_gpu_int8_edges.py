@@ -50,3 +50,24 @@ def test_norms_with_weights_near_the_ends_of_32_bits(D):
             got = q[row, :D].double() * s[row].double()
             # half a step of the integers and, far below it, the 32-bit scale's and borders' roundings (a scale below 2^-126 has steps of 2^-149)
             assert float((got - want).abs().max()) <= float(want.abs().max()) / 127 * 0.501, (size, weight, eps, row)
+
+
+@pytest.mark.parametrize("T", [8, 400])
+def test_additions_of_values_below_the_least_normal_one(T):
+    """What a product is added to, the product and the sum may be subnormal: kept by every form, so that a row's result does not depend on the others in the call."""
+    k = _kernels()
+    g = torch.Generator(device=DEV).manual_seed(T)
+    for N in (256, 257, 130):
+        _, a, s, _ = _product(k, g, T, 64, N)
+        s *= 2.0 ** -15
+        q = torch.randint(-127, 128, (N, 64), generator=g, device=DEV, dtype=torch.int8)
+        w = k.int8_weight(q, (0.01 + torch.rand(N, generator=g, device=DEV)) * 2.0 ** -120)
+        want = ((a.double() @ q.double().T).float() * s[:, None]) * w.scales
+        assert float(((want != 0) & (want.abs() < 2.0 ** -126)).float().mean()) > 0.05
+        for base in (torch.zeros_like(want), torch.randn(T, N, generator=g, device=DEV) * 2.0 ** -130, -want, want * 0.75):
+            for plan in (None, ("few", 8, 1, 0), ("many", 1), ("many", 2)):
+                for room in (0, 3):
+                    out = torch.full((T, N + room), 7.0, device=DEV)
+                    out[:, :N] = base
+                    k.int8_product(a, s, w, out[:, :N], accumulate=True, plan=plan)
+                    assert torch.equal(out[:, :N], base + want) and (out[:, N:] == 7).all(), (N, plan, room)
