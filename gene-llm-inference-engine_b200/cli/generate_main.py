@@ -21,7 +21,8 @@ USAGE = (
     "  DIR holds config.json and model.safetensors. --steps is the maximum number of positions including the\n"
     "  prompt (default: the context length). --weights f32 (= --dtype fp32) runs the whole model in true 32-bit;\n"
     "  int8: the layers' projections in 8-bit integers with a scale a channel, rounded when the model is loaded, and their inputs\n"
-    "  with a scale a row (with --draft-model: of the model of --model). It does not go with --adapter.\n"
+    "  with a scale a row (with --draft-model: of the model of --model); --dtype, before or behind it, is the type of everything else.\n"
+    "  It does not go with --adapter.\n"
     "  --random-weights SEED --config FILE first writes such a folder (random bfloat16 weights from the seed, for the\n"
     "  configuration in FILE, a config.json) to DIR, or to a temporary folder when no --model is given.\n"
     "  --adapter DIR: a low-rank adapter (adapter_config.json, adapter_model.safetensors) beside the model's weights.\n"
@@ -59,7 +60,7 @@ def parse(argv: List[str]) -> dict:
     o = {"model": "", "prompt_ids": None, "steps": 0, "max_seq_len": 0, "weights": "native", "device": "cuda",
          "profile": False, "temperature": 0.8, "top_k": None, "top_p": None, "seed": None, "stop_ids": [],
          "page_size": 16, "kv_pages": None, "echo": True, "quiet": False, "dump_tokens": "", "random_weights": None,
-         "config": "", "help": False, "adapter": "", "draft_model": "", "drafts": 4}
+         "config": "", "help": False, "adapter": "", "draft_model": "", "drafts": 4, "int8": False, "dtype": "bfloat16"}
     i = 0
     while i < len(argv):
         flag = argv[i]
@@ -88,14 +89,17 @@ def parse(argv: List[str]) -> dict:
         elif flag == "--bos": pass
         elif flag == "--steps": o["steps"] = _int(flag, value())
         elif flag == "--max-seq-len": o["max_seq_len"] = _int(flag, value())
-        elif flag == "--weights": o["weights"] = value()
+        elif flag == "--weights":
+            o["weights"] = value()
+            o["int8"] = o["weights"] == "int8"
         elif flag == "--dtype":
             name = value().lower()
             if name not in ("bf16", "bfloat16", "fp32", "f32", "float32"):
                 raise UsageError("--dtype must be bf16 or fp32")
-            if name not in ("bf16", "bfloat16"):
+            o["dtype"] = "bfloat16" if name in ("bf16", "bfloat16") else "float32"
+            if o["dtype"] == "float32":
                 o["weights"] = "f32"
-            elif o["weights"] != "int8":            # (which computes in bfloat16 besides)
+            elif o["weights"] != "int8":
                 o["weights"] = "native"
         elif flag == "--random-weights": o["random_weights"] = _int(flag, value())
         elif flag == "--config": o["config"] = value()
@@ -128,8 +132,10 @@ def parse(argv: List[str]) -> dict:
         raise UsageError("--prompt-ids or --prompt-ids-file is required (at least one token id)")
     if o["weights"] not in ("native", "f32", "int8"):
         raise UsageError("--weights must be native, f32 or int8")
-    if o["weights"] == "int8" and o["adapter"]:
+    if o["int8"] and o["adapter"]:
         raise UsageError("--weights int8 cannot be combined with --adapter")
+    if not o["int8"]:               # (--dtype is another name of --weights native or f32: the last of them holds)
+        o["dtype"] = "float32" if o["weights"] == "f32" else "bfloat16"
     if not o["device"].startswith("cuda"):
         raise UsageError("--device must be cuda: this engine has no CPU or emulated device")
     if o["draft_model"] and (o["top_k"] or (o["top_p"] is not None and o["top_p"] < 1.0)):
@@ -162,9 +168,9 @@ def _with_drafts(o: dict, device: str) -> int:
     context = o["max_seq_len"] or read_config(o["model"])[1].model_spec().max_position
     positions = min(o["steps"], context) if o["steps"] > 0 else context
     rank = _adapter_rank(o["adapter"]) if o["adapter"] else 0
-    engine = SpeculativeEngine(o["model"], o["draft_model"], drafts=o["drafts"], dtype="float32" if o["weights"] == "f32" else "bfloat16", device=device,
+    engine = SpeculativeEngine(o["model"], o["draft_model"], drafts=o["drafts"], dtype=o["dtype"], device=device,
                                max_running=1, max_seq_len=positions, page_size=o["page_size"], adapter_slots=1 if rank else 0, adapter_rank=rank or 16,
-                               weights="int8" if o["weights"] == "int8" else "native")
+                               weights="int8" if o["int8"] else "native")
     if rank:
         engine.load_adapter(0, o["adapter"])
     if engine.context < positions and not o["quiet"]:
@@ -226,10 +232,10 @@ def main(argv: Optional[List[str]] = None) -> int:
             return _with_drafts(o, device)
         t0 = time.perf_counter()
         rank = _adapter_rank(o["adapter"]) if o["adapter"] else 0
-        engine = Engine(o["model"], dtype="float32" if o["weights"] == "f32" else "bfloat16", device=device,
+        engine = Engine(o["model"], dtype=o["dtype"], device=device,
                         max_seq_len=o["max_seq_len"] or None, page_size=o["page_size"], kv_pages=o["kv_pages"],
                         max_running=1, prefix_cache=False, adapter_slots=1 if rank else 0, adapter_rank=rank or 16,
-                        weights="int8" if o["weights"] == "int8" else "native")
+                        weights="int8" if o["int8"] else "native")
         if rank:
             engine.load_adapter(0, o["adapter"])
         load_s = time.perf_counter() - t0

@@ -149,3 +149,15 @@ def test_command_line():
                               gf.model_dir("c"), "--temperature", "0", "--steps", "20", "--no-echo", "--prompt-ids", " ".join(map(str, prompt))],
                              stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
     assert drafted.returncode == 0 and len(drafted.stdout.split()) == len(want), drafted.stderr
+
+
+@pytest.mark.parametrize("flags", [["--weights", "int8", "--dtype", "fp32"], ["--dtype", "fp32", "--weights", "int8"]])
+def test_command_line_in_32_bit_besides_the_projections(flags):
+    from geneinfer_b200 import Engine
+    prompt = tc.random_tokens(7, 256, 5)
+    run = subprocess.run([sys.executable, os.path.join(ROOT, "bin", "gi_generate"), "--model", gf.model_dir("a"), *flags, "--temperature", "0", "--steps", "20", "--no-echo",
+                          "--prompt-ids", " ".join(map(str, prompt))], stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
+    assert run.returncode == 0, run.stderr
+    engine = Engine(gf.model_dir("a"), dtype="float32", weights="int8", max_running=1, prefix_cache=False)
+    assert [int(t) for t in run.stdout.split()] == engine.generate([prompt], max_new_tokens=20 - len(prompt) + 1, temperature=0.0)[0]
+    assert engine.model.layers[0].int8 and engine.model.dtype is torch.float32

@@ -161,3 +161,19 @@ def test_plans_that_do_not_exist_are_refused():
                           (lambda: many(0), "groups of 0"), (lambda: many(1, ldo=0), "overlap")):
         with pytest.raises(k.KernelError, match=message):
             k.check(code(), "int8_product")
+
+
+def test_command_line_weights_and_type_in_either_order():
+    """``--weights int8`` and ``--dtype`` say two things, and neither is lost to the other's place."""
+    from geneinfer_b200.cli.generate_main import UsageError, parse
+    base = ["--model", "m", "--prompt-ids", "1 2"]
+    int8, fp32, bf16, f32, native = ["--weights", "int8"], ["--dtype", "fp32"], ["--dtype", "bf16"], ["--weights", "f32"], ["--weights", "native"]
+    for flags, want in (([], (False, "bfloat16")), (int8, (True, "bfloat16")), (int8 + fp32, (True, "float32")), (fp32 + int8, (True, "float32")),
+                        (int8 + bf16, (True, "bfloat16")), (bf16 + int8, (True, "bfloat16")), (fp32 + int8 + bf16, (True, "bfloat16")), (fp32, (False, "float32")),
+                        (f32, (False, "float32")), (f32 + int8, (True, "bfloat16")), (int8 + f32, (False, "float32")), (fp32 + native, (False, "bfloat16")),
+                        (f32 + bf16, (False, "bfloat16")), (native + fp32, (False, "float32")), (int8 + fp32 + native, (False, "bfloat16"))):
+        o = parse(base + flags)
+        assert (o["int8"], o["dtype"]) == want, flags
+    for flags in (int8 + fp32, fp32 + int8):
+        with pytest.raises(UsageError, match="--adapter"):
+            parse(base + flags + ["--adapter", "a"])
