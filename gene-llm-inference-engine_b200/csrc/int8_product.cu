@@ -894,6 +894,7 @@ int int8_many_impl(const void* a, const float* a_scales, int T, int width, const
     GI_REQUIRE(T == 1 || ldo >= N, "int8_product: rows of the output overlap");
     GI_REQUIRE(!gated || out_dtype == kBF16, "int8_product: a gated product has a bfloat16 output");
     GI_REQUIRE(act >= 0 && act < kActCount, "int8_product: unknown activation %d", act);
+    GI_REQUIRE(!(gated && act == kActCappedSwish && limit < 0.f), "int8_product: a bound of %g (not below zero)", limit);
     GI_REQUIRE(group_t >= 1, "int8_product: groups of %d tiles", group_t);
     ManyParams p{};
     p.a_scales = a_scales;

@@ -338,6 +338,7 @@ int rows_int8_impl(int kind, const void* x, int x_dtype, long long ldx, const vo
     GI_REQUIRE(x_dtype == kF32 || x_dtype == kBF16, "rows_int8: unsupported dtype code %d", x_dtype);
     GI_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0, "rows_int8: the output must be 16-byte aligned");
     GI_REQUIRE(act >= 0 && act < kActCount, "rows_int8: unknown activation %d", act);
+    GI_REQUIRE(!(act == kActCappedSwish && limit < 0.f), "rows_int8: a bound of %g (not below zero: zeros behind a row have to stay zeros)", limit);
     GI_REQUIRE(ldx >= (kind == kRowsGated ? 2ll : 1ll) * D || T == 1, "rows_int8: rows of x overlap");
     const RowsParams p{x, add, weight, static_cast<int8_t*>(q), scales, ldx, T, D, width, act, limit, eps, w_constant};
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -1823,7 +1823,7 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, scale
 def gated_act_int8(gate_up: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, activation: str = "silu", limit: float = 0.0,
                    bias: Optional[torch.Tensor] = None) -> None:
     """act(gate_up[:, :I]) * gate_up[:, I:], rounded to bfloat16, in 8 bits: ``gate_up`` [T, 2I] (32-bit or bfloat16; rows may lie apart), ``out``
-    [T, int8_width(I)] int8, ``scales`` [T]; ``activation``, ``limit`` and ``bias`` [2I] as ``gated_act`` has them."""
+    [T, int8_width(I)] int8, ``scales`` [T]; ``activation``, ``limit`` (not below zero) and ``bias`` [2I] as ``gated_act`` has them."""
     if gate_up.dim() != 2 or gate_up.shape[1] % 2 or (bias is not None and bias.numel() != gate_up.shape[1]):
         raise KernelError("gated_act_int8: gate_up must be [T, 2I] (and the bias [2I])")
     if activation not in ACTIVATIONS:

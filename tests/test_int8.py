@@ -177,3 +177,22 @@ def test_command_line_weights_and_type_in_either_order():
     for flags in (int8 + fp32, fp32 + int8):
         with pytest.raises(UsageError, match="--adapter"):
             parse(base + flags + ["--adapter", "a"])
+
+
+def test_a_bound_below_zero_is_refused():
+    """Such a bound makes something of the zeros behind a row (min(0, limit)), which would go into its integers and its scale. No GPU needed."""
+    x, q, s = torch.zeros(2, 40), torch.zeros(2, 32, dtype=torch.int8), torch.zeros(2)
+    room = torch.zeros(64 + 16, dtype=torch.int8)
+    at = room.data_ptr() + -room.data_ptr() % 16
+
+    def rows(limit, activation):
+        return k.lib().gi_rows_int8(2, x.data_ptr(), k.F32, 40, 0, 0, 0, 0.0, k.ACTIVATIONS[activation], limit, at, 32, s.data_ptr(), 2, 20, 0, 0)
+
+    with pytest.raises(k.KernelError, match="bound of -1"):
+        k.check(rows(-1.0, "capped_swish"), "gated_act_int8")
+    tiles = torch.zeros(2 * 16384 + 128, dtype=torch.int8)
+    a = torch.zeros(2 * 16 + 16, dtype=torch.int8)
+    code = k.lib().gi_int8_product_many(a.data_ptr() + -a.data_ptr() % 16, s.data_ptr(), 2, 16, tiles.data_ptr() + -tiles.data_ptr() % 128, s.data_ptr(), 20, 1,
+                                        k.ACTIVATIONS["capped_swish"], -1.0, 0, x.data_ptr(), k.BF16, 24, 0, 1, s.data_ptr(), 0)
+    with pytest.raises(k.KernelError, match="bound of -1"):
+        k.check(code, "int8_gated")
