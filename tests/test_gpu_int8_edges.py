@@ -71,3 +71,24 @@ def test_additions_of_values_below_the_least_normal_one(T):
                     out[:, :N] = base
                     k.int8_product(a, s, w, out[:, :N], accumulate=True, plan=plan)
                     assert torch.equal(out[:, :N], base + want) and (out[:, N:] == 7).all(), (N, plan, room)
+
+
+@pytest.mark.parametrize("activation", ["silu", "relu", "gelu_tanh", "capped_swish"])
+@pytest.mark.parametrize("T,K,I", [(2048, 512, 1024), (1500, 130, 4099), (700, 777, 8200)])
+def test_activated_rows_of_few_and_of_many_are_the_same(T, K, I, activation):
+    """With few rows the products go through memory in 32 bits, with many the activation is the product's epilogue: the same integers and scales, to the bit."""
+    k = _kernels()
+    g = torch.Generator(device=DEV).manual_seed(T + I)
+    q, ws = torch.randint(-127, 128, (2 * I, K), generator=g, device=DEV, dtype=torch.int8), (0.01 + torch.rand(2 * I, generator=g, device=DEV)) / (4900 * math.sqrt(K))
+    w = k.int8_weight(q, ws, gated=True)
+    _, a, s, _ = _product(k, g, T, K, 1)
+    for bias in (None, 0.2 * torch.randn(2 * I, generator=g, device=DEV)):
+        got = []
+        for n in (T, 60, 1):
+            out, scales = torch.full((n, k.int8_width(I)), 77, dtype=torch.int8, device=DEV), torch.full((n,), -1.0, device=DEV)
+            k.int8_gated(a[:n], s[:n], w, out, scales, torch.empty(k.int8_gated_work(n, w), device=DEV), activation, 2.0, bias)
+            got.append((out, scales))
+            assert k._int8_plan(n, w)[0] == ("many" if n == T else "few")
+        for out, scales in got[1:]:
+            n = scales.numel()
+            assert torch.equal(out, got[0][0][:n]) and torch.equal(scales, got[0][1][:n])

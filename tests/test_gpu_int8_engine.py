@@ -161,3 +161,58 @@ def test_command_line_in_32_bit_besides_the_projections(flags):
     engine = Engine(gf.model_dir("a"), dtype="float32", weights="int8", max_running=1, prefix_cache=False)
     assert [int(t) for t in run.stdout.split()] == engine.generate([prompt], max_new_tokens=20 - len(prompt) + 1, temperature=0.0)[0]
     assert engine.model.layers[0].int8 and engine.model.dtype is torch.float32
+
+
+def _logits(engine, name, tokens, portion, wanted):
+    """32-bit logits of the wanted positions of a prompt fed in portions; the request is closed again."""
+    from geneinfer_b200.engine.step import StepEntry
+    engine.open(name)
+    rows = []
+    for at in range(0, len(tokens), portion):
+        here = tokens[at:at + portion]
+        out = engine.step([StepEntry(name, here, [p - at for p in wanted if at <= p < at + len(here)])])
+        if out is not None:
+            rows.append(out.clone())
+    engine.close(name)
+    return torch.cat(rows)
+
+
+@pytest.mark.parametrize("length", [700, 1300])
+def test_long_prompts_in_one_step_and_in_portions(length):
+    """A step of more rows than any projection takes as few (1,300 at these widths; at 700 some of each) gives what portions of 64 and of 7 tokens give, to the bit, the
+    first time and from the recorded launches."""
+    from geneinfer_b200.engine.loading import load_model
+    from geneinfer_b200.engine.step import StepEngine
+    from geneinfer_b200.ops import kernels
+    model = load_model(gf.model_dir("w"), dtype="float32", weights="int8", max_position=2048)
+    engine = StepEngine(model, n_pages=256, max_requests=2, max_step_tokens=1400, debug_checks=True)
+    layer = model.layers[0]
+    forms = {kernels._int8_plan(length, linear.weight)[0] for linear in (layer.mixer.w_qkv, layer.mixer.w_o, layer.feed_forward.w_gate_up, layer.feed_forward.w_down)}
+    assert forms == ({"many"} if length == 1300 else {"few", "many"})
+    tokens = tc.random_tokens(length, 128256, length)
+    wanted = [0, 5, 63, 64, 300, length - 1]
+    whole = _logits(engine, "whole", tokens, length, wanted)
+    assert bool(whole.isfinite().all())
+    before = engine.program_runs
+    assert torch.equal(_logits(engine, "again", tokens, length, wanted), whole) and engine.program_runs > before
+    assert torch.equal(_logits(engine, "portions", tokens, 64, wanted), whole)
+    assert torch.equal(_logits(engine, "small", tokens[:301], 7, wanted[:5]), whole[:5])
+    assert kernels.gemm_tc_status(engine.device) == 0
+
+
+def test_long_prompts_of_the_serving_path():
+    """bfloat16, steps of 1,400 tokens: products of many rows, the gated epilogue, the addition with the norm; twice the same, and near the 32-bit path."""
+    from geneinfer_b200.engine.loading import load_model
+    from geneinfer_b200.engine.step import StepEngine
+    from geneinfer_b200.ops import kernels
+    tokens, wanted = tc.random_tokens(1300, 128256, 3), [0, 300, 1299]
+    rows = {}
+    for dtype in ("bfloat16", "float32"):
+        engine = StepEngine(load_model(gf.model_dir("w"), dtype=dtype, weights="int8", max_position=2048), n_pages=256, max_requests=2, max_step_tokens=1400, debug_checks=True)
+        rows[dtype] = _logits(engine, "first", tokens, 1300, wanted)
+        assert torch.equal(_logits(engine, "again", tokens, 1300, wanted), rows[dtype])
+        assert kernels.gemm_tc_status(engine.device) == 0
+    # The cache, the attention and the head's input round to bfloat16, 2^-9 of a value: half a step of 127 and more, so that the rows of a projection round apart. Two
+    # roundings of one value that know nothing of each other differ by sqrt(1/6) of a step, a step is 1/127 of a row's largest value, that at most 6 times its root mean
+    # square: 6 / 127 / sqrt(6) = 0.019 of a row. Eight projections (four in each of two layers), in squares: 0.055; the bfloat16 roundings themselves are a tenth of it.
+    assert _off(rows["bfloat16"], rows["float32"].double()) < 0.0625
