@@ -1847,6 +1847,14 @@ class Int8Weight:
     none behind them start early). Who writes them by other means sets it to False. ``scales`` are read behind the wait and may be the launch's before."""
 
     def __init__(self, tiles: torch.Tensor, scales: torch.Tensor, channels: int, width: int, gated: bool, constant: bool = False):
+        parts = 2 if gated else 1
+        size = parts * ((channels + 127) // 128) * ((width + 127) // 128) * 128 * 128
+        if channels < 1 or width < 16 or width % 16 or width > INT8_WIDTH_MOST:
+            raise KernelError(f"Int8Weight: {channels} channels of {width} values (a width is a multiple of 16, at most {INT8_WIDTH_MOST})")
+        if tiles.dtype is not torch.int8 or not tiles.is_contiguous() or tiles.numel() != size:
+            raise KernelError(f"Int8Weight: the tiles must be int8, {size} of them side by side")
+        if scales.dtype is not torch.float32 or not scales.is_contiguous() or scales.numel() != parts * channels:
+            raise KernelError(f"Int8Weight: the scales must be 32-bit, {parts * channels} of them side by side")
         self.tiles, self.scales, self.channels, self.width, self.gated, self.constant = tiles, scales, channels, width, gated, constant
         self.plans, self.works = {}, {}      # rows -> the plan of a product of so many, and the scratch: sizes decide, once
 

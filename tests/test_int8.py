@@ -196,3 +196,17 @@ def test_a_bound_below_zero_is_refused():
                                         k.ACTIVATIONS["capped_swish"], -1.0, 0, x.data_ptr(), k.BF16, 24, 0, 1, s.data_ptr(), 0)
     with pytest.raises(k.KernelError, match="bound of -1"):
         k.check(code, "int8_gated")
+
+
+def test_tiles_put_together_by_hand_have_to_be_the_weights():
+    """The kernels take sizes from the weight: tiles or scales that are fewer would be read behind their end."""
+    w = k.int8_weight(torch.zeros(300, 200, dtype=torch.int8), torch.ones(300))
+    pair = k.int8_weight(torch.zeros(300, 200, dtype=torch.int8), torch.ones(300), gated=True)
+    assert k.Int8Weight(w.tiles, w.scales, 300, 208, False).constant is False and w.constant and pair.constant
+    k.Int8Weight(pair.tiles, pair.scales, 150, 208, True)
+    for tiles, scales, channels, width, gated in ((w.tiles[:-1], w.scales, 300, 208, False), (w.tiles, w.scales, 300, 257 + 15, False), (w.tiles, w.scales, 385, 208, False),
+                                                  (w.tiles, w.scales, 300, 208, True), (w.tiles, w.scales[:299], 300, 208, False), (w.tiles, w.scales.double(), 300, 208, False),
+                                                  (w.tiles.float(), w.scales, 300, 208, False), (w.tiles, w.scales, 300, 200, False), (w.tiles, w.scales, 0, 208, False),
+                                                  (w.tiles.view(2, -1).T, w.scales, 300, 208, False), (pair.tiles, pair.scales[:150], 150, 208, True)):
+        with pytest.raises(k.KernelError, match="Int8Weight"):
+            k.Int8Weight(tiles, scales, channels, width, gated)
