@@ -15,7 +15,7 @@
 // NaN. A norm whose squares or products with the weights leave the range of 32 bits is taken again: the squares from values 2^-80 times as large, or
 // 2^80 times where they vanish beside an eps that is as small, and the products with the weights likewise, each by a factor of its own (values near 1 with weights
 // near 2^127 have squares as they should be).
-// Rows whose largest |v| is below 2^-100 count as zero (scale 0): 127 / m would leave that range at the other end.
+// Rows whose largest |v| (as it was taken last) is below 2^-100 count as zero (scale 0): 127 / m would leave that range at the other end.
 #include "common.cuh"
 
 namespace gi {
@@ -170,7 +170,7 @@ __device__ __forceinline__ unsigned top_bits(const float4 v, unsigned m) {
 // 2^60 then.)
 __device__ __forceinline__ bool other_factors(unsigned m, float ss, float eps, Factors& f) {
     if (!(ss < __uint_as_float(kInfBits))) f.squares = kDown;
-    else if (ss < kLeastSquares && eps < kLeastEps && m > 0) f.squares = kUp;
+    else if (ss < kLeastSquares && eps < kLeastEps) f.squares = kUp;
     if (m >= kInfBits) f.values = kDown;
     else if (f.squares == kUp && m < kSmallBits) f.values = kUp;
     return f.squares != 1.f || f.values != 1.f;

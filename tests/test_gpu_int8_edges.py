@@ -92,3 +92,19 @@ def test_activated_rows_of_few_and_of_many_are_the_same(T, K, I, activation):
         for out, scales in got[1:]:
             n = scales.numel()
             assert torch.equal(out, got[0][0][:n]) and torch.equal(scales, got[0][1][:n])
+
+
+@pytest.mark.parametrize("D", [300, 9001, 33000])
+def test_small_norms_with_small_weights(D):
+    """Rows without an eps whose products with the weights vanish in 32 bits altogether, though the normed values do not."""
+    k = _kernels()
+    g = torch.Generator(device=DEV).manual_seed(D)
+    x = torch.randn(2, D, generator=g, device=DEV) * 1e-30
+    x[1] = 0
+    w = (0.5 + 0.5 * torch.rand(D, generator=g, device=DEV)) * 1e-20
+    assert not (x * w).any()
+    q, s = torch.empty(2, k.int8_width(D), dtype=torch.int8, device=DEV), torch.empty(2, device=DEV)
+    k.rmsnorm_int8(x, w, q, s, 0.0)
+    want = x[0].double() / x[0].double().square().mean().sqrt() * w.double()
+    assert float((q[0, :D].double() * s[0].double() - want).abs().max()) <= float(want.abs().max()) / 127 * 0.501
+    assert float(s[1]) == 0 and not q[1].any()
