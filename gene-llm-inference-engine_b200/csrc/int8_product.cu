@@ -4,7 +4,8 @@
 //
 // tcgen05.mma kind::i8 adds the products in 32-bit integers in tensor memory. They are exact (K up to 131,056, which the host
 // checks), so a result depends neither on how K is cut nor on which of the two kernels below computed it: every sum is turned
-// into a float once, multiplied by the row's scale, then by the channel's, in that order everywhere.
+// into a float once, multiplied by the row's scale, then by the channel's, in that order everywhere (so the sum times the row's scale has to lie within the
+// range of 32 bits), and what it is added to is added once, rounded to nearest, subnormals kept, by either kernel.
 //
 // The weights lie in tiles of 128 channels x 128 values of K, 16 KB each, [channel tile][block of K][128][128] with K padded to whole
 // blocks by zeros and every row's eight 16-byte pieces permuted by piece ^ (row % 8): a tile in memory is what tcgen05.mma
@@ -18,7 +19,7 @@
 //
 // Many rows (int8_many_kernel). Pairs of CTAs (cta_group::2) on tiles of 256 rows x 256 channels, persistent, accumulators
 // twice in tensor memory so that the epilogue of a tile runs beside the products of the next. Epilogues: 32-bit store or addition and
-// bfloat16 store by TMA from a staging buffer (or by plain stores, where the output's rows are not whole 16 bytes), and act(gate) * up in
+// bfloat16 store by TMA from a staging buffer (or by the lanes' loads and stores, where the output's rows are not whole 16 bytes), and act(gate) * up in
 // bfloat16 for gated weights.
 //
 // Every wait is bounded: where a limit is hit the kernel records a code in the status word, stops issuing work, lets its own copies

@@ -210,8 +210,9 @@ __device__ __forceinline__ float2 row_factors(unsigned m_bits, float ss, const R
 
 // G threads to a row, V groups of four values each in registers, read in batches: 64 registers, so that an SM holds 1,024 threads of it (of two rows at least,
 // up to 16,384 values). 8,192 rows of 4,096 with a 32-bit addition: 64 us, 6.8 TB/s (the measured copy rate is 6.55; some of it stays in L2); 8,192 of 16,384
-// from 16 bits: 78 us, 5.1 TB/s; 4,096 activated rows of 14,336: from 32 bits 90 us, 5.9 TB/s, from 16 bits 67 us, 4.4 TB/s (23 instructions a value at 2.3 of 4 a
-// cycle). One row of 2,048: 1.8 us in a stream of launches.
+// from 16 bits: 78 us, 5.1 TB/s; 4,096 activated rows of 14,336: from 32 bits 90 us, 5.9 TB/s, from 16 bits 67 us, 4.4 TB/s (neither memory, at half its rate, nor
+// the issue of instructions, 23 a value at 2.3 of 4 a cycle, is full: a row's loads, arithmetic and stores follow each other, and two rows are all that an SM holds).
+// One row of 2,048: 1.8 us in a stream of launches.
 template <int KIND, typename TX, typename TA, int G, int V, bool VEC>
 __global__ void __launch_bounds__(G < 128 ? 128 : G, G <= 512 ? 1024 / (G < 128 ? 128 : G) : 1)
 rows_int8_kernel(const RowsParams p) {

@@ -3,6 +3,10 @@
 Each function checks device, dtype, contiguity and sizes of what it is given (a kernel never sees
 a pointer it could misread) and raises ``KernelError`` with the library's message when the library
 refuses a size. Nothing here computes on the host.
+
+Kernels begin while the one ahead still runs and wait before they read what it writes. A model's weights are no launch's output, so that several entry
+points (``rmsnorm``, ``gemm_tc`` and what is built on them, convolutions, head norms, routers) read them ahead of that wait: such a weight must not be written by a
+launch of this library that may still be running. Those with ``w_constant`` (and ``Int8Weight.constant``) read weights behind it unless they are told.
 """
 from __future__ import annotations
 
@@ -1950,7 +1954,8 @@ def _int8_operands(name: str, a: torch.Tensor, a_scales: torch.Tensor, w: Int8We
 def int8_product(a: torch.Tensor, a_scales: torch.Tensor, w: Int8Weight, out: torch.Tensor, accumulate: bool = False, plan=None) -> None:
     """out[t, n] (+)= a_scales[t] * w.scales[n] * sum over k of a[t, k] * w[n, k]: ``a`` [T, w.width] int8 with ``a_scales`` [T], ``out``
     [T, N] 32-bit (``accumulate``: added to) or bfloat16; its rows may lie apart. The sums are exact integers: a row's result does
-    not depend on the other rows of the call."""
+    not depend on the other rows of the call. A sum times its row's scale has to lie within the range of 32 bits. ``plan``: a form to take instead of the
+    chosen one (``_int8_plan_of``), with the same results."""
     T = _int8_operands("int8_product", a, a_scales, w, out)
     if w.gated:
         raise KernelError("int8_product: the weight is laid out for int8_gated")
